@@ -415,6 +415,58 @@ enum rh_post_stage {
   RH_POST_ALL = 7
 };
 
+/* ------------------------------------------------------------------ classifier over a large label set */
+/* Element types of the entry points below. */
+enum rh_dtype { RH_F32 = 0, RH_BF16 = 1, RH_F16 = 2 };
+
+enum rh_ce_reduction { RH_CE_MEAN = 0, RH_CE_SUM = 1 };
+
+enum rh_ce_flags {
+  RH_CE_GRAD_X = 1,       /* of the workspace query: dx / dw / db will be asked for */
+  RH_CE_GRAD_W = 2,
+  RH_CE_GRAD_B = 4,
+  RH_CE_COPY_WEIGHT = 8   /* w's rows are not whole, aligned 16-byte pieces (d * element size, ldw *
+                             element size or the address): the call works on a padded copy */
+};
+
+/* Softmax cross entropy of the logits x w^T + bias, with its gradients, in pieces of the classes: the
+ * logits are never stored whole.  A row whose label is ignore_index takes no part (no loss, zero gradient,
+ * whatever its features hold); so does one with a label outside [0, v), which also sets
+ * RH_STATUS_LABEL_RANGE.  A call without a counted row has loss 0 and zero gradients.
+ * dx / dw / db (each may be NULL) hold the gradients times `grad`, for an upstream gradient of that size. */
+typedef struct rh_linear_ce_args {
+  const void* x;           /* device [n][ldx]: features                                           */
+  const void* w;           /* device [v][ldw]: one row a class                                    */
+  const void* bias;        /* device [v] or NULL                                                  */
+  const void* labels;      /* device [n], int64 or int32                                          */
+  int64_t n, v;
+  int64_t ldx, ldw;        /* row strides in elements                                             */
+  int32_t d;
+  int32_t dtype;           /* rh_dtype of x, w, bias and the gradients                            */
+  int32_t labels_int64;
+  int32_t reduction;       /* rh_ce_reduction                                                     */
+  int64_t ignore_index;
+  const float* divisor;    /* device [1] or NULL: what the mean divides by instead of this call's
+                              counted rows (a sharded batch passes the count over all ranks)      */
+  float grad;
+  int32_t flags;           /* RH_CE_COPY_WEIGHT                                                   */
+  float* row_loss;         /* device [n] out                                                      */
+  float* small;            /* device [4] out: loss, rows counted, 1 / divisor, status (int32)     */
+  void* dx;                /* device [n][d] out                                                   */
+  void* dw;                /* device [v][d] out                                                   */
+  void* db;                /* device [v] out                                                      */
+  void* workspace;
+  size_t workspace_bytes;
+} rh_linear_ce_args;
+
+/* 0 for sizes out of range: n <= 2^26, d <= 2^17, v <= 2^24. */
+size_t rh_linear_ce_workspace_bytes(int64_t n, int32_t d, int64_t v, int32_t dtype, int32_t flags);
+int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream);
+
+/* x *= *scale / assumed in place; nothing is touched when *scale == assumed (no host read). */
+int rh_scale_gradient(void* x, int64_t count, int32_t dtype, const float* scale, float assumed,
+                      rh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

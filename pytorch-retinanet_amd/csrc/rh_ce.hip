@@ -1,0 +1,886 @@
+// Softmax cross entropy of a classifier's last projection over a large label set, forward and
+// backward, without the logits ever being kept (gfx950).
+//
+//   z[n][v] = x[n] . w[v] + b[v],   lse[n] = log sum_v exp z[n][v]
+//   row[n]  = lse[n] - z[n][y_n],   loss = s sum_n row[n],   s = 1 / max(1, rows counted)  or  1
+//   P[n][v] = exp(z[n][v] - lse[n]) - [v == y_n]
+//   dX = s P W,   dW = s P^T X,   db = s sum_n P
+//
+// Rows whose label is ignore_index, or outside [0, V), take no part: the features of the others are
+// laid out one after the other in a scratch copy first (its rows padded to whole tile steps), so
+// what stands in a row left out never meets a product, not even as 0 * inf, and costs nothing.
+#include "rh_gemm.h"
+
+namespace rh {
+namespace ce {
+
+using namespace gemm;
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp as the loss needs it: for float results the accurate one; for 16-bit ones the hardware exp2 of a
+// rounded product (|x| * 6e-8 relative, far below the 2^-9 of the type the result is rounded to).
+template <typename T>
+__device__ __forceinline__ float exp_for(const float x) {
+  return __builtin_amdgcn_exp2f(x * kLog2e);
+}
+template <>
+__device__ __forceinline__ float exp_for<float>(const float x) {
+  return expf(x);
+}
+
+// P is the matrix units' operand and so is rounded to the inputs' type.  float16 has no room for
+// small probabilities (2^-24 is its smallest value, one of 131 072 equal classes has 2^-17): there P
+// is kept times 2^15, which |P| <= 1 allows, and the products' results are scaled back, both exact.
+template <typename T>
+struct PScale {
+  static constexpr float up = 1.0f, down = 1.0f;
+};
+template <>
+struct PScale<_Float16> {
+  static constexpr float up = 32768.0f, down = 1.0f / 32768.0f;
+};
+
+// ---------------------------------------------------------------------------------------------
+// Labels, rows
+// ---------------------------------------------------------------------------------------------
+struct Labels {
+  const void* p;
+  int wide;             // int64, else int32
+  long long ignore;
+  int v;
+  __device__ __forceinline__ long long at(const long long i) const {
+    return wide ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
+  }
+  __device__ __forceinline__ bool counts(const long long y) const { return y != ignore && y >= 0 && y < v; }
+};
+
+// Per block of `per` rows: how many count, and whether a label lies outside [0, V).
+__global__ __launch_bounds__(64) void count_rows_kernel(const Labels y, const int n, const int per,
+                                                       int2* __restrict__ blocks) {
+  const long long lo = (long long)blockIdx.x * per, hi = min((long long)n, lo + per);
+  int count = 0, bad = 0;
+  for (long long i = lo + threadIdx.x; i < hi; i += 64) {
+    const long long t = y.at(i);
+    count += y.counts(t);
+    bad |= t != y.ignore && (t < 0 || t >= y.v);
+  }
+  count = wave_sum(count);
+  bad = __any(bad);
+  if (threadIdx.x == 0) blocks[blockIdx.x] = make_int2(count, bad);
+}
+
+struct RowInfo {
+  int* map;        // [n] place -> row
+  int* label;      // [n] place -> label
+  int* n_valid;    // [1]
+  float* scale;    // [1] s * expected upstream gradient
+};
+
+// Copies the rows that count to their places, zero-padded to ldp values; sets what a row left out
+// gets: no loss, no gradient.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void place_rows_kernel(
+    const T* __restrict__ x, const long long ldx, const int d, const Labels y, const int n, const int per,
+    const int2* __restrict__ blocks, T* __restrict__ xp, const int ldp, const RowInfo info,
+    float* __restrict__ row_loss, T* __restrict__ dx, float* __restrict__ small, int* __restrict__ status,
+    const float* __restrict__ total, const int mean, const float grad) {
+  __shared__ int s_red[4], s_bad[4];
+  __shared__ int s_place[kThreads];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  int before = 0, all = 0, bad = 0;
+  for (int i = t; i < (int)gridDim.x; i += kThreads) {
+    const int2 c = blocks[i];
+    if (i < (int)blockIdx.x) before += c.x;
+    all += c.x;
+    bad |= c.y;
+  }
+  before = wave_sum(before);
+  all = wave_sum(all);
+  bad = __any(bad);
+  if (lane == 0) {
+    s_red[wave] = before;
+    s_bad[wave] = bad;
+  }
+  __syncthreads();
+  before = s_red[0] + s_red[1] + s_red[2] + s_red[3];
+  bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    if (lane == 0) s_red[wave] = all;
+    __syncthreads();
+    if (t == 0) {
+      all = s_red[0] + s_red[1] + s_red[2] + s_red[3];
+      *info.n_valid = all;
+      const float div = mean ? fmaxf(total ? *total : (float)all, 1.0f) : 1.0f;
+      *info.scale = grad / div;
+      small[1] = (float)all;
+      small[2] = 1.0f / div;
+      *status = bad ? RH_STATUS_LABEL_RANGE : 0;
+    }
+    __syncthreads();
+  }
+  // this block's rows: place within the block by a ballot count (per <= 256)
+  const long long lo = (long long)blockIdx.x * per;
+  const int rows = (int)min((long long)per, n - lo);
+  bool keep = false;
+  long long label = 0;
+  if (t < rows) {
+    label = y.at(lo + t);
+    keep = y.counts(label);
+  }
+  const unsigned long long kept = __ballot(keep);
+  if (lane == 0) s_red[wave] = __popcll(kept);
+  __syncthreads();
+  int at = before + __popcll(kept & ((1ull << lane) - 1ull));
+  for (int i = 0; i < wave; ++i) at += s_red[i];
+  if (t < rows) {
+    s_place[t] = keep ? at : -1;
+    if (keep) {
+      info.map[at] = (int)(lo + t);
+      info.label[at] = (int)label;
+    } else {
+      row_loss[lo + t] = 0.0f;
+    }
+  }
+  __syncthreads();
+  const bool wide = ((ldx * (long long)sizeof(T)) & 15) == 0 && ((uintptr_t)x & 15) == 0;
+  constexpr int kV = 16 / (int)sizeof(T);
+  for (int r = wave; r < rows; r += 4) {
+    const int to = s_place[r];
+    const T* src = x + (lo + r) * ldx;
+    if (to >= 0) {
+      T* dst = xp + (long long)to * ldp;
+      if (wide) {
+        int c = lane * kV;
+        for (; c + kV <= d; c += 64 * kV) *(u32x4*)(dst + c) = *(const u32x4*)(src + c);
+        for (; c < ldp; c += 64 * kV)
+          for (int k = 0; k < kV; ++k) dst[c + k] = c + k < d ? src[c + k] : (T)0.0f;
+      } else {
+        for (int c = lane; c < ldp; c += 64) dst[c] = c < d ? src[c] : (T)0.0f;
+      }
+    } else if (dx) {
+      T* dst = dx + (lo + r) * (long long)d;
+      for (int c = lane; c < d; c += 64) dst[c] = (T)0.0f;
+    }
+  }
+}
+
+// A copy of the weights with rows of whole 16-byte pieces, for a row length or stride that has none.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* __restrict__ w, const long long ldw,
+                                                            const int d, const int v, T* __restrict__ out,
+                                                            const int ldp) {
+  const int lane = threadIdx.x & 63;
+  for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < v; r += (long long)gridDim.x * 4)
+    for (int c = lane; c < ldp; c += 64) out[r * ldp + c] = c < d ? w[r * ldw + c] : (T)0.0f;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Logits of one tile, and what becomes of them
+// ---------------------------------------------------------------------------------------------
+struct Grid {
+  int m, n;        // tiles
+};
+
+// Tiles in groups of eight rows of tiles, down a group's column first: the workgroups that run side
+// by side on an XCD share both operands' rows in its L2.
+__device__ __forceinline__ int2 tile_at(const Grid g, const int id) {
+  const int t = xcd_run(id, g.m * g.n);
+  const int span = 8 * g.n, first = t / span * 8, rows = min(8, g.m - first), in = t % span;
+  return make_int2(first + in % rows, in / rows);
+}
+
+template <typename T>
+struct LogitArgs {
+  const T* x;          // placed rows, ldx apart, zero-padded
+  long long ldx;
+  const T* w;          // first class of this call
+  long long ldw, w_bytes;
+  const T* bias;
+  int steps;           // of k
+  int w_limit;         // bytes of the last step that are the weights' rows
+  int v0, v;           // first class, how many
+  Grid grid;
+  RowInfo info;
+  float2* stats;       // [tile of classes][place]  (max, sum of exp above it)
+  long long ld_stats;
+  float* z_label;      // [place]
+  const float* lse;    // [place]
+  T* p;                // [place][ldp]
+  int ldp;
+};
+
+enum What { kStats, kProb };
+
+template <typename T, typename S, What kWhat>
+__global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_kernel(const LogitArgs<T> a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  RH_LDS char* lds = (RH_LDS char*)smem;
+  const int2 at = tile_at(a.grid, blockIdx.x);
+  const int rows = *a.info.n_valid, m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  if (m0 >= rows) return;
+  Tile<T, kRows, kRows, S> tile;
+  tile.run(a.x + m0 * a.ldx, a.ldx, ((long long)rows - m0) * a.ldx * (int)sizeof(T),
+           a.w + n0 * a.ldw, a.ldw, a.w_bytes - (long long)n0 * a.ldw * (int)sizeof(T), a.steps, lds, a.w_limit);
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
+  const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32;
+  const int left = a.v - n0 - wn - 4 * half;      // this lane's columns (32 j + 8 q + r) below it exist
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int c = min(32 * j + 8 * (r >> 2) + (r & 3), left - 1);       // past the last class: any
+        const float b = TypeOf<T>::to_float(a.bias[max(a.v0 + n0 + wn + 4 * half + c, 0)]);
+#pragma unroll
+        for (int i = 0; i < S::kFM; ++i) tile.acc[i][j][r] += b;
+      }
+  }
+  if constexpr (kWhat == kStats) {
+    if (a.v - n0 < S::kBN) {      // classes that do not exist
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool none = 32 * j + 8 * (r >> 2) + (r & 3) >= left;
+#pragma unroll
+          for (int i = 0; i < S::kFM; ++i) tile.acc[i][j][r] = none ? -__builtin_inff() : tile.acc[i][j][r];
+        }
+    }
+    RH_LDS float2* red = (RH_LDS float2*)lds;      // [kWN][kBM]
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::kFM; ++i) {
+      const int m = wm + 32 * i + (lane & 31), row = m0 + m;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, tile.acc[i][j][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += exp_for<T>(tile.acc[i][j][r] - base);
+      sum += __shfl_xor(sum, 32, 64);
+      if (half == 0) {
+        float2 pair = make_float2(top, sum);
+        red[(wave % S::kWN) * S::kBM + m].x = pair.x;
+        red[(wave % S::kWN) * S::kBM + m].y = pair.y;
+      }
+      const int c = row < rows ? a.info.label[row] - (a.v0 + n0 + wn + 4 * half) : -1;
+      const bool mine = c >= 0 && c < S::kFN * 32 && (c & 7) < 4;
+      if (__any(mine)) {
+        float z = 0.0f;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z = c == 32 * j + 8 * (r >> 2) + (r & 3) ? tile.acc[i][j][r] : z;
+        if (mine) a.z_label[row] = z;
+      }
+      __builtin_amdgcn_sched_barrier(0);      // one fragment row's registers at a time
+    }
+    __syncthreads();
+    if (t < S::kBM && m0 + t < rows) {
+      float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < S::kWN; ++k) top = fmaxf(top, red[k * S::kBM + t].x);
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+      for (int k = 0; k < S::kWN; ++k)
+        sum += red[k * S::kBM + t].y * exp_for<T>(red[k * S::kBM + t].x - base);
+      a.stats[(long long)(a.v0 / S::kBN + at.y) * a.ld_stats + m0 + t] = make_float2(top, sum);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::kFM; ++i) {
+      const int row = m0 + wm + 32 * i + (lane & 31);
+      if (row < rows) {
+        const float lse = a.lse[row];
+        const int c = a.info.label[row] - (a.v0 + n0 + wn + 4 * half);
+        const int room = a.ldp - n0 - wn - 4 * half;      // columns up to ldp are written, with zeros past v
+        T* out = a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int at0 = 32 * j + 8 * q;
+            Vec4<T> v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float p = exp_for<T>(tile.acc[i][j][4 * q + r] - lse);
+              p = (c == at0 + r ? p - 1.0f : p) * PScale<T>::up;
+              v.v[r] = TypeOf<T>::from_float(at0 + r < left ? p : 0.0f);
+            }
+            if (at0 < room) *(Vec4<T>*)(out + at0) = v;
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);      // one fragment row's registers at a time
+    }
+  }
+}
+
+// lse and row loss of every place from the tiles' pairs: eight threads a row, each an eighth of the
+// tiles, joined by (max, sum) pairs.
+__global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __restrict__ stats,
+                                                              const long long ld, const int tiles,
+                                                              const RowInfo info,
+                                                              const float* __restrict__ z_label,
+                                                              float* __restrict__ lse,
+                                                              float* __restrict__ row_loss,
+                                                              double* __restrict__ partial) {
+  __shared__ float s_top[8][32], s_sum[8][32];
+  const int rows = *info.n_valid, r = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + r;
+  float top = -__builtin_inff(), sum = 0.0f;
+  if (row < rows) {
+    for (int t = part; t < tiles; t += 8) {
+      const float2 p = stats[t * ld + row];
+      const float up = fmaxf(top, p.x), base = up == -__builtin_inff() ? 0.0f : up;
+      sum = sum * expf(top - base) + p.y * expf(p.x - base);
+      top = up;
+    }
+  }
+  s_top[part][r] = top;
+  s_sum[part][r] = sum;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    double loss = 0.0;
+    if (part == 0 && row < rows) {
+      top = -__builtin_inff();
+      sum = 0.0f;
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, s_top[k][r]);
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      for (int k = 0; k < 8; ++k) sum += s_sum[k][r] * expf(s_top[k][r] - base);
+      const float l = top + logf(sum), v = l - z_label[row];
+      lse[row] = l;
+      row_loss[info.map[row]] = v;
+      loss = (double)v;
+    }
+    loss = wave_sum(loss);
+    if (threadIdx.x == 0) partial[blockIdx.x] = loss;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __restrict__ partial, const int n,
+                                                               float* __restrict__ small) {
+  __shared__ double s_red[4];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) sum += partial[i];
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) small[0] = (float)(((s_red[0] + s_red[1]) + (s_red[2] + s_red[3])) * (double)small[2]);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradients
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+struct ProductArgs {
+  const T* a;
+  long long lda;
+  const T* b;
+  long long ldb, b_bytes;      // readable from b on (kCols: its rows end with the sum instead)
+  int m, n, k;                 // on the host's side; rows that count bound m or k on the device
+  const int* rows;             // bounds m (kRows A) or k (kCols A)
+  Grid grid;
+  int split_steps;             // k steps a split takes
+  const float* scale;
+  float down;
+  T* out;                      // [map[m] or m][ldo]
+  const int* map;
+  long long ldo;
+  float* part;                 // [split][m][ldpart] instead of out
+  long long ldpart, plane;
+  int add;                     // part += instead of part =
+};
+
+enum To { kParts, kQuads, kSingly };     // float parts; the result, rows of whole groups of four values or not
+
+template <typename T, Layout kLA, Layout kLB, typename S, To kTo>
+__global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  RH_LDS char* lds = (RH_LDS char*)smem;
+  constexpr int kStepK = kStepBytes / (int)sizeof(T);
+  const int2 at = tile_at(a.grid, blockIdx.x);
+  const int rows = *a.rows, m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  const int m = kLA == kRows ? min(a.m, rows) : a.m, k = kLA == kCols ? min(a.k, rows) : a.k;
+  if (m0 >= m) return;
+  const long long size = sizeof(T);
+  const long long k0 = (long long)blockIdx.y * a.split_steps * kStepK;
+  const int steps = (int)max(0ll, min((long long)a.split_steps, (k - k0 + kStepK - 1) / kStepK));
+  const T* pa;
+  const T* pb;
+  long long a_bytes, b_bytes;
+  if (kLA == kRows) {
+    pa = a.a + m0 * a.lda + k0;
+    a_bytes = (((long long)m - m0 - 1) * a.lda + k - k0) * size;
+  } else {
+    pa = a.a + k0 * a.lda + m0;
+    a_bytes = ((k - k0) * a.lda - m0) * size;
+  }
+  static_assert(kLB == kCols, "the second operand of both products has the sum down its columns");
+  pb = a.b + k0 * a.ldb + n0;
+  b_bytes = min(a.b_bytes - (k0 * a.ldb + n0) * size, ((k - k0) * a.ldb - n0) * size);
+  Tile<T, kLA, kLB, S> tile;
+  tile.run(pa, a.lda, a_bytes, pb, a.ldb, b_bytes, steps, lds);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32 + 4 * (lane >> 5);
+  const float s = *a.scale * a.down;
+  const int room = a.n - n0 - wn;      // this lane's columns (32 j + 8 q + r) below it exist
+#pragma unroll
+  for (int i = 0; i < S::kFM; ++i) {
+    const int row = m0 + wm + 32 * i + (lane & 31);
+    if (row < m) {
+      if constexpr (kTo == kParts) {      // ldpart is a multiple of four, 16-byte aligned
+        float* part = a.part + blockIdx.y * a.plane + row * a.ldpart + n0 + wn;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (32 * j + 8 * q < room) {
+              f32x4 v = {tile.acc[i][j][4 * q], tile.acc[i][j][4 * q + 1], tile.acc[i][j][4 * q + 2],
+                         tile.acc[i][j][4 * q + 3]};
+              if (a.add) v += *(const f32x4*)(part + 32 * j + 8 * q);
+              *(f32x4*)(part + 32 * j + 8 * q) = v;
+            }
+      } else {
+        T* out = a.out + (a.map ? a.map[row] : row) * a.ldo + n0 + wn;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            Vec4<T> v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v.v[r] = TypeOf<T>::from_float(tile.acc[i][j][4 * q + r] * s);
+            T* to = out + 32 * j + 8 * q;
+            if constexpr (kTo == kQuads) {
+              if (32 * j + 8 * q < room) *(Vec4<T>*)to = v;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (32 * j + 8 * q + r < room) to[r] = v.v[r];
+            }
+          }
+      }
+    }
+  }
+}
+
+// out[map[m] or m][:] = scale * sum of the splits' parts, in their order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __restrict__ part, const int splits,
+                                                              const long long plane, const long long ldpart,
+                                                              const int m, const int n,
+                                                              const int* __restrict__ rows,
+                                                              const float* __restrict__ scale, const float down,
+                                                              const int* __restrict__ map, T* __restrict__ out,
+                                                              const long long ldo) {
+  const long long quads = (n + 3) / 4, top = min(m, rows ? *rows : m) * quads;
+  const float s = *scale * down;
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < top; i += (long long)gridDim.x * kThreads) {
+    const long long r = i / quads;
+    const int c = (int)(i - r * quads) * 4;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < splits; ++k) v += *(const f32x4*)(part + k * plane + r * ldpart + c);
+    T* to = out + (map ? map[r] : r) * ldo + c;
+    if ((n & 3) == 0) {
+      Vec4<T> o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o.v[j] = TypeOf<T>::from_float(v[j] * s);
+      *(Vec4<T>*)to = o;
+    } else {
+      for (int j = 0; j < 4 && c + j < n; ++j) to[j] = TypeOf<T>::from_float(v[j] * s);
+    }
+  }
+}
+
+// Column sums of P over the rows that count: a block takes 256 columns and every splits-th run of rows.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sum_columns_kernel(const T* __restrict__ p, const int ldp, const int v,
+                                                               const int* __restrict__ rows_at, const int splits,
+                                                               float* __restrict__ part) {
+  const int c = blockIdx.x * kThreads + threadIdx.x, rows = *rows_at;
+  const int per = (rows + splits - 1) / splits, lo = blockIdx.y * per, hi = min(rows, lo + per);
+  if (c >= v) return;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int r = lo; r < hi; ++r) sum += TypeOf<T>::to_float(p[(long long)r * ldp + c]);
+  part[(long long)blockIdx.y * v + c] = sum;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_columns_kernel(const float* __restrict__ part, const int splits,
+                                                                const int v, const float* __restrict__ scale,
+                                                                const float down, T* __restrict__ db) {
+  const int c = blockIdx.x * kThreads + threadIdx.x;
+  if (c >= v) return;
+  float sum = 0.0f;
+  for (int k = 0; k < splits; ++k) sum += part[(long long)k * v + c];
+  db[c] = TypeOf<T>::from_float(sum * (*scale * down));
+}
+
+// x *= scale / assumed in place, one rounding; an array whose scale is the assumed one is not touched.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void upstream_kernel(T* __restrict__ x, const long long n,
+                                                            const float* __restrict__ scale, const float assumed) {
+  const float s = *scale;
+  if (s == assumed) return;
+  const float f = s / assumed;
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads)
+    x[i] = TypeOf<T>::from_float(TypeOf<T>::to_float(x[i]) * f);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+typedef Shape<2, 2, 4, 4> Large;      // 256 x 256, 4 waves
+typedef Shape<2, 2, 2, 2> Small;      // 128 x 128, 4 waves
+
+constexpr long long kPieceBytes = 256ll << 20;
+constexpr long long kPieceMost = 1 << 18;      // a tile's byte offsets into P stay below 2^31
+constexpr int kColumnSplits = 32;
+
+static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+struct Plan {
+  int size, step_k;
+  int per, row_blocks;          // rows a placing block takes
+  int ldx, ldw_pad;             // padded rows of the placed features; of the copied weights (0: none)
+  bool large_logits, large_dx, large_dw;
+  int bn;                       // classes a tile of the logits takes
+  int piece, pieces, ldp;       // classes of P at a time
+  int dx_splits, dx_steps, dw_splits, dw_steps;
+  long long ldpart_dx, ldpart_dw;
+  int tiles_v;
+};
+
+// Tiles of 256 x 256 move half the bytes per product of those of 128 x 128, which fill the card
+// with a quarter of the work.
+static bool take_large(long long m, long long n) {
+  return m > 128 && n > 128 && (long long)ceil_div(m, 256) * ceil_div(n, 256) >= 128;
+}
+
+// Splits of the sum over k: as many as fill the card, each of eight steps at least.
+static int splits_for(long long m, long long n, int steps, bool large) {
+  const long long tiles = large ? (long long)ceil_div(m, 256) * ceil_div(n, 256)
+                                : (long long)ceil_div(m, 128) * ceil_div(n, 128);
+  const long long want = large ? 256 : 512;
+  long long s = tiles >= want ? 1 : want / tiles;
+  if (s > steps / 8) s = steps / 8;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : (int)s;
+}
+
+static Plan make_plan(int n, int d, int v, int dtype, int flags) {
+  Plan p = {};
+  p.size = dtype == RH_F32 ? 4 : 2;
+  p.step_k = kStepBytes / p.size;
+  p.per = n > 65536 ? 256 : 32;
+  p.row_blocks = ceil_div(n, p.per);
+  p.ldx = ceil_div(d, p.step_k) * p.step_k;
+  p.ldw_pad = flags & RH_CE_COPY_WEIGHT ? p.ldx : 0;
+  long long piece = kPieceBytes / ((long long)n * p.size) / 256 * 256;
+  if (piece < 4096) piece = 4096;
+  if (piece > kPieceMost) piece = kPieceMost;
+  if (piece > v) piece = v;
+  p.pieces = ceil_div(v, piece);
+  if (p.pieces > 1) piece = ceil_div(ceil_div(v, p.pieces), 256) * 256;     // of even size
+  p.pieces = ceil_div(v, piece);
+  p.piece = (int)piece;
+  p.ldp = ceil_div(piece, 64) * 64;
+  p.large_logits = take_large(n, piece);
+  p.bn = p.large_logits ? 256 : 128;
+  p.tiles_v = ceil_div(v, p.bn);
+  p.large_dx = take_large(n, d);
+  p.large_dw = take_large(piece, d);
+  const int k_dx = ceil_div(p.ldp, p.step_k), k_dw = ceil_div(n, p.step_k);
+  p.dx_splits = splits_for(n, d, k_dx, p.large_dx);
+  p.dx_steps = ceil_div(k_dx, p.dx_splits);
+  p.dw_splits = splits_for(piece, d, k_dw, p.large_dw);
+  p.dw_steps = ceil_div(k_dw, p.dw_splits);
+  p.ldpart_dx = ceil_div(d, 4) * 4;
+  p.ldpart_dw = ceil_div(d, 4) * 4;
+  return p;
+}
+
+struct Space {
+  int2* blocks;
+  RowInfo info;
+  char* x;
+  char* w;
+  float2* stats;
+  float* z_label;
+  float* lse;
+  double* loss;
+  char* p;
+  float* dx_part;
+  float* dw_part;
+  float* db_part;
+  size_t bytes;
+};
+
+static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
+  Carver c(base);
+  Space s = {};
+  s.blocks = c.take<int2>(p.row_blocks);
+  s.info.map = c.take<int>(n);
+  s.info.label = c.take<int>(n);
+  s.info.n_valid = c.take<int>(1);
+  s.info.scale = c.take<float>(1);
+  s.x = c.take<char>((size_t)n * p.ldx * p.size);
+  if (p.ldw_pad) s.w = c.take<char>((size_t)v * p.ldw_pad * p.size);
+  s.stats = c.take<float2>((size_t)p.tiles_v * n);
+  s.z_label = c.take<float>(n);
+  s.lse = c.take<float>(n);
+  s.loss = c.take<double>(ceil_div(n, 32));
+  if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) s.p = c.take<char>((size_t)n * p.ldp * p.size);
+  if ((flags & RH_CE_GRAD_X) && (p.pieces > 1 || p.dx_splits > 1))
+    s.dx_part = c.take<float>((size_t)p.dx_splits * n * p.ldpart_dx);
+  if ((flags & RH_CE_GRAD_W) && p.dw_splits > 1)
+    s.dw_part = c.take<float>((size_t)p.dw_splits * p.piece * p.ldpart_dw);
+  if (flags & RH_CE_GRAD_B) s.db_part = c.take<float>((size_t)kColumnSplits * p.piece);
+  s.bytes = c.off;
+  return s;
+}
+
+template <typename K>
+static int raise_lds(K kernel, int bytes) {
+  RH_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return RH_OK;
+}
+
+template <typename T, typename S, What kWhat>
+static int launch_logits(LogitArgs<T> a, int n, hipStream_t stream) {
+  a.grid = Grid{ceil_div(n, S::kBM), ceil_div(a.v, S::kBN)};
+  auto kernel = logits_kernel<T, S, kWhat>;
+  if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n), dim3(S::kThreads), S::kLdsBytes, stream, a);
+  RH_CHECK_LAUNCH("logits_kernel");
+  return RH_OK;
+}
+
+template <typename T, Layout kLA, typename S>
+static int launch_product(ProductArgs<T> a, int splits, hipStream_t stream) {
+  a.grid = Grid{ceil_div(a.m, S::kBM), ceil_div(a.n, S::kBN)};
+  auto kernel = a.part         ? product_kernel<T, kLA, kCols, S, kParts>
+                : a.n % 4 == 0 ? product_kernel<T, kLA, kCols, S, kQuads>
+                               : product_kernel<T, kLA, kCols, S, kSingly>;
+  if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n, splits), dim3(S::kThreads), S::kLdsBytes, stream, a);
+  RH_CHECK_LAUNCH("product_kernel");
+  return RH_OK;
+}
+
+template <typename T>
+static int join_parts(const float* part, int splits, long long plane, long long ldpart, int m, int n, const int* rows,
+                      const float* scale, const int* map, T* out, hipStream_t stream) {
+  long long blocks = ((long long)m * ((n + 3) / 4) + kThreads - 1) / kThreads;
+  if (blocks > 256 * 8) blocks = 256 * 8;
+  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, part, splits, plane,
+                     ldpart, m, n, rows, scale, PScale<T>::down, map, out, (long long)n);
+  RH_CHECK_LAUNCH("join_parts_kernel");
+  return RH_OK;
+}
+
+template <typename T>
+static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStream_t stream) {
+  const int n = (int)q.n, d = q.d, v = (int)q.v;
+  const Labels labels{q.labels, q.labels_int64, q.ignore_index, v};
+  T* const x = (T*)s.x;
+  hipLaunchKernelGGL(count_rows_kernel, dim3(p.row_blocks), dim3(64), 0, stream, labels, n, p.per, s.blocks);
+  RH_CHECK_LAUNCH("count_rows_kernel");
+  hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
+                     d, labels, n, p.per, s.blocks, x, p.ldx, s.info, q.row_loss, (T*)q.dx, q.small,
+                     (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
+  RH_CHECK_LAUNCH("place_rows_kernel");
+  const T* w = (const T*)q.w;
+  long long ldw = q.ldw;
+  if (p.ldw_pad) {
+    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(v < 8192 ? ceil_div(v, 4) : 2048), dim3(kThreads), 0, stream, w, ldw, d, v,
+                       (T*)s.w, p.ldw_pad);
+    RH_CHECK_LAUNCH("pad_rows_kernel");
+    w = (const T*)s.w;
+    ldw = p.ldw_pad;
+  }
+  const long long d_w = p.ldw_pad ? p.ldw_pad : d;
+  const long long w_bytes = ((v - 1) * ldw + d_w) * p.size;
+
+  LogitArgs<T> a = {};
+  a.x = x;
+  a.ldx = p.ldx;
+  a.w = w;
+  a.ldw = ldw;
+  a.w_bytes = w_bytes;
+  a.bias = (const T*)q.bias;
+  a.steps = p.ldx / p.step_k;
+  a.w_limit = (int)(d_w * p.size - (long long)(a.steps - 1) * kStepBytes);
+  a.v = v;
+  a.info = s.info;
+  a.stats = s.stats;
+  a.ld_stats = n;
+  a.z_label = s.z_label;
+  a.lse = s.lse;
+  a.p = (T*)s.p;
+  a.ldp = p.ldp;
+  if (int rc = p.large_logits ? launch_logits<T, Large, kStats>(a, n, stream)
+                              : launch_logits<T, Small, kStats>(a, n, stream))
+    return rc;
+  const int joins = ceil_div(n, 32);
+  hipLaunchKernelGGL(join_stats_kernel, dim3(joins), dim3(kThreads), 0, stream, s.stats, (long long)n, p.tiles_v, s.info,
+                     s.z_label, s.lse, q.row_loss, s.loss);
+  RH_CHECK_LAUNCH("join_stats_kernel");
+  hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, joins, q.small);
+  RH_CHECK_LAUNCH("finish_loss_kernel");
+  if (!q.dx && !q.dw && !q.db) return RH_OK;
+
+  for (int i = 0; i < p.pieces; ++i) {
+    const int v0 = i * p.piece, vc = v - v0 < p.piece ? v - v0 : p.piece;
+    a.v0 = v0;
+    a.v = vc;
+    a.w = w + v0 * ldw;
+    a.w_bytes = w_bytes - v0 * ldw * p.size;
+    if (int rc = p.large_logits ? launch_logits<T, Large, kProb>(a, n, stream)
+                                : launch_logits<T, Small, kProb>(a, n, stream))
+      return rc;
+    if (q.dx) {
+      const bool parts = s.dx_part != nullptr;
+      ProductArgs<T> g = {};
+      g.a = (const T*)s.p;
+      g.lda = p.ldp;
+      g.b = a.w;
+      g.ldb = ldw;
+      g.b_bytes = a.w_bytes;
+      g.m = n;
+      g.n = d;
+      g.k = ceil_div(vc, 64) * 64;       // P has zeros there, the weights' records end earlier
+      g.rows = s.info.n_valid;
+      g.split_steps = p.dx_steps;
+      g.scale = s.info.scale;
+      g.down = PScale<T>::down;
+      g.out = (T*)q.dx;
+      g.map = s.info.map;
+      g.ldo = d;
+      g.part = s.dx_part;
+      g.ldpart = p.ldpart_dx;
+      g.plane = (long long)n * p.ldpart_dx;
+      g.add = parts && i > 0;
+      if (int rc = p.large_dx ? launch_product<T, kRows, Large>(g, p.dx_splits, stream)
+                              : launch_product<T, kRows, Small>(g, p.dx_splits, stream))
+        return rc;
+      if (parts && i == p.pieces - 1)
+        if (int rc = join_parts<T>(s.dx_part, p.dx_splits, g.plane, g.ldpart, n, d, s.info.n_valid, s.info.scale,
+                                   s.info.map, (T*)q.dx, stream))
+          return rc;
+    }
+    if (q.dw) {
+      ProductArgs<T> g = {};
+      g.a = (const T*)s.p;
+      g.lda = p.ldp;
+      g.b = x;
+      g.ldb = p.ldx;
+      g.b_bytes = (long long)n * p.ldx * p.size;
+      g.m = vc;
+      g.n = d;
+      g.k = n;
+      g.rows = s.info.n_valid;
+      g.split_steps = p.dw_steps;
+      g.scale = s.info.scale;
+      g.down = PScale<T>::down;
+      g.out = (T*)q.dw + (long long)v0 * d;
+      g.ldo = d;
+      g.part = s.dw_part;
+      g.ldpart = p.ldpart_dw;
+      g.plane = (long long)p.piece * p.ldpart_dw;
+      if (int rc = p.large_dw ? launch_product<T, kCols, Large>(g, p.dw_splits, stream)
+                              : launch_product<T, kCols, Small>(g, p.dw_splits, stream))
+        return rc;
+      if (s.dw_part)
+        if (int rc = join_parts<T>(s.dw_part, p.dw_splits, g.plane, g.ldpart, vc, d, nullptr, s.info.scale, nullptr,
+                                   g.out, stream))
+          return rc;
+    }
+    if (q.db) {
+      hipLaunchKernelGGL(sum_columns_kernel<T>, dim3(ceil_div(vc, kThreads), kColumnSplits), dim3(kThreads), 0, stream,
+                         (const T*)s.p, p.ldp, vc, s.info.n_valid, kColumnSplits, s.db_part);
+      RH_CHECK_LAUNCH("sum_columns_kernel");
+      hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(vc, kThreads)), dim3(kThreads), 0, stream, s.db_part,
+                         kColumnSplits, vc, s.info.scale, PScale<T>::down, (T*)q.db + v0);
+      RH_CHECK_LAUNCH("join_columns_kernel");
+    }
+  }
+  return RH_OK;
+}
+
+static int check_sizes(int64_t n, int32_t d, int64_t v, int32_t dtype) {
+  RH_REQUIRE(dtype == RH_F32 || dtype == RH_BF16 || dtype == RH_F16, RH_EINVAL, "unknown element type %d", dtype);
+  RH_REQUIRE(n >= 1 && n <= (1 << 26), RH_ESHAPE, "rows must be in 1 .. 2^26 (got %lld)", (long long)n);
+  RH_REQUIRE(d >= 1 && d <= (1 << 17), RH_ESHAPE, "features must be in 1 .. 2^17 (got %d)", d);
+  RH_REQUIRE(v >= 1 && v <= (1 << 24), RH_ESHAPE, "classes must be in 1 .. 2^24 (got %lld)", (long long)v);
+  return RH_OK;
+}
+
+}  // namespace ce
+}  // namespace rh
+
+extern "C" {
+
+size_t rh_linear_ce_workspace_bytes(int64_t n, int32_t d, int64_t v, int32_t dtype, int32_t flags) {
+  if (rh::ce::check_sizes(n, d, v, dtype) != RH_OK) return 0;
+  const rh::ce::Plan p = rh::ce::make_plan((int)n, d, (int)v, dtype, flags);
+  return rh::ce::carve(nullptr, p, (int)n, d, (int)v, flags).bytes;
+}
+
+int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream) {
+  RH_REQUIRE(args, RH_EINVAL, "null arguments");
+  const rh_linear_ce_args& q = *args;
+  if (int rc = rh::ce::check_sizes(q.n, q.d, q.v, q.dtype)) return rc;
+  RH_REQUIRE(q.x && q.w && q.labels && q.row_loss && q.small, RH_EINVAL, "null pointer");
+  RH_REQUIRE(q.reduction == RH_CE_MEAN || q.reduction == RH_CE_SUM, RH_EINVAL, "unknown reduction %d", q.reduction);
+  RH_REQUIRE(q.ldx >= q.d && q.ldw >= q.d, RH_ESHAPE, "row stride smaller than the row");
+  RH_REQUIRE(!q.db || q.bias, RH_EINVAL, "a gradient of the bias needs a bias");
+  const int size = q.dtype == RH_F32 ? 4 : 2;
+  int flags = q.flags & RH_CE_COPY_WEIGHT;
+  if (q.dx) flags |= RH_CE_GRAD_X;
+  if (q.dw) flags |= RH_CE_GRAD_W;
+  if (q.db) flags |= RH_CE_GRAD_B;
+  RH_REQUIRE((flags & RH_CE_COPY_WEIGHT) ||
+                 (rh::aligned16(q.w) && q.d * size % 16 == 0 && q.ldw * size % 16 == 0 && q.ldw < (1 << 20)),
+             RH_EALIGN, "weights whose rows are not whole 16-byte pieces need RH_CE_COPY_WEIGHT");
+  RH_REQUIRE(((uintptr_t)q.dx | (uintptr_t)q.dw) % 16 == 0, RH_EALIGN, "gradients must be 16-byte aligned");
+  const rh::ce::Plan p = rh::ce::make_plan((int)q.n, q.d, (int)q.v, q.dtype, flags);
+  const rh::ce::Space s = rh::ce::carve(q.workspace, p, (int)q.n, q.d, (int)q.v, flags);
+  RH_REQUIRE(q.workspace && q.workspace_bytes >= s.bytes, RH_EWORKSPACE, "workspace of %zu bytes, %zu needed",
+             q.workspace_bytes, s.bytes);
+  RH_REQUIRE((uintptr_t)q.workspace % 256 == 0, RH_EALIGN, "workspace must be 256-byte aligned");
+  if (q.dtype == RH_F32) return rh::ce::run<float>(q, p, s, (hipStream_t)stream);
+  if (q.dtype == RH_BF16) return rh::ce::run<__bf16>(q, p, s, (hipStream_t)stream);
+  return rh::ce::run<_Float16>(q, p, s, (hipStream_t)stream);
+}
+
+int rh_scale_gradient(void* x, int64_t count, int32_t dtype, const float* scale, float assumed, rh_stream_t stream) {
+  RH_REQUIRE(count >= 0, RH_ESHAPE, "negative count");
+  RH_REQUIRE(assumed != 0.0f, RH_EINVAL, "assumed scale must be non-zero");
+  if (count == 0) return RH_OK;
+  RH_REQUIRE(x && scale, RH_EINVAL, "null pointer");
+  long long blocks = (count + rh::ce::kThreads - 1) / rh::ce::kThreads;
+  if (blocks > 256 * 16) blocks = 256 * 16;
+  const dim3 grid((unsigned)blocks), block(rh::ce::kThreads);
+  if (dtype == RH_F32)
+    hipLaunchKernelGGL(rh::ce::upstream_kernel<float>, grid, block, 0, (hipStream_t)stream, (float*)x, (long long)count, scale, assumed);
+  else if (dtype == RH_BF16)
+    hipLaunchKernelGGL(rh::ce::upstream_kernel<__bf16>, grid, block, 0, (hipStream_t)stream, (__bf16*)x, (long long)count, scale, assumed);
+  else if (dtype == RH_F16)
+    hipLaunchKernelGGL(rh::ce::upstream_kernel<_Float16>, grid, block, 0, (hipStream_t)stream, (_Float16*)x, (long long)count, scale, assumed);
+  else
+    RH_FAIL(RH_EINVAL, "unknown element type %d", dtype);
+  RH_CHECK_LAUNCH("upstream_kernel");
+  return RH_OK;
+}
+
+}  // extern "C"

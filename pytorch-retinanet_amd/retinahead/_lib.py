@@ -62,6 +62,39 @@ class AssignAhead(C.Structure):
     ]
 
 
+RH_F32, RH_BF16, RH_F16 = 0, 1, 2
+CE_GRAD_X, CE_GRAD_W, CE_GRAD_B, CE_COPY_WEIGHT = 1, 2, 4, 8
+CE_REDUCTIONS = {"mean": 0, "sum": 1}
+
+
+class LinearCeArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("w", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("labels", C.c_void_p),
+        ("n", C.c_int64),
+        ("v", C.c_int64),
+        ("ldx", C.c_int64),
+        ("ldw", C.c_int64),
+        ("d", C.c_int32),
+        ("dtype", C.c_int32),
+        ("labels_int64", C.c_int32),
+        ("reduction", C.c_int32),
+        ("ignore_index", C.c_int64),
+        ("divisor", C.c_void_p),
+        ("grad", C.c_float),
+        ("flags", C.c_int32),
+        ("row_loss", C.c_void_p),
+        ("small", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dw", C.c_void_p),
+        ("db", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 NORM_PER_IMAGE, NORM_GLOBAL = 0, 1
 NORMALIZERS = {"per_image": NORM_PER_IMAGE, "global": NORM_GLOBAL}
 
@@ -124,6 +157,9 @@ SIGNATURES = {
     "rh_postprocess_levels": (C.c_int, [_P, _P, _P, _I32, _I32, _P, _P, _I32, _I32,
                                         C.POINTER(PostParams), _P, _P, _P, _P, _P, _P, _P, _SZ, _I32,
                                         _P]),
+    "rh_linear_ce_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I32, _I32]),
+    "rh_linear_ce": (C.c_int, [C.POINTER(LinearCeArgs), _P]),
+    "rh_scale_gradient": (C.c_int, [_P, _I64, _I32, _P, _F, _P]),
 }
 
 _lib = None

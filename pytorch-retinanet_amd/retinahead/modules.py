@@ -459,6 +459,92 @@ class GenericFocalLoss(nn.Module):
                                      bool(self.logits), bool(self.reduce))
 
 
+class _LinearCrossEntropyFn(torch.autograd.Function):
+    """As _DenseHeadLossFn: the forward call makes the gradients, backward applies the upstream one."""
+
+    @staticmethod
+    def forward(ctx, features, weight, bias, labels, divisor, cfg, grad_mode):
+        need = [grad_mode and ctx.needs_input_grad[i] for i in range(3)]
+        out = F.linear_cross_entropy(features, weight, labels, bias, ignore_index=cfg["ignore_index"],
+                                     reduction=cfg["reduction"], divisor=divisor,
+                                     expected_grad=cfg["expected_grad"], grads=need)
+        ctx.grads = [out.get(k) for k in ("d_features", "d_weight", "d_bias")]
+        ctx.expected = cfg["expected_grad"]
+        cfg["state"].set(features.device, out.without_grads())
+        small = out["small"]
+        return small.new_empty(0).set_(small.untyped_storage(), small.storage_offset(), (1,))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        if ctx.grads is None:
+            raise RetinaHeadError("the fused loss keeps one set of gradients: backward() can run "
+                                  "once per forward()")
+        grads, ctx.grads = ctx.grads, None
+        if not (ctx.expected == 1.0 and _is_unit(g)):
+            for d in grads:
+                if d is not None:
+                    F.scale_gradient_(d, g, ctx.expected)
+        return (*grads, None, None, None, None)
+
+
+class LinearCrossEntropy(nn.Module):
+    """Softmax cross entropy of a classifier's last projection, for label sets too large to keep the
+    logits of: ``forward(features[..., D], weight[V, D], labels[...], bias[V]=None)`` returns the
+    float32 [1] loss of ``features @ weight.T + bias``, differentiable with respect to features,
+    weight and bias.  The logits are made in pieces of the classes and never stored whole; as in
+    ``FocalLoss`` the forward call makes the gradients too.
+
+    Where ``FocalLoss`` scores every class by itself, this is the head for mutually exclusive classes
+    (the 601 of datasets/oid_dataset.py:47-50 count the background as one).
+
+    Element types: float32, bfloat16, float16 (one for all three; the gradients have it too).
+    Products are summed in float32, softmax statistics and losses are float32.  For 16-bit types the
+    softmax minus one-hot matrix is rounded once to the type, as an operand of the matrix units.
+
+    ignore_index: rows with this label take no part: no loss, zero gradient, whatever their features
+        hold.  A batch without a counted row has loss 0 and zero gradients.
+    reduction: 'mean' over the counted rows, or 'sum'.
+    expected_grad: the upstream gradient the stored gradients are made for (see ``FocalLoss``); any
+        other one is applied in place by ``backward``, with one more rounding for 16-bit types.
+    check_labels: read the status word after the call (one host synchronisation) and raise IndexError
+        for a label outside [0, V) other than ignore_index; without it such a row is left out.
+
+    ``forward(..., divisor=)`` takes a float32 [1] device tensor the mean divides by instead of this
+    call's counted rows (``retinahead.dist.DataParallelLinearCrossEntropy`` passes the count over all
+    ranks).  ``last`` holds the latest call's ``row_loss``, ``num_valid``, ``status``.
+    """
+
+    def __init__(self, ignore_index=-100, reduction="mean", expected_grad=1.0, check_labels=False):
+        super().__init__()
+        if reduction not in _lib.CE_REDUCTIONS:
+            raise ValueError("reduction must be 'mean' or 'sum'")
+        if float(expected_grad) == 0.0:
+            raise ValueError("expected_grad must not be zero")
+        self.cfg = dict(ignore_index=int(ignore_index), reduction=reduction,
+                        expected_grad=float(expected_grad), state=_CallState())
+        self.check_labels = bool(check_labels)
+
+    @property
+    def last(self):
+        """Device tensors of the latest call: row_loss, num_valid [1], status [1]."""
+        return self.cfg["state"].mine
+
+    @property
+    def last_by_device(self):
+        """{device index: outputs of the latest call on that device}."""
+        return self.cfg["state"].by_device
+
+    def forward(self, features, weight, labels, bias=None, divisor=None):
+        loss = _LinearCrossEntropyFn.apply(features, weight, bias, labels, divisor, self.cfg,
+                                           torch.is_grad_enabled())
+        if self.check_labels and int(self.last["status"].item()) & _lib.RH_STATUS_LABEL_RANGE:
+            raise IndexError("label outside [0, classes)")
+        loss = loss.as_subclass(_LossTensor)
+        loss._token = object()      # backward() without a gradient: seeded with the cached ones
+        return loss
+
+
 class Anchors(nn.Module):
     """Replaces Anchors (models/retinanet/anchors.py:6-45).
 

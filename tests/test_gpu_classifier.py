@@ -1,0 +1,344 @@
+"""The softmax classifier loss over a large label set (retinahead.LinearCrossEntropy) against a plain
+64-bit implementation, element by element, with bounds derived from the arithmetic.
+
+Bounds.  Let e = 2^-23 (a float32 operation is off by at most 2^-24 of its result; the matrix units'
+internal additions are granted twice that) and u = eps/2 of the element type.
+  logits      |dz| <= (D + 1) e sum_i |x_i w_i| + e |b|      =: Z (its largest over the classes of a row)
+  lse         a sum of positive terms, each off by its exponent's error, its exp and V additions (pairwise
+              within tiles, but V e bounds any order):  |d lse| <= Z + (V + 16) e + e (|max| + |lse|)
+  row loss    Z + |d lse| + e |row|
+  P           |dP| <= p (exp(Z + |d lse| + 8 e + 4 e |z - lse|) - 1) + e + u |P|   (the e: p - 1 in float32)
+  dX = s P W  s (|dP| |W| + (V + 2) e |P| |W|) + (u + 2 e) |dX| + half the type's smallest step
+and dW, db in the same way over the rows.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+E = 2.0 ** -23
+
+
+@pytest.fixture(scope="module")
+def rh():
+    import retinahead
+    retinahead.load_library()
+    return retinahead
+
+
+def make(n, d, v, dtype, bias, ignored=0.0, seed=0, scale=2.0, label_type=torch.int64):
+    g = torch.Generator().manual_seed(seed * 1009 + n * 7 + d * 3 + v)
+    w = (torch.randn(v, d, generator=g) * scale / math.sqrt(d)).to(TYPES[dtype])
+    y = torch.randint(0, v, (n,), generator=g)
+    x = torch.randn(n, d, generator=g)
+    x[::2] += 1.5 * w[y[::2]].float()
+    x = x.to(TYPES[dtype])
+    if ignored:
+        y[torch.rand(n, generator=g) < ignored] = -100
+    b = (torch.randn(v, generator=g) * 0.5).to(TYPES[dtype]) if bias else None
+    return x.cuda(), w.cuda(), y.to(label_type).cuda(), None if b is None else b.cuda()
+
+
+def oracle(x, w, y, b, reduction="mean", upstream=1.0, divisor=None, ignore=-100):
+    """Results in 64 bits and the bound of each (see the module's docstring)."""
+    tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps / 2
+    u = torch.finfo(x.dtype).eps / 2
+    n, d = x.shape
+    v = w.shape[0]
+    keep = (y != ignore) & (y >= 0) & (y < v)
+    X = torch.where(keep[:, None], x, torch.zeros_like(x)).double()
+    W, Y = w.double(), torch.where(keep, y, 0).long()
+    z = X @ W.T
+    Z = X.abs() @ W.abs().T * ((d + 1) * E)
+    if b is not None:
+        z = z + b.double()
+        Z = Z + E * b.double().abs()
+    Z = Z.amax(1, keepdim=True) + E * z.abs()
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    zy = z.gather(1, Y[:, None])
+    dlse = Z.amax(1, keepdim=True) + (v + 16) * E + E * (z.amax(1, keepdim=True).abs() + lse.abs())
+    row = torch.where(keep, (lse - zy)[:, 0], 0.0)
+    drow = torch.where(keep, (Z.gather(1, Y[:, None]) + dlse)[:, 0] + E * row.abs(), 0.0)
+    count = float(keep.sum())
+    s = 1.0 / max(1.0, count if divisor is None else divisor) if reduction == "mean" else 1.0
+    loss = row.sum() * s
+    p = (z - lse).exp()
+    k = keep.double()[:, None]
+    P = p.clone()
+    P.scatter_add_(1, Y[:, None], torch.full_like(zy, -1.0))
+    dP = (p * torch.expm1(Z + dlse + 8 * E + 4 * E * (z - lse).abs()) + E + u * P.abs()) * k
+    P = P * k
+    s *= upstream
+    a = abs(s)
+    out = {"loss": (loss, drow.sum() * abs(s / upstream) + 2 * E * loss.abs()), "row_loss": (row, drow)}
+    for name, left, dleft, right, terms in (("d_features", P, dP, W, v), ("d_weight", P.T, dP.T, X, n),
+                                            ("d_bias", P.T, dP.T, torch.ones(n, 1, dtype=torch.float64, device=x.device), n)):
+        want = s * (left @ right)
+        tol = a * (dleft @ right.abs() + (terms + 2) * E * (left.abs() @ right.abs())) + (u + 2 * E) * want.abs() + tiny
+        if name == "d_bias":
+            want, tol = want[:, 0], tol[:, 0]
+        out[name] = (want, tol)
+    return out
+
+
+def close(name, got, want):
+    value, tol = want
+    got = got.double().reshape(value.shape)
+    bad = ~((got - value).abs() <= tol)
+    assert not bad.any(), (name, int(bad.sum()), bad.numel(), float(((got - value).abs() / tol).nan_to_num(1e9).max()))
+
+
+def check_all(rh, x, w, y, b, **kw):
+    out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, b is not None), **kw)
+    want = oracle(x, w, y, b, reduction=kw.get("reduction", "mean"), upstream=kw.get("expected_grad", 1.0))
+    for name in ("loss", "row_loss", "d_features", "d_weight") + (("d_bias",) if b is not None else ()):
+        close(name, out[name], want[name])
+    return out
+
+
+SIZES = [(1, 8, 1), (1, 64, 2), (2, 1, 3), (3, 17, 5), (31, 33, 63), (64, 64, 64), (128, 128, 128), (129, 72, 257),
+         (300, 100, 1000), (257, 256, 601), (65, 520, 4099), (1000, 40, 70)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_matches_64_bits(rh, n, d, v, dtype, bias):
+    x, w, y, b = make(n, d, v, dtype, bias, ignored=0.3 if n > 2 else 0.0)
+    out = check_all(rh, x, w, y, b)
+    assert float(out["num_valid"]) == float((y != -100).sum())
+    assert int(out["status"]) == 0
+    assert out["d_features"].dtype == x.dtype and out["row_loss"].dtype == torch.float32
+    assert (out["d_features"][y == -100] == 0).all() and (out["row_loss"][y == -100] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,v", [(4099, 264, 70001), (8200, 1032, 300), (70000, 24, 90)])
+def test_large_tiles_pieces_and_many_rows(rh, n, d, v, dtype):
+    if dtype == "f32" and v > 1000:
+        n = 2051
+    x, w, y, b = make(n, d, v, dtype, True, ignored=0.1, seed=3)
+    check_all(rh, x, w, y, b)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("reduction,grad", [("sum", 1.0), ("mean", 0.25)])
+def test_reductions_and_expected_gradient(rh, dtype, reduction, grad):
+    x, w, y, b = make(50, 48, 37, dtype, True, ignored=0.2, seed=1)
+    check_all(rh, x, w, y, b, reduction=reduction, expected_grad=grad)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_left_out_may_hold_anything(rh, dtype):
+    x, w, y, b = make(140, 72, 300, dtype, True, ignored=0.4, seed=2)
+    want = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    x2 = x.clone()
+    out_rows = (y == -100).nonzero()[:, 0]
+    x2[out_rows[0::3]] = float("nan")
+    x2[out_rows[1::3]] = float("inf")
+    x2[out_rows[2::3]] = torch.finfo(x.dtype).min
+    got = rh.functional.linear_cross_entropy(x2, w, y, b, grads=(True, True, True))
+    for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+        assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_no_row_counts(rh, dtype):
+    x, w, y, b = make(70, 72, 300, dtype, True)
+    y.fill_(-100)
+    out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    assert float(out["loss"]) == 0.0 and float(out["num_valid"]) == 0.0
+    for k in ("row_loss", "d_features", "d_weight", "d_bias"):
+        assert (out[k] == 0).all(), k
+    e = rh.functional.linear_cross_entropy(x[:0], w, y[:0], b, grads=(True, True, True))
+    assert float(e["loss"]) == 0.0 and e["d_features"].shape == (0, 72) and (e["d_weight"] == 0).all()
+
+
+def test_labels_outside_are_left_out_and_reported(rh):
+    x, w, y, b = make(40, 64, 30, "f32", True)
+    bad = y.clone()
+    bad[3], bad[7], bad[11] = 30, -1, 1 << 40
+    ref = y.clone()
+    ref[[3, 7, 11]] = -100
+    got = rh.functional.linear_cross_entropy(x, w, bad, b, grads=(True, True, True))
+    want = rh.functional.linear_cross_entropy(x, w, ref, b, grads=(True, True, True))
+    assert int(got["status"]) == 1 and int(want["status"]) == 0
+    for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+        assert torch.equal(got[k], want[k])
+    with pytest.raises(IndexError):
+        rh.LinearCrossEntropy(check_labels=True)(x, w, bad, b)
+    rh.LinearCrossEntropy(check_labels=True)(x, w, ref, b)
+
+
+@pytest.mark.parametrize("value", [float("-inf"), "lowest"])
+def test_classes_masked_by_the_bias(rh, value):
+    x, w, y, b = make(90, 64, 200, "bf16", True, seed=4)
+    y.clamp_(max=99)
+    low = torch.finfo(b.dtype).min if value == "lowest" else value
+    b[100:] = low
+    out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    want = rh.functional.linear_cross_entropy(x, w[:100].contiguous(), y, b[:100].contiguous(), grads=(True, True, True))
+    for k in ("loss", "row_loss"):
+        assert torch.allclose(out[k], want[k], rtol=1e-5)     # other tiles: sums in another order (10 e)
+    assert (out["d_weight"][100:] == 0).all() and (out["d_bias"][100:] == 0).all()
+    # lse may differ in its last bits, and with it now and then which way an entry of P rounds (a
+    # step of 2^-8 |P| <= 2^-8): two such entries in one sum, and one step of the result
+    flips = 2 * 2.0 ** -8 * float(x.abs().max()) / 90
+    assert torch.allclose(out["d_weight"][:100].float(), want["d_weight"].float(), rtol=2.0 ** -7, atol=flips)
+
+
+def test_nan_and_inf_reach_the_loss(rh):
+    x, w, y, b = make(40, 64, 30, "f32", True)
+    x[5, 3] = float("nan")
+    out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    assert torch.isnan(out["loss"]).all() and torch.isnan(out["row_loss"][5])
+    good = torch.arange(40, device="cuda") != 5
+    assert torch.isfinite(out["row_loss"][good]).all() and torch.isfinite(out["d_features"][good]).all()
+    x[5, 3] = 0.0
+    b[2] = float("inf")
+    assert torch.isnan(rh.functional.linear_cross_entropy(x, w, y, b)["loss"]).all()
+
+
+def test_strides_and_label_types(rh):
+    x, w, y, b = make(60, 72, 130, "bf16", True, ignored=0.2, seed=5)
+    want = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    wide = torch.full((60, 200), float("nan"), dtype=x.dtype, device="cuda")
+    wide[:, 8:80] = x
+    odd = torch.full((60, 201), float("nan"), dtype=x.dtype, device="cuda")
+    odd[:, 3:75] = x
+    ww = torch.full((130, 160), float("nan"), dtype=x.dtype, device="cuda")
+    ww[:, 16:88] = w
+    wo = torch.full((130, 161), float("nan"), dtype=x.dtype, device="cuda")
+    wo[:, 5:77] = w
+    yy = torch.full((60, 3), -7, dtype=torch.int32, device="cuda")
+    yy[:, 1] = y
+    for xs in (x, wide[:, 8:80], odd[:, 3:75], x.t().contiguous().t()):
+        for ws in (w, ww[:, 16:88], wo[:, 5:77], w.t().contiguous().t()):
+            got = rh.functional.linear_cross_entropy(xs, ws, yy[:, 1], b, grads=(True, True, True))
+            for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+                assert torch.equal(got[k], want[k]), k
+    batched = rh.functional.linear_cross_entropy(x.view(5, 12, 72), w, y.view(5, 12), b, grads=(True, False, False))
+    assert batched["row_loss"].shape == (5, 12) and batched["d_features"].shape == (5, 12, 72)
+    assert torch.equal(batched["d_features"].view(60, 72), want["d_features"]) and "d_weight" not in batched
+    broad = rh.functional.linear_cross_entropy(x[:1].expand(60, 72), w, y, b)
+    copied = rh.functional.linear_cross_entropy(x[:1].repeat(60, 1), w, y, b)
+    assert torch.equal(broad["row_loss"], copied["row_loss"])
+
+
+# ------------------------------------------------------------------ the module
+def test_module_gradients_and_upstream(rh):
+    x, w, y, b = make(80, 64, 200, "f32", True, ignored=0.1, seed=6)
+    want = oracle(x, w, y, b)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    fn = rh.LinearCrossEntropy()
+    loss = fn(leaves[0], leaves[1], y, leaves[2])
+    loss.backward()
+    close("loss", loss.detach(), want["loss"])
+    for t, k in zip(leaves, ("d_features", "d_weight", "d_bias")):
+        close(k, t.grad, want[k])
+    assert torch.equal(fn.last["row_loss"], rh.functional.linear_cross_entropy(x, w, y, b)["row_loss"])
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    # any other upstream gradient, through other operations: exact powers of two
+    first = [t.grad.clone() for t in leaves]
+    for t in leaves:
+        t.grad = None
+    (fn(leaves[0], leaves[1], y, leaves[2]) * 0.5 + 1.0).backward()
+    for t, g in zip(leaves, first):
+        assert torch.equal(t.grad, g * 0.5)
+    # gradients accumulate, and only where they are asked for
+    leaves[0].grad = None
+    fn(leaves[0], w, y, b).backward()
+    fn(leaves[0], w, y, b).backward()
+    assert torch.equal(leaves[0].grad, first[0] * 2)
+    with torch.no_grad():
+        assert not fn(leaves[0], leaves[1], y, leaves[2]).requires_grad
+
+
+def test_gradient_against_differences(rh):
+    x, w, y, b = make(12, 16, 20, "f32", True, seed=7)
+    out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    h = 2.0 ** -6
+    # central differences of the 64-bit loss: h^2/6 |f'''|, with |f'''| <= 2 max|w|^3 (softmax cumulants)
+    for t, k in ((x, "d_features"), (w, "d_weight"), (b, "d_bias")):
+        flat = t.view(-1)
+        for i in range(0, flat.numel(), max(1, flat.numel() // 7)):
+            keep = flat[i].clone()
+            flat[i] = keep + h
+            up = oracle(x, w, y, b)["loss"][0]
+            hi = flat[i].double()
+            flat[i] = keep - h
+            down = oracle(x, w, y, b)["loss"][0]
+            lo = flat[i].double()
+            flat[i] = keep
+            slope = float((up - down) / (hi - lo))
+            reach = max(1.0, float(x.abs().max()), float(w.abs().max()))
+            assert abs(slope - float(out[k].view(-1)[i])) <= h * h / 3 * reach ** 3 + 1e-5, (k, i)
+
+
+def test_tied_weight_and_frozen_parts(rh):
+    """The same weight feeds an embedding and the loss: both gradients arrive."""
+    x, w, y, _ = make(30, 32, 50, "f32", False, seed=8)
+    w = w.requires_grad_(True)
+    emb = w[y]
+    rh.LinearCrossEntropy()(emb, w, y).backward()
+    got = w.grad.clone()
+    want = oracle(emb.detach(), w.detach(), y, None)
+    expect = want["d_weight"][0].clone()
+    expect.index_add_(0, y, want["d_features"][0])
+    tol = want["d_weight"][1].clone()
+    tol.index_add_(0, y, want["d_features"][1] + 4 * E * want["d_features"][0].abs())
+    assert ((got.double() - expect).abs() <= tol + 4 * E * expect.abs()).all()
+
+
+def test_streams_and_repeated_calls_agree(rh):
+    x, w, y, b = make(500, 256, 3001, "bf16", True, ignored=0.1, seed=9)
+    first = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        s = streams[i % 2]
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True)))
+    torch.cuda.synchronize()
+    for o in outs:
+        for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+            assert torch.equal(o[k], first[k]), k
+
+
+def test_captured_training_step(rh):
+    """Forward and backward in one graph, replayed with new inputs between eager calls."""
+    x, w, y, b = make(200, 64, 300, "bf16", True, ignored=0.1, seed=10)
+    fn = rh.LinearCrossEntropy()
+    sx = x.clone().requires_grad_(True)
+    sw = w.clone().requires_grad_(True)
+    sy = y.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sx.grad = sw.grad = None
+        loss = fn(sx, sw, sy)
+        loss.backward()
+        del loss
+        sx.grad = sw.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = fn(sx, sw, sy)
+        static.backward()
+    for seed in range(4):
+        x2, w2, y2, _ = make(200, 64, 300, "bf16", False, ignored=0.1 * seed, seed=20 + seed)
+        with torch.no_grad():
+            sx.copy_(x2)
+            sw.copy_(w2)
+            sy.copy_(y2)
+        graph.replay()
+        want = rh.functional.linear_cross_entropy(x2, w2, y2, grads=(True, True, False))
+        torch.cuda.synchronize()
+        assert torch.equal(static.detach(), want["loss"])
+        assert torch.equal(sx.grad, want["d_features"]) and torch.equal(sw.grad, want["d_weight"])

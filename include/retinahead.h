@@ -467,6 +467,38 @@ int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream);
 int rh_scale_gradient(void* x, int64_t count, int32_t dtype, const float* scale, float assumed,
                       rh_stream_t stream);
 
+/* ------------------------------------------------------------------ gradient norm and clipping */
+/* One tensor of a list: dense memory, aligned to its element. */
+typedef struct rh_tensor_ref {
+  void* data;          /* device */
+  int64_t count;       /* elements; 0: skipped */
+  int32_t dtype;       /* rh_dtype */
+  int32_t reserved;
+} rh_tensor_ref;
+
+enum rh_grad_norm_type { RH_NORM_2 = 0, RH_NORM_1 = 1, RH_NORM_INF = 2 };
+enum rh_clip_stages { RH_CLIP_NORM = 1, RH_CLIP_SCALE = 2, RH_CLIP_ALL = 3 };
+
+/* train.py's step between backward and the optimizer: the norm over every value of the list, then every
+ * value times min(1, max_norm / (norm + 1e-6)) in place (element types may be mixed; each value is
+ * rounded once).  A NaN norm makes every value NaN.  `tensors` is host memory, read before the call
+ * returns.  Ranks that hold parts of one model run RH_CLIP_NORM, reduce `total` (sum; RH_NORM_INF: max)
+ * and run RH_CLIP_SCALE. */
+typedef struct rh_grad_clip_args {
+  const rh_tensor_ref* tensors;   /* host */
+  int32_t count;
+  int32_t norm_type;              /* rh_grad_norm_type */
+  int32_t stages;                 /* rh_clip_stages */
+  float max_norm;
+  double* total;                  /* device [1]: sum of squares / sum of magnitudes / largest magnitude */
+  float* norm;                    /* device [1] out */
+  void* workspace;                /* RH_CLIP_NORM */
+  size_t workspace_bytes;
+} rh_grad_clip_args;
+
+size_t rh_grad_clip_workspace_bytes(const rh_tensor_ref* tensors, int32_t count);
+int rh_grad_clip(const rh_grad_clip_args* args, rh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -95,6 +95,32 @@ class LinearCeArgs(C.Structure):
     ]
 
 
+class TensorRef(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("count", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class GradClipArgs(C.Structure):
+    _fields_ = [
+        ("tensors", C.c_void_p),
+        ("count", C.c_int32),
+        ("norm_type", C.c_int32),
+        ("stages", C.c_int32),
+        ("max_norm", C.c_float),
+        ("total", C.c_void_p),
+        ("norm", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
+GRAD_NORMS = {2.0: 0, 1.0: 1, float("inf"): 2}
+CLIP_NORM, CLIP_SCALE, CLIP_ALL = 1, 2, 3
+
 NORM_PER_IMAGE, NORM_GLOBAL = 0, 1
 NORMALIZERS = {"per_image": NORM_PER_IMAGE, "global": NORM_GLOBAL}
 
@@ -159,6 +185,8 @@ SIGNATURES = {
                                         _P]),
     "rh_linear_ce_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I32, _I32]),
     "rh_linear_ce": (C.c_int, [C.POINTER(LinearCeArgs), _P]),
+    "rh_grad_clip_workspace_bytes": (_SZ, [_P, _I32]),
+    "rh_grad_clip": (C.c_int, [C.POINTER(GradClipArgs), _P]),
     "rh_scale_gradient": (C.c_int, [_P, _I64, _I32, _P, _F, _P]),
 }
 

@@ -31,17 +31,21 @@ def shard_bounds(global_batch, rank, world_size):
     return lo, lo + base + (1 if rank < rem else 0)
 
 
+def _all_reduce_(t, op, group):
+    if t.is_cuda and dist_.get_backend(group) != "nccl":
+        host = t.detach().cpu()
+        dist_.all_reduce(host, op=op, group=group)
+        t.copy_(host)
+    else:
+        dist_.all_reduce(t, op=op, group=group)
+    return t
+
+
 def all_reduce_sum_(t, group=None):
     """In-place sum of ``t`` over the ranks of ``group``.  RCCL (backend "nccl") reduces device
     tensors directly; a host-side backend (gloo: CPU tests, several ranks rehearsing on one
     card) gets a device tensor staged through the host."""
-    if t.is_cuda and dist_.get_backend(group) != "nccl":
-        host = t.detach().cpu()
-        dist_.all_reduce(host, op=dist_.ReduceOp.SUM, group=group)
-        t.copy_(host)
-    else:
-        dist_.all_reduce(t, op=dist_.ReduceOp.SUM, group=group)
-    return t
+    return _all_reduce_(t, dist_.ReduceOp.SUM, group)
 
 
 class _GlobalValue(torch.autograd.Function):
@@ -110,3 +114,46 @@ class DataParallelFocalLoss(torch.nn.Module):
         self.last_global = {"num_pos": vec[2], "images": vec[3]}
         return {"classification_loss": _GlobalValue.apply(cls_l.reshape(1), vec[0:1]),
                 "regression_loss": _GlobalValue.apply(reg_l.reshape(1), vec[1:2])}
+
+
+def count_valid(labels, num_classes, ignore_index=-100):
+    """float32 [1]: rows of ``labels`` that take part in the classifier loss (exact below 2^24)."""
+    keep = (labels >= 0) & (labels < num_classes) & (labels != ignore_index)
+    return keep.sum(dtype=torch.float32).reshape(1)
+
+
+class DataParallelLinearCrossEntropy(torch.nn.Module):
+    """``retinahead.LinearCrossEntropy(reduction='mean')`` over a batch sharded by rows: the mean runs
+    over the counted rows of all ranks (one 4-byte all-reduce before the call), the loss returned is the
+    global one (one more after it).  Each rank's gradients are its share of the global loss's, so the
+    weight's gradients are SUMMED over ranks (torch's DistributedDataParallel averages: multiply the loss
+    by the world size there)."""
+
+    def __init__(self, loss_fn, group=None):
+        super().__init__()
+        if loss_fn.cfg["reduction"] != "mean":
+            raise ValueError("a sum over ranks needs no wrapper: use reduction='mean'")
+        self.loss_fn = loss_fn
+        self.group = group
+
+    def forward(self, features, weight, labels, bias=None):
+        if not (dist_.is_available() and dist_.is_initialized()) or dist_.get_world_size(self.group) == 1:
+            return self.loss_fn(features, weight, labels, bias)
+        total = all_reduce_sum_(count_valid(labels, weight.shape[0], self.loss_fn.cfg["ignore_index"]),
+                                self.group)
+        local = self.loss_fn(features, weight, labels, bias, divisor=total)
+        value = all_reduce_sum_(local.detach().clone(), self.group)
+        return _GlobalValue.apply(local, value)
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, group=None):
+    """``retinahead.clip_grad_norm_`` for parameters sharded over the ranks of ``group``: the norm runs
+    over every rank's gradients (one 8-byte all-reduce between the norm's pass and the scaling one).  All
+    ranks call it, those without a gradient too.  Replicated parameters, whose gradients are equal on all
+    ranks, take ``retinahead.clip_grad_norm_``."""
+    from .modules import _clip
+    if not (dist_.is_available() and dist_.is_initialized()) or dist_.get_world_size(group) == 1:
+        return _clip(parameters, max_norm, norm_type, error_if_nonfinite, None)
+    op = dist_.ReduceOp.MAX if float(norm_type) == float("inf") else dist_.ReduceOp.SUM
+    return _clip(parameters, max_norm, norm_type, error_if_nonfinite,
+                 lambda total: _all_reduce_(total, op, group))

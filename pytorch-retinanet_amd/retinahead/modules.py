@@ -545,6 +545,57 @@ class LinearCrossEntropy(nn.Module):
         return loss
 
 
+def grad_norm(tensors, norm_type=2.0):
+    """float32 [] device tensor: the 2-, 1- or infinity norm over every value of ``tensors`` (one
+    tensor or an iterable; float32, bfloat16 and float16 may be mixed).  Values and squares are summed
+    in float64.  An empty list has norm 0."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    F._norm_code(norm_type)
+    if not tensors:
+        return torch.tensor(0.0)
+    return F.grad_clip(tensors, norm_type=norm_type, stages=_lib.CLIP_NORM)["norm"]
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scales the gradients of ``parameters`` in place so that their norm over all of them is at most
+    ``max_norm`` (each times min(1, max_norm / (norm + 1e-6))), and returns that norm from before as a
+    float32 [] device tensor: the step between ``loss.backward()`` and ``optimizer.step()`` of
+    train.py:190-203.  The signature is that of torch.nn.utils.clip_grad_norm_; nothing is read back
+    unless ``error_if_nonfinite`` asks for it.
+
+    Gradients may be float32, bfloat16 and float16 in one call, in any dense order of dimensions and at
+    any address, but two must not share memory.  A NaN or infinite gradient has the effect it has in
+    torch: a NaN norm makes every gradient NaN, an infinite one makes them 0 (NaN where infinite).
+    When every rank of a data-parallel job holds the same (already reduced) gradients this is the call;
+    for parameters sharded over ranks see ``retinahead.dist.clip_grad_norm_``."""
+    return _clip(parameters, max_norm, norm_type, error_if_nonfinite, None)
+
+
+def _clip(parameters, max_norm, norm_type, error_if_nonfinite, reduce_total):
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    F._norm_code(norm_type)
+    if not float(max_norm) >= 0.0:
+        raise ValueError("max_norm must be a number from 0 on")
+    if not grads:
+        if reduce_total is None:
+            return torch.tensor(0.0)
+        total = reduce_total(torch.zeros(1, dtype=torch.float64,
+                                         device=parameters[0].device if parameters else "cpu"))
+        return (total.sqrt() if float(norm_type) == 2.0 else total).float().reshape(())
+    if reduce_total is None and not error_if_nonfinite:
+        return F.grad_clip(grads, max_norm, norm_type)["norm"]
+    out = F.grad_clip(grads, max_norm, norm_type, stages=_lib.CLIP_NORM)
+    norm = out["norm"]
+    if reduce_total is not None:
+        reduce_total(out["total"])
+        norm = out["total"].sqrt() if float(norm_type) == 2.0 else out["total"]
+    if error_if_nonfinite and not bool(torch.isfinite(norm)):
+        raise RuntimeError(f"the norm of order {norm_type} of the gradients is not finite, so they "
+                           "cannot be clipped")
+    return F.grad_clip(grads, max_norm, norm_type, stages=_lib.CLIP_SCALE, out=out)["norm"]
+
+
 class Anchors(nn.Module):
     """Replaces Anchors (models/retinanet/anchors.py:6-45).
 

@@ -1,0 +1,80 @@
+"""What the gradient norm and clipping refuse, and their host-side logic (no GPU needed)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import retinahead as rh
+from retinahead import _lib
+from retinahead import functional as F
+
+
+def test_dense_orders():
+    x = torch.zeros(2, 3, 5, 7)
+    for t in (x, x.permute(3, 0, 2, 1), x.to(memory_format=torch.channels_last), x[:, :, :1].contiguous(), x[0], x[:, None],
+              torch.zeros(()), torch.zeros(0, 4), torch.zeros(1, 4).t()):
+        assert F._is_dense(t), t.shape
+    for t in (x[:, ::2], x[:, :, 1:], x[..., 1:], torch.zeros(1).expand(4), torch.zeros(4, 4).as_strided((3, 3), (1, 1))):
+        assert not F._is_dense(t), t.stride()
+
+
+def test_refuses_host_tensors_and_values():
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+    with pytest.raises(rh.RetinaHeadError, match="HIP device"):
+        rh.clip_grad_norm_([p], 1.0)
+    with pytest.raises(rh.RetinaHeadError, match="HIP device"):
+        rh.grad_norm(p.grad)
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            rh.clip_grad_norm_([p], bad)
+    with pytest.raises(ValueError, match="norm_type"):
+        rh.clip_grad_norm_([p], 1.0, norm_type=0.5)
+    assert float(rh.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0)) == 0.0
+    assert float(rh.grad_norm([])) == 0.0
+
+
+def _refs(*items):
+    a = np.zeros(len(items), F._REF)
+    for i, it in enumerate(items):
+        a[i] = tuple(it) + (0,)
+    return a
+
+
+def _args(refs, **kw):
+    a = _lib.GradClipArgs(refs.ctypes.data, len(refs), 0, _lib.CLIP_ALL, 1.0, 4096, 8192, 16384, 1 << 20)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("items,kw,code,text", [
+    ([(4096, 4, 3)], {}, -1, "element type"),
+    ([(4096, -1, 0)], {}, -2, "element count"),
+    ([(0, 4, 0)], {}, -1, "null pointer"),
+    ([(4098, 4, 0)], {}, -5, "aligned"),
+    ([(4097, 4, 1)], {}, -5, "aligned"),
+    ([(4096, 100, 0), (4096, 100, 0)], {}, -1, "share memory"),
+    ([(8192, 100, 0), (4096, 1025, 0)], {}, -1, "share memory"),
+    ([(4096, 4, 0)], dict(stages=0), -1, "stages"),
+    ([(4096, 4, 0)], dict(stages=4), -1, "stages"),
+    ([(4096, 4, 0)], dict(norm_type=3), -1, "norm"),
+    ([(4096, 4, 0)], dict(total=None), -1, "null"),
+    ([(4096, 4, 0)], dict(workspace_bytes=8), -4, "workspace"),
+    ([(4096, 4, 0)], dict(workspace=None), -4, "workspace"),
+    ([(4096, 4, 0)], dict(workspace=16400), -5, "256"),
+])
+def test_entry_point_refuses(items, kw, code, text):
+    refs = _refs(*items)
+    assert rh.load_library().rh_grad_clip(C.byref(_args(refs, **kw)), None) == code
+    assert text in _lib.last_error()
+
+
+def test_workspace_query():
+    q = rh.load_library().rh_grad_clip_workspace_bytes
+    one = _refs((4096, 5, 0))
+    assert q(one.ctypes.data, 1) == 256 and q(None, 0) == 256
+    assert q(None, 1) == 0 and q(one.ctypes.data, -1) == 0
+    big = _refs((4096, 1 << 34, 0))
+    assert q(big.ctypes.data, 1) < 1 << 20

@@ -192,9 +192,38 @@ __device__ __forceinline__ int2 tile_at(const Grid g, const int id) {
   return make_int2(first + in % rows, in / rows);
 }
 
+// The rows of a call come in chunks: this chunk's are `first` on, at most `most` of them.
+struct Chunk {
+  int first, most;
+  __device__ __forceinline__ int rows(const int* n_valid) const {
+    return min(most, *n_valid - first);
+  }
+};
+
+// How a logit waits for its row's sum where it is kept: as it is (float), or for the 16-bit types as
+// its distance below the tile's largest in the row, in steps of 2^-kBits: an error of at most half a
+// step, which changes p by 2^-12 (bfloat16) or 2^-13 (float16) relative, a sixteenth and a quarter of
+// what rounding p to the type does.  The last code is probability 0; it stands for what is more than
+// 32 or 16 below the largest (p < 2^-46 or 2^-23 of that one's).
+template <typename T>
+struct Kept {
+  typedef unsigned short type;
+  static constexpr int kBits = sizeof(T) == 2 ? 11 : 0;
+};
+template <>
+struct Kept<_Float16> {
+  typedef unsigned short type;
+  static constexpr int kBits = 12;
+};
+template <>
+struct Kept<float> {
+  typedef float type;
+  static constexpr int kBits = 0;
+};
+
 template <typename T>
 struct LogitArgs {
-  const T* x;          // placed rows, ldx apart, zero-padded
+  const T* x;          // the chunk's placed rows, ldx apart, zero-padded
   long long ldx;
   const T* w;          // first class of this call
   long long ldw, w_bytes;
@@ -203,23 +232,26 @@ struct LogitArgs {
   int w_limit;         // bytes of the last step that are the weights' rows
   int v0, v;           // first class, how many
   Grid grid;
-  RowInfo info;
+  Chunk chunk;
+  const int* n_valid;
+  const int* label;    // [place], as everything below by the chunk's places
   float2* stats;       // [tile of classes][place]  (max, sum of exp above it)
   long long ld_stats;
   float* z_label;      // [place]
-  const float* lse;    // [place]
-  T* p;                // [place][ldp]
+  const float2* row;   // [place]  (max, 1 / sum) over all classes
+  void* p;             // [place][ldp]  P, or the logits kept for it
   int ldp;
 };
 
-enum What { kStats, kProb };
+// kStats: the tiles' (max, sum) only.  kKeep: and the logits.  kProb: P, from rows' sums known before.
+enum What { kStats, kKeep, kProb };
 
 template <typename T, typename S, What kWhat>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_kernel(const LogitArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
   const int2 at = tile_at(a.grid, blockIdx.x);
-  const int rows = *a.info.n_valid, m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  const int rows = a.chunk.rows(a.n_valid), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   if (m0 >= rows) return;
   Tile<T, kRows, kRows, S> tile;
   tile.run(a.x + m0 * a.ldx, a.ldx, ((long long)rows - m0) * a.ldx * (int)sizeof(T),
@@ -227,83 +259,95 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
   const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32;
   const int left = a.v - n0 - wn - 4 * half;      // this lane's columns (32 j + 8 q + r) below it exist
+  const int room = a.ldp - n0 - wn - 4 * half;    // and those below it are stored
+  float bias[S::kFN][16];      // what a column's logits get; -inf where there is no class
+#pragma unroll
+  for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bias[j][r] = 32 * j + 8 * (r >> 2) + (r & 3) < left ? 0.0f : -__builtin_inff();
   if (a.bias) {
 #pragma unroll
     for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int c = min(32 * j + 8 * (r >> 2) + (r & 3), left - 1);       // past the last class: any
-        const float b = TypeOf<T>::to_float(a.bias[max(a.v0 + n0 + wn + 4 * half + c, 0)]);
-#pragma unroll
-        for (int i = 0; i < S::kFM; ++i) tile.acc[i][j][r] += b;
+        bias[j][r] += TypeOf<T>::to_float(a.bias[max(a.v0 + n0 + wn + 4 * half + c, 0)]);
       }
   }
-  if constexpr (kWhat == kStats) {
-    if (a.v - n0 < S::kBN) {      // classes that do not exist
-#pragma unroll
-      for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool none = 32 * j + 8 * (r >> 2) + (r & 3) >= left;
-#pragma unroll
-          for (int i = 0; i < S::kFM; ++i) tile.acc[i][j][r] = none ? -__builtin_inff() : tile.acc[i][j][r];
-        }
-    }
-    RH_LDS float2* red = (RH_LDS float2*)lds;      // [kWN][kBM]
-    __syncthreads();
+  if constexpr (kWhat != kProb) {
+    RH_LDS float* tops = (RH_LDS float*)lds;       // [kWN][kBM]
+    RH_LDS float* sums = tops + S::kWN * S::kBM;   // [kWN][kBM]
 #pragma unroll
     for (int i = 0; i < S::kFM; ++i) {
-      const int m = wm + 32 * i + (lane & 31), row = m0 + m;
       float top = -__builtin_inff();
 #pragma unroll
       for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, tile.acc[i][j][r]);
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, tile.acc[i][j][r] + bias[j][r]);
       top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (half == 0) tops[(wave % S::kWN) * S::kBM + wm + 32 * i + lane] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::kFM; ++i) {
+      const int m = wm + 32 * i + (lane & 31), row = m0 + m;
+      float top = tops[m];
+#pragma unroll
+      for (int k = 1; k < S::kWN; ++k) top = fmaxf(top, tops[k * S::kBM + m]);
       const float base = top == -__builtin_inff() ? 0.0f : top;
+      typename Kept<T>::type* out = (typename Kept<T>::type*)a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += exp_for<T>(tile.acc[i][j][r] - base);
+        for (int q = 0; q < 4; ++q) {
+          Vec4<typename Kept<T>::type> kept;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float z = tile.acc[i][j][4 * q + r] + bias[j][4 * q + r];
+            sum += exp_for<T>(z - base);
+            if constexpr (sizeof(T) == 4) {
+              kept.v[r] = z;
+            } else {
+              const float steps = __builtin_fmaf(base - z, (float)(1 << Kept<T>::kBits), 0.5f);
+              kept.v[r] = (unsigned short)(unsigned)fminf(steps, 65535.0f);
+            }
+          }
+          if (kWhat == kKeep && row < rows && 32 * j + 8 * q < room)
+            *(Vec4<typename Kept<T>::type>*)(out + 32 * j + 8 * q) = kept;
+        }
       sum += __shfl_xor(sum, 32, 64);
-      if (half == 0) {
-        float2 pair = make_float2(top, sum);
-        red[(wave % S::kWN) * S::kBM + m].x = pair.x;
-        red[(wave % S::kWN) * S::kBM + m].y = pair.y;
-      }
-      const int c = row < rows ? a.info.label[row] - (a.v0 + n0 + wn + 4 * half) : -1;
+      if (half == 0) sums[(wave % S::kWN) * S::kBM + m] = sum;
+      const int c = row < rows ? a.label[row] - (a.v0 + n0 + wn + 4 * half) : -1;
       const bool mine = c >= 0 && c < S::kFN * 32 && (c & 7) < 4;
       if (__any(mine)) {
         float z = 0.0f;
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) z = c == 32 * j + 8 * (r >> 2) + (r & 3) ? tile.acc[i][j][r] : z;
+          for (int r = 0; r < 16; ++r) z = c == 32 * j + 8 * (r >> 2) + (r & 3) ? tile.acc[i][j][r] + bias[j][r] : z;
         if (mine) a.z_label[row] = z;
       }
       __builtin_amdgcn_sched_barrier(0);      // one fragment row's registers at a time
     }
     __syncthreads();
-    if (t < S::kBM && m0 + t < rows) {
-      float top = -__builtin_inff(), sum = 0.0f;
+    for (int m = t; m < S::kBM && m0 + m < rows; m += S::kThreads) {
+      float top = tops[m], sum = sums[m];
 #pragma unroll
-      for (int k = 0; k < S::kWN; ++k) top = fmaxf(top, red[k * S::kBM + t].x);
-      const float base = top == -__builtin_inff() ? 0.0f : top;
-#pragma unroll
-      for (int k = 0; k < S::kWN; ++k)
-        sum += red[k * S::kBM + t].y * exp_for<T>(red[k * S::kBM + t].x - base);
-      a.stats[(long long)(a.v0 / S::kBN + at.y) * a.ld_stats + m0 + t] = make_float2(top, sum);
+      for (int k = 1; k < S::kWN; ++k) {
+        top = fmaxf(top, tops[k * S::kBM + m]);
+        sum += sums[k * S::kBM + m];
+      }
+      a.stats[(long long)(a.v0 / S::kBN + at.y) * a.ld_stats + m0 + m] = make_float2(top, sum);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < S::kFM; ++i) {
       const int row = m0 + wm + 32 * i + (lane & 31);
       if (row < rows) {
-        const float lse = a.lse[row];
-        const int c = a.info.label[row] - (a.v0 + n0 + wn + 4 * half);
-        const int room = a.ldp - n0 - wn - 4 * half;      // columns up to ldp are written, with zeros past v
-        T* out = a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
+        const float2 of_row = a.row[row];
+        const int c = a.label[row] - (a.v0 + n0 + wn + 4 * half);
+        T* out = (T*)a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
@@ -312,29 +356,91 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
             Vec4<T> v;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              float p = exp_for<T>(tile.acc[i][j][4 * q + r] - lse);
-              p = (c == at0 + r ? p - 1.0f : p) * PScale<T>::up;
-              v.v[r] = TypeOf<T>::from_float(at0 + r < left ? p : 0.0f);
+              const float p = exp_for<T>((tile.acc[i][j][4 * q + r] + bias[j][4 * q + r]) - of_row.x) * of_row.y;
+              v.v[r] = TypeOf<T>::from_float((c == at0 + r ? p - 1.0f : p) * PScale<T>::up);
             }
             if (at0 < room) *(Vec4<T>*)(out + at0) = v;
           }
       }
-      __builtin_amdgcn_sched_barrier(0);      // one fragment row's registers at a time
     }
   }
 }
 
-// lse and row loss of every place from the tiles' pairs: eight threads a row, each an eighth of the
-// tiles, joined by (max, sum) pairs.
+// P from the kept logits, in their place: p = e^(z - tile's top) * (e^(tile's top - row's top) / row's
+// sum), the first factor from the code.  A workgroup takes kRows rows of 16 bytes of columns a thread;
+// column_sums (or NULL): [row block][v] sums of P over its rows.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept, const int ldp, const int v,
+                                                         const Chunk chunk, const int* __restrict__ n_valid,
+                                                         const int* __restrict__ label,
+                                                         const float2* __restrict__ row_stats,
+                                                         const float2* __restrict__ stats, const long long ld_stats,
+                                                         const int tile, const int per,
+                                                         float* __restrict__ column_sums) {
+  constexpr int kV = 16 / (int)sizeof(T);
+  const int rows = chunk.rows(n_valid), lo = blockIdx.y * per, hi = min(rows, lo + per);
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * kV;
+  if (c >= ldp) return;
+  const float2* top = stats + (long long)(c / tile) * ld_stats;
+  float sums[kV];
+#pragma unroll
+  for (int k = 0; k < kV; ++k) sums[k] = 0.0f;
+#pragma unroll 4
+  for (int r = lo; r < hi; ++r) {
+    u32x4* const at = (u32x4*)((T*)kept + (long long)r * ldp + c);
+    const u32x4 z = *at;
+    const float2 of_row = row_stats[r];
+    const int y = label[r] - c;
+    u32x4 out;
+    float p[kV];
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 f = __builtin_bit_cast(f32x4, z);
+#pragma unroll
+      for (int k = 0; k < kV; ++k) p[k] = expf(f[k] - of_row.x) * of_row.y;
+    } else {
+      const float f = exp_for<T>(top[r].x - of_row.x) * of_row.y;
+#pragma unroll
+      for (int k = 0; k < kV; ++k) {
+        const unsigned w = z[k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
+        const float e = __builtin_amdgcn_exp2f((float)code * (-kLog2e / (1 << Kept<T>::kBits)));
+        p[k] = (code == 0xffffu ? 0.0f : e) * f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+      p[k] = y == k ? p[k] - 1.0f : p[k];
+      sums[k] += p[k];
+    }
+    if constexpr (sizeof(T) == 4) {
+      f32x4 o;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = c + k < v ? p[k] : 0.0f;
+      out = __builtin_bit_cast(u32x4, o);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const T a = TypeOf<T>::from_float(p[2 * k] * PScale<T>::up), b = TypeOf<T>::from_float(p[2 * k + 1] * PScale<T>::up);
+        out[k] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
+      }
+    }
+    *at = out;
+  }
+  if (column_sums)
+    for (int k = 0; k < kV && c + k < v; ++k) column_sums[(long long)blockIdx.y * v + c + k] = sums[k];
+}
+
+// Row loss and (max, 1 / sum) of every place from the tiles' pairs: eight threads a row, each an
+// eighth of the tiles.
 __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __restrict__ stats,
                                                               const long long ld, const int tiles,
-                                                              const RowInfo info,
+                                                              const Chunk chunk, const int* __restrict__ n_valid,
+                                                              const int* __restrict__ map,
                                                               const float* __restrict__ z_label,
-                                                              float* __restrict__ lse,
+                                                              float2* __restrict__ row_stats,
                                                               float* __restrict__ row_loss,
                                                               double* __restrict__ partial) {
   __shared__ float s_top[8][32], s_sum[8][32];
-  const int rows = *info.n_valid, r = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int rows = chunk.rows(n_valid), r = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int row = blockIdx.x * 32 + r;
   float top = -__builtin_inff(), sum = 0.0f;
   if (row < rows) {
@@ -356,9 +462,9 @@ __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __re
       for (int k = 0; k < 8; ++k) top = fmaxf(top, s_top[k][r]);
       const float base = top == -__builtin_inff() ? 0.0f : top;
       for (int k = 0; k < 8; ++k) sum += s_sum[k][r] * expf(s_top[k][r] - base);
-      const float l = top + logf(sum), v = l - z_label[row];
-      lse[row] = l;
-      row_loss[info.map[row]] = v;
+      const float v = (top - z_label[row]) + logf(sum);
+      row_stats[row] = make_float2(top, 1.0f / sum);
+      row_loss[map[row]] = v;
       loss = (double)v;
     }
     loss = wave_sum(loss);
@@ -387,7 +493,8 @@ struct ProductArgs {
   const T* b;
   long long ldb, b_bytes;      // readable from b on (kCols: its rows end with the sum instead)
   int m, n, k;                 // on the host's side; rows that count bound m or k on the device
-  const int* rows;             // bounds m (kRows A) or k (kCols A)
+  const int* n_valid;          // with the chunk: bounds m (kRows A) or k (kCols A)
+  Chunk chunk;
   Grid grid;
   int split_steps;             // k steps a split takes
   const float* scale;
@@ -408,7 +515,7 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
   RH_LDS char* lds = (RH_LDS char*)smem;
   constexpr int kStepK = kStepBytes / (int)sizeof(T);
   const int2 at = tile_at(a.grid, blockIdx.x);
-  const int rows = *a.rows, m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  const int rows = max(a.chunk.rows(a.n_valid), 0), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   const int m = kLA == kRows ? min(a.m, rows) : a.m, k = kLA == kCols ? min(a.k, rows) : a.k;
   if (m0 >= m) return;
   const long long size = sizeof(T);
@@ -477,11 +584,11 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __restrict__ part, const int splits,
                                                               const long long plane, const long long ldpart,
                                                               const int m, const int n,
-                                                              const int* __restrict__ rows,
+                                                              const Chunk chunk, const int* __restrict__ n_valid,
                                                               const float* __restrict__ scale, const float down,
                                                               const int* __restrict__ map, T* __restrict__ out,
                                                               const long long ldo) {
-  const long long quads = (n + 3) / 4, top = min(m, rows ? *rows : m) * quads;
+  const long long quads = (n + 3) / 4, top = (n_valid ? chunk.rows(n_valid) : m) * quads;
   const float s = *scale * down;
   for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < top; i += (long long)gridDim.x * kThreads) {
     const long long r = i / quads;
@@ -503,9 +610,9 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __res
 // Column sums of P over the rows that count: a block takes 256 columns and every splits-th run of rows.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sum_columns_kernel(const T* __restrict__ p, const int ldp, const int v,
-                                                               const int* __restrict__ rows_at, const int splits,
-                                                               float* __restrict__ part) {
-  const int c = blockIdx.x * kThreads + threadIdx.x, rows = *rows_at;
+                                                               const Chunk chunk, const int* __restrict__ n_valid,
+                                                               const int splits, float* __restrict__ part) {
+  const int c = blockIdx.x * kThreads + threadIdx.x, rows = max(chunk.rows(n_valid), 0);
   const int per = (rows + splits - 1) / splits, lo = blockIdx.y * per, hi = min(rows, lo + per);
   if (c >= v) return;
   float sum = 0.0f;
@@ -542,21 +649,31 @@ __global__ __launch_bounds__(kThreads) void upstream_kernel(T* __restrict__ x, c
 typedef Shape<2, 2, 4, 4> Large;      // 256 x 256, 4 waves
 typedef Shape<2, 2, 2, 2> Small;      // 128 x 128, 4 waves
 
-constexpr long long kPieceBytes = 256ll << 20;
-constexpr long long kPieceMost = 1 << 18;      // a tile's byte offsets into P stay below 2^31
+constexpr long long kPieceBytes = 256ll << 20;      // of P where the logits are made twice
+constexpr long long kPieceMost = 1 << 18;           // classes; a tile's byte offsets into P stay below 2^31
+constexpr long long kKeptBytes = 2ll << 30;         // of logits where they are made once
 constexpr int kColumnSplits = 32;
+constexpr int kProbRows = 64;
+constexpr int kKeepFrom = 512;                      // features
 
 static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+// The call's work is cut so that no more than a bounded piece of the logits exists at a time:
+//   keep    all classes of `chunk` rows: logits once (6 n d v operations in all), P made in their
+//           place; with more than one chunk the weight's gradient is added up in float32.
+//   !keep   `piece` classes of all rows: one pass for the rows' sums, then piece by piece the logits
+//           again, as P (8 n d v operations); each piece's part of the weight's gradient is complete.
 struct Plan {
   int size, step_k;
   int per, row_blocks;          // rows a placing block takes
   int ldx, ldw_pad;             // padded rows of the placed features; of the copied weights (0: none)
+  bool keep;
+  int chunk, chunks;            // rows at a time
+  int piece, pieces, ldp;       // classes of P at a time
   bool large_logits, large_dx, large_dw;
   int bn;                       // classes a tile of the logits takes
-  int piece, pieces, ldp;       // classes of P at a time
   int dx_splits, dx_steps, dw_splits, dw_steps;
-  long long ldpart_dx, ldpart_dw;
+  long long ldpart;
   int tiles_v;
 };
 
@@ -585,27 +702,42 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   p.row_blocks = ceil_div(n, p.per);
   p.ldx = ceil_div(d, p.step_k) * p.step_k;
   p.ldw_pad = flags & RH_CE_COPY_WEIGHT ? p.ldx : 0;
-  long long piece = kPieceBytes / ((long long)n * p.size) / 256 * 256;
-  if (piece < 4096) piece = 4096;
-  if (piece > kPieceMost) piece = kPieceMost;
-  if (piece > v) piece = v;
-  p.pieces = ceil_div(v, piece);
-  if (p.pieces > 1) piece = ceil_div(ceil_div(v, p.pieces), 256) * 256;     // of even size
-  p.pieces = ceil_div(v, piece);
-  p.piece = (int)piece;
-  p.ldp = ceil_div(piece, 64) * 64;
-  p.large_logits = take_large(n, piece);
+  const bool grads = flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B);
+  const long long row_bytes = (long long)ceil_div(v, 64) * 64 * p.size;
+  p.chunk = n;
+  p.chunks = 1;
+  p.keep = grads && d >= kKeepFrom && row_bytes * 256 < kKeptBytes;
+  if (p.keep) {
+    const long long rows = kKeptBytes / row_bytes / 256 * 256;
+    if (n > rows) {
+      p.chunks = ceil_div(n, rows);
+      p.chunk = ceil_div(ceil_div(n, p.chunks), 256) * 256;      // of even size
+      p.chunks = ceil_div(n, p.chunk);
+    }
+    p.piece = v;
+    p.pieces = 1;
+  } else {
+    long long piece = kPieceBytes / ((long long)n * p.size) / 256 * 256;
+    if (piece < 4096) piece = 4096;
+    if (piece > kPieceMost) piece = kPieceMost;
+    if (piece > v) piece = v;
+    p.pieces = ceil_div(v, piece);
+    if (p.pieces > 1) piece = ceil_div(ceil_div(v, p.pieces), 256) * 256;
+    p.pieces = ceil_div(v, piece);
+    p.piece = (int)piece;
+  }
+  p.ldp = ceil_div(p.piece, 64) * 64;
+  p.large_logits = take_large(p.chunk, p.piece);
   p.bn = p.large_logits ? 256 : 128;
   p.tiles_v = ceil_div(v, p.bn);
-  p.large_dx = take_large(n, d);
-  p.large_dw = take_large(piece, d);
-  const int k_dx = ceil_div(p.ldp, p.step_k), k_dw = ceil_div(n, p.step_k);
-  p.dx_splits = splits_for(n, d, k_dx, p.large_dx);
+  p.large_dx = take_large(p.chunk, d);
+  p.large_dw = take_large(p.piece, d);
+  const int k_dx = ceil_div(p.ldp, p.step_k), k_dw = ceil_div(p.chunk, p.step_k);
+  p.dx_splits = splits_for(p.chunk, d, k_dx, p.large_dx);
   p.dx_steps = ceil_div(k_dx, p.dx_splits);
-  p.dw_splits = splits_for(piece, d, k_dw, p.large_dw);
+  p.dw_splits = splits_for(p.piece, d, k_dw, p.large_dw);
   p.dw_steps = ceil_div(k_dw, p.dw_splits);
-  p.ldpart_dx = ceil_div(d, 4) * 4;
-  p.ldpart_dw = ceil_div(d, 4) * 4;
+  p.ldpart = ceil_div(d, 4) * 4;
   return p;
 }
 
@@ -616,12 +748,13 @@ struct Space {
   char* w;
   float2* stats;
   float* z_label;
-  float* lse;
+  float2* row_stats;
   double* loss;
   char* p;
   float* dx_part;
   float* dw_part;
   float* db_part;
+  int db_splits;      // parts of a column's sum, of all chunks
   size_t bytes;
 };
 
@@ -635,16 +768,19 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   s.info.scale = c.take<float>(1);
   s.x = c.take<char>((size_t)n * p.ldx * p.size);
   if (p.ldw_pad) s.w = c.take<char>((size_t)v * p.ldw_pad * p.size);
-  s.stats = c.take<float2>((size_t)p.tiles_v * n);
+  s.stats = c.take<float2>((size_t)p.tiles_v * p.chunk);
   s.z_label = c.take<float>(n);
-  s.lse = c.take<float>(n);
+  s.row_stats = c.take<float2>(n);
   s.loss = c.take<double>(ceil_div(n, 32));
-  if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) s.p = c.take<char>((size_t)n * p.ldp * p.size);
+  if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) s.p = c.take<char>((size_t)p.chunk * p.ldp * p.size);
   if ((flags & RH_CE_GRAD_X) && (p.pieces > 1 || p.dx_splits > 1))
-    s.dx_part = c.take<float>((size_t)p.dx_splits * n * p.ldpart_dx);
-  if ((flags & RH_CE_GRAD_W) && p.dw_splits > 1)
-    s.dw_part = c.take<float>((size_t)p.dw_splits * p.piece * p.ldpart_dw);
-  if (flags & RH_CE_GRAD_B) s.db_part = c.take<float>((size_t)kColumnSplits * p.piece);
+    s.dx_part = c.take<float>((size_t)p.dx_splits * p.chunk * p.ldpart);
+  if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw_splits > 1))
+    s.dw_part = c.take<float>((size_t)p.dw_splits * p.piece * p.ldpart);
+  if (flags & RH_CE_GRAD_B) {
+    s.db_splits = p.keep ? ceil_div(p.chunk, kProbRows) * p.chunks : kColumnSplits;
+    s.db_part = c.take<float>((size_t)s.db_splits * p.piece);
+  }
   s.bytes = c.off;
   return s;
 }
@@ -656,8 +792,8 @@ static int raise_lds(K kernel, int bytes) {
 }
 
 template <typename T, typename S, What kWhat>
-static int launch_logits(LogitArgs<T> a, int n, hipStream_t stream) {
-  a.grid = Grid{ceil_div(n, S::kBM), ceil_div(a.v, S::kBN)};
+static int launch_logits(LogitArgs<T> a, hipStream_t stream) {
+  a.grid = Grid{ceil_div(a.chunk.most, S::kBM), ceil_div(a.v, S::kBN)};
   auto kernel = logits_kernel<T, S, kWhat>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n), dim3(S::kThreads), S::kLdsBytes, stream, a);
@@ -678,13 +814,81 @@ static int launch_product(ProductArgs<T> a, int splits, hipStream_t stream) {
 }
 
 template <typename T>
-static int join_parts(const float* part, int splits, long long plane, long long ldpart, int m, int n, const int* rows,
-                      const float* scale, const int* map, T* out, hipStream_t stream) {
-  long long blocks = ((long long)m * ((n + 3) / 4) + kThreads - 1) / kThreads;
+static int join_parts(const ProductArgs<T>& g, int splits, bool by_rows, hipStream_t stream) {
+  long long blocks = ((long long)g.m * ((g.n + 3) / 4) + kThreads - 1) / kThreads;
   if (blocks > 256 * 8) blocks = 256 * 8;
-  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, part, splits, plane,
-                     ldpart, m, n, rows, scale, PScale<T>::down, map, out, (long long)n);
+  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, g.part, splits, g.plane,
+                     g.ldpart, g.m, g.n, g.chunk, by_rows ? g.n_valid : nullptr, g.scale, g.down, g.map, g.out, g.ldo);
   RH_CHECK_LAUNCH("join_parts_kernel");
+  return RH_OK;
+}
+
+// dX of a chunk from a piece of P (all of it, or the piece-th).
+template <typename T>
+static int features_gradient(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a,
+                             int piece, hipStream_t stream) {
+  ProductArgs<T> g = {};
+  g.a = (const T*)s.p;
+  g.lda = p.ldp;
+  g.b = a.w;
+  g.ldb = a.ldw;
+  g.b_bytes = a.w_bytes;
+  g.m = a.chunk.most;
+  g.n = q.d;
+  g.k = ceil_div(a.v, 64) * 64;       // P has zeros there, the weights' records end earlier
+  g.n_valid = a.n_valid;
+  g.chunk = a.chunk;
+  g.split_steps = p.dx_steps;
+  g.scale = s.info.scale;
+  g.down = PScale<T>::down;
+  g.out = (T*)q.dx;
+  g.map = s.info.map + a.chunk.first;
+  g.ldo = q.d;
+  g.part = s.dx_part;
+  g.ldpart = p.ldpart;
+  g.plane = (long long)p.chunk * p.ldpart;
+  g.add = piece > 0;
+  if (int rc = p.large_dx ? launch_product<T, kRows, Large>(g, p.dx_splits, stream)
+                          : launch_product<T, kRows, Small>(g, p.dx_splits, stream))
+    return rc;
+  return s.dx_part && piece == p.pieces - 1 ? join_parts(g, p.dx_splits, true, stream) : RH_OK;
+}
+
+// dW of a piece's classes from a chunk of P.
+template <typename T>
+static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a,
+                           int chunk, hipStream_t stream) {
+  ProductArgs<T> g = {};
+  g.a = (const T*)s.p;
+  g.lda = p.ldp;
+  g.b = a.x;
+  g.ldb = a.ldx;
+  g.b_bytes = (long long)a.chunk.most * a.ldx * p.size;
+  g.m = a.v;
+  g.n = q.d;
+  g.k = a.chunk.most;
+  g.n_valid = a.n_valid;
+  g.chunk = a.chunk;
+  g.split_steps = p.dw_steps;
+  g.scale = s.info.scale;
+  g.down = PScale<T>::down;
+  g.out = (T*)q.dw + (long long)a.v0 * q.d;
+  g.ldo = q.d;
+  g.part = s.dw_part;
+  g.ldpart = p.ldpart;
+  g.plane = (long long)p.piece * p.ldpart;
+  g.add = chunk > 0;
+  if (int rc = p.large_dw ? launch_product<T, kCols, Large>(g, p.dw_splits, stream)
+                          : launch_product<T, kCols, Small>(g, p.dw_splits, stream))
+    return rc;
+  return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, p.dw_splits, false, stream) : RH_OK;
+}
+
+template <typename T>
+static int bias_gradient(const rh_linear_ce_args& q, const Space& s, int v0, int vc, float down, hipStream_t stream) {
+  hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(vc, kThreads)), dim3(kThreads), 0, stream, s.db_part,
+                     s.db_splits, vc, s.info.scale, down, (T*)q.db + v0);
+  RH_CHECK_LAUNCH("join_columns_kernel");
   return RH_OK;
 }
 
@@ -712,7 +916,6 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   const long long w_bytes = ((v - 1) * ldw + d_w) * p.size;
 
   LogitArgs<T> a = {};
-  a.x = x;
   a.ldx = p.ldx;
   a.w = w;
   a.ldw = ldw;
@@ -720,100 +923,67 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   a.bias = (const T*)q.bias;
   a.steps = p.ldx / p.step_k;
   a.w_limit = (int)(d_w * p.size - (long long)(a.steps - 1) * kStepBytes);
-  a.v = v;
-  a.info = s.info;
+  a.n_valid = s.info.n_valid;
   a.stats = s.stats;
-  a.ld_stats = n;
-  a.z_label = s.z_label;
-  a.lse = s.lse;
-  a.p = (T*)s.p;
+  a.ld_stats = p.chunk;
+  a.p = s.p;
   a.ldp = p.ldp;
-  if (int rc = p.large_logits ? launch_logits<T, Large, kStats>(a, n, stream)
-                              : launch_logits<T, Small, kStats>(a, n, stream))
-    return rc;
-  const int joins = ceil_div(n, 32);
-  hipLaunchKernelGGL(join_stats_kernel, dim3(joins), dim3(kThreads), 0, stream, s.stats, (long long)n, p.tiles_v, s.info,
-                     s.z_label, s.lse, q.row_loss, s.loss);
-  RH_CHECK_LAUNCH("join_stats_kernel");
-  hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, joins, q.small);
-  RH_CHECK_LAUNCH("finish_loss_kernel");
-  if (!q.dx && !q.dw && !q.db) return RH_OK;
-
-  for (int i = 0; i < p.pieces; ++i) {
-    const int v0 = i * p.piece, vc = v - v0 < p.piece ? v - v0 : p.piece;
-    a.v0 = v0;
-    a.v = vc;
-    a.w = w + v0 * ldw;
-    a.w_bytes = w_bytes - v0 * ldw * p.size;
-    if (int rc = p.large_logits ? launch_logits<T, Large, kProb>(a, n, stream)
-                                : launch_logits<T, Small, kProb>(a, n, stream))
+  for (int c = 0; c < p.chunks; ++c) {
+    a.chunk = Chunk{c * p.chunk, n - c * p.chunk < p.chunk ? n - c * p.chunk : p.chunk};
+    const int first = a.chunk.first;
+    a.x = x + (long long)first * p.ldx;
+    a.label = s.info.label + first;
+    a.z_label = s.z_label + first;
+    a.row = s.row_stats + first;
+    a.v0 = 0;
+    a.v = v;
+    if (int rc = p.keep ? p.large_logits ? launch_logits<T, Large, kKeep>(a, stream)
+                                         : launch_logits<T, Small, kKeep>(a, stream)
+                        : p.large_logits ? launch_logits<T, Large, kStats>(a, stream)
+                                         : launch_logits<T, Small, kStats>(a, stream))
       return rc;
-    if (q.dx) {
-      const bool parts = s.dx_part != nullptr;
-      ProductArgs<T> g = {};
-      g.a = (const T*)s.p;
-      g.lda = p.ldp;
-      g.b = a.w;
-      g.ldb = ldw;
-      g.b_bytes = a.w_bytes;
-      g.m = n;
-      g.n = d;
-      g.k = ceil_div(vc, 64) * 64;       // P has zeros there, the weights' records end earlier
-      g.rows = s.info.n_valid;
-      g.split_steps = p.dx_steps;
-      g.scale = s.info.scale;
-      g.down = PScale<T>::down;
-      g.out = (T*)q.dx;
-      g.map = s.info.map;
-      g.ldo = d;
-      g.part = s.dx_part;
-      g.ldpart = p.ldpart_dx;
-      g.plane = (long long)n * p.ldpart_dx;
-      g.add = parts && i > 0;
-      if (int rc = p.large_dx ? launch_product<T, kRows, Large>(g, p.dx_splits, stream)
-                              : launch_product<T, kRows, Small>(g, p.dx_splits, stream))
-        return rc;
-      if (parts && i == p.pieces - 1)
-        if (int rc = join_parts<T>(s.dx_part, p.dx_splits, g.plane, g.ldpart, n, d, s.info.n_valid, s.info.scale,
-                                   s.info.map, (T*)q.dx, stream))
-          return rc;
+    hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, 32)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
+                       p.tiles_v, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,
+                       s.loss + first / 32);
+    RH_CHECK_LAUNCH("join_stats_kernel");
+    if (c == p.chunks - 1) {
+      hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, 32), q.small);
+      RH_CHECK_LAUNCH("finish_loss_kernel");
     }
-    if (q.dw) {
-      ProductArgs<T> g = {};
-      g.a = (const T*)s.p;
-      g.lda = p.ldp;
-      g.b = x;
-      g.ldb = p.ldx;
-      g.b_bytes = (long long)n * p.ldx * p.size;
-      g.m = vc;
-      g.n = d;
-      g.k = n;
-      g.rows = s.info.n_valid;
-      g.split_steps = p.dw_steps;
-      g.scale = s.info.scale;
-      g.down = PScale<T>::down;
-      g.out = (T*)q.dw + (long long)v0 * d;
-      g.ldo = d;
-      g.part = s.dw_part;
-      g.ldpart = p.ldpart_dw;
-      g.plane = (long long)p.piece * p.ldpart_dw;
-      if (int rc = p.large_dw ? launch_product<T, kCols, Large>(g, p.dw_splits, stream)
-                              : launch_product<T, kCols, Small>(g, p.dw_splits, stream))
-        return rc;
-      if (s.dw_part)
-        if (int rc = join_parts<T>(s.dw_part, p.dw_splits, g.plane, g.ldpart, vc, d, nullptr, s.info.scale, nullptr,
-                                   g.out, stream))
-          return rc;
+    if (!q.dx && !q.dw && !q.db) continue;
+    if (p.keep) {
+      const int per_chunk = ceil_div(p.chunk, kProbRows);
+      const dim3 grid(ceil_div(p.ldp, kThreads * (16 / p.size)), per_chunk);      // column sums: every part is written
+      hipLaunchKernelGGL(probs_kernel<T>, grid, dim3(kThreads), 0, stream, s.p, p.ldp, v, a.chunk, s.info.n_valid, a.label,
+                         a.row, s.stats, a.ld_stats, p.bn, kProbRows,
+                         s.db_part ? s.db_part + (long long)c * per_chunk * v : nullptr);
+      RH_CHECK_LAUNCH("probs_kernel");
+      if (q.dx)
+        if (int rc = features_gradient(q, p, s, a, 0, stream)) return rc;
+      if (q.dw)
+        if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
+      continue;
     }
-    if (q.db) {
-      hipLaunchKernelGGL(sum_columns_kernel<T>, dim3(ceil_div(vc, kThreads), kColumnSplits), dim3(kThreads), 0, stream,
-                         (const T*)s.p, p.ldp, vc, s.info.n_valid, kColumnSplits, s.db_part);
-      RH_CHECK_LAUNCH("sum_columns_kernel");
-      hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(vc, kThreads)), dim3(kThreads), 0, stream, s.db_part,
-                         kColumnSplits, vc, s.info.scale, PScale<T>::down, (T*)q.db + v0);
-      RH_CHECK_LAUNCH("join_columns_kernel");
+    for (int i = 0; i < p.pieces; ++i) {
+      a.v0 = i * p.piece;
+      a.v = v - a.v0 < p.piece ? v - a.v0 : p.piece;
+      a.w = w + a.v0 * ldw;
+      a.w_bytes = w_bytes - a.v0 * ldw * p.size;
+      if (int rc = p.large_logits ? launch_logits<T, Large, kProb>(a, stream) : launch_logits<T, Small, kProb>(a, stream))
+        return rc;
+      if (q.dx)
+        if (int rc = features_gradient(q, p, s, a, i, stream)) return rc;
+      if (q.dw)
+        if (int rc = weight_gradient(q, p, s, a, 0, stream)) return rc;
+      if (q.db) {
+        hipLaunchKernelGGL(sum_columns_kernel<T>, dim3(ceil_div(a.v, kThreads), kColumnSplits), dim3(kThreads), 0, stream,
+                           (const T*)s.p, p.ldp, a.v, a.chunk, s.info.n_valid, kColumnSplits, s.db_part);
+        RH_CHECK_LAUNCH("sum_columns_kernel");
+        if (int rc = bias_gradient<T>(q, s, a.v0, a.v, PScale<T>::down, stream)) return rc;
+      }
     }
   }
+  if (q.db && p.keep) return bias_gradient<T>(q, s, 0, v, 1.0f, stream);
   return RH_OK;
 }
 

@@ -7,7 +7,9 @@ internal additions are granted twice that) and u = eps/2 of the element type.
   lse         a sum of positive terms, each off by its exponent's error, its exp and V additions (pairwise
               within tiles, but V e bounds any order):  |d lse| <= Z + (V + 16) e + e (|max| + |lse|)
   row loss    Z + |d lse| + e |row|
-  P           |dP| <= p (exp(Z + |d lse| + 8 e + 4 e |z - lse|) - 1) + e + u |P|   (the e: p - 1 in float32)
+  P           |dP| <= p (exp(Z + |d lse| + 8 e + 4 e |z - lse| + k) - 1) + e + u |P|
+              (the e: p - 1 in float32, and what is so far below its row's largest that it counts as 0;
+              k: half a step of the kept logit, 2^-12 for bfloat16 and 2^-13 for float16)
   dX = s P W  s (|dP| |W| + (V + 2) e |P| |W|) + (u + 2 e) |dX| + half the type's smallest step
 and dW, db in the same way over the rows.
 """
@@ -69,7 +71,8 @@ def oracle(x, w, y, b, reduction="mean", upstream=1.0, divisor=None, ignore=-100
     k = keep.double()[:, None]
     P = p.clone()
     P.scatter_add_(1, Y[:, None], torch.full_like(zy, -1.0))
-    dP = (p * torch.expm1(Z + dlse + 8 * E + 4 * E * (z - lse).abs()) + E + u * P.abs()) * k
+    kept = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -12, torch.float16: 2.0 ** -13}[x.dtype]
+    dP = (p * torch.expm1(Z + dlse + 8 * E + 4 * E * (z - lse).abs() + kept) + E + u * P.abs()) * k
     P = P * k
     s *= upstream
     a = abs(s)
@@ -122,6 +125,49 @@ def test_large_tiles_pieces_and_many_rows(rh, n, d, v, dtype):
         n = 2051
     x, w, y, b = make(n, d, v, dtype, True, ignored=0.1, seed=3)
     check_all(rh, x, w, y, b)
+
+
+SIZES_WIDE = [(5, 512, 33), (130, 520, 1), (129, 1000, 2049), (700, 513, 4100), (64, 1544, 129)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("n,d,v", SIZES_WIDE)
+def test_wide_features(rh, n, d, v, dtype, bias):
+    """The logits are kept between the passes from a feature width on."""
+    x, w, y, b = make(n, d, v, dtype, bias, ignored=0.3, seed=11, scale=4.0)
+    check_all(rh, x, w, y, b)
+
+
+def test_rows_in_chunks(rh):
+    """More rows than logits may be kept of: the same sums as the two halves by themselves."""
+    x, w, y, b = make(17001, 520, 70001, "bf16", True, seed=12)
+    y[:9000:3] = -100
+    kw = dict(reduction="sum", grads=(True, True, True))
+    both = rh.functional.linear_cross_entropy(x, w, y, b, **kw)
+    halves = [rh.functional.linear_cross_entropy(x[i], w, y[i], b, **kw) for i in (slice(0, 8000), slice(8000, 17001))]
+    assert torch.allclose(both["row_loss"], torch.cat([h["row_loss"] for h in halves]), rtol=64 * E, atol=64 * E)
+    for part in (slice(0, 300), slice(8500, 9000), slice(16800, 17001)):      # a row's results need that row alone
+        close("d_features", both["d_features"][part], oracle(x[part], w, y[part], b, reduction="sum")["d_features"])
+    assert abs(float(both["loss"]) - sum(float(h["loss"]) for h in halves)) <= 3 * 2.0 ** -24 * float(both["loss"])
+    u = 2.0 ** -8
+    for k, rows in (("d_weight", x), ("d_bias", torch.ones(17001, 1, device="cuda"))):
+        a, c = (h[k].double() for h in halves)
+        # each side rounds once per result; the sums inside are float32 in another order: 17001 terms of
+        # |P| |x| <= |P| max|x|, and sum_n |P| <= 2 (count of the label) + the class's probability mass
+        mass = 2.0 * torch.bincount(y[y >= 0], minlength=70001).double() + halves[0]["d_bias"].double().abs() \
+            + halves[1]["d_bias"].double().abs() + 1.0
+        slack = 64 * E * float(rows.abs().max()) * (mass[:, None] if k == "d_weight" else mass)
+        bad = (both[k].double() - (a + c)).abs() > u * (a.abs() + c.abs() + (a + c).abs()) + slack
+        assert not bad.any(), (k, int(bad.sum()))
+    y[:] = -100
+    y[16000:] = 5
+    some = rh.functional.linear_cross_entropy(x, w, y, b, **kw)
+    want = oracle(x[16000:], w, y[16000:], b, reduction="sum")
+    close("d_features", some["d_features"][16000:], want["d_features"])
+    assert (some["d_features"][:16000] == 0).all()
+    for k in ("loss", "d_weight", "d_bias"):
+        close(k, some[k], want[k])
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))

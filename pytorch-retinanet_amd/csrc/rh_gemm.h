@@ -257,42 +257,48 @@ struct Tile {
       if (s == 0) stage_wait();
     }
     u32x4 x[2][S::kFM], y[2][S::kFN];
-    auto read = [&](const int to, const RH_LDS char* stage, const int kk) {
-#pragma unroll
-      for (int i = 0; i < S::kFM; ++i) x[to][i] = fa.read(stage, i, kk);
-#pragma unroll
-      for (int j = 0; j < S::kFN; ++j) y[to][j] = fb.read(stage + kOffB, j, kk);
+    constexpr int kSlots = S::kFM * S::kFN, kFragments = S::kFM + S::kFN;
+    // Fragment f of a quarter, in the order the products take them: y0 x0 y1 .. yn x1 .. xm.
+    auto read = [&](const int to, const RH_LDS char* stage, const int kk, const int f) {
+      if (f == 0) y[to][0] = fb.read(stage + kOffB, 0, kk);
+      else if (f == 1) x[to][0] = fa.read(stage, 0, kk);
+      else if (f <= S::kFN) y[to][f - 1] = fb.read(stage + kOffB, f - 1, kk);
+      else x[to][f - S::kFN] = fa.read(stage, f - S::kFN, kk);
     };
-    auto multiply = [&](const int from, const int i) {
+    // A quarter's products, with what comes next issued between them: while one instruction runs on
+    // the matrix unit (32 cycles) the wave has time for about seven others.
+    auto quarter = [&](const int from, const RH_LDS char* stage, const int kk, const bool load) {
 #pragma unroll
-      for (int j = 0; j < S::kFN; ++j) acc[i][j] = TypeOf<T>::mma(y[from][j], x[from][i], acc[i][j]);
+      for (int t = 0; t < kSlots; ++t) {
+        acc[t / S::kFN][t % S::kFN] =
+            TypeOf<T>::mma(y[from][t % S::kFN], x[from][t / S::kFN], acc[t / S::kFN][t % S::kFN]);
+        if (t < kFragments) read(from ^ 1, stage, kk, t);
+        if (load) {
+          constexpr int kA = kOpsA / kSlots, kB = kOpsB / kSlots;
+          static_assert(kSlots <= 4 || kOpsA + kOpsB == kSlots, "a load a slot");
+          if constexpr (kOpsA + kOpsB == kSlots) {
+            if (t < kOpsA) la.template load<false>(t, 1);
+            else lb.template load<kTail>(t - kOpsA, 1);
+          } else {
+            la.template load<false>(t * kA, kA);
+            lb.template load<kTail>(t * kB, kB);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
-    auto multiply_all = [&](const int from) {
 #pragma unroll
-      for (int i = 0; i < S::kFM; ++i) multiply(from, i);
-      __builtin_amdgcn_sched_barrier(0);      // the next reads stay behind these instructions' issue
-    };
-    read(0, lds, 0);
+    for (int f = 0; f < kFragments; ++f) read(0, lds, 0, f);
     for (int s = 0; s < steps; ++s) {
       RH_LDS char* here = lds + (s & 1) * S::kStage;
       RH_LDS char* next = lds + ((s + 1) & 1) * S::kStage;
-      read(1, here, 1);
-      multiply_all(0);
-      read(0, here, 2);
-      multiply_all(1);
-      read(1, here, 3);
-      multiply_all(0);
+      quarter(0, here, 1, false);
+      quarter(1, here, 2, false);
+      quarter(0, here, 3, false);
       stage_wait();
-      read(0, next, 0);
       la.begin(here, s + 2 < steps, kStepBytes);
       lb.begin(here + kOffB, s + 2 < steps, s + 3 == steps ? b_limit : kStepBytes);
-#pragma unroll
-      for (int i = 0; i < S::kFM; ++i) {
-        la.template load<false>(i * (kOpsA / S::kFM), kOpsA / S::kFM);
-        lb.template load<kTail>(i * (kOpsB / S::kFM), kOpsB / S::kFM);
-        multiply(1, i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      quarter(1, next, 0, true);
     }
     stage_wait();      // LDS is the caller's again
   }

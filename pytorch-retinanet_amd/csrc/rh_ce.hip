@@ -201,24 +201,24 @@ struct Chunk {
 };
 
 // How a logit waits for its row's sum where it is kept: as it is (float), or for the 16-bit types as
-// its distance below the tile's largest in the row, in steps of 2^-kBits: an error of at most half a
-// step, which changes p by 2^-12 (bfloat16) or 2^-13 (float16) relative, a sixteenth and a quarter of
-// what rounding p to the type does.  The last code is probability 0; it stands for what is more than
-// 32 or 16 below the largest (p < 2^-46 or 2^-23 of that one's).
+// its distance below the largest of its group of columns in the row, in steps of 1 / kSteps of a
+// factor of two: an error of at most half a step, which changes p by less than 2^-12 (bfloat16) or
+// 2^-13 (float16) relative, a sixteenth and a quarter of what rounding p to the type does.  The last
+// code is probability 0; it stands for p < 2^-32 or 2^-23 of the largest.
 template <typename T>
 struct Kept {
   typedef unsigned short type;
-  static constexpr int kBits = sizeof(T) == 2 ? 11 : 0;
+  static constexpr float kSteps = 2048.0f;
 };
 template <>
 struct Kept<_Float16> {
   typedef unsigned short type;
-  static constexpr int kBits = 12;
+  static constexpr float kSteps = 2840.0f;
 };
 template <>
 struct Kept<float> {
   typedef float type;
-  static constexpr int kBits = 0;
+  static constexpr float kSteps = 1.0f;
 };
 
 template <typename T>
@@ -235,7 +235,7 @@ struct LogitArgs {
   Chunk chunk;
   const int* n_valid;
   const int* label;    // [place], as everything below by the chunk's places
-  float2* stats;       // [tile of classes][place]  (max, sum of exp above it)
+  float2* stats;       // [group of classes][place]  (max, sum of exp above it)
   long long ld_stats;
   float* z_label;      // [place]
   const float2* row;   // [place]  (max, 1 / sum) over all classes
@@ -243,8 +243,129 @@ struct LogitArgs {
   int ldp;
 };
 
-// kStats: the tiles' (max, sum) only.  kKeep: and the logits.  kProb: P, from rows' sums known before.
+// kStats: the groups' (max, sum) only, a group being a wave's part of the tile's classes.  kKeep: and the logits.  kProb: P, from rows' sums known before.
 enum What { kStats, kKeep, kProb };
+
+// What becomes of a tile's logits.  kPlain: every class is there and none has a bias; else each column
+// gets something, minus infinity where there is no class.
+template <typename T, typename S, What kWhat, bool kPlain, typename Acc>
+__device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& tile, const int m0, const int n0,
+                                              const int rows) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
+  const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32;
+  const int left = a.v - n0 - wn - 4 * half;      // this lane's columns (32 j + 8 q + r) below it exist
+  [[maybe_unused]] const int room = a.ldp - n0 - wn - 4 * half;      // and those below it are stored (float)
+  [[maybe_unused]] float bias[S::kFN][16];
+  if constexpr (!kPlain) {
+#pragma unroll
+    for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int c = 32 * j + 8 * (r >> 2) + (r & 3), in = min(c, left - 1);       // past the last class: any
+        const float b = a.bias ? TypeOf<T>::to_float(a.bias[max(a.v0 + n0 + wn + 4 * half + in, 0)]) : 0.0f;
+        bias[j][r] = c < left ? b : -__builtin_inff();
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < S::kFM; ++i) {
+    const int row = m0 + wm + 32 * i + (lane & 31);
+    const bool there = row < rows;
+    f32x16 z[S::kFN];
+#pragma unroll
+    for (int j = 0; j < S::kFN; ++j) {
+      z[j] = tile.acc[i][j];
+      if constexpr (!kPlain)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[j][r] += bias[j][r];
+    }
+    const int c = there ? a.label[row] - (a.v0 + n0 + wn + 4 * half) : -1;
+    // in place of z: kProb: P; else, kept as 16 bits, the distance below the group's largest in steps
+    if constexpr (kWhat == kProb) {
+      const float2 of_row = there ? a.row[row] : make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = exp_for<T>(z[j][r] - of_row.x) * of_row.y;
+          z[j][r] = (c == 32 * j + 8 * (r >> 2) + (r & 3) ? p - 1.0f : p) * PScale<T>::up;
+        }
+    } else {
+      const bool mine = c >= 0 && c < S::kFN * 32 && (c & 7) < 4;
+      if (__any(mine)) {
+        float zy = 0.0f;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) zy = c == 32 * j + 8 * (r >> 2) + (r & 3) ? z[j][r] : zy;
+        if (mine) a.z_label[row] = zy;
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, z[j][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if constexpr (sizeof(T) == 4) {
+            sum += expf(z[j][r] - base);
+          } else {
+            const float below = z[j][r] - base;      // first: z and base may be the type's lowest
+            sum += exp_for<T>(below);
+            z[j][r] = __builtin_fmaf(below, -kLog2e * Kept<T>::kSteps, 0.5f);
+          }
+        }
+      sum += __shfl_xor(sum, 32, 64);
+      const int group = (a.v0 + n0 + wn) / (S::kFN * 32);
+      if (there && half == 0) a.stats[group * a.ld_stats + row] = make_float2(top, sum);
+    }
+    if constexpr (kWhat != kStats) {
+      if constexpr (sizeof(T) == 4) {
+        float* to = (float*)a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (there && 32 * j + 8 * q < room)
+              *(f32x4*)(to + 32 * j + 8 * q) =
+                  f32x4{z[j][4 * q], z[j][4 * q + 1], z[j][4 * q + 2], z[j][4 * q + 3]};
+      } else {
+        // eight neighbouring columns a lane: the lower half of the wave takes the even groups of eight
+        unsigned short* to = (unsigned short*)a.p + (long long)row * a.ldp + n0 + wn + 8 * half;
+        const int space = a.ldp - n0 - wn - 8 * half;
+#pragma unroll
+        for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            unsigned long long half_group[2];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              unsigned w[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float lo = z[j][4 * (q + g) + 2 * k], hi = z[j][4 * (q + g) + 2 * k + 1];
+                if constexpr (kWhat == kProb) {
+                  const T x = TypeOf<T>::from_float(lo), y = TypeOf<T>::from_float(hi);
+                  w[k] = (unsigned)__builtin_bit_cast(unsigned short, x) |
+                         (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
+                } else {
+                  w[k] = (unsigned)fminf(lo, 65535.0f) | (unsigned)fminf(hi, 65535.0f) << 16;
+                }
+              }
+              half_group[g] = (unsigned long long)w[1] << 32 | w[0];
+            }
+            const u32x4 eight = whole_group(half_group[0], half_group[1]);
+            if (there && 32 * j + 8 * q < space) *(u32x4*)(to + 32 * j + 8 * q) = eight;
+          }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);      // one fragment row's registers at a time
+  }
+}
 
 template <typename T, typename S, What kWhat>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_kernel(const LogitArgs<T> a) {
@@ -256,117 +377,13 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
   Tile<T, kRows, kRows, S> tile;
   tile.run(a.x + m0 * a.ldx, a.ldx, ((long long)rows - m0) * a.ldx * (int)sizeof(T),
            a.w + n0 * a.ldw, a.ldw, a.w_bytes - (long long)n0 * a.ldw * (int)sizeof(T), a.steps, lds, a.w_limit);
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
-  const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32;
-  const int left = a.v - n0 - wn - 4 * half;      // this lane's columns (32 j + 8 q + r) below it exist
-  const int room = a.ldp - n0 - wn - 4 * half;    // and those below it are stored
-  float bias[S::kFN][16];      // what a column's logits get; -inf where there is no class
-#pragma unroll
-  for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) bias[j][r] = 32 * j + 8 * (r >> 2) + (r & 3) < left ? 0.0f : -__builtin_inff();
-  if (a.bias) {
-#pragma unroll
-    for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int c = min(32 * j + 8 * (r >> 2) + (r & 3), left - 1);       // past the last class: any
-        bias[j][r] += TypeOf<T>::to_float(a.bias[max(a.v0 + n0 + wn + 4 * half + c, 0)]);
-      }
-  }
-  if constexpr (kWhat != kProb) {
-    RH_LDS float* tops = (RH_LDS float*)lds;       // [kWN][kBM]
-    RH_LDS float* sums = tops + S::kWN * S::kBM;   // [kWN][kBM]
-#pragma unroll
-    for (int i = 0; i < S::kFM; ++i) {
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, tile.acc[i][j][r] + bias[j][r]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (half == 0) tops[(wave % S::kWN) * S::kBM + wm + 32 * i + lane] = top;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < S::kFM; ++i) {
-      const int m = wm + 32 * i + (lane & 31), row = m0 + m;
-      float top = tops[m];
-#pragma unroll
-      for (int k = 1; k < S::kWN; ++k) top = fmaxf(top, tops[k * S::kBM + m]);
-      const float base = top == -__builtin_inff() ? 0.0f : top;
-      typename Kept<T>::type* out = (typename Kept<T>::type*)a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          Vec4<typename Kept<T>::type> kept;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float z = tile.acc[i][j][4 * q + r] + bias[j][4 * q + r];
-            sum += exp_for<T>(z - base);
-            if constexpr (sizeof(T) == 4) {
-              kept.v[r] = z;
-            } else {
-              const float steps = __builtin_fmaf(base - z, (float)(1 << Kept<T>::kBits), 0.5f);
-              kept.v[r] = (unsigned short)(unsigned)fminf(steps, 65535.0f);
-            }
-          }
-          if (kWhat == kKeep && row < rows && 32 * j + 8 * q < room)
-            *(Vec4<typename Kept<T>::type>*)(out + 32 * j + 8 * q) = kept;
-        }
-      sum += __shfl_xor(sum, 32, 64);
-      if (half == 0) sums[(wave % S::kWN) * S::kBM + m] = sum;
-      const int c = row < rows ? a.label[row] - (a.v0 + n0 + wn + 4 * half) : -1;
-      const bool mine = c >= 0 && c < S::kFN * 32 && (c & 7) < 4;
-      if (__any(mine)) {
-        float z = 0.0f;
-#pragma unroll
-        for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) z = c == 32 * j + 8 * (r >> 2) + (r & 3) ? tile.acc[i][j][r] + bias[j][r] : z;
-        if (mine) a.z_label[row] = z;
-      }
-      __builtin_amdgcn_sched_barrier(0);      // one fragment row's registers at a time
-    }
-    __syncthreads();
-    for (int m = t; m < S::kBM && m0 + m < rows; m += S::kThreads) {
-      float top = tops[m], sum = sums[m];
-#pragma unroll
-      for (int k = 1; k < S::kWN; ++k) {
-        top = fmaxf(top, tops[k * S::kBM + m]);
-        sum += sums[k * S::kBM + m];
-      }
-      a.stats[(long long)(a.v0 / S::kBN + at.y) * a.ld_stats + m0 + m] = make_float2(top, sum);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < S::kFM; ++i) {
-      const int row = m0 + wm + 32 * i + (lane & 31);
-      if (row < rows) {
-        const float2 of_row = a.row[row];
-        const int c = a.label[row] - (a.v0 + n0 + wn + 4 * half);
-        T* out = (T*)a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
-#pragma unroll
-        for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int at0 = 32 * j + 8 * q;
-            Vec4<T> v;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float p = exp_for<T>((tile.acc[i][j][4 * q + r] + bias[j][4 * q + r]) - of_row.x) * of_row.y;
-              v.v[r] = TypeOf<T>::from_float((c == at0 + r ? p - 1.0f : p) * PScale<T>::up);
-            }
-            if (at0 < room) *(Vec4<T>*)(out + at0) = v;
-          }
-      }
-    }
-  }
+  if (!a.bias && n0 + S::kBN <= a.v)
+    finish_logits<T, S, kWhat, true>(a, tile, m0, n0, rows);
+  else
+    finish_logits<T, S, kWhat, false>(a, tile, m0, n0, rows);
 }
 
-// P from the kept logits, in their place: p = e^(z - tile's top) * (e^(tile's top - row's top) / row's
+// P from the kept logits, in their place: p = e^(z - group's top) * (e^(group's top - row's top) / row's
 // sum), the first factor from the code.  A workgroup takes kRows rows of 16 bytes of columns a thread;
 // column_sums (or NULL): [row block][v] sums of P over its rows.
 template <typename T>
@@ -375,13 +392,13 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept
                                                          const int* __restrict__ label,
                                                          const float2* __restrict__ row_stats,
                                                          const float2* __restrict__ stats, const long long ld_stats,
-                                                         const int tile, const int per,
+                                                         const int group, const int per,
                                                          float* __restrict__ column_sums) {
   constexpr int kV = 16 / (int)sizeof(T);
   const int rows = chunk.rows(n_valid), lo = blockIdx.y * per, hi = min(rows, lo + per);
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kV;
   if (c >= ldp) return;
-  const float2* top = stats + (long long)(c / tile) * ld_stats;
+  const float2* top = stats + (long long)(c / group) * ld_stats;
   float sums[kV];
 #pragma unroll
   for (int k = 0; k < kV; ++k) sums[k] = 0.0f;
@@ -402,7 +419,7 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
         const unsigned w = z[k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
-        const float e = __builtin_amdgcn_exp2f((float)code * (-kLog2e / (1 << Kept<T>::kBits)));
+        const float e = __builtin_amdgcn_exp2f((float)code * (-1.0f / Kept<T>::kSteps));
         p[k] = (code == 0xffffu ? 0.0f : e) * f;
       }
     }
@@ -507,7 +524,8 @@ struct ProductArgs {
   int add;                     // part += instead of part =
 };
 
-enum To { kParts, kQuads, kSingly };     // float parts; the result, rows of whole groups of four values or not
+// float parts; the result, in rows of whole groups of eight 16-bit values, of four of either size, or not
+enum To { kParts, kOctets, kQuads, kSingly };
 
 template <typename T, Layout kLA, Layout kLB, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
@@ -558,6 +576,7 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
             }
       } else {
         T* out = a.out + (a.map ? a.map[row] : row) * a.ldo + n0 + wn;
+        [[maybe_unused]] unsigned long long half_group[2];
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
@@ -568,6 +587,13 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
             T* to = out + 32 * j + 8 * q;
             if constexpr (kTo == kQuads) {
               if (32 * j + 8 * q < room) *(Vec4<T>*)to = v;
+            } else if constexpr (kTo == kOctets) {
+              half_group[q & 1] = __builtin_bit_cast(unsigned long long, v);
+              if (q & 1) {      // eight neighbouring columns a lane
+                const u32x4 eight = whole_group(half_group[0], half_group[1]);
+                const int c = 32 * j + 8 * (q - 1) + 4 * (lane >> 5);      // from this lane's first column
+                if (c < room) *(u32x4*)(out + c) = eight;
+              }
             } else {
 #pragma unroll
               for (int r = 0; r < 4; ++r)
@@ -671,10 +697,10 @@ struct Plan {
   int chunk, chunks;            // rows at a time
   int piece, pieces, ldp;       // classes of P at a time
   bool large_logits, large_dx, large_dw;
-  int bn;                       // classes a tile of the logits takes
+  int group;                    // classes a wave of the logits' tiles takes
   int dx_splits, dx_steps, dw_splits, dw_steps;
   long long ldpart;
-  int tiles_v;
+  int groups;
 };
 
 // Tiles of 256 x 256 move half the bytes per product of those of 128 x 128, which fill the card
@@ -728,8 +754,8 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   }
   p.ldp = ceil_div(p.piece, 64) * 64;
   p.large_logits = take_large(p.chunk, p.piece);
-  p.bn = p.large_logits ? 256 : 128;
-  p.tiles_v = ceil_div(v, p.bn);
+  p.group = p.large_logits ? Large::kFN * 32 : Small::kFN * 32;
+  p.groups = ceil_div(v, p.large_logits ? Large::kBN : Small::kBN) * (p.large_logits ? Large::kWN : Small::kWN);
   p.large_dx = take_large(p.chunk, d);
   p.large_dw = take_large(p.piece, d);
   const int k_dx = ceil_div(p.ldp, p.step_k), k_dw = ceil_div(p.chunk, p.step_k);
@@ -768,7 +794,7 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   s.info.scale = c.take<float>(1);
   s.x = c.take<char>((size_t)n * p.ldx * p.size);
   if (p.ldw_pad) s.w = c.take<char>((size_t)v * p.ldw_pad * p.size);
-  s.stats = c.take<float2>((size_t)p.tiles_v * p.chunk);
+  s.stats = c.take<float2>((size_t)p.groups * p.chunk);
   s.z_label = c.take<float>(n);
   s.row_stats = c.take<float2>(n);
   s.loss = c.take<double>(ceil_div(n, 32));
@@ -804,9 +830,10 @@ static int launch_logits(LogitArgs<T> a, hipStream_t stream) {
 template <typename T, Layout kLA, typename S>
 static int launch_product(ProductArgs<T> a, int splits, hipStream_t stream) {
   a.grid = Grid{ceil_div(a.m, S::kBM), ceil_div(a.n, S::kBN)};
-  auto kernel = a.part         ? product_kernel<T, kLA, kCols, S, kParts>
-                : a.n % 4 == 0 ? product_kernel<T, kLA, kCols, S, kQuads>
-                               : product_kernel<T, kLA, kCols, S, kSingly>;
+  constexpr To kWide = sizeof(T) == 2 ? kOctets : kQuads;
+  auto kernel = a.part                                   ? product_kernel<T, kLA, kCols, S, kParts>
+                : a.n % (sizeof(T) == 2 ? 8 : 4) == 0    ? product_kernel<T, kLA, kCols, S, kWide>
+                                                         : product_kernel<T, kLA, kCols, S, kSingly>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n, splits), dim3(S::kThreads), S::kLdsBytes, stream, a);
   RH_CHECK_LAUNCH("product_kernel");
@@ -943,7 +970,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
                                          : launch_logits<T, Small, kStats>(a, stream))
       return rc;
     hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, 32)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
-                       p.tiles_v, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,
+                       p.groups, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,
                        s.loss + first / 32);
     RH_CHECK_LAUNCH("join_stats_kernel");
     if (c == p.chunks - 1) {
@@ -955,7 +982,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
       const int per_chunk = ceil_div(p.chunk, kProbRows);
       const dim3 grid(ceil_div(p.ldp, kThreads * (16 / p.size)), per_chunk);      // column sums: every part is written
       hipLaunchKernelGGL(probs_kernel<T>, grid, dim3(kThreads), 0, stream, s.p, p.ldp, v, a.chunk, s.info.n_valid, a.label,
-                         a.row, s.stats, a.ld_stats, p.bn, kProbRows,
+                         a.row, s.stats, a.ld_stats, p.group, kProbRows,
                          s.db_part ? s.db_part + (long long)c * per_chunk * v : nullptr);
       RH_CHECK_LAUNCH("probs_kernel");
       if (q.dx)

@@ -67,6 +67,15 @@ struct TypeOf<_Float16> {
   static __device__ __forceinline__ _Float16 from_float(float v) { return (_Float16)v; }
 };
 
+// A lane of the lower half of the wave has four values of each of two groups of eight, x of the first
+// and y of the second (as 8 bytes), its partner 32 lanes on the other four: afterwards the lower lane
+// has the first group whole, the upper one the second.
+__device__ __forceinline__ u32x4 whole_group(const unsigned long long x, const unsigned long long y) {
+  const auto lo = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)y, false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap((unsigned)(x >> 32), (unsigned)(y >> 32), false, false);
+  return u32x4{lo[0], hi[0], lo[1], hi[1]};
+}
+
 template <typename T>
 struct Vec4 {
   T v[4];

@@ -9,26 +9,11 @@
 // Rows whose label is ignore_index, or outside [0, V), take no part: the features of the others are
 // laid out one after the other in a scratch copy first (its rows padded to whole tile steps), so
 // what stands in a row left out never meets a product, not even as 0 * inf, and costs nothing.
-#include "rh_gemm.h"
+#include "rh_ce.h"
 
 namespace rh {
 namespace ce {
 
-using namespace gemm;
-
-constexpr int kThreads = 256;
-constexpr float kLog2e = 1.4426950408889634f;
-
-// exp as the loss needs it: for float results the accurate one; for 16-bit ones the hardware exp2 of a
-// rounded product (|x| * 6e-8 relative, far below the 2^-9 of the type the result is rounded to).
-template <typename T>
-__device__ __forceinline__ float exp_for(const float x) {
-  return __builtin_amdgcn_exp2f(x * kLog2e);
-}
-template <>
-__device__ __forceinline__ float exp_for<float>(const float x) {
-  return expf(x);
-}
 
 // P is the matrix units' operand and so is rounded to the inputs' type.  float16 has no room for
 // small probabilities (2^-24 is its smallest value, one of 131 072 equal classes has 2^-17): there P
@@ -45,17 +30,6 @@ struct PScale<_Float16> {
 // ---------------------------------------------------------------------------------------------
 // Labels, rows
 // ---------------------------------------------------------------------------------------------
-struct Labels {
-  const void* p;
-  int wide;             // int64, else int32
-  long long ignore;
-  int v;
-  __device__ __forceinline__ long long at(const long long i) const {
-    return wide ? ((const long long*)p)[i] : (long long)((const int*)p)[i];
-  }
-  __device__ __forceinline__ bool counts(const long long y) const { return y != ignore && y >= 0 && y < v; }
-};
-
 // Per block of `per` rows: how many count, and whether a label lies outside [0, V).
 __global__ __launch_bounds__(64) void count_rows_kernel(const Labels y, const int n, const int per,
                                                        int2* __restrict__ blocks) {
@@ -682,8 +656,6 @@ constexpr int kColumnSplits = 32;
 constexpr int kProbRows = 64;
 constexpr int kKeepFrom = 512;                      // features
 
-static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
-
 // The call's work is cut so that no more than a bounded piece of the logits exists at a time:
 //   keep    all classes of `chunk` rows: logits once (6 n d v operations in all), P made in their
 //           place; with more than one chunk the weight's gradient is added up in float32.
@@ -1029,6 +1001,7 @@ extern "C" {
 
 size_t rh_linear_ce_workspace_bytes(int64_t n, int32_t d, int64_t v, int32_t dtype, int32_t flags) {
   if (rh::ce::check_sizes(n, d, v, dtype) != RH_OK) return 0;
+  if (n <= rh::ce::kFewRows) return rh::ce::few_workspace_bytes((int)n, d, (int)v, dtype, flags);
   const rh::ce::Plan p = rh::ce::make_plan((int)n, d, (int)v, dtype, flags);
   return rh::ce::carve(nullptr, p, (int)n, d, (int)v, flags).bytes;
 }
@@ -1050,6 +1023,13 @@ int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream) {
                  (rh::aligned16(q.w) && q.d * size % 16 == 0 && q.ldw * size % 16 == 0 && q.ldw < (1 << 20)),
              RH_EALIGN, "weights whose rows are not whole 16-byte pieces need RH_CE_COPY_WEIGHT");
   RH_REQUIRE(((uintptr_t)q.dx | (uintptr_t)q.dw) % 16 == 0, RH_EALIGN, "gradients must be 16-byte aligned");
+  if (q.n <= rh::ce::kFewRows) {
+    const size_t need = rh::ce::few_workspace_bytes((int)q.n, q.d, (int)q.v, q.dtype, flags);
+    RH_REQUIRE(q.workspace && q.workspace_bytes >= need, RH_EWORKSPACE, "workspace of %zu bytes, %zu needed",
+               q.workspace_bytes, need);
+    RH_REQUIRE((uintptr_t)q.workspace % 256 == 0, RH_EALIGN, "workspace must be 256-byte aligned");
+    return rh::ce::run_few(q, flags, (hipStream_t)stream);
+  }
   const rh::ce::Plan p = rh::ce::make_plan((int)q.n, q.d, (int)q.v, q.dtype, flags);
   const rh::ce::Space s = rh::ce::carve(q.workspace, p, (int)q.n, q.d, (int)q.v, flags);
   RH_REQUIRE(q.workspace && q.workspace_bytes >= s.bytes, RH_EWORKSPACE, "workspace of %zu bytes, %zu needed",

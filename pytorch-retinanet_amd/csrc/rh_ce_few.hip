@@ -1,0 +1,468 @@
+// The classifier loss for a few rows (gfx950).  With so few rows the weights' bytes are what counts:
+// they are read for the logits and again for the gradients, whose bytes are written.  Four launches:
+//
+//   logits      z[row][class] in float32, 16 classes x 16 rows to a matrix instruction that takes the
+//               weights straight from memory, and each workgroup's (max, sum of exp) of every row
+//   rows        the rows' (max, 1 / sum), losses and the call's loss
+//   gradients   one more pass over the weights: dW rows written, dX summed per workgroup; P stays float32
+//   features    the workgroups' parts of dX joined
+#include "rh_ce.h"
+
+namespace rh {
+namespace ce {
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+
+template <typename T>
+struct Mma16;      // 16 classes x 16 rows, 16 bytes of k a lane: lane % 16 is the class / row, lane / 16 the piece
+template <>
+struct Mma16<float> {
+  static __device__ __forceinline__ f32x4 run(const u32x4 a, const u32x4 b, f32x4 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[0], y[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[1], y[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[2], y[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], y[3], c, 0, 0, 0);
+    return c;
+  }
+};
+template <>
+struct Mma16<__bf16> {
+  static __device__ __forceinline__ f32x4 run(const u32x4 a, const u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                   0, 0, 0);
+  }
+};
+template <>
+struct Mma16<_Float16> {
+  static __device__ __forceinline__ f32x4 run(const u32x4 a, const u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                  0, 0);
+  }
+};
+
+// 16 bytes of values from p on, of which `have` exist (the others read as zero).
+template <typename T, bool kWide>
+__device__ __forceinline__ u32x4 load_values(const T* p, const int have) {
+  constexpr int kV = 16 / (int)sizeof(T);
+  if constexpr (kWide) {
+    return have >= kV ? *(const u32x4*)p : u32x4{0, 0, 0, 0};      // rows are whole pieces: all or none
+  } else {
+    union {
+      T v[kV];
+      u32x4 u;
+    } r;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) r.v[i] = i < have ? p[i] : (T)0.0f;
+    return r.u;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void to_floats(const u32x4 u, float (&f)[16 / sizeof(T)]) {
+  union {
+    u32x4 u;
+    T v[16 / sizeof(T)];
+  } r;
+  r.u = u;
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) f[i] = TypeOf<T>::to_float(r.v[i]);
+}
+
+struct FewSpace {
+  float* z;            // [n][ldz]
+  float2* part;        // [kFewRows][blocks]
+  float2* row;         // [kFewRows]  (max, 1 / sum), of a row that counts
+  float* scale;        // [1]
+  float* dx_part;      // [parts][n][ldpart]
+  size_t bytes;
+};
+
+struct FewPlan {
+  int groups, waves, blocks;        // logits: groups of 16 classes
+  int ldz;
+  int tpr, subsets, slices;         // gradients: threads a row of weights, rows side by side, column slices
+  int grad_blocks, per;             // classes a workgroup takes
+  int parts, ldpart;
+  bool wide_w;
+};
+
+static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
+  FewPlan p = {};
+  const int vals = dtype == RH_F32 ? 4 : 8;
+  p.groups = ceil_div(v, 16);
+  p.waves = p.groups < 2048 ? p.groups : 2048;
+  p.blocks = ceil_div(p.waves, 4);
+  p.ldz = ceil_div(v, 16) * 16;
+  p.tpr = 16;
+  while (p.tpr < kThreads && p.tpr * vals < d) p.tpr *= 2;
+  p.subsets = kThreads / p.tpr;
+  p.slices = ceil_div(d, p.tpr * vals);
+  int blocks = 512 / (p.slices < 512 ? p.slices : 512);
+  const int most = ceil_div(v, 4 * p.subsets);
+  if (blocks > most) blocks = most;
+  if (blocks < 1) blocks = 1;
+  p.per = ceil_div(ceil_div(v, blocks), p.subsets) * p.subsets;
+  p.grad_blocks = ceil_div(v, p.per);
+  p.parts = p.grad_blocks * p.subsets;
+  p.ldpart = p.slices * p.tpr * vals;
+  p.wide_w = !(flags & RH_CE_COPY_WEIGHT);      // here that only says how the weights are read
+  return p;
+}
+
+static FewSpace few_space(void* base, const FewPlan& p, int n, int flags) {
+  Carver c(base);
+  FewSpace s = {};
+  s.z = c.take<float>((size_t)n * p.ldz);
+  s.part = c.take<float2>((size_t)kFewRows * p.blocks);
+  s.row = c.take<float2>(kFewRows);
+  s.scale = c.take<float>(1);
+  if (flags & RH_CE_GRAD_X) s.dx_part = c.take<float>((size_t)p.parts * n * p.ldpart);
+  s.bytes = c.off;
+  return s;
+}
+
+size_t few_workspace_bytes(int n, int d, int v, int dtype, int flags) {
+  return few_space(nullptr, few_plan(n, d, v, dtype, flags), n, flags).bytes;
+}
+
+constexpr int kBatch = 8;                 // groups of classes a wave carries through the features
+constexpr int kChunkBytes = 4096;         // of a row of features in LDS at a time
+constexpr int kPitch = kChunkBytes + 16;  // rows a bank group apart
+constexpr int kAhead = 8;                 // loads of weights in flight a lane
+
+template <typename T, bool kWide>
+__global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restrict__ x, const long long ldx, const int n,
+                                                              const int d, const T* __restrict__ w, const long long ldw,
+                                                              const int v, const T* __restrict__ bias,
+                                                              const int groups, const int waves,
+                                                              float* __restrict__ z, const int ldz,
+                                                              float2* __restrict__ part) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float2 s_part[4][16];
+  constexpr int kV = 16 / (int)sizeof(T), kStepK = 4 * kV, kChunk = kChunkBytes / (int)sizeof(T);
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15, piece = lane >> 4;
+  const int me = blockIdx.x * 4 + wave;
+  float top = -__builtin_inff(), sum = 0.0f;      // of row `in`, over this lane's classes
+  for (int g0 = 0; g0 * waves < groups; g0 += kBatch) {
+    f32x4 acc[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int mine = me < waves ? min(kBatch, (groups - me + waves - 1) / waves - g0) : 0;
+    for (int k0 = 0; k0 < d; k0 += kChunk) {
+      const int len = min(kChunk, d - k0);
+      __syncthreads();
+      for (int i = t; i < 16 * (kChunkBytes / 16); i += kThreads) {
+        const int r = i / (kChunkBytes / 16), c = i % (kChunkBytes / 16) * kV;
+        if (c < (len + kAhead * kStepK - 1) / (kAhead * kStepK) * (kAhead * kStepK))      // zeros behind the row
+          *(u32x4*)(smem + r * kPitch + c * (int)sizeof(T)) =
+              r < n ? load_values<T, false>(x + r * ldx + k0 + c, len - c) : u32x4{0, 0, 0, 0};
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (i < mine) {
+          const int c = (me + (g0 + i) * waves) * 16 + in;
+          const T* row = w + (long long)min(c, v - 1) * ldw + k0 + piece * kV;
+          const char* xs = smem + in * kPitch + piece * 16;
+#pragma unroll 1
+          for (int k = 0; k < len; k += kAhead * kStepK) {
+            u32x4 a[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+              a[u] = load_values<T, kWide>(row + k + u * kStepK, len - k - u * kStepK - piece * kV);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+              acc[i] = Mma16<T>::run(a[u], *(const u32x4*)(xs + (k + u * kStepK) * (int)sizeof(T)), acc[i]);
+          }
+        }
+      }
+    }
+    // acc: row `in`, classes 4 * piece + r of the group
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i < mine) {
+      const int c = (me + (g0 + i) * waves) * 16 + 4 * piece;
+      f32x4 out;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float b = bias && c + r < v ? TypeOf<T>::to_float(bias[c + r]) : 0.0f;
+        out[r] = c + r < v ? acc[i][r] + b : -__builtin_inff();
+        const float up = fmaxf(top, out[r]), base = up == -__builtin_inff() ? 0.0f : up;
+        sum = sum * expf(top - base) + expf(out[r] - base);
+        top = up;
+      }
+      if (in < n) *(f32x4*)(z + (long long)in * ldz + c) = out;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    const float other = __shfl_xor(top, o, 64), more = __shfl_xor(sum, o, 64);
+    const float up = fmaxf(top, other), base = up == -__builtin_inff() ? 0.0f : up;
+    sum = sum * expf(top - base) + more * expf(other - base);
+    top = up;
+  }
+  if (lane < 16) s_part[wave][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (t < 16) {
+    top = -__builtin_inff();
+    sum = 0.0f;
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, s_part[k][t].x);
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    for (int k = 0; k < 4; ++k) sum += s_part[k][t].y * expf(s_part[k][t].x - base);
+    part[t * gridDim.x + blockIdx.x] = make_float2(top, sum);
+  }
+}
+
+// One wave a row.
+__global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* __restrict__ part, const int blocks,
+                                                                 const Labels y, const int n,
+                                                                 const float* __restrict__ z, const int ldz,
+                                                                 const float* __restrict__ divisor, const int mean,
+                                                                 const float grad, float2* __restrict__ row,
+                                                                 float* __restrict__ scale,
+                                                                 float* __restrict__ row_loss,
+                                                                 float* __restrict__ small, int* __restrict__ status) {
+  __shared__ float s_loss[kFewRows];
+  __shared__ int s_keep[kFewRows], s_bad[kFewRows];
+  const int r = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float top = -__builtin_inff(), sum = 0.0f;
+  for (int i = lane; i < blocks; i += 64) {
+    const float2 p = part[r * blocks + i];
+    const float up = fmaxf(top, p.x), base = up == -__builtin_inff() ? 0.0f : up;
+    sum = sum * expf(top - base) + p.y * expf(p.x - base);
+    top = up;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float other = __shfl_xor(top, o, 64), more = __shfl_xor(sum, o, 64);
+    const float up = fmaxf(top, other), base = up == -__builtin_inff() ? 0.0f : up;
+    sum = sum * expf(top - base) + more * expf(other - base);
+    top = up;
+  }
+  if (lane == 0) {
+    const long long label = r < n ? y.at(r) : y.ignore;
+    const bool keep = r < n && y.counts(label);
+    float loss = 0.0f;
+    if (keep) {
+      loss = (top - z[(long long)r * ldz + label]) + logf(sum);
+      row[r] = make_float2(top, 1.0f / sum);
+    }
+    if (r < n) row_loss[r] = loss;
+    s_loss[r] = loss;
+    s_keep[r] = keep;
+    s_bad[r] = r < n && label != y.ignore && (label < 0 || label >= y.v);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double total = 0.0;
+    int count = 0, bad = 0;
+    for (int i = 0; i < n; ++i) {
+      total += (double)s_loss[i];
+      count += s_keep[i];
+      bad |= s_bad[i];
+    }
+    const float div = mean ? fmaxf(divisor ? *divisor : (float)count, 1.0f) : 1.0f;
+    *scale = grad / div;
+    small[0] = (float)(total * (double)(1.0f / div));
+    small[1] = (float)count;
+    small[2] = 1.0f / div;
+    *status = bad ? RH_STATUS_LABEL_RANGE : 0;
+  }
+}
+
+// A thread has 16 bytes of columns; kN rows of features beside them in registers.  The workgroup's
+// classes are taken `subsets` at a time, a class by tpr threads.
+template <typename T, int kN, bool kWide>
+__global__ __launch_bounds__(kThreads) void few_gradients_kernel(
+    const T* __restrict__ x, const long long ldx, const int n, const int d, const T* __restrict__ w,
+    const long long ldw, const int v, const Labels y, const float* __restrict__ z, const int ldz,
+    const float2* __restrict__ row, const float* __restrict__ scale, const int per, const int tpr,
+    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ dx_part, const int ldpart) {
+  constexpr int kV = 16 / (int)sizeof(T);
+  constexpr int kAtOnce = 128;      // classes whose probabilities wait in LDS
+  __shared__ float s_p[kAtOnce][kN];
+  __shared__ float2 s_row[kN];
+  __shared__ int s_label[kN];
+  const int t = threadIdx.x, subsets = kThreads / tpr, subset = t / tpr;
+  const int c = (blockIdx.y * tpr + t % tpr) * kV;
+  const float s = *scale;
+  if (t < kN) {
+    const long long label = t < n ? y.at(t) : y.ignore;
+    s_label[t] = t < n && y.counts(label) ? (int)label : -1;
+    s_row[t] = s_label[t] >= 0 ? row[t] : make_float2(0.0f, 0.0f);
+  }
+  __syncthreads();
+  // 16 rows beside 16 sums of eight columns each leave no room for the rows as floats
+  constexpr bool kPacked = kN * kV > 64;
+  constexpr int kAtATime = kN <= 2 ? 4 : kN <= 8 ? 2 : 1;      // rows of weights in flight a thread
+  [[maybe_unused]] float xs[kPacked ? 1 : kN][kV];
+  [[maybe_unused]] u32x4 xp[kPacked ? kN : 1];
+  float acc[kN][kV];
+#pragma unroll
+  for (int r = 0; r < kN; ++r) {
+    // what a row left out holds must not meet its zeros
+    const u32x4 u = s_label[r] >= 0 ? load_values<T, false>(x + r * ldx + c, d - c) : u32x4{0, 0, 0, 0};
+    if constexpr (kPacked) xp[r] = u;
+    else to_floats<T>(u, xs[r]);
+#pragma unroll
+    for (int k = 0; k < kV; ++k) acc[r][k] = 0.0f;
+  }
+  const int lo = blockIdx.x * per, hi = min(v, lo + per);
+  for (int v0 = lo; v0 < hi; v0 += kAtOnce) {
+    const int count = min(kAtOnce, hi - v0);
+    __syncthreads();
+    for (int i = t; i < count * kN; i += kThreads) {
+      const int r = i / count, a = i - r * count;
+      float p = 0.0f;
+      if (s_label[r] >= 0) {
+        p = expf(z[(long long)r * ldz + v0 + a] - s_row[r].x) * s_row[r].y;
+        p = (s_label[r] == v0 + a ? p - 1.0f : p) * s;
+      }
+      s_p[a][r] = p;
+    }
+    __syncthreads();
+    if (db && blockIdx.y == 0)
+      for (int a = t; a < count; a += kThreads) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kN; ++r) sum += s_p[a][r];
+        db[v0 + a] = TypeOf<T>::from_float(sum);
+      }
+    if (c >= d) continue;
+#pragma unroll 1
+    for (int a0 = subset; a0 < count; a0 += kAtATime * subsets) {
+      u32x4 ws[kAtATime];
+      if (dx_part) {
+#pragma unroll
+        for (int u = 0; u < kAtATime; ++u) {
+          const int a = min(a0 + u * subsets, count - 1);
+          ws[u] = load_values<T, kWide>(w + (long long)(v0 + a) * ldw + c, d - c);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAtATime; ++u) {
+        const int a = a0 + u * subsets;
+        if (a >= count) continue;
+        float f[kV], g[kV];
+        if (dx_part) to_floats<T>(ws[u], f);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) g[k] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kN; ++r) {
+          const float p = s_p[a][r];
+          if (dx_part)
+#pragma unroll
+            for (int k = 0; k < kV; ++k) acc[r][k] = __builtin_fmaf(p, f[k], acc[r][k]);
+          if (dw) {
+            float xr[kV];
+            if constexpr (kPacked) {
+              to_floats<T>(xp[r], xr);
+            } else {
+#pragma unroll
+              for (int k = 0; k < kV; ++k) xr[k] = xs[r][k];
+            }
+#pragma unroll
+            for (int k = 0; k < kV; ++k) g[k] = __builtin_fmaf(p, xr[k], g[k]);
+          }
+        }
+        if (dw) {
+          union {
+            T v[kV];
+            u32x4 u;
+          } out;
+#pragma unroll
+          for (int k = 0; k < kV; ++k) out.v[k] = TypeOf<T>::from_float(g[k]);
+          T* to = dw + (long long)(v0 + a) * d + c;
+          if (d % kV == 0) {
+            *(u32x4*)to = out.u;
+          } else {
+#pragma unroll
+            for (int k = 0; k < kV; ++k)
+              if (c + k < d) to[k] = out.v[k];
+          }
+        }
+      }
+    }
+  }
+  if (dx_part && c < ldpart) {
+#pragma unroll
+    for (int r = 0; r < kN; ++r) {
+      if (r < n) {
+      float* to = dx_part + ((long long)(blockIdx.x * subsets + subset) * n + r) * ldpart + c;
+#pragma unroll
+      for (int k = 0; k < kV; k += 4) *(f32x4*)(to + k) = f32x4{acc[r][k], acc[r][k + 1], acc[r][k + 2], acc[r][k + 3]};
+      }
+    }
+  }
+}
+
+// Four columns of a row by 16 threads, each every 16th part.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __restrict__ part, const int parts,
+                                                                const int n, const int ldpart, const int d,
+                                                                T* __restrict__ dx) {
+  __shared__ f32x4 s_sum[16][16];
+  const int quad = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int c = (blockIdx.x * 16 + quad) * 4, r = blockIdx.y;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < ldpart) {
+#pragma unroll 4
+    for (int i = slice; i < parts; i += 16) sum += *(const f32x4*)(part + ((long long)i * n + r) * ldpart + c);
+  }
+  s_sum[slice][quad] = sum;
+  __syncthreads();
+  if (slice == 0 && c < d) {
+    for (int k = 1; k < 16; ++k) sum += s_sum[k][quad];
+    for (int k = 0; k < 4 && c + k < d; ++k) dx[(long long)r * d + c + k] = TypeOf<T>::from_float(sum[k]);
+  }
+}
+
+template <typename T, int kN>
+static int launch_gradients(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
+                            hipStream_t stream) {
+  auto kernel = p.wide_w ? few_gradients_kernel<T, kN, true> : few_gradients_kernel<T, kN, false>;
+  hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
+                     (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per, p.tpr,
+                     (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart);
+  RH_CHECK_LAUNCH("few_gradients_kernel");
+  return RH_OK;
+}
+
+template <typename T>
+static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) {
+  const int n = (int)q.n, v = (int)q.v;
+  const FewPlan p = few_plan(n, q.d, v, q.dtype, flags);
+  const FewSpace s = few_space(q.workspace, p, n, flags);
+  const Labels y{q.labels, q.labels_int64, q.ignore_index, v};
+  auto logits = p.wide_w ? few_logits_kernel<T, true> : few_logits_kernel<T, false>;
+  hipLaunchKernelGGL(logits, dim3(p.blocks), dim3(kThreads), 16 * kPitch, stream, (const T*)q.x, (long long)q.ldx, n, q.d,
+                     (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, s.z, p.ldz, s.part);
+  RH_CHECK_LAUNCH("few_logits_kernel");
+  hipLaunchKernelGGL(few_rows_kernel, dim3(1), dim3(64 * kFewRows), 0, stream, s.part, p.blocks, y, n, s.z, p.ldz, q.divisor,
+                     q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3));
+  RH_CHECK_LAUNCH("few_rows_kernel");
+  if (!q.dx && !q.dw && !q.db) return RH_OK;
+  if (int rc = n <= 1   ? launch_gradients<T, 1>(q, p, s, y, stream)
+               : n <= 2 ? launch_gradients<T, 2>(q, p, s, y, stream)
+               : n <= 4 ? launch_gradients<T, 4>(q, p, s, y, stream)
+               : n <= 8 ? launch_gradients<T, 8>(q, p, s, y, stream)
+                        : launch_gradients<T, 16>(q, p, s, y, stream))
+    return rc;
+  if (q.dx) {
+    hipLaunchKernelGGL(few_features_kernel<T>, dim3(ceil_div(q.d, 64), n), dim3(kThreads), 0, stream, s.dx_part, p.parts, n,
+                       p.ldpart, q.d, (T*)q.dx);
+    RH_CHECK_LAUNCH("few_features_kernel");
+  }
+  return RH_OK;
+}
+
+int run_few(const rh_linear_ce_args& q, int flags, hipStream_t stream) {
+  if (q.dtype == RH_F32) return run_typed<float>(q, flags, stream);
+  if (q.dtype == RH_BF16) return run_typed<__bf16>(q, flags, stream);
+  return run_typed<_Float16>(q, flags, stream);
+}
+
+}  // namespace ce
+}  // namespace rh

@@ -139,6 +139,33 @@ def test_wide_features(rh, n, d, v, dtype, bias):
     check_all(rh, x, w, y, b)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("d,v", [(8, 17), (33, 200), (2048, 40), (2056, 3000), (5000, 130), (256, 40001)])
+def test_few_rows(rh, n, d, v, dtype):
+    x, w, y, b = make(n, d, v, dtype, True, ignored=0.25 if n > 4 else 0.0, seed=13)
+    check_all(rh, x, w, y, b)
+
+
+def test_few_rows_of_very_many_classes(rh):
+    """More classes than the waves take in one go, and a workspace row past 2^31 bytes of weights."""
+    x, w, y, b = make(3, 16, 300_001, "bf16", True, seed=14)
+    check_all(rh, x, w, y, b)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.randn(600_000, 2048, generator=g, device="cuda").mul_(0.03).bfloat16()      # 2.4 GB
+    x = torch.randn(2, 2048, generator=g, device="cuda").bfloat16()
+    y = torch.tensor([599_999, 3], device="cuda")
+    out = rh.functional.linear_cross_entropy(x, w, y, grads=(True, True, False))
+    z = torch.cat([x.double() @ w[i:i + 50_000].double().T for i in range(0, 600_000, 50_000)], 1)
+    row = torch.logsumexp(z, 1) - z.gather(1, y[:, None])[:, 0]
+    assert ((out["row_loss"].double() - row).abs() <= 4096 * E * row).all()
+    p = (z - torch.logsumexp(z, 1, keepdim=True)).exp()
+    p[torch.arange(2), y] -= 1.0
+    for c in (0, 3, 299_999, 599_999):
+        want = (p[:, c, None] * x.double()).sum(0) / 2
+        assert ((out["d_weight"][c].double() - want).abs() <= 2.0 ** -7 * want.abs() + 1e-9).all()
+
+
 def test_rows_in_chunks(rh):
     """More rows than logits may be kept of: the same sums as the two halves by themselves."""
     x, w, y, b = make(17001, 520, 70001, "bf16", True, seed=12)

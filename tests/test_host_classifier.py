@@ -61,7 +61,8 @@ def test_workspace_query():
     assert q(4, 0, 5, 0, 0) == 0 and "features" in _lib.last_error()
     assert q(4, 8, 0, 0, 0) == 0 and "classes" in _lib.last_error()
     assert q(4, 8, 5, 3, 0) == 0 and "element type" in _lib.last_error()
-    assert 0 < q(4, 8, 5, 0, 0) < q(4, 8, 5, 0, full) < q(4, 8, 5, 0, full | _lib.CE_COPY_WEIGHT)
+    assert 0 < q(400, 8, 500, 0, 0) < q(400, 8, 500, 0, full) < q(400, 8, 500, 0, full | _lib.CE_COPY_WEIGHT)
+    assert 0 < q(4, 8, 5, 0, 0) < q(4, 8, 5, 0, full)
     # the logits of this call would take 8 GiB in 16 bits
     assert q(1 << 15, 1024, 1 << 17, _lib.RH_BF16, full) < 3 << 30
 

@@ -17,13 +17,14 @@ namespace norm {
 
 constexpr int kThreads = 256;
 constexpr int kPieceBytes = 32768;
-constexpr int kMostTensors = 160;      // of one launch: its table takes 3.8 KiB of the 4 KiB of arguments
-constexpr int kMostBlocks = 2048;      // of one launch
+constexpr int kMostTensors = 240;      // of one launch: its table takes 3.8 KiB of the 4 KiB of arguments
+constexpr int kMostBlocks = 1024;      // of one launch
+constexpr long long kMostValues = 1ll << 29;      // of an entry: a larger tensor takes several
 
 struct Table {
   const char* p[kMostTensors];
-  long long n[kMostTensors];           // values * 4 + element type
-  int end[kMostTensors];               // pieces up to and with this tensor
+  unsigned n[kMostTensors];            // values * 4 + element type
+  int end[kMostTensors];               // pieces up to and with this entry
   int tensors;
   int pieces;
 };
@@ -182,10 +183,10 @@ __device__ __forceinline__ void each_piece(const Table& t, const F f) {
   for (int i = lo; i < hi; ++i) {
     while (t.end[a] <= i) ++a;
     const int first = i - (a ? t.end[a - 1] : 0);
-    const int type = (int)(t.n[a] & 3);
+    const int type = (int)(t.n[a] & 3u);
     Range r;
     r.begin = t.p[a];
-    r.end = r.begin + (t.n[a] >> 2) * (type == RH_F32 ? 4 : 2);
+    r.end = r.begin + (unsigned long long)(t.n[a] >> 2) * (type == RH_F32 ? 4 : 2);
     r.from = (const char*)((uintptr_t)r.begin & ~(uintptr_t)15) + (long long)first * kPieceBytes;
     f(type, r);
   }
@@ -235,12 +236,18 @@ __global__ __launch_bounds__(kThreads) void total_kernel(const double* __restric
   }
 }
 
+// partials: how many workgroups' sums `total` is still to be joined from (every workgroup does, in
+// the same order: it costs less than a launch); 0: it is there.
 template <int kKind>
-__global__ __launch_bounds__(kThreads) void clip_kernel(const Table t, const double* __restrict__ total,
+__global__ __launch_bounds__(kThreads) void clip_kernel(const Table t, const double* __restrict__ partial,
+                                                        const int partials, double* __restrict__ total,
                                                         const float max_norm, float* __restrict__ norm) {
-  const double s = *total;
+  const double s = partials ? total_of<kKind>(partial, partials) : *total;
   const float length = (float)(kKind == kSquares ? __builtin_sqrt(s) : s);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = length;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (partials) *total = s;
+    *norm = length;
+  }
   const float c = max_norm / (length + 1e-6f);
   if (c >= 1.0f) return;      // times one: nothing to write (a NaN goes on, and into every gradient)
   // from the list's end, which the norm's pass has read last and the caches still hold
@@ -273,27 +280,30 @@ static int each_table(const rh_tensor_ref* list, int count, const F f) {
   Table t;
   t.tensors = 0;
   long long pieces = 0;
-  for (int i = 0; i <= count; ++i) {
-    long long more = 0;
-    if (i < count) {
-      if (list[i].count == 0) continue;
-      more = pieces_of(list[i].data, list[i].count * (list[i].dtype == RH_F32 ? 4 : 2));
-    }
-    if (t.tensors && (i == count || t.tensors == kMostTensors || pieces + more > 0x7fffffffll)) {
-      t.pieces = (int)pieces;
-      if (int rc = f(t, blocks_for(pieces))) return rc;
-      t.tensors = 0;
-      pieces = 0;
-    }
-    if (i < count) {
+  auto flush = [&]() -> int {
+    if (!t.tensors) return RH_OK;
+    t.pieces = (int)pieces;
+    const int rc = f(t, blocks_for(pieces));
+    t.tensors = 0;
+    pieces = 0;
+    return rc;
+  };
+  for (int i = 0; i < count; ++i) {
+    const int size = list[i].dtype == RH_F32 ? 4 : 2;
+    for (long long at = 0; at < list[i].count; at += kMostValues) {
+      const long long n = list[i].count - at < kMostValues ? list[i].count - at : kMostValues;
+      const char* p = (const char*)list[i].data + at * size;
+      const long long more = pieces_of(p, n * size);
+      if (t.tensors == kMostTensors || pieces + more > 0x7fffffffll)
+        if (int rc = flush()) return rc;
       pieces += more;
-      t.p[t.tensors] = (const char*)list[i].data;
-      t.n[t.tensors] = list[i].count * 4 + list[i].dtype;
+      t.p[t.tensors] = p;
+      t.n[t.tensors] = (unsigned)(n * 4 + list[i].dtype);
       t.end[t.tensors] = (int)pieces;
       ++t.tensors;
     }
   }
-  return RH_OK;
+  return flush();
 }
 
 static int check_list(const rh_tensor_ref* list, int32_t count, bool written) {
@@ -332,26 +342,27 @@ static int check_list(const rh_tensor_ref* list, int32_t count, bool written) {
 template <int kKind>
 static int run(const rh_grad_clip_args& q, hipStream_t stream) {
   double* partial = (double*)q.workspace;
+  int blocks = 0;
   if (q.stages & RH_CLIP_NORM) {
-    int at = 0;
-    int rc = each_table(q.tensors, q.count, [&](const Table& t, int blocks) -> int {
-      hipLaunchKernelGGL(norm_kernel<kKind>, dim3(blocks), dim3(kThreads), 0, stream, t, partial + at);
+    int rc = each_table(q.tensors, q.count, [&](const Table& t, int b) -> int {
+      hipLaunchKernelGGL(norm_kernel<kKind>, dim3(b), dim3(kThreads), 0, stream, t, partial + blocks);
       RH_CHECK_LAUNCH("norm_kernel");
-      at += blocks;
+      blocks += b;
       return RH_OK;
     });
     if (rc) return rc;
-    hipLaunchKernelGGL(total_kernel<kKind>, dim3(1), dim3(kThreads), 0, stream, partial, at, q.total, q.norm);
+  }
+  if (!(q.stages & RH_CLIP_SCALE) || (blocks == 0 && (q.stages & RH_CLIP_NORM))) {
+    hipLaunchKernelGGL(total_kernel<kKind>, dim3(1), dim3(kThreads), 0, stream, partial, blocks, q.total, q.norm);
     RH_CHECK_LAUNCH("total_kernel");
+    return RH_OK;
   }
-  if (q.stages & RH_CLIP_SCALE) {
-    return each_table(q.tensors, q.count, [&](const Table& t, int blocks) -> int {
-      hipLaunchKernelGGL(clip_kernel<kKind>, dim3(blocks), dim3(kThreads), 0, stream, t, q.total, q.max_norm, q.norm);
-      RH_CHECK_LAUNCH("clip_kernel");
-      return RH_OK;
-    });
-  }
-  return RH_OK;
+  return each_table(q.tensors, q.count, [&](const Table& t, int b) -> int {
+    hipLaunchKernelGGL(clip_kernel<kKind>, dim3(b), dim3(kThreads), 0, stream, t, partial, blocks, q.total, q.max_norm,
+                       q.norm);
+    RH_CHECK_LAUNCH("clip_kernel");
+    return RH_OK;
+  });
 }
 
 }  // namespace norm

@@ -10,10 +10,9 @@ import threading
 from collections import OrderedDict
 from typing import Optional
 
-import numpy as np
 import torch
 
-from . import _lib
+from . import _host, _lib
 from ._lib import RetinaHeadError
 
 # Caches shared by every thread that calls into the package (nn.DataParallel drives its replicas
@@ -682,33 +681,14 @@ def scale_gradient_(grad, scale, assumed=1.0):
 
 
 # --------------------------------------------------------------------------- gradient norm
-_REF = np.dtype([("data", np.uint64), ("count", np.int64), ("dtype", np.int32), ("reserved", np.int32)])
-
-
-def _is_dense(t):
-    """Every address between a tensor's first and last value is one of its values, once."""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _tensor_refs(tensors):
-    """(device, table of the list as rh_tensor_ref)."""
-    refs = np.zeros(len(tensors), _REF)
-    if any(t.layout != torch.strided for t in tensors):
-        raise RetinaHeadError("gradients must be dense tensors, not sparse ones")
-    dev = _dev_check(*tensors)
-    if not all(map(_is_dense, tensors)):
-        raise RetinaHeadError("gradients must fill their memory: a strided or expanded view does not")
-    refs["data"] = [t.data_ptr() for t in tensors]
-    refs["count"] = [t.numel() for t in tensors]
-    refs["dtype"] = [_dtype_code(t) for t in tensors]
-    return dev, refs
+def _tensor_table(tensors, grads=False):
+    """(device, list as rh_tensor_ref in bytes) of the tensors, or of their gradients where they have
+    one; device None where there is nothing."""
+    table = _host.tensor_table(tensors, grads)
+    if isinstance(table, str):
+        raise RetinaHeadError(table)
+    index, refs = table
+    return (None if index < 0 else torch.device("cuda", index)), refs
 
 
 def _norm_code(norm_type):
@@ -718,32 +698,33 @@ def _norm_code(norm_type):
     return code
 
 
-def grad_clip(tensors, max_norm=None, norm_type=2.0, stages=_lib.CLIP_ALL, out=None):
+def grad_clip(tensors, max_norm=None, norm_type=2.0, stages=_lib.CLIP_ALL, out=None, grads=False):
     """The norm over every value of ``tensors`` (stage ``CLIP_NORM``) and their scaling in place by
-    min(1, max_norm / (norm + 1e-6)) (stage ``CLIP_SCALE``), without a host read.  Returns a dict of
-    device tensors: ``norm`` float32 [], ``total`` float64 [1] (what ranks sum, or for the infinity norm
-    maximise, between the two stages; pass the dict as ``out``)."""
+    min(1, max_norm / (norm + 1e-6)) (stage ``CLIP_SCALE``), without a host read; with ``grads`` of the
+    tensors' gradients, those without one left out.  Returns a dict of device tensors: ``norm`` float32 [],
+    ``total`` float64 [1] (what ranks sum, or for the infinity norm maximise, between the two stages;
+    pass the dict as ``out``), or None where there is no tensor."""
     code = _norm_code(norm_type)
     if stages & _lib.CLIP_SCALE and (max_norm is None or not float(max_norm) >= 0.0):
         raise ValueError("max_norm must be a number from 0 on")
-    dev, refs = _tensor_refs(tensors)
+    dev, refs = _tensor_table(tensors, grads)
     if dev is None:
-        raise RetinaHeadError("grad_clip needs at least one tensor")
+        return None
     if out is None:
         out = {"norm": torch.empty((), dtype=torch.float32, device=dev),
                "total": torch.empty((1,), dtype=torch.float64, device=dev)}
     lib = _lib.load()
+    at, count = C.cast(C.c_char_p(refs), C.c_void_p).value, len(refs) // C.sizeof(_lib.TensorRef)
     with _on_device(dev) as stream:
         ws, room = None, 0
         if stages & _lib.CLIP_NORM:
-            room = lib.rh_grad_clip_workspace_bytes(refs.ctypes.data, len(refs))
+            room = lib.rh_grad_clip_workspace_bytes(at, count)
             if room == 0:
                 raise RetinaHeadError("grad_clip: " + _lib.last_error())
             ws = workspace(dev, room, "grad_clip", stream)
-        args = _lib.GradClipArgs(refs.ctypes.data, len(refs), code, int(stages),
-                                 0.0 if max_norm is None else float(max_norm), out["total"].data_ptr(),
-                                 out["norm"].data_ptr(), None if ws is None else ws.data_ptr(),
-                                 0 if ws is None else ws.numel())
+        args = _lib.GradClipArgs(at, count, code, int(stages), 0.0 if max_norm is None else float(max_norm),
+                                 out["total"].data_ptr(), out["norm"].data_ptr(),
+                                 None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
         _lib.check(lib.rh_grad_clip(C.byref(args), stream), "rh_grad_clip")
     return out
 

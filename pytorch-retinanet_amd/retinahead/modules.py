@@ -550,10 +550,8 @@ def grad_norm(tensors, norm_type=2.0):
     tensor or an iterable; float32, bfloat16 and float16 may be mixed).  Values and squares are summed
     in float64.  An empty list has norm 0."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    F._norm_code(norm_type)
-    if not tensors:
-        return torch.tensor(0.0)
-    return F.grad_clip(tensors, norm_type=norm_type, stages=_lib.CLIP_NORM)["norm"]
+    out = F.grad_clip(tensors, norm_type=norm_type, stages=_lib.CLIP_NORM)
+    return torch.tensor(0.0) if out is None else out["norm"]
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -573,27 +571,26 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 
 def _clip(parameters, max_norm, norm_type, error_if_nonfinite, reduce_total):
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    grads = [g for g in [p.grad for p in parameters] if g is not None]
-    F._norm_code(norm_type)
     if not float(max_norm) >= 0.0:
         raise ValueError("max_norm must be a number from 0 on")
-    if not grads:
-        if reduce_total is None:
-            return torch.tensor(0.0)
-        total = reduce_total(torch.zeros(1, dtype=torch.float64,
-                                         device=parameters[0].device if parameters else "cpu"))
-        return (total.sqrt() if float(norm_type) == 2.0 else total).float().reshape(())
-    if reduce_total is None and not error_if_nonfinite:
-        return F.grad_clip(grads, max_norm, norm_type)["norm"]
-    out = F.grad_clip(grads, max_norm, norm_type, stages=_lib.CLIP_NORM)
-    norm = out["norm"]
+    in_one = reduce_total is None and not error_if_nonfinite
+    out = F.grad_clip(parameters, max_norm, norm_type, grads=True,
+                      stages=_lib.CLIP_ALL if in_one else _lib.CLIP_NORM)
+    if in_one:
+        return torch.tensor(0.0) if out is None else out["norm"]
+    if out is None:
+        total = torch.zeros(1, dtype=torch.float64, device=parameters[0].device if parameters else "cpu")
+    else:
+        total = out["total"]
     if reduce_total is not None:
-        reduce_total(out["total"])
-        norm = out["total"].sqrt() if float(norm_type) == 2.0 else out["total"]
+        reduce_total(total)
+    norm = total.sqrt() if float(norm_type) == 2.0 else total
     if error_if_nonfinite and not bool(torch.isfinite(norm)):
         raise RuntimeError(f"the norm of order {norm_type} of the gradients is not finite, so they "
                            "cannot be clipped")
-    return F.grad_clip(grads, max_norm, norm_type, stages=_lib.CLIP_SCALE, out=out)["norm"]
+    if out is None:
+        return norm.float().reshape(())
+    return F.grad_clip(parameters, max_norm, norm_type, grads=True, stages=_lib.CLIP_SCALE, out=out)["norm"]
 
 
 class Anchors(nn.Module):

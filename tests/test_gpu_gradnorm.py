@@ -246,3 +246,32 @@ def test_training_step_of_a_classifier(rh, dtype):
             pb -= pb.grad
         losses.append(float(loss))
     assert all(math.isfinite(v) for v in losses)
+
+
+def test_tensor_larger_than_an_entry_of_the_table(rh):
+    n = (1 << 30) + (1 << 29) + 12345
+    g = torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda")
+    g[-1] = 3.0
+    want = math.sqrt((n - 1) * 0.25 + 9.0)
+    got = rh.clip_grad_norm_(params_of([g]), 100.0)
+    assert abs(float(got) - want) <= 2.0 ** -23 * want
+    scaled = torch.tensor(0.5 * (100.0 / (want + 1e-6)), dtype=torch.float64)
+    assert (g[:-1] == g[0]).all() and abs(float(g[0]) - float(scaled)) <= 2.0 ** -8 * float(scaled)
+    assert abs(float(g[-1]) - 6.0 * float(scaled)) <= 2.0 ** -8 * 6.0 * float(scaled)
+
+
+def test_sharded_stages(rh):
+    """The two stages apart, with a sum over ranks put between them."""
+    F = rh.functional
+    from retinahead import _lib
+    a = [rand(1000, "f32", 40), rand(33, "bf16", 41)]
+    other = [rand(500, "f16", 42)]
+    both = norm64(a + other, 2.0)
+    out = F.grad_clip(a, stages=_lib.CLIP_NORM)
+    out["total"] += F.grad_clip(other, stages=_lib.CLIP_NORM)["total"]
+    before = [t.clone() for t in a]
+    F.grad_clip(a, 1.0, stages=_lib.CLIP_SCALE, out=out)
+    assert abs(float(out["norm"]) - both) <= 2.0 ** -23 * both
+    for t, b in zip(a, before):
+        exact = b.double() * (1.0 / (both + 1e-6))
+        assert ((t.double() - exact).abs() <= exact.abs() * (torch.finfo(t.dtype).eps / 2 + 2.0 ** -22)).all()

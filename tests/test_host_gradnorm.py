@@ -7,16 +7,6 @@ import torch
 
 import retinahead as rh
 from retinahead import _lib
-from retinahead import functional as F
-
-
-def test_dense_orders():
-    x = torch.zeros(2, 3, 5, 7)
-    for t in (x, x.permute(3, 0, 2, 1), x.to(memory_format=torch.channels_last), x[:, :, :1].contiguous(), x[0], x[:, None],
-              torch.zeros(()), torch.zeros(0, 4), torch.zeros(1, 4).t()):
-        assert F._is_dense(t), t.shape
-    for t in (x[:, ::2], x[:, :, 1:], x[..., 1:], torch.zeros(1).expand(4), torch.zeros(4, 4).as_strided((3, 3), (1, 1))):
-        assert not F._is_dense(t), t.stride()
 
 
 def test_refuses_host_tensors_and_values():
@@ -33,10 +23,18 @@ def test_refuses_host_tensors_and_values():
         rh.clip_grad_norm_([p], 1.0, norm_type=0.5)
     assert float(rh.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0)) == 0.0
     assert float(rh.grad_norm([])) == 0.0
+    with pytest.raises(rh.RetinaHeadError, match="list of tensors"):
+        rh.grad_norm([1.0])
+    with pytest.raises(TypeError):
+        rh.grad_norm(3)
+
+
+REF = np.dtype([("data", np.uint64), ("count", np.int64), ("dtype", np.int32), ("reserved", np.int32)])
 
 
 def _refs(*items):
-    a = np.zeros(len(items), F._REF)
+    assert REF.itemsize == C.sizeof(_lib.TensorRef)
+    a = np.zeros(len(items), REF)
     for i, it in enumerate(items):
         a[i] = tuple(it) + (0,)
     return a

@@ -429,8 +429,8 @@ enum rh_ce_flags {
                              element size or the address): the call works on a padded copy */
 };
 
-/* Softmax cross entropy of the logits x w^T + bias, with its gradients, in pieces of the classes: the
- * logits are never stored whole.  A row whose label is ignore_index takes no part (no loss, zero gradient,
+/* Softmax cross entropy of the logits x w^T + bias, with its gradients, in pieces: no more than 2 GiB of
+ * logits (or 256 rows of them) exist at a time.  A row whose label is ignore_index takes no part (no loss, zero gradient,
  * whatever its features hold); so does one with a label outside [0, v), which also sets
  * RH_STATUS_LABEL_RANGE.  A call without a counted row has loss 0 and zero gradients.
  * dx / dw / db (each may be NULL) hold the gradients times `grad`, for an upstream gradient of that size. */
@@ -459,7 +459,7 @@ typedef struct rh_linear_ce_args {
   size_t workspace_bytes;
 } rh_linear_ce_args;
 
-/* 0 for sizes out of range: n <= 2^26, d <= 2^17, v <= 2^24. */
+/* 0 for sizes out of range: n <= 2^26, d <= 2^17, v <= 2^21. */
 size_t rh_linear_ce_workspace_bytes(int64_t n, int32_t d, int64_t v, int32_t dtype, int32_t flags);
 int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream);
 

@@ -52,15 +52,23 @@ struct RowInfo {
   float* scale;    // [1] s * expected upstream gradient
 };
 
-// Copies the rows that count to their places, zero-padded to ldp values; sets what a row left out
-// gets: no loss, no gradient.
+// Where column `c` of the chunk's place `r` lies in an array of panels of `rows` rows (in elements).
+template <typename T>
+__device__ __forceinline__ long long in_panels(const int r, const int c, const long long rows) {
+  constexpr int kC = kStepBytes / (int)sizeof(T);
+  return ((long long)(c / kC) * rows + r) * kC + c % kC;
+}
+
+// Copies the rows that count to their places in the chunks' panels, padded with zeros to whole panels; sets
+// what a row left out gets: no loss, no gradient.  A workgroup takes `per` rows and every gridDim.y-th panel;
+// a wave 16 rows of a panel at a time, a kilobyte where they are neighbours.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void place_rows_kernel(
     const T* __restrict__ x, const long long ldx, const int d, const Labels y, const int n, const int per,
-    const int2* __restrict__ blocks, T* __restrict__ xp, const int ldp, const RowInfo info,
+    const int2* __restrict__ blocks, T* __restrict__ xp, const int panels, const int chunk, const RowInfo info,
     float* __restrict__ row_loss, T* __restrict__ dx, float* __restrict__ small, int* __restrict__ status,
     const float* __restrict__ total, const int mean, const float grad) {
-  __shared__ int s_red[4], s_bad[4];
+  __shared__ int s_red[4], s_all[4], s_bad[4];
   __shared__ int s_place[kThreads];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   int before = 0, all = 0, bad = 0;
@@ -75,26 +83,22 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
   bad = __any(bad);
   if (lane == 0) {
     s_red[wave] = before;
+    s_all[wave] = all;
     s_bad[wave] = bad;
   }
   __syncthreads();
   before = s_red[0] + s_red[1] + s_red[2] + s_red[3];
-  bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
-  __syncthreads();
-  if (blockIdx.x == 0) {
-    if (lane == 0) s_red[wave] = all;
-    __syncthreads();
-    if (t == 0) {
-      all = s_red[0] + s_red[1] + s_red[2] + s_red[3];
-      *info.n_valid = all;
-      const float div = mean ? fmaxf(total ? *total : (float)all, 1.0f) : 1.0f;
-      *info.scale = grad / div;
-      small[1] = (float)all;
-      small[2] = 1.0f / div;
-      *status = bad ? RH_STATUS_LABEL_RANGE : 0;
-    }
-    __syncthreads();
+  const bool first = blockIdx.y == 0;
+  if (first && blockIdx.x == 0 && t == 0) {
+    all = s_all[0] + s_all[1] + s_all[2] + s_all[3];
+    *info.n_valid = all;
+    const float div = mean ? fmaxf(total ? *total : (float)all, 1.0f) : 1.0f;
+    *info.scale = grad / div;
+    small[1] = (float)all;
+    small[2] = 1.0f / div;
+    *status = (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) ? RH_STATUS_LABEL_RANGE : 0;
   }
+  __syncthreads();
   // this block's rows: place within the block by a ballot count (per <= 256)
   const long long lo = (long long)blockIdx.x * per;
   const int rows = (int)min((long long)per, n - lo);
@@ -111,34 +115,45 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
   for (int i = 0; i < wave; ++i) at += s_red[i];
   if (t < rows) {
     s_place[t] = keep ? at : -1;
-    if (keep) {
-      info.map[at] = (int)(lo + t);
-      info.label[at] = (int)label;
-    } else {
-      row_loss[lo + t] = 0.0f;
+    if (first) {
+      if (keep) {
+        info.map[at] = (int)(lo + t);
+        info.label[at] = (int)label;
+      } else {
+        row_loss[lo + t] = 0.0f;
+      }
     }
   }
   __syncthreads();
   const bool wide = ((ldx * (long long)sizeof(T)) & 15) == 0 && ((uintptr_t)x & 15) == 0;
-  constexpr int kV = 16 / (int)sizeof(T);
-  for (int r = wave; r < rows; r += 4) {
-    const int to = s_place[r];
-    const T* src = x + (lo + r) * ldx;
-    if (to >= 0) {
-      T* dst = xp + (long long)to * ldp;
-      if (wide) {
-        int c = lane * kV;
-        for (; c + kV <= d; c += 64 * kV) *(u32x4*)(dst + c) = *(const u32x4*)(src + c);
-        for (; c < ldp; c += 64 * kV)
-          for (int k = 0; k < kV; ++k) dst[c + k] = c + k < d ? src[c + k] : (T)0.0f;
+  constexpr int kV = 16 / (int)sizeof(T), kC = kStepBytes / (int)sizeof(T);
+  for (int p = blockIdx.y + gridDim.y * wave; p < panels; p += gridDim.y * 4) {
+    const int c = p * kC + (lane & 3) * kV;
+#pragma unroll 2
+    for (int r = lane >> 2; r < rows; r += 16) {
+      const int to = s_place[r];
+      if (to < 0) continue;
+      const T* src = x + (lo + r) * ldx + c;
+      union {
+        T v[kV];
+        u32x4 u;
+      } w;
+      if (wide && c + kV <= d) {
+        w.u = *(const u32x4*)src;
       } else {
-        for (int c = lane; c < ldp; c += 64) dst[c] = c < d ? src[c] : (T)0.0f;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) w.v[k] = c + k < d ? src[k] : (T)0.0f;
       }
-    } else if (dx) {
-      T* dst = dx + (lo + r) * (long long)d;
-      for (int c = lane; c < d; c += 64) dst[c] = (T)0.0f;
+      const int in = to / chunk;
+      *(u32x4*)(xp + (long long)in * chunk * panels * kC + in_panels<T>(to - in * chunk, c, chunk)) = w.u;
     }
   }
+  if (dx && first)
+    for (int r = wave; r < rows; r += 4)
+      if (s_place[r] < 0) {
+        T* dst = dx + (lo + r) * (long long)d;
+        for (int c = lane; c < d; c += 64) dst[c] = (T)0.0f;
+      }
 }
 
 // A copy of the weights with rows of whole 16-byte pieces, for a row length or stride that has none.
@@ -164,6 +179,17 @@ __device__ __forceinline__ int2 tile_at(const Grid g, const int id) {
   const int t = xcd_run(id, g.m * g.n);
   const int span = 8 * g.n, first = t / span * 8, rows = min(8, g.m - first), in = t % span;
   return make_int2(first + in % rows, in / rows);
+}
+
+// The call's loss from the row blocks' sums, by one workgroup.
+__device__ __forceinline__ void add_losses(const double* __restrict__ parts, const int n, float* __restrict__ small) {
+  __shared__ double s_red[4];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) sum += parts[i];
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) small[0] = (float)(((s_red[0] + s_red[1]) + (s_red[2] + s_red[3])) * (double)small[2]);
 }
 
 // The rows of a call come in chunks: this chunk's are `first` on, at most `most` of them.
@@ -197,14 +223,15 @@ struct Kept<float> {
 
 template <typename T>
 struct LogitArgs {
-  const T* x;          // the chunk's placed rows, ldx apart, zero-padded
-  long long ldx;
+  const T* x;          // the chunk's placed rows, in panels of chunk_rows
+  long long x_bytes;
+  int chunk_rows;
   const T* w;          // first class of this call
   long long ldw, w_bytes;
   const T* bias;
   int steps;           // of k
   int w_limit;         // bytes of the last step that are the weights' rows
-  int v0, v;           // first class, how many
+  int v;
   Grid grid;
   Chunk chunk;
   const int* n_valid;
@@ -212,13 +239,13 @@ struct LogitArgs {
   float2* stats;       // [group of classes][place]  (max, sum of exp above it)
   long long ld_stats;
   float* z_label;      // [place]
-  const float2* row;   // [place]  (max, 1 / sum) over all classes
-  void* p;             // [place][ldp]  P, or the logits kept for it
+  void* p;             // the logits kept, in panels of chunk_rows, of ldp columns
   int ldp;
 };
 
-// kStats: the groups' (max, sum) only, a group being a wave's part of the tile's classes.  kKeep: and the logits.  kProb: P, from rows' sums known before.
-enum What { kStats, kKeep, kProb };
+// kStats: the groups' (max, sum) only, a group being a wave's part of the tile's classes.  kKeep: and the
+// logits.
+enum What { kStats, kKeep };
 
 // What becomes of a tile's logits.  kPlain: every class is there and none has a bias; else each column
 // gets something, minus infinity where there is no class.
@@ -236,7 +263,7 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int c = 32 * j + 8 * (r >> 2) + (r & 3), in = min(c, left - 1);       // past the last class: any
-        const float b = a.bias ? TypeOf<T>::to_float(a.bias[max(a.v0 + n0 + wn + 4 * half + in, 0)]) : 0.0f;
+        const float b = a.bias ? TypeOf<T>::to_float(a.bias[max(n0 + wn + 4 * half + in, 0)]) : 0.0f;
         bias[j][r] = c < left ? b : -__builtin_inff();
       }
   }
@@ -252,18 +279,9 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[j][r] += bias[j][r];
     }
-    const int c = there ? a.label[row] - (a.v0 + n0 + wn + 4 * half) : -1;
-    // in place of z: kProb: P; else, kept as 16 bits, the distance below the group's largest in steps
-    if constexpr (kWhat == kProb) {
-      const float2 of_row = there ? a.row[row] : make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = exp_for<T>(z[j][r] - of_row.x) * of_row.y;
-          z[j][r] = (c == 32 * j + 8 * (r >> 2) + (r & 3) ? p - 1.0f : p) * PScale<T>::up;
-        }
-    } else {
+    const int c = there ? a.label[row] - (n0 + wn + 4 * half) : -1;
+    // (kept as 16 bits, z becomes the distance below the group's largest in steps)
+    {
       const bool mine = c >= 0 && c < S::kFN * 32 && (c & 7) < 4;
       if (__any(mine)) {
         float zy = 0.0f;
@@ -294,23 +312,22 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
           }
         }
       sum += __shfl_xor(sum, 32, 64);
-      const int group = (a.v0 + n0 + wn) / (S::kFN * 32);
+      const int group = (n0 + wn) / (S::kFN * 32);
       if (there && half == 0) a.stats[group * a.ld_stats + row] = make_float2(top, sum);
     }
-    if constexpr (kWhat != kStats) {
+    if constexpr (kWhat == kKeep) {
+      const int c0 = n0 + wn + 4 * half;
       if constexpr (sizeof(T) == 4) {
-        float* to = (float*)a.p + (long long)row * a.ldp + n0 + wn + 4 * half;
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (there && 32 * j + 8 * q < room)
-              *(f32x4*)(to + 32 * j + 8 * q) =
+              *(f32x4*)((float*)a.p + in_panels<float>(row, c0 + 32 * j + 8 * q, a.chunk_rows)) =
                   f32x4{z[j][4 * q], z[j][4 * q + 1], z[j][4 * q + 2], z[j][4 * q + 3]};
       } else {
-        // eight neighbouring columns a lane: the lower half of the wave takes the even groups of eight
-        unsigned short* to = (unsigned short*)a.p + (long long)row * a.ldp + n0 + wn + 8 * half;
-        const int space = a.ldp - n0 - wn - 8 * half;
+        // eight neighbouring columns a lane: the lower half of the wave takes the even groups of eight; two
+        // stores fill a panel's 32 rows
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
@@ -322,18 +339,14 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 const float lo = z[j][4 * (q + g) + 2 * k], hi = z[j][4 * (q + g) + 2 * k + 1];
-                if constexpr (kWhat == kProb) {
-                  const T x = TypeOf<T>::from_float(lo), y = TypeOf<T>::from_float(hi);
-                  w[k] = (unsigned)__builtin_bit_cast(unsigned short, x) |
-                         (unsigned)__builtin_bit_cast(unsigned short, y) << 16;
-                } else {
-                  w[k] = (unsigned)fminf(lo, 65535.0f) | (unsigned)fminf(hi, 65535.0f) << 16;
-                }
+                w[k] = (unsigned)fminf(lo, 65535.0f) | (unsigned)fminf(hi, 65535.0f) << 16;
               }
               half_group[g] = (unsigned long long)w[1] << 32 | w[0];
             }
             const u32x4 eight = whole_group(half_group[0], half_group[1]);
-            if (there && 32 * j + 8 * q < space) *(u32x4*)(to + 32 * j + 8 * q) = eight;
+            if (there && n0 + wn + 32 * j < a.ldp)
+              *(u32x4*)((unsigned short*)a.p +
+                        in_panels<T>(row, n0 + wn + 32 * j, a.chunk_rows) + 8 * q + 8 * half) = eight;
           }
       }
     }
@@ -348,82 +361,107 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
   const int2 at = tile_at(a.grid, blockIdx.x);
   const int rows = a.chunk.rows(a.n_valid), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   if (m0 >= rows) return;
-  Tile<T, kRows, kRows, S> tile;
-  tile.run(a.x + m0 * a.ldx, a.ldx, ((long long)rows - m0) * a.ldx * (int)sizeof(T),
-           a.w + n0 * a.ldw, a.ldw, a.w_bytes - (long long)n0 * a.ldw * (int)sizeof(T), a.steps, lds, a.w_limit);
+  constexpr long long size = sizeof(T);
+  Tile<T, kRows, kPanels, kRows, gemm::kPlain, S> tile;
+  tile.run(a.x + (long long)m0 * (kStepBytes / size), (long long)a.chunk_rows * kStepBytes,
+           a.x_bytes - (long long)m0 * kStepBytes, a.w + n0 * a.ldw, a.ldw * size, a.w_bytes - n0 * a.ldw * size,
+           a.steps, lds, kStepBytes, a.w_limit);
   if (!a.bias && n0 + S::kBN <= a.v)
     finish_logits<T, S, kWhat, true>(a, tile, m0, n0, rows);
   else
     finish_logits<T, S, kWhat, false>(a, tile, m0, n0, rows);
 }
 
+constexpr int kProbRows = 256;
+
 // P from the kept logits, in their place: p = e^(z - group's top) * (e^(group's top - row's top) / row's
-// sum), the first factor from the code.  A workgroup takes kRows rows of 16 bytes of columns a thread;
-// column_sums (or NULL): [row block][v] sums of P over its rows.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept, const int ldp, const int v,
-                                                         const Chunk chunk, const int* __restrict__ n_valid,
+// sum), the first factor from the code.  A workgroup takes a group of classes (kPanelsOf panels) of
+// kProbRows places, a thread 16 bytes of each panel's row.  column_sums (or NULL): [row block][v] sums of P
+// over its rows.  The first workgroup of the last chunk also adds up the loss (losses > 0).
+template <typename T, int kPanelsOf>
+__global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept, const int chunk_rows, const int ldp,
+                                                         const int v, const Chunk chunk,
+                                                         const int* __restrict__ n_valid,
                                                          const int* __restrict__ label,
                                                          const float2* __restrict__ row_stats,
                                                          const float2* __restrict__ stats, const long long ld_stats,
-                                                         const int group, const int per,
-                                                         float* __restrict__ column_sums) {
-  constexpr int kV = 16 / (int)sizeof(T);
-  const int rows = chunk.rows(n_valid), lo = blockIdx.y * per, hi = min(rows, lo + per);
-  const int c = (blockIdx.x * kThreads + threadIdx.x) * kV;
-  if (c >= ldp) return;
-  const float2* top = stats + (long long)(c / group) * ld_stats;
-  float sums[kV];
+                                                         float* __restrict__ column_sums,
+                                                         const double* __restrict__ loss_parts, const int losses,
+                                                         float* __restrict__ small) {
+  constexpr int kV = 16 / (int)sizeof(T), kC = kStepBytes / (int)sizeof(T);
+  __shared__ float s_sum[4][kPanelsOf * kC];
+  if (losses && blockIdx.x == 0 && blockIdx.y == 0) add_losses(loss_parts, losses, small);
+  const int rows = chunk.rows(n_valid), lo = blockIdx.y * kProbRows, hi = min(rows, lo + kProbRows);
+  const int t = threadIdx.x, first = blockIdx.x * kPanelsOf * kC, c = first + (t & 3) * kV;
+  const float2* top = stats + (long long)blockIdx.x * ld_stats;
+  float sums[kPanelsOf][kV];
 #pragma unroll
-  for (int k = 0; k < kV; ++k) sums[k] = 0.0f;
-#pragma unroll 4
-  for (int r = lo; r < hi; ++r) {
-    u32x4* const at = (u32x4*)((T*)kept + (long long)r * ldp + c);
-    const u32x4 z = *at;
+  for (int i = 0; i < kPanelsOf; ++i)
+#pragma unroll
+    for (int k = 0; k < kV; ++k) sums[i][k] = 0.0f;
+  for (int r = lo + (t >> 2); r < hi; r += kThreads / 4) {
+    u32x4* const at = (u32x4*)((T*)kept + in_panels<T>(r, c, chunk_rows));
+    const long long next = (long long)chunk_rows * kStepBytes / 16;      // panel
+    u32x4 z[kPanelsOf];
+#pragma unroll
+    for (int i = 0; i < kPanelsOf; ++i)
+      if (first + i * kC < ldp) z[i] = at[i * next];
     const float2 of_row = row_stats[r];
     const int y = label[r] - c;
-    u32x4 out;
-    float p[kV];
-    if constexpr (sizeof(T) == 4) {
-      const f32x4 f = __builtin_bit_cast(f32x4, z);
+    const float f = sizeof(T) == 4 ? of_row.y : exp_for<T>(top[r].x - of_row.x) * of_row.y;
 #pragma unroll
-      for (int k = 0; k < kV; ++k) p[k] = expf(f[k] - of_row.x) * of_row.y;
-    } else {
-      const float f = exp_for<T>(top[r].x - of_row.x) * of_row.y;
+    for (int i = 0; i < kPanelsOf; ++i) {
+      if (first + i * kC >= ldp) continue;
+      float p[kV];
+      if constexpr (sizeof(T) == 4) {
+        const f32x4 w = __builtin_bit_cast(f32x4, z[i]);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) p[k] = expf(w[k] - of_row.x) * f;
+      } else {
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+          const unsigned w = z[i][k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
+          const float e = __builtin_amdgcn_exp2f((float)code * (-1.0f / Kept<T>::kSteps));
+          p[k] = (code == 0xffffu ? 0.0f : e) * f;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
-        const unsigned w = z[k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
-        const float e = __builtin_amdgcn_exp2f((float)code * (-1.0f / Kept<T>::kSteps));
-        p[k] = (code == 0xffffu ? 0.0f : e) * f;
+        p[k] = y == i * kC + k ? p[k] - 1.0f : p[k];
+        sums[i][k] += p[k];
       }
+      u32x4 out;
+      if constexpr (sizeof(T) == 4) {
+        out = __builtin_bit_cast(u32x4, f32x4{p[0], p[1], p[2], p[3]});
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const T a = TypeOf<T>::from_float(p[2 * k] * PScale<T>::up), b = TypeOf<T>::from_float(p[2 * k + 1] * PScale<T>::up);
+          out[k] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
+        }
+      }
+      at[i * next] = out;
     }
+  }
+  if (!column_sums) return;
+#pragma unroll
+  for (int i = 0; i < kPanelsOf; ++i)
 #pragma unroll
     for (int k = 0; k < kV; ++k) {
-      p[k] = y == k ? p[k] - 1.0f : p[k];
-      sums[k] += p[k];
-    }
-    if constexpr (sizeof(T) == 4) {
-      f32x4 o;
+      float s = sums[i][k];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = c + k < v ? p[k] : 0.0f;
-      out = __builtin_bit_cast(u32x4, o);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const T a = TypeOf<T>::from_float(p[2 * k] * PScale<T>::up), b = TypeOf<T>::from_float(p[2 * k + 1] * PScale<T>::up);
-        out[k] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
-      }
+      for (int o = 4; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
+      if ((t & 63) < 4) s_sum[t >> 6][i * kC + (t & 3) * kV + k] = s;
     }
-    *at = out;
-  }
-  if (column_sums)
-    for (int k = 0; k < kV && c + k < v; ++k) column_sums[(long long)blockIdx.y * v + c + k] = sums[k];
+  __syncthreads();
+  for (int i = t; i < kPanelsOf * kC && first + i < v; i += kThreads)
+    column_sums[(long long)blockIdx.y * v + first + i] = (s_sum[0][i] + s_sum[1][i]) + (s_sum[2][i] + s_sum[3][i]);
 }
 
 // Row loss and (max, 1 / sum) of every place from the tiles' pairs: eight threads a row, each an
 // eighth of the tiles.
 __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __restrict__ stats,
-                                                              const long long ld, const int tiles,
+                                                              const long long ld, const int groups,
                                                               const Chunk chunk, const int* __restrict__ n_valid,
                                                               const int* __restrict__ map,
                                                               const float* __restrict__ z_label,
@@ -435,10 +473,18 @@ __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __re
   const int row = blockIdx.x * 32 + r;
   float top = -__builtin_inff(), sum = 0.0f;
   if (row < rows) {
-    for (int t = part; t < tiles; t += 8) {
-      const float2 p = stats[t * ld + row];
-      const float up = fmaxf(top, p.x), base = up == -__builtin_inff() ? 0.0f : up;
-      sum = sum * expf(top - base) + p.y * expf(p.x - base);
+    for (int t0 = part; t0 < groups; t0 += 64) {      // eight at a time, their loads together
+      float2 p[8];
+      float up = top;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        p[k] = t0 + 8 * k < groups ? stats[(t0 + 8 * k) * ld + row] : make_float2(-__builtin_inff(), 0.0f);
+        up = fmaxf(up, p[k].x);
+      }
+      const float base = up == -__builtin_inff() ? 0.0f : up;
+      sum *= expf(top - base);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += p[k].y * expf(p[k].x - base);
       top = up;
     }
   }
@@ -463,15 +509,9 @@ __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __re
   }
 }
 
-__global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __restrict__ partial, const int n,
+__global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __restrict__ parts, const int n,
                                                                float* __restrict__ small) {
-  __shared__ double s_red[4];
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += kThreads) sum += partial[i];
-  sum = wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) small[0] = (float)(((s_red[0] + s_red[1]) + (s_red[2] + s_red[3])) * (double)small[2]);
+  add_losses(parts, n, small);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -479,12 +519,13 @@ __global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __r
 // ---------------------------------------------------------------------------------------------
 template <typename T>
 struct ProductArgs {
-  const T* a;
-  long long lda;
-  const T* b;
-  long long ldb, b_bytes;      // readable from b on (kCols: its rows end with the sum instead)
-  int m, n, k;                 // on the host's side; rows that count bound m or k on the device
-  const int* n_valid;          // with the chunk: bounds m (kRows A) or k (kCols A)
+  const T* p;                  // P in panels of chunk_rows
+  long long p_bytes;
+  int chunk_rows;
+  const T* b;                  // dX: the weights, ldb apart; dW: the features in panels of chunk_rows
+  long long ldb, b_bytes;
+  int m, n, k;                 // rows that count bound m (dX) or k (dW) on the device
+  const int* n_valid;
   Chunk chunk;
   Grid grid;
   int split_steps;             // k steps a split takes
@@ -501,33 +542,28 @@ struct ProductArgs {
 // float parts; the result, in rows of whole groups of eight 16-bit values, of four of either size, or not
 enum To { kParts, kOctets, kQuads, kSingly };
 
-template <typename T, Layout kLA, Layout kLB, typename S, To kTo>
+// kLA = kRows: dX = P W, the sum over the classes; kCols: dW = P^T X, over the chunk's rows.
+template <typename T, Layout kLA, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  constexpr int kStepK = kStepBytes / (int)sizeof(T);
+  constexpr long long size = sizeof(T);
+  constexpr int kC = kStepBytes / (int)sizeof(T);      // values of k a step, columns a panel
   const int2 at = tile_at(a.grid, blockIdx.x);
   const int rows = max(a.chunk.rows(a.n_valid), 0), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
-  const int m = kLA == kRows ? min(a.m, rows) : a.m, k = kLA == kCols ? min(a.k, rows) : a.k;
+  const int m = kLA == kRows ? rows : a.m, k = kLA == kCols ? rows : a.k;
   if (m0 >= m) return;
-  const long long size = sizeof(T);
-  const long long k0 = (long long)blockIdx.y * a.split_steps * kStepK;
-  const int steps = (int)max(0ll, min((long long)a.split_steps, (k - k0 + kStepK - 1) / kStepK));
-  const T* pa;
-  const T* pb;
-  long long a_bytes, b_bytes;
-  if (kLA == kRows) {
-    pa = a.a + m0 * a.lda + k0;
-    a_bytes = (((long long)m - m0 - 1) * a.lda + k - k0) * size;
-  } else {
-    pa = a.a + k0 * a.lda + m0;
-    a_bytes = ((k - k0) * a.lda - m0) * size;
-  }
-  static_assert(kLB == kCols, "the second operand of both products has the sum down its columns");
-  pb = a.b + k0 * a.ldb + n0;
-  b_bytes = min(a.b_bytes - (k0 * a.ldb + n0) * size, ((k - k0) * a.ldb - n0) * size);
-  Tile<T, kLA, kLB, S> tile;
-  tile.run(pa, a.lda, a_bytes, pb, a.ldb, b_bytes, steps, lds);
+  const int k0 = blockIdx.y * a.split_steps * kC;
+  const int steps = max(0, min(a.split_steps, (k - k0 + kC - 1) / kC));
+  const int last = k - k0 - (steps - 1) * kC;          // values of k in the last step
+  const long long panel = (long long)a.chunk_rows * kStepBytes;
+  const long long from = kLA == kRows ? k0 / kC * panel + (long long)m0 * kStepBytes
+                                      : m0 / kC * panel + (long long)k0 * kStepBytes;
+  constexpr bool kPB = kLA == kCols;
+  const long long from_b = kPB ? n0 / kC * panel + (long long)k0 * kStepBytes : (k0 * a.ldb + n0) * size;
+  Tile<T, kLA, kPanels, kCols, kPB, S> tile;
+  tile.run((const char*)a.p + from, panel, a.p_bytes - from, (const char*)a.b + from_b, kPB ? panel : a.ldb * size,
+           a.b_bytes - from_b, steps, lds, last, last);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32 + 4 * (lane >> 5);
   const float s = *a.scale * a.down;
@@ -607,29 +643,23 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __res
   }
 }
 
-// Column sums of P over the rows that count: a block takes 256 columns and every splits-th run of rows.
+// db from the row blocks' column sums: 32 columns a workgroup, eight threads a column.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sum_columns_kernel(const T* __restrict__ p, const int ldp, const int v,
-                                                               const Chunk chunk, const int* __restrict__ n_valid,
-                                                               const int splits, float* __restrict__ part) {
-  const int c = blockIdx.x * kThreads + threadIdx.x, rows = max(chunk.rows(n_valid), 0);
-  const int per = (rows + splits - 1) / splits, lo = blockIdx.y * per, hi = min(rows, lo + per);
-  if (c >= v) return;
-  float sum = 0.0f;
-#pragma unroll 8
-  for (int r = lo; r < hi; ++r) sum += TypeOf<T>::to_float(p[(long long)r * ldp + c]);
-  part[(long long)blockIdx.y * v + c] = sum;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void join_columns_kernel(const float* __restrict__ part, const int splits,
+__global__ __launch_bounds__(kThreads) void join_columns_kernel(const float* __restrict__ part, const int parts,
                                                                 const int v, const float* __restrict__ scale,
-                                                                const float down, T* __restrict__ db) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= v) return;
+                                                                T* __restrict__ db) {
+  __shared__ float s_sum[8][32];
+  const int in = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + in;
   float sum = 0.0f;
-  for (int k = 0; k < splits; ++k) sum += part[(long long)k * v + c];
-  db[c] = TypeOf<T>::from_float(sum * (*scale * down));
+  if (c < v)
+#pragma unroll 8
+    for (int k = slice; k < parts; k += 8) sum += part[(long long)k * v + c];
+  s_sum[slice][in] = sum;
+  __syncthreads();
+  if (slice == 0 && c < v) {
+    for (int k = 1; k < 8; ++k) sum += s_sum[k][in];
+    db[c] = TypeOf<T>::from_float(sum * *scale);
+  }
 }
 
 // x *= scale / assumed in place, one rounding; an array whose scale is the assumed one is not touched.
@@ -649,30 +679,23 @@ __global__ __launch_bounds__(kThreads) void upstream_kernel(T* __restrict__ x, c
 typedef Shape<2, 2, 4, 4> Large;      // 256 x 256, 4 waves
 typedef Shape<2, 2, 2, 2> Small;      // 128 x 128, 4 waves
 
-constexpr long long kPieceBytes = 256ll << 20;      // of P where the logits are made twice
-constexpr long long kPieceMost = 1 << 18;           // classes; a tile's byte offsets into P stay below 2^31
-constexpr long long kKeptBytes = 2ll << 30;         // of logits where they are made once
-constexpr int kColumnSplits = 32;
-constexpr int kProbRows = 64;
-constexpr int kKeepFrom = 512;                      // features
+constexpr long long kKeptBytes = 2ll << 30;      // of logits at a time, or 256 rows of them
+constexpr int kMostChunk = 1 << 22;              // rows; eight panels' offsets stay below 2^31
 
-// The call's work is cut so that no more than a bounded piece of the logits exists at a time:
-//   keep    all classes of `chunk` rows: logits once (6 n d v operations in all), P made in their
-//           place; with more than one chunk the weight's gradient is added up in float32.
-//   !keep   `piece` classes of all rows: one pass for the rows' sums, then piece by piece the logits
-//           again, as P (8 n d v operations); each piece's part of the weight's gradient is complete.
+// The call's rows are taken in chunks whose logits take kKeptBytes at most: they are made once (6 n d v
+// operations in all), P takes their place, and the chunk's part of the weight's gradient is added to the
+// others' in float32 where there are several.
 struct Plan {
   int size, step_k;
   int per, row_blocks;          // rows a placing block takes
-  int ldx, ldw_pad;             // padded rows of the placed features; of the copied weights (0: none)
-  bool keep;
+  int panels;                   // of the features
+  int ldw_pad;                  // row of the copied weights (0: not copied)
   int chunk, chunks;            // rows at a time
-  int piece, pieces, ldp;       // classes of P at a time
+  int ldp;                      // columns of P
   bool large_logits, large_dx, large_dw;
-  int group;                    // classes a wave of the logits' tiles takes
+  int group, groups;            // classes a wave of the logits' tiles takes
   int dx_splits, dx_steps, dw_splits, dw_steps;
   long long ldpart;
-  int groups;
 };
 
 // Tiles of 256 x 256 move half the bytes per product of those of 128 x 128, which fill the card
@@ -698,42 +721,28 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   p.step_k = kStepBytes / p.size;
   p.per = n > 65536 ? 256 : 32;
   p.row_blocks = ceil_div(n, p.per);
-  p.ldx = ceil_div(d, p.step_k) * p.step_k;
-  p.ldw_pad = flags & RH_CE_COPY_WEIGHT ? p.ldx : 0;
-  const bool grads = flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B);
-  const long long row_bytes = (long long)ceil_div(v, 64) * 64 * p.size;
+  p.panels = ceil_div(d, p.step_k);
+  p.ldw_pad = flags & RH_CE_COPY_WEIGHT ? ceil_div(d, p.step_k) * p.step_k : 0;
+  p.ldp = ceil_div(v, 64) * 64;
+  long long rows = kKeptBytes / ((long long)p.ldp * p.size) / 256 * 256;
+  if (rows < 256) rows = 256;
+  if (rows > kMostChunk) rows = kMostChunk;
   p.chunk = n;
   p.chunks = 1;
-  p.keep = grads && d >= kKeepFrom && row_bytes * 256 < kKeptBytes;
-  if (p.keep) {
-    const long long rows = kKeptBytes / row_bytes / 256 * 256;
-    if (n > rows) {
-      p.chunks = ceil_div(n, rows);
-      p.chunk = ceil_div(ceil_div(n, p.chunks), 256) * 256;      // of even size
-      p.chunks = ceil_div(n, p.chunk);
-    }
-    p.piece = v;
-    p.pieces = 1;
-  } else {
-    long long piece = kPieceBytes / ((long long)n * p.size) / 256 * 256;
-    if (piece < 4096) piece = 4096;
-    if (piece > kPieceMost) piece = kPieceMost;
-    if (piece > v) piece = v;
-    p.pieces = ceil_div(v, piece);
-    if (p.pieces > 1) piece = ceil_div(ceil_div(v, p.pieces), 256) * 256;
-    p.pieces = ceil_div(v, piece);
-    p.piece = (int)piece;
+  if (n > rows) {
+    p.chunks = ceil_div(n, rows);
+    p.chunk = ceil_div(ceil_div(n, p.chunks), 256) * 256;      // of even size
+    p.chunks = ceil_div(n, p.chunk);
   }
-  p.ldp = ceil_div(p.piece, 64) * 64;
-  p.large_logits = take_large(p.chunk, p.piece);
+  p.large_logits = take_large(p.chunk, v);
   p.group = p.large_logits ? Large::kFN * 32 : Small::kFN * 32;
   p.groups = ceil_div(v, p.large_logits ? Large::kBN : Small::kBN) * (p.large_logits ? Large::kWN : Small::kWN);
   p.large_dx = take_large(p.chunk, d);
-  p.large_dw = take_large(p.piece, d);
+  p.large_dw = take_large(v, d);
   const int k_dx = ceil_div(p.ldp, p.step_k), k_dw = ceil_div(p.chunk, p.step_k);
   p.dx_splits = splits_for(p.chunk, d, k_dx, p.large_dx);
   p.dx_steps = ceil_div(k_dx, p.dx_splits);
-  p.dw_splits = splits_for(p.piece, d, k_dw, p.large_dw);
+  p.dw_splits = splits_for(v, d, k_dw, p.large_dw);
   p.dw_steps = ceil_div(k_dw, p.dw_splits);
   p.ldpart = ceil_div(d, 4) * 4;
   return p;
@@ -752,7 +761,7 @@ struct Space {
   float* dx_part;
   float* dw_part;
   float* db_part;
-  int db_splits;      // parts of a column's sum, of all chunks
+  int db_parts;       // of a column's sum, of all chunks
   size_t bytes;
 };
 
@@ -764,20 +773,20 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   s.info.label = c.take<int>(n);
   s.info.n_valid = c.take<int>(1);
   s.info.scale = c.take<float>(1);
-  s.x = c.take<char>((size_t)n * p.ldx * p.size);
+  s.x = c.take<char>((size_t)p.chunks * p.chunk * p.panels * kStepBytes);
   if (p.ldw_pad) s.w = c.take<char>((size_t)v * p.ldw_pad * p.size);
   s.stats = c.take<float2>((size_t)p.groups * p.chunk);
   s.z_label = c.take<float>(n);
   s.row_stats = c.take<float2>(n);
   s.loss = c.take<double>(ceil_div(n, 32));
   if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) s.p = c.take<char>((size_t)p.chunk * p.ldp * p.size);
-  if ((flags & RH_CE_GRAD_X) && (p.pieces > 1 || p.dx_splits > 1))
+  if ((flags & RH_CE_GRAD_X) && p.dx_splits > 1)
     s.dx_part = c.take<float>((size_t)p.dx_splits * p.chunk * p.ldpart);
   if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw_splits > 1))
-    s.dw_part = c.take<float>((size_t)p.dw_splits * p.piece * p.ldpart);
+    s.dw_part = c.take<float>((size_t)p.dw_splits * v * p.ldpart);
   if (flags & RH_CE_GRAD_B) {
-    s.db_splits = p.keep ? ceil_div(p.chunk, kProbRows) * p.chunks : kColumnSplits;
-    s.db_part = c.take<float>((size_t)s.db_splits * p.piece);
+    s.db_parts = ceil_div(p.chunk, kProbRows) * p.chunks;
+    s.db_part = c.take<float>((size_t)s.db_parts * v);
   }
   s.bytes = c.off;
   return s;
@@ -803,12 +812,24 @@ template <typename T, Layout kLA, typename S>
 static int launch_product(ProductArgs<T> a, int splits, hipStream_t stream) {
   a.grid = Grid{ceil_div(a.m, S::kBM), ceil_div(a.n, S::kBN)};
   constexpr To kWide = sizeof(T) == 2 ? kOctets : kQuads;
-  auto kernel = a.part                                   ? product_kernel<T, kLA, kCols, S, kParts>
-                : a.n % (sizeof(T) == 2 ? 8 : 4) == 0    ? product_kernel<T, kLA, kCols, S, kWide>
-                                                         : product_kernel<T, kLA, kCols, S, kSingly>;
+  auto kernel = a.part                                ? product_kernel<T, kLA, S, kParts>
+                : a.n % (sizeof(T) == 2 ? 8 : 4) == 0 ? product_kernel<T, kLA, S, kWide>
+                                                      : product_kernel<T, kLA, S, kSingly>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n, splits), dim3(S::kThreads), S::kLdsBytes, stream, a);
   RH_CHECK_LAUNCH("product_kernel");
+  return RH_OK;
+}
+
+template <typename T, int kPanelsOf>
+static int launch_probs(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a, int chunk,
+                        hipStream_t stream) {
+  const int blocks = ceil_div(p.chunk, kProbRows);
+  hipLaunchKernelGGL((probs_kernel<T, kPanelsOf>), dim3(ceil_div(p.ldp, p.group), blocks), dim3(kThreads), 0, stream, s.p,
+                     p.chunk, p.ldp, a.v, a.chunk, a.n_valid, a.label, s.row_stats + a.chunk.first, s.stats, a.ld_stats,
+                     s.db_part ? s.db_part + (long long)chunk * blocks * a.v : nullptr, s.loss,
+                     chunk == p.chunks - 1 ? ceil_div(q.n, 32) : 0, q.small);
+  RH_CHECK_LAUNCH("probs_kernel");
   return RH_OK;
 }
 
@@ -822,73 +843,62 @@ static int join_parts(const ProductArgs<T>& g, int splits, bool by_rows, hipStre
   return RH_OK;
 }
 
-// dX of a chunk from a piece of P (all of it, or the piece-th).
+// What the two products share.
+template <typename T>
+static ProductArgs<T> product_args(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a) {
+  ProductArgs<T> g = {};
+  g.p = (const T*)s.p;
+  g.p_bytes = (long long)p.chunk * p.ldp * p.size;
+  g.chunk_rows = p.chunk;
+  g.n = q.d;
+  g.n_valid = a.n_valid;
+  g.chunk = a.chunk;
+  g.scale = s.info.scale;
+  g.down = PScale<T>::down;
+  g.ldo = q.d;
+  g.ldpart = p.ldpart;
+  return g;
+}
+
+// dX of a chunk.
 template <typename T>
 static int features_gradient(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a,
-                             int piece, hipStream_t stream) {
-  ProductArgs<T> g = {};
-  g.a = (const T*)s.p;
-  g.lda = p.ldp;
+                             hipStream_t stream) {
+  ProductArgs<T> g = product_args(q, p, s, a);
   g.b = a.w;
   g.ldb = a.ldw;
   g.b_bytes = a.w_bytes;
   g.m = a.chunk.most;
-  g.n = q.d;
-  g.k = ceil_div(a.v, 64) * 64;       // P has zeros there, the weights' records end earlier
-  g.n_valid = a.n_valid;
-  g.chunk = a.chunk;
+  g.k = a.v;
   g.split_steps = p.dx_steps;
-  g.scale = s.info.scale;
-  g.down = PScale<T>::down;
   g.out = (T*)q.dx;
   g.map = s.info.map + a.chunk.first;
-  g.ldo = q.d;
   g.part = s.dx_part;
-  g.ldpart = p.ldpart;
   g.plane = (long long)p.chunk * p.ldpart;
-  g.add = piece > 0;
   if (int rc = p.large_dx ? launch_product<T, kRows, Large>(g, p.dx_splits, stream)
                           : launch_product<T, kRows, Small>(g, p.dx_splits, stream))
     return rc;
-  return s.dx_part && piece == p.pieces - 1 ? join_parts(g, p.dx_splits, true, stream) : RH_OK;
+  return s.dx_part ? join_parts(g, p.dx_splits, true, stream) : RH_OK;
 }
 
-// dW of a piece's classes from a chunk of P.
+// dW, or a chunk's part of it.
 template <typename T>
 static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a,
                            int chunk, hipStream_t stream) {
-  ProductArgs<T> g = {};
-  g.a = (const T*)s.p;
-  g.lda = p.ldp;
+  ProductArgs<T> g = product_args(q, p, s, a);
   g.b = a.x;
-  g.ldb = a.ldx;
-  g.b_bytes = (long long)a.chunk.most * a.ldx * p.size;
+  g.b_bytes = a.x_bytes;
   g.m = a.v;
-  g.n = q.d;
   g.k = a.chunk.most;
-  g.n_valid = a.n_valid;
-  g.chunk = a.chunk;
   g.split_steps = p.dw_steps;
-  g.scale = s.info.scale;
-  g.down = PScale<T>::down;
-  g.out = (T*)q.dw + (long long)a.v0 * q.d;
-  g.ldo = q.d;
+  g.out = (T*)q.dw;
   g.part = s.dw_part;
-  g.ldpart = p.ldpart;
-  g.plane = (long long)p.piece * p.ldpart;
+  g.plane = (long long)a.v * p.ldpart;
   g.add = chunk > 0;
   if (int rc = p.large_dw ? launch_product<T, kCols, Large>(g, p.dw_splits, stream)
                           : launch_product<T, kCols, Small>(g, p.dw_splits, stream))
     return rc;
   return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, p.dw_splits, false, stream) : RH_OK;
-}
-
-template <typename T>
-static int bias_gradient(const rh_linear_ce_args& q, const Space& s, int v0, int vc, float down, hipStream_t stream) {
-  hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(vc, kThreads)), dim3(kThreads), 0, stream, s.db_part,
-                     s.db_splits, vc, s.info.scale, down, (T*)q.db + v0);
-  RH_CHECK_LAUNCH("join_columns_kernel");
-  return RH_OK;
 }
 
 template <typename T>
@@ -898,9 +908,10 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   T* const x = (T*)s.x;
   hipLaunchKernelGGL(count_rows_kernel, dim3(p.row_blocks), dim3(64), 0, stream, labels, n, p.per, s.blocks);
   RH_CHECK_LAUNCH("count_rows_kernel");
-  hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
-                     d, labels, n, p.per, s.blocks, x, p.ldx, s.info, q.row_loss, (T*)q.dx, q.small,
-                     (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
+  const int side = ceil_div(p.panels, 16) < 8 ? ceil_div(p.panels, 16) : 8;
+  hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks, side), dim3(kThreads), 0, stream, (const T*)q.x,
+                     (long long)q.ldx, d, labels, n, p.per, s.blocks, x, p.panels, p.chunk, s.info, q.row_loss, (T*)q.dx,
+                     q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
   RH_CHECK_LAUNCH("place_rows_kernel");
   const T* w = (const T*)q.w;
   long long ldw = q.ldw;
@@ -912,16 +923,18 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     ldw = p.ldw_pad;
   }
   const long long d_w = p.ldw_pad ? p.ldw_pad : d;
-  const long long w_bytes = ((v - 1) * ldw + d_w) * p.size;
+  const bool grads = q.dx || q.dw || q.db;
 
   LogitArgs<T> a = {};
-  a.ldx = p.ldx;
+  a.chunk_rows = p.chunk;
+  a.x_bytes = (long long)p.chunk * p.panels * kStepBytes;
   a.w = w;
   a.ldw = ldw;
-  a.w_bytes = w_bytes;
+  a.w_bytes = ((v - 1) * ldw + d_w) * p.size;
   a.bias = (const T*)q.bias;
-  a.steps = p.ldx / p.step_k;
+  a.steps = p.panels;
   a.w_limit = (int)(d_w * p.size - (long long)(a.steps - 1) * kStepBytes);
+  a.v = v;
   a.n_valid = s.info.n_valid;
   a.stats = s.stats;
   a.ld_stats = p.chunk;
@@ -930,59 +943,38 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   for (int c = 0; c < p.chunks; ++c) {
     a.chunk = Chunk{c * p.chunk, n - c * p.chunk < p.chunk ? n - c * p.chunk : p.chunk};
     const int first = a.chunk.first;
-    a.x = x + (long long)first * p.ldx;
+    a.x = x + (long long)first * p.panels * p.step_k;
     a.label = s.info.label + first;
     a.z_label = s.z_label + first;
-    a.row = s.row_stats + first;
-    a.v0 = 0;
-    a.v = v;
-    if (int rc = p.keep ? p.large_logits ? launch_logits<T, Large, kKeep>(a, stream)
-                                         : launch_logits<T, Small, kKeep>(a, stream)
-                        : p.large_logits ? launch_logits<T, Large, kStats>(a, stream)
-                                         : launch_logits<T, Small, kStats>(a, stream))
+    if (int rc = grads ? p.large_logits ? launch_logits<T, Large, kKeep>(a, stream)
+                                        : launch_logits<T, Small, kKeep>(a, stream)
+                       : p.large_logits ? launch_logits<T, Large, kStats>(a, stream)
+                                        : launch_logits<T, Small, kStats>(a, stream))
       return rc;
     hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, 32)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
                        p.groups, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,
                        s.loss + first / 32);
     RH_CHECK_LAUNCH("join_stats_kernel");
-    if (c == p.chunks - 1) {
-      hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, 32), q.small);
-      RH_CHECK_LAUNCH("finish_loss_kernel");
-    }
-    if (!q.dx && !q.dw && !q.db) continue;
-    if (p.keep) {
-      const int per_chunk = ceil_div(p.chunk, kProbRows);
-      const dim3 grid(ceil_div(p.ldp, kThreads * (16 / p.size)), per_chunk);      // column sums: every part is written
-      hipLaunchKernelGGL(probs_kernel<T>, grid, dim3(kThreads), 0, stream, s.p, p.ldp, v, a.chunk, s.info.n_valid, a.label,
-                         a.row, s.stats, a.ld_stats, p.group, kProbRows,
-                         s.db_part ? s.db_part + (long long)c * per_chunk * v : nullptr);
-      RH_CHECK_LAUNCH("probs_kernel");
-      if (q.dx)
-        if (int rc = features_gradient(q, p, s, a, 0, stream)) return rc;
-      if (q.dw)
-        if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
-      continue;
-    }
-    for (int i = 0; i < p.pieces; ++i) {
-      a.v0 = i * p.piece;
-      a.v = v - a.v0 < p.piece ? v - a.v0 : p.piece;
-      a.w = w + a.v0 * ldw;
-      a.w_bytes = w_bytes - a.v0 * ldw * p.size;
-      if (int rc = p.large_logits ? launch_logits<T, Large, kProb>(a, stream) : launch_logits<T, Small, kProb>(a, stream))
-        return rc;
-      if (q.dx)
-        if (int rc = features_gradient(q, p, s, a, i, stream)) return rc;
-      if (q.dw)
-        if (int rc = weight_gradient(q, p, s, a, 0, stream)) return rc;
-      if (q.db) {
-        hipLaunchKernelGGL(sum_columns_kernel<T>, dim3(ceil_div(a.v, kThreads), kColumnSplits), dim3(kThreads), 0, stream,
-                           (const T*)s.p, p.ldp, a.v, a.chunk, s.info.n_valid, kColumnSplits, s.db_part);
-        RH_CHECK_LAUNCH("sum_columns_kernel");
-        if (int rc = bias_gradient<T>(q, s, a.v0, a.v, PScale<T>::down, stream)) return rc;
-      }
-    }
+    if (!grads) continue;
+    const int panels = p.group * p.size / kStepBytes;      // of a group of classes
+    if (int rc = panels == 8   ? launch_probs<T, 8>(q, p, s, a, c, stream)
+                 : panels == 4 ? launch_probs<T, 4>(q, p, s, a, c, stream)
+                               : launch_probs<T, 2>(q, p, s, a, c, stream))
+      return rc;
+    if (q.dx)
+      if (int rc = features_gradient(q, p, s, a, stream)) return rc;
+    if (q.dw)
+      if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
   }
-  if (q.db && p.keep) return bias_gradient<T>(q, s, 0, v, 1.0f, stream);
+  if (!grads) {
+    hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, 32), q.small);
+    RH_CHECK_LAUNCH("finish_loss_kernel");
+  }
+  if (q.db) {
+    hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(v, 32)), dim3(kThreads), 0, stream, s.db_part, s.db_parts, v,
+                       s.info.scale, (T*)q.db);
+    RH_CHECK_LAUNCH("join_columns_kernel");
+  }
   return RH_OK;
 }
 
@@ -990,7 +982,7 @@ static int check_sizes(int64_t n, int32_t d, int64_t v, int32_t dtype) {
   RH_REQUIRE(dtype == RH_F32 || dtype == RH_BF16 || dtype == RH_F16, RH_EINVAL, "unknown element type %d", dtype);
   RH_REQUIRE(n >= 1 && n <= (1 << 26), RH_ESHAPE, "rows must be in 1 .. 2^26 (got %lld)", (long long)n);
   RH_REQUIRE(d >= 1 && d <= (1 << 17), RH_ESHAPE, "features must be in 1 .. 2^17 (got %d)", d);
-  RH_REQUIRE(v >= 1 && v <= (1 << 24), RH_ESHAPE, "classes must be in 1 .. 2^24 (got %lld)", (long long)v);
+  RH_REQUIRE(v >= 1 && v <= (1 << 21), RH_ESHAPE, "classes must be in 1 .. 2^21 (got %lld)", (long long)v);
   return RH_OK;
 }
 

@@ -1,12 +1,15 @@
 // Matrix-product core of the classifier loss (gfx950): C[m][n] = sum_k A(m,k) B(n,k) on the matrix
-// units, operands staged to LDS by direct loads, two stages deep.
+// units, operands staged to LDS by direct loads through a ring of four stages.
 //
 // An operand comes in one of two layouts, so that the loss's three products need no transposed
 // copies:   kRows  element (i,k) at  base + i*ld + k   (the sum runs along a row)
 //           kCols  element (i,k) at  base + k*ld + i   (the sum runs down a column)
-// Both are staged as they lie in memory.  A kRows tile holds 128 bytes of k per row and its 16-byte
+// Both are staged as they lie in memory.  A kRows tile holds 64 bytes of k per row and its 16-byte
 // fragments are read as they are; a kCols tile of a 16-bit type is read with the transposing LDS
 // load, one of a 32-bit type element by element.
+//
+// What this library lays out itself (the features, P) it lays out in panels of 64 bytes of columns, the
+// rows of a panel one after the other: the tiles of either layout are then runs of whole kilobytes.
 //
 // Every global read goes through a buffer descriptor whose record count ends at the operand's last
 // valid element: what a tile reaches beyond it reads as zero and touches no memory.
@@ -27,9 +30,12 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 
 enum Layout { kRows = 0, kCols = 1 };
+constexpr bool kPlain = false, kPanels = true;
 
-// 128 bytes of k per tile step: 64 values of a 16-bit type, 32 of float.
-constexpr int kStepBytes = 128;
+// 64 bytes of k per tile step: 32 values of a 16-bit type, 16 of float; two quarters (kk) of the matrix
+// instructions' depth each.
+constexpr int kStepBytes = 64;
+constexpr int kRing = 4;
 
 template <typename T>
 struct TypeOf;
@@ -88,41 +94,53 @@ __device__ __forceinline__ int xcd_run(const int id, const int total) {
   return x * per + min(x, rest) + at;
 }
 
-// One operand's descriptor for a tile: bytes readable from its first element on.
+constexpr unsigned kMostBytes = 0xffffff00u;
+constexpr int kNowhere = (int)0xffffff80u;      // an offset no descriptor reaches: reads as zero
+
+// One operand's descriptor: `bytes` readable from base on.
 __device__ __forceinline__ u32x4 make_rsrc(const char* base, const long long bytes) {
   const unsigned long long at = (unsigned long long)base;
-  const long long top = 0x7fffff00ll;
+  const unsigned low = (unsigned)bytes, high = (unsigned)((unsigned long long)bytes >> 32);
   u32x4 r;
   r[0] = __builtin_amdgcn_readfirstlane((unsigned)at);
-  r[1] = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32) & 0xffffu);
-  r[2] = __builtin_amdgcn_readfirstlane((unsigned)(bytes <= 0 ? 0 : bytes < top ? bytes : top));
+  r[1] = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));      // 47 bits of address, no stride
+  r[2] = __builtin_amdgcn_readfirstlane(high ? kMostBytes : min(low, kMostBytes));
   r[3] = 0x00020000u;
-  // a lane instruction may have written these registers: a memory instruction that takes them has to
-  // stay five cycles behind, which nobody else sees to for the written-out ones below
-  asm volatile("s_nop 4" : "+s"(r));
   return r;
 }
-constexpr int kNowhere = 0x7fffff80;      // an offset no descriptor reaches: reads as zero
 
 // 16 bytes per lane from the buffer to LDS, lane after lane from `lds` on.  Written out, because
 // the compiler waits for every such load of its own before any LDS read; here stage_wait() does.
+template <int kAt>
 __device__ __forceinline__ void load_to_lds(const u32x4 rsrc, const unsigned lds, const int offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
-               : "s"(lds), "v"(offset), "s"(rsrc)
-               : "memory");
+               : "s"(lds), "v"(offset), "s"(rsrc), "n"(kAt)
+               : "memory", "scc");
 }
-// This wave's loads have landed and its LDS reads have returned; then every wave's.
+// All but this wave's latest kLeft loads have landed and its LDS reads have returned; then every wave's.
+template <int kLeft>
 __device__ __forceinline__ void stage_wait() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+}
+
+template <int k>
+struct Int {
+  static constexpr int value = k;
+};
+template <int kN, int kI = 0, typename F>
+__device__ __forceinline__ void each(const F f) {      // f(Int<0>) .. f(Int<kN - 1>)
+  if constexpr (kI < kN) {
+    f(Int<kI>());
+    each<kN, kI + 1>(f);
+  }
 }
 
 // Moves one stage of an operand's tile (kR rows or columns of the result, kStepBytes of k) to LDS.
-template <typename T, Layout kL, int kR, int kThreads>
+template <typename T, Layout kL, bool kPaneled, int kR, int kThreads>
 struct Loader {
   static constexpr int kStepK = kStepBytes / (int)sizeof(T);
-  static constexpr int kBytes = kR * kStepBytes;
-  static constexpr int kOps = kBytes / (kThreads * 16);
+  static constexpr int kOps = kR * kStepBytes / (kThreads * 16);
   static constexpr int kRowBytes = kL == kRows ? kStepBytes : kR * (int)sizeof(T);
   static constexpr int kChunks = kRowBytes / 16;             // 16-byte chunks of a staged row
   static constexpr int kRowsPerOp = kThreads / kChunks;      // staged rows one pass of all threads covers
@@ -131,38 +149,50 @@ struct Loader {
   long long left;         // bytes readable from base on
   long long step;         // bytes from one step to the next
 
+  static __device__ __forceinline__ int row_of(const int i) { return i * kRowsPerOp + (int)threadIdx.x / kChunks; }
   static __device__ __forceinline__ int chunk_of(const int i) {
-    const int row = i * kRowsPerOp + (int)threadIdx.x / kChunks, at = (int)threadIdx.x % kChunks;
-    if (kL == kRows) return at ^ ((row >> 1) & 7);
+    const int row = row_of(i), at = (int)threadIdx.x % kChunks;
+    if (kL == kRows) return at ^ ((row >> 2) & 3);
     return sizeof(T) == 2 ? at ^ ((row & 3) << 2) : at;    // 16 bits: 32-byte blocks, block ^ 2*(k & 3)
   }
-  // origin: first element of the tile at k = 0; ld in elements; bytes: readable from origin on.
-  __device__ __forceinline__ void init(const void* origin, long long ld, long long bytes) {
+  // origin: first element of the tile at k = 0; stride: bytes from row to row, or from panel to panel;
+  // bytes: readable from origin on.
+  __device__ __forceinline__ void init(const void* origin, long long stride, long long bytes) {
     base = (const char*)origin;
     left = bytes;
-    step = kL == kRows ? kStepBytes : (long long)kStepK * ld * (int)sizeof(T);
+    if (kPaneled) step = kL == kRows ? stride : kStepK * kStepBytes;
+    else step = kL == kRows ? kStepBytes : kStepK * stride;
 #pragma unroll
-    for (int i = 0; i < kOps; ++i)
-      offset[i] = (int)((i * kRowsPerOp + (int)threadIdx.x / kChunks) * ld * (int)sizeof(T)) + chunk_of(i) * 16;
+    for (int i = 0; i < kOps; ++i) {
+      const int row = row_of(i), chunk = chunk_of(i);
+      if (!kPaneled) offset[i] = (int)(row * stride) + chunk * 16;
+      else if (kL == kRows) offset[i] = row * kStepBytes + chunk * 16;
+      else offset[i] = (int)((chunk >> 2) * stride) + row * kStepBytes + (chunk & 3) * 16;
+    }
   }
-  // The coming step's loads to a stage: begin(), then load<i>() for each of the kOps.  A step that
-  // is not `there` reads zeros and touches no memory; limit (kRows): bytes of k that belong to the rows.
-  u32x4 rsrc;
+  // A step's loads: plan() works out the descriptor of the coming one, begin() makes it the one that
+  // load() takes.  A step that is not `there` reads zeros and touches no memory.  limit: bytes (kRows) or
+  // values (kCols) of its k that belong to the operand, the others read as zero.
+  u32x4 rsrc, coming;
   unsigned to;
   int limit;
-  __device__ __forceinline__ void begin(RH_LDS char* stage, const bool there, const int k_bytes) {
-    rsrc = make_rsrc(base, there ? left : 0);
-    to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)stage + (threadIdx.x >> 6) * 1024);
-    limit = k_bytes;
+  __device__ __forceinline__ void plan(const bool there) {
+    coming = make_rsrc(base, there ? left : 0);
+    // a lane instruction may have written these registers: a memory instruction that takes them has to
+    // stay five cycles behind, which nobody else sees to for the written-out ones
+    asm volatile("s_nop 4" : "+s"(coming));
     base += step;
     left -= step;
   }
-  template <bool kTail>
-  __device__ __forceinline__ void load(const int first, const int count) const {
-#pragma unroll
-    for (int i = first; i < first + count; ++i)
-      load_to_lds(rsrc, to + i * kThreads * 16,
-                  !kTail || chunk_of(i) * 16 < limit ? offset[i] : kNowhere);
+  __device__ __forceinline__ void begin(const unsigned stage, const int k_limit) {
+    rsrc = coming;
+    to = stage;
+    limit = k_limit;
+  }
+  template <bool kTail, int i>
+  __device__ __forceinline__ void load() const {
+    const bool in = !kTail || (kL == kRows ? chunk_of(i) * 16 < limit : row_of(i) < limit);
+    load_to_lds<i * kThreads * 16>(rsrc, to, in ? offset[i] : kNowhere);
   }
 };
 
@@ -171,14 +201,14 @@ struct Loader {
 template <typename T, Layout kL, int kR, int kF>
 struct Fragments {
   static constexpr int kRowBytes = kR * (int)sizeof(T);      // kCols only
-  static constexpr int kAddr = kL == kRows ? 4 : (sizeof(T) == 2 ? kF : 1);
+  static constexpr int kAddr = kL == kRows ? 2 : (sizeof(T) == 2 ? kF : 1);
   int addr[kAddr];
   __device__ __forceinline__ void init(const int first) {
     const int l = (int)threadIdx.x & 63;
     if (kL == kRows) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        addr[kk] = (first + (l & 31)) * kStepBytes + (((2 * kk + (l >> 5)) ^ ((l >> 1) & 7)) << 4);
+      for (int kk = 0; kk < 2; ++kk)
+        addr[kk] = (first + (l & 31)) * kStepBytes + (((2 * kk + (l >> 5)) ^ ((l >> 2) & 3)) << 4);
     } else if (sizeof(T) == 2) {
       const int q = (l >> 2) & 3;
 #pragma unroll
@@ -218,27 +248,30 @@ struct Shape {
   static constexpr int kBM = kWM * kFM * 32, kBN = kWN * kFN * 32;
   static constexpr int kThreads = kWM * kWN * 64;
   static constexpr int kStage = (kBM + kBN) * kStepBytes;
-  static constexpr int kLdsBytes = 2 * kStage;
+  static constexpr int kLdsBytes = kRing * kStage;
 };
 
 // acc[i][j][r]: result row m = 32 i + lane % 32 and column n = 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4
 // of the wave's part: a lane owns rows, four neighbouring columns at a time.
-template <typename T, Layout kLA, Layout kLB, typename S>
+template <typename T, Layout kLA, bool kPA, Layout kLB, bool kPB, typename S>
 struct Tile {
   static constexpr int kStepK = kStepBytes / (int)sizeof(T);
   f32x16 acc[S::kFM][S::kFN];
 
-  // a / b: first elements of the tile's operands at the first k; *_bytes: readable from there;
-  // steps: k steps (of kStepK values); b_limit (kRows B): bytes of the last step that are b's.
+  // a / b: first elements of the tile's operands at the first k; lda, ldb: bytes from row to row or from
+  // panel to panel; *_bytes: readable from there; steps: k steps (of kStepK values); a_limit, b_limit: how
+  // much of the last one is the operand's (kCols: values; plain kRows: bytes of a row).
   //
-  // A step's fragments are read a quarter ahead of the instructions that take them.  The wait for the
-  // next stage stands before the last quarter's instructions, which then cover the barrier, the first
-  // reads of that stage and the launch of the loads that refill the one just read out.
+  // Fragments are read one half step ahead of the instructions that take them, and the loads of a
+  // stage are spread over the step that frees its place in the ring, nearly three steps before it is
+  // read.  8192 x 4096 x 16384 in bfloat16, uniform values: two stages of twice the depth, their loads in one
+  // burst, 1.04-1.10 PFLOP/s; this 1.12-1.16 (1.6-1.7 on zeros: the card's power sets its clock).
   __device__ __forceinline__ void run(const void* a, long long lda, long long a_bytes, const void* b,
                                       long long ldb, long long b_bytes, const int steps,
-                                      RH_LDS char* lds, const int b_limit = kStepBytes) {
-    Loader<T, kLA, S::kBM, S::kThreads> la;
-    Loader<T, kLB, S::kBN, S::kThreads> lb;
+                                      RH_LDS char* lds, const int a_limit = kStepBytes,
+                                      const int b_limit = kStepBytes) {
+    Loader<T, kLA, kPA, S::kBM, S::kThreads> la;
+    Loader<T, kLB, kPB, S::kBN, S::kThreads> lb;
     Fragments<T, kLA, S::kBM, S::kFM> fa;
     Fragments<T, kLB, S::kBN, S::kFN> fb;
     constexpr int kOffB = S::kBM * kStepBytes;
@@ -254,17 +287,34 @@ struct Tile {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     if (steps <= 0) return;
-    constexpr bool kTail = kLB == kRows;      // rows of b may end inside the last step
-    constexpr int kOpsA = Loader<T, kLA, S::kBM, S::kThreads>::kOps;
-    constexpr int kOpsB = Loader<T, kLB, S::kBN, S::kThreads>::kOps;
+    // where k ends inside the last step: the rows of a plain kRows operand do, and kCols ones (panels are
+    // padded in k along the row)
+    constexpr bool kTailA = kLA == kCols, kTailB = kLB == kCols || !kPB;
+    constexpr int kFull = kStepBytes;      // more than either kind of limit needs
+    constexpr int kOpsA = Loader<T, kLA, kPA, S::kBM, S::kThreads>::kOps;
+    constexpr int kOpsB = Loader<T, kLB, kPB, S::kBN, S::kThreads>::kOps;
+    static_assert(kOpsA == kOpsB, "both operands' tiles are of one size");
+    // where this wave's loads of a stage go
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds + wave * 1024);
+    auto plan = [&](const int s) {
+      la.plan(s < steps);
+      lb.plan(s < steps);
+    };
+    auto begin = [&](const int s) {      // step s's loads, to its place in the ring
+      const unsigned stage = to + (s & (kRing - 1)) * S::kStage;
+      la.begin(stage, s + 1 == steps ? a_limit : kFull);
+      lb.begin(stage + kOffB, s + 1 == steps ? b_limit : kFull);
+    };
+    auto load_a = [&](auto i) { la.template load<kTailA, decltype(i)::value>(); };
+    auto load_b = [&](auto i) { lb.template load<kTailB, decltype(i)::value>(); };
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      la.begin(lds + s * S::kStage, s < steps, kStepBytes);
-      lb.begin(lds + s * S::kStage + kOffB, s < steps, s + 1 == steps ? b_limit : kStepBytes);
-      la.template load<false>(0, kOpsA);
-      lb.template load<kTail>(0, kOpsB);
-      if (s == 0) stage_wait();
+    for (int s = 0; s < kRing; ++s) {
+      plan(s);
+      begin(s);
+      each<kOpsA>(load_a);
+      if (s < kRing - 1) each<kOpsB>(load_b);      // the last one's follow in the loop
     }
+    stage_wait<(kRing - 1) * (kOpsA + kOpsB) - kOpsB>();
     u32x4 x[2][S::kFM], y[2][S::kFN];
     constexpr int kSlots = S::kFM * S::kFN, kFragments = S::kFM + S::kFN;
     // Fragment f of a quarter, in the order the products take them: y0 x0 y1 .. yn x1 .. xm.
@@ -274,42 +324,32 @@ struct Tile {
       else if (f <= S::kFN) y[to][f - 1] = fb.read(stage + kOffB, f - 1, kk);
       else x[to][f - S::kFN] = fa.read(stage, f - S::kFN, kk);
     };
-    // A quarter's products, with what comes next issued between them: while one instruction runs on
+    // A half step's products, with what comes next issued between them: while one instruction runs on
     // the matrix unit (32 cycles) the wave has time for about seven others.
-    auto quarter = [&](const int from, const RH_LDS char* stage, const int kk, const bool load) {
-#pragma unroll
-      for (int t = 0; t < kSlots; ++t) {
+    auto half_step = [&](auto from, const RH_LDS char* stage, auto kk, auto load, auto beside) {
+      constexpr int kFrom = decltype(from)::value;
+      each<kSlots>([&](auto slot) {
+        constexpr int t = decltype(slot)::value;
         acc[t / S::kFN][t % S::kFN] =
-            TypeOf<T>::mma(y[from][t % S::kFN], x[from][t / S::kFN], acc[t / S::kFN][t % S::kFN]);
-        if (t < kFragments) read(from ^ 1, stage, kk, t);
-        if (load) {
-          constexpr int kA = kOpsA / kSlots, kB = kOpsB / kSlots;
-          static_assert(kSlots <= 4 || kOpsA + kOpsB == kSlots, "a load a slot");
-          if constexpr (kOpsA + kOpsB == kSlots) {
-            if (t < kOpsA) la.template load<false>(t, 1);
-            else lb.template load<kTail>(t - kOpsA, 1);
-          } else {
-            la.template load<false>(t * kA, kA);
-            lb.template load<kTail>(t * kB, kB);
-          }
-        }
+            TypeOf<T>::mma(y[kFrom][t % S::kFN], x[kFrom][t / S::kFN], acc[t / S::kFN][t % S::kFN]);
+        if constexpr (t < kFragments) read(kFrom ^ 1, stage, decltype(kk)::value, t);
+        if constexpr (t * kOpsA % kSlots == 0) load(Int<t * kOpsA / kSlots>());
+        else if constexpr (t == kSlots / 2 + 1) beside();
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
     };
+    static_assert(kSlots >= kFragments && kSlots % kOpsA == 0, "a fragment, and at most one load, a product");
 #pragma unroll
     for (int f = 0; f < kFragments; ++f) read(0, lds, 0, f);
     for (int s = 0; s < steps; ++s) {
-      RH_LDS char* here = lds + (s & 1) * S::kStage;
-      RH_LDS char* next = lds + ((s + 1) & 1) * S::kStage;
-      quarter(0, here, 1, false);
-      quarter(1, here, 2, false);
-      quarter(0, here, 3, false);
-      stage_wait();
-      la.begin(here, s + 2 < steps, kStepBytes);
-      lb.begin(here + kOffB, s + 2 < steps, s + 3 == steps ? b_limit : kStepBytes);
-      quarter(1, next, 0, true);
+      const RH_LDS char* const here = lds + (s & (kRing - 1)) * S::kStage;
+      const RH_LDS char* const next = lds + ((s + 1) & (kRing - 1)) * S::kStage;
+      half_step(Int<0>(), here, Int<1>(), load_b, [&] { plan(s + kRing); });
+      stage_wait<(kRing - 2) * (kOpsA + kOpsB)>();      // step s is read out, step s + 1 has landed
+      begin(s + kRing);
+      half_step(Int<1>(), next, Int<0>(), load_a, [] {});
     }
-    stage_wait();      // LDS is the caller's again
+    stage_wait<0>();      // LDS is the caller's again
   }
 };
 

@@ -52,11 +52,76 @@ struct RowInfo {
   float* scale;    // [1] s * expected upstream gradient
 };
 
-// Where column `c` of the chunk's place `r` lies in an array of panels of `rows` rows (in elements).
-template <typename T>
+// Where column `c` of row `r` lies in an array of panels of `rows` rows (in elements).
 __device__ __forceinline__ long long in_panels(const int r, const int c, const long long rows) {
-  constexpr int kC = kStepBytes / (int)sizeof(T);
-  return ((long long)(c / kC) * rows + r) * kC + c % kC;
+  return ((long long)(c / kStepK) * rows + r) * kStepK + c % kStepK;
+}
+
+// Eight values as the matrix units' operand: the values themselves, or a float's three parts.
+template <typename T>
+struct Eight {
+  u32x4 part[TypeOf<T>::kParts];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> in_parts(const float (&f)[8]) {
+  typedef typename TypeOf<T>::Part P;
+  Eight<T> out;
+  union {
+    P v[8];
+    u32x4 u;
+  } w[TypeOf<T>::kParts];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    float left = f[k];
+#pragma unroll
+    for (int i = 0; i < TypeOf<T>::kParts; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        // the nearest bfloat16, but not infinity for a finite number
+        const float most = 3.38953139e38f;
+        const float near = __builtin_fabsf(left) > most && __builtin_fabsf(left) < __builtin_inff()
+                               ? __builtin_copysignf(most, left) : left;
+        w[i].v[k] = (P)near;
+        left -= (float)w[i].v[k];
+      } else {
+        w[i].v[k] = (P)left;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TypeOf<T>::kParts; ++i) out.part[i] = w[i].u;
+  return out;
+}
+
+// Eight values from p on, of which `have` exist (the others are zero), in parts.
+template <typename T>
+__device__ __forceinline__ Eight<T> load_parts(const T* p, const int have, const bool wide) {
+  if constexpr (sizeof(T) == 2) {
+    union {
+      T v[8];
+      Eight<T> e;
+    } w;
+    if (wide && have >= 8) {
+      w.e.part[0] = *(const u32x4*)p;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w.v[k] = k < have ? p[k] : (T)0.0f;
+    }
+    return w.e;
+  } else {
+    float f[8];
+    if (wide && have >= 8) {
+      const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f[k] = a[k];
+        f[4 + k] = b[k];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = k < have ? p[k] : 0.0f;
+    }
+    return in_parts<T>(f);
+  }
 }
 
 // Copies the rows that count to their places in the chunks' panels, padded with zeros to whole panels; sets
@@ -65,7 +130,8 @@ __device__ __forceinline__ long long in_panels(const int r, const int c, const l
 template <typename T>
 __global__ __launch_bounds__(kThreads) void place_rows_kernel(
     const T* __restrict__ x, const long long ldx, const int d, const Labels y, const int n, const int per,
-    const int2* __restrict__ blocks, T* __restrict__ xp, const int panels, const int chunk, const RowInfo info,
+    const int2* __restrict__ blocks, char* __restrict__ xp, const long long part, const int panels, const int chunk,
+    const RowInfo info,
     float* __restrict__ row_loss, T* __restrict__ dx, float* __restrict__ small, int* __restrict__ status,
     const float* __restrict__ total, const int mean, const float grad) {
   __shared__ int s_red[4], s_all[4], s_bad[4];
@@ -126,26 +192,17 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
   }
   __syncthreads();
   const bool wide = ((ldx * (long long)sizeof(T)) & 15) == 0 && ((uintptr_t)x & 15) == 0;
-  constexpr int kV = 16 / (int)sizeof(T), kC = kStepBytes / (int)sizeof(T);
   for (int p = blockIdx.y + gridDim.y * wave; p < panels; p += gridDim.y * 4) {
-    const int c = p * kC + (lane & 3) * kV;
+    const int c = p * kStepK + (lane & 3) * 8;
 #pragma unroll 2
     for (int r = lane >> 2; r < rows; r += 16) {
       const int to = s_place[r];
       if (to < 0) continue;
-      const T* src = x + (lo + r) * ldx + c;
-      union {
-        T v[kV];
-        u32x4 u;
-      } w;
-      if (wide && c + kV <= d) {
-        w.u = *(const u32x4*)src;
-      } else {
-#pragma unroll
-        for (int k = 0; k < kV; ++k) w.v[k] = c + k < d ? src[k] : (T)0.0f;
-      }
+      const Eight<T> w = load_parts<T>(x + (lo + r) * ldx + c, d - c, wide);
       const int in = to / chunk;
-      *(u32x4*)(xp + (long long)in * chunk * panels * kC + in_panels<T>(to - in * chunk, c, chunk)) = w.u;
+      char* dst = xp + ((long long)in * chunk * panels * kStepK + in_panels(to - in * chunk, c, chunk)) * 2;
+#pragma unroll
+      for (int i = 0; i < TypeOf<T>::kParts; ++i) *(u32x4*)(dst + i * part) = w.part[i];
     }
   }
   if (dx && first)
@@ -164,6 +221,23 @@ __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* __restrict_
   const int lane = threadIdx.x & 63;
   for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < v; r += (long long)gridDim.x * 4)
     for (int c = lane; c < ldp; c += 64) out[r * ldp + c] = c < d ? w[r * ldw + c] : (T)0.0f;
+}
+
+// The weights in panels and parts (float).
+template <typename T>
+__global__ __launch_bounds__(kThreads) void take_apart_kernel(const T* __restrict__ w, const long long ldw, const int d,
+                                                              const int v, const int panels, char* __restrict__ out,
+                                                              const long long part) {
+  const bool wide = ((ldw * (long long)sizeof(T)) & 15) == 0 && ((uintptr_t)w & 15) == 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 16 + (lane >> 2);
+  if (r >= v) return;
+  for (int p = blockIdx.y * 4 + wave; p < panels; p += gridDim.y * 4) {
+    const int c = p * kStepK + (lane & 3) * 8;
+    const Eight<T> e = load_parts<T>(w + (long long)r * ldw + c, d - c, wide);
+    char* dst = out + in_panels(r, c, v) * 2;
+#pragma unroll
+    for (int i = 0; i < TypeOf<T>::kParts; ++i) *(u32x4*)(dst + i * part) = e.part[i];
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -223,11 +297,11 @@ struct Kept<float> {
 
 template <typename T>
 struct LogitArgs {
-  const T* x;          // the chunk's placed rows, in panels of chunk_rows
-  long long x_bytes;
+  const char* x;       // the chunk's placed rows, in panels of chunk_rows
+  long long x_bytes, x_part;
   int chunk_rows;
-  const T* w;          // first class of this call
-  long long ldw, w_bytes;
+  const char* w;       // the weights: rows ldw bytes apart, or (float) panels, ldw from one to the next
+  long long ldw, w_bytes, w_part;
   const T* bias;
   int steps;           // of k
   int w_limit;         // bytes of the last step that are the weights' rows
@@ -239,7 +313,7 @@ struct LogitArgs {
   float2* stats;       // [group of classes][place]  (max, sum of exp above it)
   long long ld_stats;
   float* z_label;      // [place]
-  void* p;             // the logits kept, in panels of chunk_rows, of ldp columns
+  void* z;             // the logits kept, in panels of chunk_rows, of ldp columns
   int ldp;
 };
 
@@ -323,7 +397,7 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (there && 32 * j + 8 * q < room)
-              *(f32x4*)((float*)a.p + in_panels<float>(row, c0 + 32 * j + 8 * q, a.chunk_rows)) =
+              *(f32x4*)((float*)a.z + in_panels(row, c0 + 32 * j + 8 * q, a.chunk_rows)) =
                   f32x4{z[j][4 * q], z[j][4 * q + 1], z[j][4 * q + 2], z[j][4 * q + 3]};
       } else {
         // eight neighbouring columns a lane: the lower half of the wave takes the even groups of eight; two
@@ -345,8 +419,8 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
             }
             const u32x4 eight = whole_group(half_group[0], half_group[1]);
             if (there && n0 + wn + 32 * j < a.ldp)
-              *(u32x4*)((unsigned short*)a.p +
-                        in_panels<T>(row, n0 + wn + 32 * j, a.chunk_rows) + 8 * q + 8 * half) = eight;
+              *(u32x4*)((unsigned short*)a.z + in_panels(row, n0 + wn + 32 * j, a.chunk_rows) + 8 * q +
+                        8 * half) = eight;
           }
       }
     }
@@ -361,11 +435,11 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
   const int2 at = tile_at(a.grid, blockIdx.x);
   const int rows = a.chunk.rows(a.n_valid), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   if (m0 >= rows) return;
-  constexpr long long size = sizeof(T);
-  Tile<T, kRows, kPanels, kRows, gemm::kPlain, S> tile;
-  tile.run(a.x + (long long)m0 * (kStepBytes / size), (long long)a.chunk_rows * kStepBytes,
-           a.x_bytes - (long long)m0 * kStepBytes, a.w + n0 * a.ldw, a.ldw * size, a.w_bytes - n0 * a.ldw * size,
-           a.steps, lds, kStepBytes, a.w_limit);
+  constexpr bool kPW = sizeof(T) == 4;
+  const long long from = n0 * (kPW ? (long long)kStepBytes : a.ldw);
+  Tile<T, kRows, kPanels, kRows, kPW, S> tile;
+  tile.run(a.x + (long long)m0 * kStepBytes, (long long)a.chunk_rows * kStepBytes, a.x_bytes - (long long)m0 * kStepBytes,
+           a.x_part, a.w + from, a.ldw, a.w_bytes - from, a.w_part, a.steps, lds, kStepBytes, a.w_limit);
   if (!a.bias && n0 + S::kBN <= a.v)
     finish_logits<T, S, kWhat, true>(a, tile, m0, n0, rows);
   else
@@ -374,12 +448,13 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
 
 constexpr int kProbRows = 256;
 
-// P from the kept logits, in their place: p = e^(z - group's top) * (e^(group's top - row's top) / row's
+// P from the kept logits, in their place (float: beside them, in parts): p = e^(z - group's top) * (e^(group's top - row's top) / row's
 // sum), the first factor from the code.  A workgroup takes a group of classes (kPanelsOf panels) of
-// kProbRows places, a thread 16 bytes of each panel's row.  column_sums (or NULL): [row block][v] sums of P
+// kProbRows places, a thread eight columns of each panel's row.  column_sums (or NULL): [row block][v] sums of P
 // over its rows.  The first workgroup of the last chunk also adds up the loss (losses > 0).
 template <typename T, int kPanelsOf>
-__global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept, const int chunk_rows, const int ldp,
+__global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict__ kept, char* __restrict__ p_out,
+                                                         const long long part, const int chunk_rows, const int ldp,
                                                          const int v, const Chunk chunk,
                                                          const int* __restrict__ n_valid,
                                                          const int* __restrict__ label,
@@ -388,73 +463,63 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(void* __restrict__ kept
                                                          float* __restrict__ column_sums,
                                                          const double* __restrict__ loss_parts, const int losses,
                                                          float* __restrict__ small) {
-  constexpr int kV = 16 / (int)sizeof(T), kC = kStepBytes / (int)sizeof(T);
-  __shared__ float s_sum[4][kPanelsOf * kC];
+  constexpr int kWords = sizeof(T) == 4 ? 2 : 1;      // of 16 bytes that hold eight logits
+  __shared__ float s_sum[4][kPanelsOf * kStepK];
   if (losses && blockIdx.x == 0 && blockIdx.y == 0) add_losses(loss_parts, losses, small);
   const int rows = chunk.rows(n_valid), lo = blockIdx.y * kProbRows, hi = min(rows, lo + kProbRows);
-  const int t = threadIdx.x, first = blockIdx.x * kPanelsOf * kC, c = first + (t & 3) * kV;
+  const int t = threadIdx.x, first = blockIdx.x * kPanelsOf * kStepK, c = first + (t & 3) * 8;
   const float2* top = stats + (long long)blockIdx.x * ld_stats;
-  float sums[kPanelsOf][kV];
+  float sums[kPanelsOf][8];
 #pragma unroll
   for (int i = 0; i < kPanelsOf; ++i)
 #pragma unroll
-    for (int k = 0; k < kV; ++k) sums[i][k] = 0.0f;
+    for (int k = 0; k < 8; ++k) sums[i][k] = 0.0f;
   for (int r = lo + (t >> 2); r < hi; r += kThreads / 4) {
-    u32x4* const at = (u32x4*)((T*)kept + in_panels<T>(r, c, chunk_rows));
-    const long long next = (long long)chunk_rows * kStepBytes / 16;      // panel
-    u32x4 z[kPanelsOf];
+    const long long at = in_panels(r, c, chunk_rows), next = (long long)chunk_rows * kStepK;
+    u32x4 z[kPanelsOf][kWords];
 #pragma unroll
     for (int i = 0; i < kPanelsOf; ++i)
-      if (first + i * kC < ldp) z[i] = at[i * next];
+#pragma unroll
+      for (int k = 0; k < kWords; ++k)
+        if (first + i * kStepK < ldp) z[i][k] = ((const u32x4*)kept)[(at + i * next) / 8 * kWords + k];
     const float2 of_row = row_stats[r];
     const int y = label[r] - c;
     const float f = sizeof(T) == 4 ? of_row.y : exp_for<T>(top[r].x - of_row.x) * of_row.y;
 #pragma unroll
     for (int i = 0; i < kPanelsOf; ++i) {
-      if (first + i * kC >= ldp) continue;
-      float p[kV];
-      if constexpr (sizeof(T) == 4) {
-        const f32x4 w = __builtin_bit_cast(f32x4, z[i]);
+      if (first + i * kStepK >= ldp) continue;
+      float p[8];
 #pragma unroll
-        for (int k = 0; k < kV; ++k) p[k] = expf(w[k] - of_row.x) * f;
-      } else {
-#pragma unroll
-        for (int k = 0; k < kV; ++k) {
-          const unsigned w = z[i][k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
+      for (int k = 0; k < 8; ++k) {
+        if constexpr (sizeof(T) == 4) {
+          const unsigned w = z[i][k >> 2][k & 3];
+          p[k] = expf(__builtin_bit_cast(float, w) - of_row.x) * f;
+        } else {
+          const unsigned w = z[i][0][k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
           const float e = __builtin_amdgcn_exp2f((float)code * (-1.0f / Kept<T>::kSteps));
           p[k] = (code == 0xffffu ? 0.0f : e) * f;
         }
-      }
-#pragma unroll
-      for (int k = 0; k < kV; ++k) {
-        p[k] = y == i * kC + k ? p[k] - 1.0f : p[k];
+        p[k] = y == i * kStepK + k ? p[k] - 1.0f : p[k];
         sums[i][k] += p[k];
+        p[k] *= PScale<T>::up;
       }
-      u32x4 out;
-      if constexpr (sizeof(T) == 4) {
-        out = __builtin_bit_cast(u32x4, f32x4{p[0], p[1], p[2], p[3]});
-      } else {
+      const Eight<T> out = in_parts<T>(p);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const T a = TypeOf<T>::from_float(p[2 * k] * PScale<T>::up), b = TypeOf<T>::from_float(p[2 * k + 1] * PScale<T>::up);
-          out[k] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
-        }
-      }
-      at[i * next] = out;
+      for (int k = 0; k < TypeOf<T>::kParts; ++k) *(u32x4*)(p_out + k * part + (at + i * next) * 2) = out.part[k];
     }
   }
   if (!column_sums) return;
 #pragma unroll
   for (int i = 0; i < kPanelsOf; ++i)
 #pragma unroll
-    for (int k = 0; k < kV; ++k) {
+    for (int k = 0; k < 8; ++k) {
       float s = sums[i][k];
 #pragma unroll
       for (int o = 4; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
-      if ((t & 63) < 4) s_sum[t >> 6][i * kC + (t & 3) * kV + k] = s;
+      if ((t & 63) < 4) s_sum[t >> 6][i * kStepK + (t & 3) * 8 + k] = s;
     }
   __syncthreads();
-  for (int i = t; i < kPanelsOf * kC && first + i < v; i += kThreads)
+  for (int i = t; i < kPanelsOf * kStepK && first + i < v; i += kThreads)
     column_sums[(long long)blockIdx.y * v + first + i] = (s_sum[0][i] + s_sum[1][i]) + (s_sum[2][i] + s_sum[3][i]);
 }
 
@@ -519,11 +584,11 @@ __global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __r
 // ---------------------------------------------------------------------------------------------
 template <typename T>
 struct ProductArgs {
-  const T* p;                  // P in panels of chunk_rows
-  long long p_bytes;
+  const char* p;               // P in panels of chunk_rows
+  long long p_bytes, p_part;
   int chunk_rows;
-  const T* b;                  // dX: the weights, ldb apart; dW: the features in panels of chunk_rows
-  long long ldb, b_bytes;
+  const char* b;               // dX: the weights (rows, or panels, ldb bytes apart); dW: the features in panels
+  long long ldb, b_bytes, b_part;
   int m, n, k;                 // rows that count bound m (dX) or k (dW) on the device
   const int* n_valid;
   Chunk chunk;
@@ -547,23 +612,21 @@ template <typename T, Layout kLA, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  constexpr long long size = sizeof(T);
-  constexpr int kC = kStepBytes / (int)sizeof(T);      // values of k a step, columns a panel
   const int2 at = tile_at(a.grid, blockIdx.x);
   const int rows = max(a.chunk.rows(a.n_valid), 0), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   const int m = kLA == kRows ? rows : a.m, k = kLA == kCols ? rows : a.k;
   if (m0 >= m) return;
-  const int k0 = blockIdx.y * a.split_steps * kC;
-  const int steps = max(0, min(a.split_steps, (k - k0 + kC - 1) / kC));
-  const int last = k - k0 - (steps - 1) * kC;          // values of k in the last step
+  const int k0 = blockIdx.y * a.split_steps * kStepK;
+  const int steps = max(0, min(a.split_steps, (k - k0 + kStepK - 1) / kStepK));
+  const int last = k - k0 - (steps - 1) * kStepK;      // values of k in the last step
   const long long panel = (long long)a.chunk_rows * kStepBytes;
-  const long long from = kLA == kRows ? k0 / kC * panel + (long long)m0 * kStepBytes
-                                      : m0 / kC * panel + (long long)k0 * kStepBytes;
-  constexpr bool kPB = kLA == kCols;
-  const long long from_b = kPB ? n0 / kC * panel + (long long)k0 * kStepBytes : (k0 * a.ldb + n0) * size;
+  const long long from = kLA == kRows ? k0 / kStepK * panel + (long long)m0 * kStepBytes
+                                      : m0 / kStepK * panel + (long long)k0 * kStepBytes;
+  constexpr bool kPB = kLA == kCols || sizeof(T) == 4;
+  const long long from_b = kPB ? n0 / kStepK * a.ldb + (long long)k0 * kStepBytes : k0 * a.ldb + n0 * (int)sizeof(T);
   Tile<T, kLA, kPanels, kCols, kPB, S> tile;
-  tile.run((const char*)a.p + from, panel, a.p_bytes - from, (const char*)a.b + from_b, kPB ? panel : a.ldb * size,
-           a.b_bytes - from_b, steps, lds, last, last);
+  tile.run(a.p + from, panel, a.p_bytes - from, a.p_part, a.b + from_b, a.ldb, a.b_bytes - from_b, a.b_part, steps, lds, last,
+           last);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32 + 4 * (lane >> 5);
   const float s = *a.scale * a.down;
@@ -686,7 +749,8 @@ constexpr int kMostChunk = 1 << 22;              // rows; eight panels' offsets 
 // operations in all), P takes their place, and the chunk's part of the weight's gradient is added to the
 // others' in float32 where there are several.
 struct Plan {
-  int size, step_k;
+  int size, parts;              // bytes of a value; numbers that it is taken apart into
+  int kept_size;                // bytes of a kept logit
   int per, row_blocks;          // rows a placing block takes
   int panels;                   // of the features
   int ldw_pad;                  // row of the copied weights (0: not copied)
@@ -718,13 +782,14 @@ static int splits_for(long long m, long long n, int steps, bool large) {
 static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   Plan p = {};
   p.size = dtype == RH_F32 ? 4 : 2;
-  p.step_k = kStepBytes / p.size;
+  p.parts = dtype == RH_F32 ? 3 : 1;
+  p.kept_size = dtype == RH_F32 ? 4 : 2;
   p.per = n > 65536 ? 256 : 32;
   p.row_blocks = ceil_div(n, p.per);
-  p.panels = ceil_div(d, p.step_k);
-  p.ldw_pad = flags & RH_CE_COPY_WEIGHT ? ceil_div(d, p.step_k) * p.step_k : 0;
+  p.panels = ceil_div(d, kStepK);
+  p.ldw_pad = dtype != RH_F32 && (flags & RH_CE_COPY_WEIGHT) ? p.panels * kStepK : 0;
   p.ldp = ceil_div(v, 64) * 64;
-  long long rows = kKeptBytes / ((long long)p.ldp * p.size) / 256 * 256;
+  long long rows = kKeptBytes / ((long long)p.ldp * p.kept_size) / 256 * 256;
   if (rows < 256) rows = 256;
   if (rows > kMostChunk) rows = kMostChunk;
   p.chunk = n;
@@ -739,7 +804,7 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   p.groups = ceil_div(v, p.large_logits ? Large::kBN : Small::kBN) * (p.large_logits ? Large::kWN : Small::kWN);
   p.large_dx = take_large(p.chunk, d);
   p.large_dw = take_large(v, d);
-  const int k_dx = ceil_div(p.ldp, p.step_k), k_dw = ceil_div(p.chunk, p.step_k);
+  const int k_dx = ceil_div(p.ldp, kStepK), k_dw = ceil_div(p.chunk, kStepK);
   p.dx_splits = splits_for(p.chunk, d, k_dx, p.large_dx);
   p.dx_steps = ceil_div(k_dx, p.dx_splits);
   p.dw_splits = splits_for(v, d, k_dw, p.large_dw);
@@ -752,12 +817,16 @@ struct Space {
   int2* blocks;
   RowInfo info;
   char* x;
+  long long x_part;      // bytes of each of the features' parts, ...
   char* w;
+  long long w_part;
   float2* stats;
   float* z_label;
   float2* row_stats;
   double* loss;
-  char* p;
+  char* z;
+  char* p;               // z's place for the 16-bit types
+  long long p_part;
   float* dx_part;
   float* dw_part;
   float* db_part;
@@ -773,13 +842,22 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   s.info.label = c.take<int>(n);
   s.info.n_valid = c.take<int>(1);
   s.info.scale = c.take<float>(1);
-  s.x = c.take<char>((size_t)p.chunks * p.chunk * p.panels * kStepBytes);
+  s.x_part = (long long)p.chunks * p.chunk * p.panels * kStepBytes;
+  s.x = c.take<char>((size_t)s.x_part * p.parts);
   if (p.ldw_pad) s.w = c.take<char>((size_t)v * p.ldw_pad * p.size);
+  if (p.parts > 1) {
+    s.w_part = (long long)v * p.panels * kStepBytes;
+    s.w = c.take<char>((size_t)s.w_part * p.parts);
+  }
   s.stats = c.take<float2>((size_t)p.groups * p.chunk);
   s.z_label = c.take<float>(n);
   s.row_stats = c.take<float2>(n);
   s.loss = c.take<double>(ceil_div(n, 32));
-  if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) s.p = c.take<char>((size_t)p.chunk * p.ldp * p.size);
+  if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) {
+    s.z = c.take<char>((size_t)p.chunk * p.ldp * p.kept_size);
+    s.p_part = (long long)p.chunk * p.ldp * 2;
+    s.p = p.parts > 1 ? c.take<char>((size_t)s.p_part * p.parts) : s.z;
+  }
   if ((flags & RH_CE_GRAD_X) && p.dx_splits > 1)
     s.dx_part = c.take<float>((size_t)p.dx_splits * p.chunk * p.ldpart);
   if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw_splits > 1))
@@ -825,8 +903,8 @@ template <typename T, int kPanelsOf>
 static int launch_probs(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a, int chunk,
                         hipStream_t stream) {
   const int blocks = ceil_div(p.chunk, kProbRows);
-  hipLaunchKernelGGL((probs_kernel<T, kPanelsOf>), dim3(ceil_div(p.ldp, p.group), blocks), dim3(kThreads), 0, stream, s.p,
-                     p.chunk, p.ldp, a.v, a.chunk, a.n_valid, a.label, s.row_stats + a.chunk.first, s.stats, a.ld_stats,
+  hipLaunchKernelGGL((probs_kernel<T, kPanelsOf>), dim3(ceil_div(p.ldp, p.group), blocks), dim3(kThreads), 0, stream, s.z,
+                     s.p, s.p_part, p.chunk, p.ldp, a.v, a.chunk, a.n_valid, a.label, s.row_stats + a.chunk.first, s.stats, a.ld_stats,
                      s.db_part ? s.db_part + (long long)chunk * blocks * a.v : nullptr, s.loss,
                      chunk == p.chunks - 1 ? ceil_div(q.n, 32) : 0, q.small);
   RH_CHECK_LAUNCH("probs_kernel");
@@ -847,8 +925,9 @@ static int join_parts(const ProductArgs<T>& g, int splits, bool by_rows, hipStre
 template <typename T>
 static ProductArgs<T> product_args(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a) {
   ProductArgs<T> g = {};
-  g.p = (const T*)s.p;
-  g.p_bytes = (long long)p.chunk * p.ldp * p.size;
+  g.p = s.p;
+  g.p_bytes = s.p_part;
+  g.p_part = s.p_part;
   g.chunk_rows = p.chunk;
   g.n = q.d;
   g.n_valid = a.n_valid;
@@ -868,6 +947,7 @@ static int features_gradient(const rh_linear_ce_args& q, const Plan& p, const Sp
   g.b = a.w;
   g.ldb = a.ldw;
   g.b_bytes = a.w_bytes;
+  g.b_part = a.w_part;
   g.m = a.chunk.most;
   g.k = a.v;
   g.split_steps = p.dx_steps;
@@ -887,7 +967,9 @@ static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Spac
                            int chunk, hipStream_t stream) {
   ProductArgs<T> g = product_args(q, p, s, a);
   g.b = a.x;
+  g.ldb = (long long)p.chunk * kStepBytes;
   g.b_bytes = a.x_bytes;
+  g.b_part = a.x_part;
   g.m = a.v;
   g.k = a.chunk.most;
   g.split_steps = p.dw_steps;
@@ -905,45 +987,53 @@ template <typename T>
 static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStream_t stream) {
   const int n = (int)q.n, d = q.d, v = (int)q.v;
   const Labels labels{q.labels, q.labels_int64, q.ignore_index, v};
-  T* const x = (T*)s.x;
   hipLaunchKernelGGL(count_rows_kernel, dim3(p.row_blocks), dim3(64), 0, stream, labels, n, p.per, s.blocks);
   RH_CHECK_LAUNCH("count_rows_kernel");
   const int side = ceil_div(p.panels, 16) < 8 ? ceil_div(p.panels, 16) : 8;
   hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks, side), dim3(kThreads), 0, stream, (const T*)q.x,
-                     (long long)q.ldx, d, labels, n, p.per, s.blocks, x, p.panels, p.chunk, s.info, q.row_loss, (T*)q.dx,
-                     q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
+                     (long long)q.ldx, d, labels, n, p.per, s.blocks, s.x, s.x_part, p.panels, p.chunk, s.info, q.row_loss,
+                     (T*)q.dx, q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
   RH_CHECK_LAUNCH("place_rows_kernel");
-  const T* w = (const T*)q.w;
-  long long ldw = q.ldw;
-  if (p.ldw_pad) {
-    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(v < 8192 ? ceil_div(v, 4) : 2048), dim3(kThreads), 0, stream, w, ldw, d, v,
-                       (T*)s.w, p.ldw_pad);
-    RH_CHECK_LAUNCH("pad_rows_kernel");
-    w = (const T*)s.w;
-    ldw = p.ldw_pad;
-  }
-  const long long d_w = p.ldw_pad ? p.ldw_pad : d;
   const bool grads = q.dx || q.dw || q.db;
-
   LogitArgs<T> a = {};
   a.chunk_rows = p.chunk;
   a.x_bytes = (long long)p.chunk * p.panels * kStepBytes;
-  a.w = w;
-  a.ldw = ldw;
-  a.w_bytes = ((v - 1) * ldw + d_w) * p.size;
-  a.bias = (const T*)q.bias;
+  a.x_part = s.x_part;
+  a.w = (const char*)q.w;
+  a.ldw = q.ldw * p.size;
+  a.w_bytes = (v - 1) * a.ldw + (long long)d * p.size;
   a.steps = p.panels;
-  a.w_limit = (int)(d_w * p.size - (long long)(a.steps - 1) * kStepBytes);
+  a.w_limit = d * 2 - (a.steps - 1) * kStepBytes;
+  if (p.ldw_pad) {
+    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(v < 8192 ? ceil_div(v, 4) : 2048), dim3(kThreads), 0, stream, (const T*)q.w,
+                       (long long)q.ldw, d, v, (T*)s.w, p.ldw_pad);
+    RH_CHECK_LAUNCH("pad_rows_kernel");
+    a.w = s.w;
+    a.ldw = (long long)p.ldw_pad * p.size;
+    a.w_bytes = v * a.ldw;
+    a.w_limit = kStepBytes;
+  }
+  if (p.parts > 1) {
+    hipLaunchKernelGGL(take_apart_kernel<T>, dim3(ceil_div(v, 16), ceil_div(p.panels, 16) < 16 ? ceil_div(p.panels, 16) : 16),
+                       dim3(kThreads), 0, stream, (const T*)q.w, (long long)q.ldw, d, v, p.panels, s.w, s.w_part);
+    RH_CHECK_LAUNCH("take_apart_kernel");
+    a.w = s.w;
+    a.ldw = (long long)v * kStepBytes;
+    a.w_bytes = s.w_part;
+    a.w_part = s.w_part;
+    a.w_limit = kStepBytes;
+  }
+  a.bias = (const T*)q.bias;
   a.v = v;
   a.n_valid = s.info.n_valid;
   a.stats = s.stats;
   a.ld_stats = p.chunk;
-  a.p = s.p;
+  a.z = s.z;
   a.ldp = p.ldp;
   for (int c = 0; c < p.chunks; ++c) {
     a.chunk = Chunk{c * p.chunk, n - c * p.chunk < p.chunk ? n - c * p.chunk : p.chunk};
     const int first = a.chunk.first;
-    a.x = x + (long long)first * p.panels * p.step_k;
+    a.x = s.x + (long long)first * p.panels * kStepBytes;
     a.label = s.info.label + first;
     a.z_label = s.z_label + first;
     if (int rc = grads ? p.large_logits ? launch_logits<T, Large, kKeep>(a, stream)
@@ -956,10 +1046,8 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
                        s.loss + first / 32);
     RH_CHECK_LAUNCH("join_stats_kernel");
     if (!grads) continue;
-    const int panels = p.group * p.size / kStepBytes;      // of a group of classes
-    if (int rc = panels == 8   ? launch_probs<T, 8>(q, p, s, a, c, stream)
-                 : panels == 4 ? launch_probs<T, 4>(q, p, s, a, c, stream)
-                               : launch_probs<T, 2>(q, p, s, a, c, stream))
+    if (int rc = p.large_logits ? launch_probs<T, Large::kFN * 32 / kStepK>(q, p, s, a, c, stream)
+                                : launch_probs<T, Small::kFN * 32 / kStepK>(q, p, s, a, c, stream))
       return rc;
     if (q.dx)
       if (int rc = features_gradient(q, p, s, a, stream)) return rc;
@@ -1012,7 +1100,7 @@ int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream) {
   if (q.dw) flags |= RH_CE_GRAD_W;
   if (q.db) flags |= RH_CE_GRAD_B;
   RH_REQUIRE((flags & RH_CE_COPY_WEIGHT) ||
-                 (rh::aligned16(q.w) && q.d * size % 16 == 0 && q.ldw * size % 16 == 0 && q.ldw < (1 << 20)),
+                 q.dtype == RH_F32 || (rh::aligned16(q.w) && q.d * size % 16 == 0 && q.ldw * size % 16 == 0 && q.ldw < (1 << 20)),
              RH_EALIGN, "weights whose rows are not whole 16-byte pieces need RH_CE_COPY_WEIGHT");
   RH_REQUIRE(((uintptr_t)q.dx | (uintptr_t)q.dw) % 16 == 0, RH_EALIGN, "gradients must be 16-byte aligned");
   if (q.n <= rh::ce::kFewRows) {

@@ -5,8 +5,13 @@
 // copies:   kRows  element (i,k) at  base + i*ld + k   (the sum runs along a row)
 //           kCols  element (i,k) at  base + k*ld + i   (the sum runs down a column)
 // Both are staged as they lie in memory.  A kRows tile holds 64 bytes of k per row and its 16-byte
-// fragments are read as they are; a kCols tile of a 16-bit type is read with the transposing LDS
-// load, one of a 32-bit type element by element.
+// fragments are read as they are; a kCols tile is read with the transposing LDS load.
+//
+// float operands are taken apart into three bfloat16 numbers, x = x0 + x1 + x2, each the nearest to what
+// is left: |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, exact but for what lies below bfloat16's range.  Of the nine
+// products of two of them the six of 2^-18 and up are summed, smallest first; the rest is below 2^-26 of
+// the product, a quarter of what one float32 rounding of it would be.  Six bfloat16 instructions do what
+// eight of float32 (32x32x2) do at a quarter of their time each.
 //
 // What this library lays out itself (the features, P) it lays out in panels of 64 bytes of columns, the
 // rows of a panel one after the other: the tiles of either layout are then runs of whole kilobytes.
@@ -32,30 +37,27 @@ typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 enum Layout { kRows = 0, kCols = 1 };
 constexpr bool kPlain = false, kPanels = true;
 
-// 64 bytes of k per tile step: 32 values of a 16-bit type, 16 of float; two quarters (kk) of the matrix
-// instructions' depth each.
+// 64 bytes of k per tile step: 32 values, two halves (kk) of the matrix instructions' depth each.  A panel
+// has as many columns.
 constexpr int kStepBytes = 64;
+constexpr int kStepK = 32;
 constexpr int kRing = 4;
 
 template <typename T>
 struct TypeOf;
 template <>
 struct TypeOf<float> {
-  static __device__ __forceinline__ f32x16 mma(const u32x4 a, const u32x4 b, f32x16 c) {
-    // lane half h holds k = 4h .. 4h+3 of eight; both operands agree, so instruction j sums the
-    // pair {j, 4+j}
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[0], y[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[1], y[1], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[2], y[2], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[3], y[3], c, 0, 0, 0);
-    return c;
-  }
+  typedef __bf16 Part;      // what the matrix units are given
+  static constexpr int kParts = 3, kTerms = 6;
+  static constexpr unsigned kOrderA = 0x010120, kOrderB = 0x001102;      // term t: parts (nibble t) of a and b
   static __device__ __forceinline__ float to_float(float v) { return v; }
   static __device__ __forceinline__ float from_float(float v) { return v; }
 };
 template <>
 struct TypeOf<__bf16> {
+  typedef __bf16 Part;
+  static constexpr int kParts = 1, kTerms = 1;
+  static constexpr unsigned kOrderA = 0, kOrderB = 0;
   static __device__ __forceinline__ f32x16 mma(const u32x4 a, const u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -65,6 +67,9 @@ struct TypeOf<__bf16> {
 };
 template <>
 struct TypeOf<_Float16> {
+  typedef _Float16 Part;
+  static constexpr int kParts = 1, kTerms = 1;
+  static constexpr unsigned kOrderA = 0, kOrderB = 0;
   static __device__ __forceinline__ f32x16 mma(const u32x4 a, const u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -136,30 +141,43 @@ __device__ __forceinline__ void each(const F f) {      // f(Int<0>) .. f(Int<kN 
   }
 }
 
-// Moves one stage of an operand's tile (kR rows or columns of the result, kStepBytes of k) to LDS.
-template <typename T, Layout kL, bool kPaneled, int kR, int kThreads>
+// Moves one stage of an operand's tile (kR rows or columns of the result, kStepBytes of k) to LDS.  The
+// steps go through k once for every term, through the part of the operand that kOrder names for it.
+template <Layout kL, bool kPaneled, int kR, int kThreads, int kTerms, unsigned kOrder>
 struct Loader {
-  static constexpr int kStepK = kStepBytes / (int)sizeof(T);
   static constexpr int kOps = kR * kStepBytes / (kThreads * 16);
-  static constexpr int kRowBytes = kL == kRows ? kStepBytes : kR * (int)sizeof(T);
+  static constexpr int kRowBytes = kL == kRows ? kStepBytes : kR * 2;
   static constexpr int kChunks = kRowBytes / 16;             // 16-byte chunks of a staged row
   static constexpr int kRowsPerOp = kThreads / kChunks;      // staged rows one pass of all threads covers
   int offset[kOps];       // this lane's byte offsets from the tile's first element
   const char* base;       // of the coming step
   long long left;         // bytes readable from base on
   long long step;         // bytes from one step to the next
+  const char* origin;
+  long long bytes, part;
+  int steps, at, term;
 
   static __device__ __forceinline__ int row_of(const int i) { return i * kRowsPerOp + (int)threadIdx.x / kChunks; }
   static __device__ __forceinline__ int chunk_of(const int i) {
     const int row = row_of(i), at = (int)threadIdx.x % kChunks;
-    if (kL == kRows) return at ^ ((row >> 2) & 3);
-    return sizeof(T) == 2 ? at ^ ((row & 3) << 2) : at;    // 16 bits: 32-byte blocks, block ^ 2*(k & 3)
+    return kL == kRows ? at ^ ((row >> 2) & 3) : at ^ ((row & 3) << 2);    // kCols: 32-byte blocks, block ^ 2*(k & 3)
   }
-  // origin: first element of the tile at k = 0; stride: bytes from row to row, or from panel to panel;
-  // bytes: readable from origin on.
-  __device__ __forceinline__ void init(const void* origin, long long stride, long long bytes) {
-    base = (const char*)origin;
+  __device__ __forceinline__ void to_term() {
+    const long long off = (kOrder >> (4 * term) & 15) * part;
+    base = origin + off;
     left = bytes;
+    at = 0;
+  }
+  // from: first element of the tile at k = 0; stride: bytes from row to row, or from panel to panel;
+  // readable: bytes from `from` on, in each part; parts: bytes from part to part; n: steps of a term.
+  __device__ __forceinline__ void init(const void* from, long long stride, long long readable, long long parts,
+                                       int n) {
+    origin = (const char*)from;
+    bytes = readable;
+    part = parts;
+    steps = n;
+    term = 0;
+    to_term();
     if (kPaneled) step = kL == kRows ? stride : kStepK * kStepBytes;
     else step = kL == kRows ? kStepBytes : kStepK * stride;
 #pragma unroll
@@ -183,6 +201,10 @@ struct Loader {
     asm volatile("s_nop 4" : "+s"(coming));
     base += step;
     left -= step;
+    if (kTerms > 1 && ++at == steps) {
+      ++term;
+      to_term();
+    }
   }
   __device__ __forceinline__ void begin(const unsigned stage, const int k_limit) {
     rsrc = coming;
@@ -198,10 +220,10 @@ struct Loader {
 
 // Reads the matrix instructions' fragments of one wave from a staged tile.  `first`: the wave's
 // first row / column of the tile (a multiple of 32); fragment f covers 32 from first + 32 f on.
-template <typename T, Layout kL, int kR, int kF>
+template <Layout kL, int kR, int kF>
 struct Fragments {
-  static constexpr int kRowBytes = kR * (int)sizeof(T);      // kCols only
-  static constexpr int kAddr = kL == kRows ? 2 : (sizeof(T) == 2 ? kF : 1);
+  static constexpr int kRowBytes = kR * 2;      // kCols only
+  static constexpr int kAddr = kL == kRows ? 2 : kF;
   int addr[kAddr];
   __device__ __forceinline__ void init(const int first) {
     const int l = (int)threadIdx.x & 63;
@@ -209,20 +231,18 @@ struct Fragments {
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
         addr[kk] = (first + (l & 31)) * kStepBytes + (((2 * kk + (l >> 5)) ^ ((l >> 2) & 3)) << 4);
-    } else if (sizeof(T) == 2) {
+    } else {
       const int q = (l >> 2) & 3;
 #pragma unroll
       for (int f = 0; f < kAddr; ++f)
         addr[f] = (8 * (l >> 5) + q) * kRowBytes + (((first / 32 + f) ^ q) << 6) + ((l >> 4) & 1) * 32 +
                   (l & 3) * 8;
-    } else {
-      addr[0] = 4 * (l >> 5) * kRowBytes + (first + (l & 31)) * 4;
     }
   }
   __device__ __forceinline__ u32x4 read(const RH_LDS char* stage, const int f, const int kk) const {
     if constexpr (kL == kRows) {
       return *(const RH_LDS u32x4*)(stage + addr[kk] + f * 32 * kStepBytes);
-    } else if constexpr (sizeof(T) == 2) {
+    } else {
       union {
         bf16x4 h[2];
         u32x4 u;
@@ -231,12 +251,6 @@ struct Fragments {
       r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((RH_LDS bf16x4*)p);
       r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((RH_LDS bf16x4*)(p + 4 * kRowBytes));
       return r.u;
-    } else {
-      const RH_LDS char* p = stage + addr[0] + f * 128 + kk * 8 * kRowBytes;
-      u32x4 r;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = *(const RH_LDS unsigned*)(p + j * kRowBytes);
-      return r;
     }
   }
 };
@@ -255,29 +269,33 @@ struct Shape {
 // of the wave's part: a lane owns rows, four neighbouring columns at a time.
 template <typename T, Layout kLA, bool kPA, Layout kLB, bool kPB, typename S>
 struct Tile {
-  static constexpr int kStepK = kStepBytes / (int)sizeof(T);
+  typedef TypeOf<T> Type;
+  typedef Loader<kLA, kPA, S::kBM, S::kThreads, Type::kTerms, Type::kOrderA> LoaderA;
+  typedef Loader<kLB, kPB, S::kBN, S::kThreads, Type::kTerms, Type::kOrderB> LoaderB;
   f32x16 acc[S::kFM][S::kFN];
 
   // a / b: first elements of the tile's operands at the first k; lda, ldb: bytes from row to row or from
-  // panel to panel; *_bytes: readable from there; steps: k steps (of kStepK values); a_limit, b_limit: how
-  // much of the last one is the operand's (kCols: values; plain kRows: bytes of a row).
+  // panel to panel; *_bytes: readable from there; *_part: bytes from one part of the numbers to the next
+  // (float); steps: k steps (of kStepK values); a_limit, b_limit: how much of the last one is the operand's
+  // (kCols: values; plain kRows: bytes of a row).
   //
   // Fragments are read one half step ahead of the instructions that take them, and the loads of a
   // stage are spread over the step that frees its place in the ring, nearly three steps before it is
   // read.  8192 x 4096 x 16384 in bfloat16, uniform values: two stages of twice the depth, their loads in one
   // burst, 1.04-1.10 PFLOP/s; this 1.12-1.16 (1.6-1.7 on zeros: the card's power sets its clock).
-  __device__ __forceinline__ void run(const void* a, long long lda, long long a_bytes, const void* b,
-                                      long long ldb, long long b_bytes, const int steps,
-                                      RH_LDS char* lds, const int a_limit = kStepBytes,
+  __device__ __forceinline__ void run(const void* a, long long lda, long long a_bytes, long long a_part,
+                                      const void* b, long long ldb, long long b_bytes, long long b_part,
+                                      const int steps_of_k, RH_LDS char* lds, const int a_limit = kStepBytes,
                                       const int b_limit = kStepBytes) {
-    Loader<T, kLA, kPA, S::kBM, S::kThreads> la;
-    Loader<T, kLB, kPB, S::kBN, S::kThreads> lb;
-    Fragments<T, kLA, S::kBM, S::kFM> fa;
-    Fragments<T, kLB, S::kBN, S::kFN> fb;
+    LoaderA la;
+    LoaderB lb;
+    Fragments<kLA, S::kBM, S::kFM> fa;
+    Fragments<kLB, S::kBN, S::kFN> fb;
+    const int steps = steps_of_k * Type::kTerms;
     constexpr int kOffB = S::kBM * kStepBytes;
     const int wave = (int)threadIdx.x >> 6;
-    la.init(a, lda, a_bytes);
-    lb.init(b, ldb, b_bytes);
+    la.init(a, lda, a_bytes, a_part, steps_of_k);
+    lb.init(b, ldb, b_bytes, b_part, steps_of_k);
     fa.init((wave / S::kWN) * S::kFM * 32);
     fb.init((wave % S::kWN) * S::kFN * 32);
 #pragma unroll
@@ -291,8 +309,8 @@ struct Tile {
     // padded in k along the row)
     constexpr bool kTailA = kLA == kCols, kTailB = kLB == kCols || !kPB;
     constexpr int kFull = kStepBytes;      // more than either kind of limit needs
-    constexpr int kOpsA = Loader<T, kLA, kPA, S::kBM, S::kThreads>::kOps;
-    constexpr int kOpsB = Loader<T, kLB, kPB, S::kBN, S::kThreads>::kOps;
+    constexpr int kOpsA = LoaderA::kOps;
+    constexpr int kOpsB = LoaderB::kOps;
     static_assert(kOpsA == kOpsB, "both operands' tiles are of one size");
     // where this wave's loads of a stage go
     const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds + wave * 1024);
@@ -300,10 +318,12 @@ struct Tile {
       la.plan(s < steps);
       lb.plan(s < steps);
     };
+    int last = steps_of_k - 1;      // the step that ends the running term
     auto begin = [&](const int s) {      // step s's loads, to its place in the ring
       const unsigned stage = to + (s & (kRing - 1)) * S::kStage;
-      la.begin(stage, s + 1 == steps ? a_limit : kFull);
-      lb.begin(stage + kOffB, s + 1 == steps ? b_limit : kFull);
+      la.begin(stage, s == last ? a_limit : kFull);
+      lb.begin(stage + kOffB, s == last ? b_limit : kFull);
+      if (Type::kTerms > 1 && s == last) last += steps_of_k;
     };
     auto load_a = [&](auto i) { la.template load<kTailA, decltype(i)::value>(); };
     auto load_b = [&](auto i) { lb.template load<kTailB, decltype(i)::value>(); };
@@ -331,7 +351,7 @@ struct Tile {
       each<kSlots>([&](auto slot) {
         constexpr int t = decltype(slot)::value;
         acc[t / S::kFN][t % S::kFN] =
-            TypeOf<T>::mma(y[kFrom][t % S::kFN], x[kFrom][t / S::kFN], acc[t / S::kFN][t % S::kFN]);
+            TypeOf<typename Type::Part>::mma(y[kFrom][t % S::kFN], x[kFrom][t / S::kFN], acc[t / S::kFN][t % S::kFN]);
         if constexpr (t < kFragments) read(kFrom ^ 1, stage, decltype(kk)::value, t);
         if constexpr (t * kOpsA % kSlots == 0) load(Int<t * kOpsA / kSlots>());
         else if constexpr (t == kSlots / 2 + 1) beside();

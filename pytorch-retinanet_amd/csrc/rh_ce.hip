@@ -745,6 +745,42 @@ typedef Shape<2, 2, 2, 2> Small;      // 128 x 128, 4 waves
 constexpr long long kKeptBytes = 2ll << 30;      // of logits at a time, or 256 rows of them
 constexpr int kMostChunk = 1 << 22;              // rows; eight panels' offsets stay below 2^31
 
+// How a product is cut up: the tiles' shape, and into how many sums along k its sum is split.
+struct Cut {
+  bool large;
+  int splits, steps;      // k steps of a split
+};
+
+// The cut of the least estimated time.  The card takes 256 tiles of 256 x 256 at a time or 512 of 128 x 128;
+// a step takes the longer the more of it is at work (the clock sinks, the tiles share the caches): 0.58 to
+// 0.88 us in a large tile, 0.26 to 0.56 in a small one.  A tile's start and end take 14 and 6 us, joining
+// the splits 4 us and their bytes' way at 4.5 TB/s.  Of 8192 x 8192 logits over 256 features, the first of
+// each pair is the small tiles' time: 80 / 94 us; over 1024: 194 / 182.  49 104 x 601 over 256: 40 / 67.
+// dX of 2048 x 1024 over 16 384 classes, float: 893 us unsplit, 499 of four splits, large and eight of
+// them 380.  200 x 512 over 10 000, bfloat16: 83 unsplit, 18 of sixteen, large 29 at best.
+static Cut cut(long long m, long long n, int steps, int terms, int most_splits) {
+  Cut best = {};
+  float least = 0.0f;
+  for (int large = 0; large < 2; ++large) {
+    const int side = large ? 256 : 128, slots = large ? 256 : 512;
+    const long long tiles = (long long)ceil_div(m, side) * ceil_div(n, side);
+    for (int splits = 1; splits <= most_splits && (splits == 1 || steps / splits >= 4); ++splits) {
+      const Cut c = {large != 0, splits, ceil_div(steps, splits)};
+      if (ceil_div(steps, c.steps) < splits) continue;      // the last would be empty
+      const long long work = tiles * splits;
+      const float filled = work < slots ? (float)work / slots : 1.0f;
+      float us = (float)((work + slots - 1) / slots) *
+                 (((large ? 0.58f : 0.26f) + 0.30f * filled) * (float)c.steps * (float)terms + (large ? 14.0f : 6.0f));
+      if (splits > 1) us += 4.0f + (float)splits * (float)m * (float)n * (4.0f / 4.5e6f);
+      if (least == 0.0f || us < least) {
+        least = us;
+        best = c;
+      }
+    }
+  }
+  return best;
+}
+
 // The call's rows are taken in chunks whose logits take kKeptBytes at most: they are made once (6 n d v
 // operations in all), P takes their place, and the chunk's part of the weight's gradient is added to the
 // others' in float32 where there are several.
@@ -756,28 +792,11 @@ struct Plan {
   int ldw_pad;                  // row of the copied weights (0: not copied)
   int chunk, chunks;            // rows at a time
   int ldp;                      // columns of P
-  bool large_logits, large_dx, large_dw;
+  bool large_logits;
   int group, groups;            // classes a wave of the logits' tiles takes
-  int dx_splits, dx_steps, dw_splits, dw_steps;
+  Cut dx, dw;
   long long ldpart;
 };
-
-// Tiles of 256 x 256 move half the bytes per product of those of 128 x 128, which fill the card
-// with a quarter of the work.
-static bool take_large(long long m, long long n) {
-  return m > 128 && n > 128 && (long long)ceil_div(m, 256) * ceil_div(n, 256) >= 128;
-}
-
-// Splits of the sum over k: as many as fill the card, each of eight steps at least.
-static int splits_for(long long m, long long n, int steps, bool large) {
-  const long long tiles = large ? (long long)ceil_div(m, 256) * ceil_div(n, 256)
-                                : (long long)ceil_div(m, 128) * ceil_div(n, 128);
-  const long long want = large ? 256 : 512;
-  long long s = tiles >= want ? 1 : want / tiles;
-  if (s > steps / 8) s = steps / 8;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : (int)s;
-}
 
 static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   Plan p = {};
@@ -799,16 +818,12 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
     p.chunk = ceil_div(ceil_div(n, p.chunks), 256) * 256;      // of even size
     p.chunks = ceil_div(n, p.chunk);
   }
-  p.large_logits = take_large(p.chunk, v);
+  const int terms = dtype == RH_F32 ? TypeOf<float>::kTerms : 1;
+  p.large_logits = cut(p.chunk, v, p.panels, terms, 1).large;
   p.group = p.large_logits ? Large::kFN * 32 : Small::kFN * 32;
   p.groups = ceil_div(v, p.large_logits ? Large::kBN : Small::kBN) * (p.large_logits ? Large::kWN : Small::kWN);
-  p.large_dx = take_large(p.chunk, d);
-  p.large_dw = take_large(v, d);
-  const int k_dx = ceil_div(p.ldp, kStepK), k_dw = ceil_div(p.chunk, kStepK);
-  p.dx_splits = splits_for(p.chunk, d, k_dx, p.large_dx);
-  p.dx_steps = ceil_div(k_dx, p.dx_splits);
-  p.dw_splits = splits_for(v, d, k_dw, p.large_dw);
-  p.dw_steps = ceil_div(k_dw, p.dw_splits);
+  p.dx = cut(p.chunk, d, p.ldp / kStepK, terms, 64);
+  p.dw = cut(v, d, ceil_div(p.chunk, kStepK), terms, 64);
   p.ldpart = ceil_div(d, 4) * 4;
   return p;
 }
@@ -858,10 +873,10 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
     s.p_part = (long long)p.chunk * p.ldp * 2;
     s.p = p.parts > 1 ? c.take<char>((size_t)s.p_part * p.parts) : s.z;
   }
-  if ((flags & RH_CE_GRAD_X) && p.dx_splits > 1)
-    s.dx_part = c.take<float>((size_t)p.dx_splits * p.chunk * p.ldpart);
-  if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw_splits > 1))
-    s.dw_part = c.take<float>((size_t)p.dw_splits * v * p.ldpart);
+  if ((flags & RH_CE_GRAD_X) && p.dx.splits > 1)
+    s.dx_part = c.take<float>((size_t)p.dx.splits * p.chunk * p.ldpart);
+  if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw.splits > 1))
+    s.dw_part = c.take<float>((size_t)p.dw.splits * v * p.ldpart);
   if (flags & RH_CE_GRAD_B) {
     s.db_parts = ceil_div(p.chunk, kProbRows) * p.chunks;
     s.db_part = c.take<float>((size_t)s.db_parts * v);
@@ -950,15 +965,15 @@ static int features_gradient(const rh_linear_ce_args& q, const Plan& p, const Sp
   g.b_part = a.w_part;
   g.m = a.chunk.most;
   g.k = a.v;
-  g.split_steps = p.dx_steps;
+  g.split_steps = p.dx.steps;
   g.out = (T*)q.dx;
   g.map = s.info.map + a.chunk.first;
   g.part = s.dx_part;
   g.plane = (long long)p.chunk * p.ldpart;
-  if (int rc = p.large_dx ? launch_product<T, kRows, Large>(g, p.dx_splits, stream)
-                          : launch_product<T, kRows, Small>(g, p.dx_splits, stream))
+  if (int rc = p.dx.large ? launch_product<T, kRows, Large>(g, p.dx.splits, stream)
+                          : launch_product<T, kRows, Small>(g, p.dx.splits, stream))
     return rc;
-  return s.dx_part ? join_parts(g, p.dx_splits, true, stream) : RH_OK;
+  return s.dx_part ? join_parts(g, p.dx.splits, true, stream) : RH_OK;
 }
 
 // dW, or a chunk's part of it.
@@ -972,15 +987,15 @@ static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Spac
   g.b_part = a.x_part;
   g.m = a.v;
   g.k = a.chunk.most;
-  g.split_steps = p.dw_steps;
+  g.split_steps = p.dw.steps;
   g.out = (T*)q.dw;
   g.part = s.dw_part;
   g.plane = (long long)a.v * p.ldpart;
   g.add = chunk > 0;
-  if (int rc = p.large_dw ? launch_product<T, kCols, Large>(g, p.dw_splits, stream)
-                          : launch_product<T, kCols, Small>(g, p.dw_splits, stream))
+  if (int rc = p.dw.large ? launch_product<T, kCols, Large>(g, p.dw.splits, stream)
+                          : launch_product<T, kCols, Small>(g, p.dw.splits, stream))
     return rc;
-  return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, p.dw_splits, false, stream) : RH_OK;
+  return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, p.dw.splits, false, stream) : RH_OK;
 }
 
 template <typename T>

@@ -1115,7 +1115,7 @@ int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream) {
   if (q.dw) flags |= RH_CE_GRAD_W;
   if (q.db) flags |= RH_CE_GRAD_B;
   RH_REQUIRE((flags & RH_CE_COPY_WEIGHT) ||
-                 q.dtype == RH_F32 || (rh::aligned16(q.w) && q.d * size % 16 == 0 && q.ldw * size % 16 == 0 && q.ldw < (1 << 20)),
+                 (rh::aligned16(q.w) && q.d * size % 16 == 0 && q.ldw * size % 16 == 0 && q.ldw < (1 << 20)),
              RH_EALIGN, "weights whose rows are not whole 16-byte pieces need RH_CE_COPY_WEIGHT");
   RH_REQUIRE(((uintptr_t)q.dx | (uintptr_t)q.dw) % 16 == 0, RH_EALIGN, "gradients must be 16-byte aligned");
   if (q.n <= rh::ce::kFewRows) {

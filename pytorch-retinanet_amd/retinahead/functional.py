@@ -574,10 +574,6 @@ class ClassifierOutputs(dict):
     def __contains__(self, key):
         return dict.__contains__(self, key) or key in _CE_SMALL_VIEWS
 
-    def without_grads(self):
-        return ClassifierOutputs(small=dict.__getitem__(self, "small"),
-                                 row_loss=dict.__getitem__(self, "row_loss"))
-
 
 def _dtype_code(t):
     code = _DTYPES.get(t.dtype)
@@ -596,74 +592,37 @@ def linear_cross_entropy(features, weight, labels, bias=None, ignore_index=-100,
     float32 [1] tensor.  Returns a dict: ``loss``, ``row_loss`` (float32, the labels' shape; 0 for a
     row left out), ``num_valid``, ``status`` and the gradients asked for as ``d_features``,
     ``d_weight``, ``d_bias``."""
-    dev = _dev_check(features, weight, labels, bias, divisor)
-    code = _dtype_code(features)
-    if weight.dtype != features.dtype or (bias is not None and bias.dtype != features.dtype):
-        raise RetinaHeadError("features, weight and bias must have one element type")
-    if weight.dim() != 2 or features.dim() < 1 or features.shape[-1] != weight.shape[1]:
-        raise RetinaHeadError("expected features [..., D] and weight [V, D]")
-    if tuple(labels.shape) != tuple(features.shape[:-1]):
-        raise RetinaHeadError("labels must have the features' shape without the last dimension")
-    if labels.dtype not in (torch.int64, torch.int32):
-        raise RetinaHeadError("labels must be int64 or int32")
-    v, d = weight.shape
-    if bias is not None and tuple(bias.shape) != (v,):
-        raise RetinaHeadError("bias must be [V]")
-    if v < 1 or d < 1:
-        raise RetinaHeadError("linear_cross_entropy needs at least one class and one feature")
+    small, row_loss, *made = _classifier_loss(features, weight, labels, bias, divisor, ignore_index,
+                                              reduction, expected_grad, grads, False)
+    out = ClassifierOutputs(small=small, row_loss=row_loss)
+    for key, grad in zip(("d_features", "d_weight", "d_bias"), made):
+        if grad is not None:
+            out[key] = grad
+    return out
+
+
+def _classifier_loss(features, weight, labels, bias, divisor, ignore_index, reduction, expected_grad, grads, node):
+    """``_host.linear_ce``: its checks of the tensors, its outputs."""
     if reduction not in _lib.CE_REDUCTIONS:
         raise ValueError("reduction must be 'mean' or 'sum'")
-    if divisor is not None and (divisor.dtype != torch.float32 or divisor.numel() != 1):
-        raise RetinaHeadError("divisor must be one float32")
     if float(expected_grad) == 0.0:
         raise ValueError("expected_grad must not be zero")
-    n = labels.numel()
-    out = ClassifierOutputs(small=torch.empty((4,), dtype=torch.float32, device=dev),
-                            row_loss=torch.empty(labels.shape, dtype=torch.float32, device=dev))
-    if grads[0]:
-        out["d_features"] = torch.empty(features.shape, dtype=features.dtype, device=dev)
-    if grads[1]:
-        out["d_weight"] = torch.empty((v, d), dtype=features.dtype, device=dev)
-    if grads[2] and bias is not None:
-        out["d_bias"] = torch.empty((v,), dtype=features.dtype, device=dev)
-    if n == 0:
-        for t in out.values():
-            t.zero_()
-        return out
-    x = features.reshape(n, d)
-    if x.stride(1) != 1 or x.stride(0) < d:
-        x = x.contiguous()
-    w = weight
-    flags = 0
-    if w.stride(1) != 1 or w.stride(0) < d:
-        w = w.contiguous()
-    size = w.element_size()
-    if d * size % 16 or w.stride(0) * size % 16 or w.data_ptr() % 16 or w.stride(0) >= 1 << 20:
-        flags = _lib.CE_COPY_WEIGHT
-    y = labels.reshape(n).contiguous()
-    b = None if bias is None else bias.contiguous()
-    ptr = lambda t: None if t is None else t.data_ptr()
-    dx, dw, db = out.get("d_features"), out.get("d_weight"), out.get("d_bias")
+    if not _bound:
+        _bind_host()
+    return _host.linear_ce(features, weight, labels, bias, divisor, ignore_index, _lib.CE_REDUCTIONS[reduction],
+                           expected_grad, *grads, node)
+
+
+_bound = False
+
+
+def _bind_host():
+    global _bound
     lib = _lib.load()
-    ask = (flags | (_lib.CE_GRAD_X if dx is not None else 0) | (_lib.CE_GRAD_W if dw is not None else 0)
-           | (_lib.CE_GRAD_B if db is not None else 0))
-    key = ("linear_ce", n, d, v, code, ask)
-    need = _ws_bytes_cache.get(key)
-    if need is None:
-        need = lib.rh_linear_ce_workspace_bytes(n, d, v, code, ask)
-        if need == 0:
-            raise RetinaHeadError("linear_cross_entropy: " + _lib.last_error())
-        _ws_bytes_cache[key] = need
-    with _on_device(dev) as stream:
-        ws = workspace(dev, need, "linear_ce", stream)
-        args = _lib.LinearCeArgs(
-            x.data_ptr(), w.data_ptr(), ptr(b), y.data_ptr(), n, v, x.stride(0) if n > 1 else d,
-            w.stride(0) if v > 1 else max(d, w.stride(0)), d, code, int(y.dtype == torch.int64),
-            _lib.CE_REDUCTIONS[reduction], int(ignore_index), ptr(divisor), float(expected_grad), flags,
-            out["row_loss"].data_ptr(), out["small"].data_ptr(), ptr(dx), ptr(dw), ptr(db), ws.data_ptr(),
-            ws.numel())
-        _lib.check(lib.rh_linear_ce(C.byref(args), stream), "rh_linear_ce")
-    return out
+    at = lambda f: C.cast(f, C.c_void_p).value
+    _host.bind(at(lib.rh_linear_ce_workspace_bytes), at(lib.rh_linear_ce), at(lib.rh_scale_gradient),
+               at(lib.rh_last_error), workspace, RetinaHeadError)
+    _bound = True
 
 
 def scale_gradient_(grad, scale, assumed=1.0):

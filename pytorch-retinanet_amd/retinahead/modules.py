@@ -12,7 +12,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _host, _lib
 from . import functional as F
 from ._lib import RetinaHeadError
 
@@ -76,7 +76,9 @@ def _unit_gradient(dev):
         with _UNIT_LOCK:        # replicas on several devices start from several threads
             unit = _UNIT.get(dev.index)
             if unit is None:
-                unit = _UNIT[dev.index] = torch.ones(1, dtype=torch.float32, device=dev)
+                unit = torch.ones(1, dtype=torch.float32, device=dev)
+                _host.know_unit(dev.index, unit.data_ptr())
+                _UNIT[dev.index] = unit
     return unit
 
 
@@ -459,33 +461,7 @@ class GenericFocalLoss(nn.Module):
                                      bool(self.logits), bool(self.reduce))
 
 
-class _LinearCrossEntropyFn(torch.autograd.Function):
-    """As _DenseHeadLossFn: the forward call makes the gradients, backward applies the upstream one."""
-
-    @staticmethod
-    def forward(ctx, features, weight, bias, labels, divisor, cfg, grad_mode):
-        need = [grad_mode and ctx.needs_input_grad[i] for i in range(3)]
-        out = F.linear_cross_entropy(features, weight, labels, bias, ignore_index=cfg["ignore_index"],
-                                     reduction=cfg["reduction"], divisor=divisor,
-                                     expected_grad=cfg["expected_grad"], grads=need)
-        ctx.grads = [out.get(k) for k in ("d_features", "d_weight", "d_bias")]
-        ctx.expected = cfg["expected_grad"]
-        cfg["state"].set(features.device, out.without_grads())
-        small = out["small"]
-        return small.new_empty(0).set_(small.untyped_storage(), small.storage_offset(), (1,))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        if ctx.grads is None:
-            raise RetinaHeadError("the fused loss keeps one set of gradients: backward() can run "
-                                  "once per forward()")
-        grads, ctx.grads = ctx.grads, None
-        if not (ctx.expected == 1.0 and _is_unit(g)):
-            for d in grads:
-                if d is not None:
-                    F.scale_gradient_(d, g, ctx.expected)
-        return (*grads, None, None, None, None)
+_NO_GRADS = (False, False, False)      # the autograd node asks for those that are needed
 
 
 class LinearCrossEntropy(nn.Module):
@@ -536,8 +512,10 @@ class LinearCrossEntropy(nn.Module):
         return self.cfg["state"].by_device
 
     def forward(self, features, weight, labels, bias=None, divisor=None):
-        loss = _LinearCrossEntropyFn.apply(features, weight, bias, labels, divisor, self.cfg,
-                                           torch.is_grad_enabled())
+        cfg = self.cfg
+        loss, small, row_loss = F._classifier_loss(features, weight, labels, bias, divisor, cfg["ignore_index"],
+                                                   cfg["reduction"], cfg["expected_grad"], _NO_GRADS, True)
+        cfg["state"].set(features.device, F.ClassifierOutputs(small=small, row_loss=row_loss))
         if self.check_labels and int(self.last["status"].item()) & _lib.RH_STATUS_LABEL_RANGE:
             raise IndexError("label outside [0, classes)")
         loss = loss.as_subclass(_LossTensor)

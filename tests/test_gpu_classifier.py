@@ -331,6 +331,41 @@ def test_module_gradients_and_upstream(rh):
         assert not fn(leaves[0], leaves[1], y, leaves[2]).requires_grad
 
 
+def test_backward_of_the_node(rh):
+    """Some of the leaves, a graph of the gradients, a kept graph, a loss changed in place."""
+    x, w, y, b = make(40, 64, 90, "f32", True, seed=16)
+    want = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    fn = rh.LinearCrossEntropy()
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    loss = fn(leaves[0], leaves[1], y, leaves[2])
+    loss.backward(inputs=[leaves[1]])
+    assert torch.equal(leaves[1].grad, want["d_weight"]) and leaves[0].grad is None and leaves[2].grad is None
+    # the gradients themselves cannot be differentiated, and say so instead of counting as constants
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    (g,) = torch.autograd.grad(fn(leaves[0], leaves[1], y, leaves[2]), leaves[0], create_graph=True)
+    assert torch.equal(g.detach(), want["d_features"])
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+    # one set of gradients, kept graph or not
+    loss = fn(leaves[0], leaves[1], y, leaves[2])
+    loss.backward(retain_graph=True)
+    with pytest.raises(rh.RetinaHeadError, match="once"):
+        loss.backward()
+    # in place, and a non-leaf input
+    for t in leaves:
+        t.grad = None
+    loss = fn(leaves[0] * 2.0, leaves[1], y, leaves[2])
+    loss /= 4
+    loss.backward()
+    double = rh.functional.linear_cross_entropy(x * 2.0, w, y, b, grads=(True, True, True))
+    assert torch.equal(leaves[0].grad, double["d_features"] * 0.5)
+    assert torch.equal(leaves[1].grad, double["d_weight"] * 0.25)
+    # under inference mode and without any tensor that requires gradients
+    with torch.inference_mode():
+        assert torch.equal(fn(x, w, y, b), want["loss"])
+    assert fn(x, w, y, b).grad_fn is None
+
+
 def test_gradient_against_differences(rh):
     x, w, y, b = make(12, 16, 20, "f32", True, seed=7)
     out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))

@@ -1,11 +1,13 @@
-// The classifier loss for a few rows (gfx950).  With so few rows the weights' bytes are what counts:
-// they are read for the logits and again for the gradients, whose bytes are written.  Four launches:
+// The classifier loss for a few rows (gfx950).  With so few rows the weights' bytes are what counts.
+// Four launches:
 //
 //   logits      z[row][class] in float32, 16 classes x 16 rows to a matrix instruction that takes the
 //               weights straight from memory, and each workgroup's (max, sum of exp) of every row
 //   rows        the rows' (max, 1 / sum), losses and the call's loss
 //   gradients   one more pass over the weights: dW rows written, dX summed per workgroup; P stays float32
 //   features    the workgroups' parts of dX joined
+//
+// Up to four rows whose sums fit a workgroup's registers read the weights once: see `online`.
 #include "rh_ce.h"
 
 namespace rh {
@@ -75,6 +77,7 @@ struct FewSpace {
   float2* row;         // [kFewRows]  (max, 1 / sum), of a row that counts
   float* scale;        // [1]
   float* dx_part;      // [parts][n][ldpart]
+  float* share;        // [n][parts]: what a row's part counts (online)
   size_t bytes;
 };
 
@@ -85,7 +88,30 @@ struct FewPlan {
   int grad_blocks, per;             // classes a workgroup takes
   int parts, ldpart;
   bool wide_w;
+  int rows, chunks;                 // online: rows (a power of two) and 16-byte pieces of columns a thread; else 0
 };
+
+// Online: dX = sum of p W without P's normalisation, which is not known before the last class.  A workgroup
+// takes whole rows of weights, so what a thread read for the logits is still in its registers when their
+// exponentials are known: dX's sum is kept relative to the running maximum and joined like a softmax's.
+// The weights are read once; dW is written by the gradients' pass, which then reads none.
+// 1 x 2048 rows, 65 536 classes, bfloat16 (268 MB of weights, as much of dW): 208 us with two readings, 145
+// with one (87 this pass, 45 the one that writes), 4.1 TB/s over both.  Loads for the next classes issued ahead, more
+// workgroups or contiguous runs of classes for each: no faster; what they read was written behind the caches.
+static void plan_online(FewPlan& p, int n, int d, int v, int vals) {
+  p.rows = n <= 1 ? 1 : n <= 2 ? 2 : 4;
+  p.chunks = ceil_div(d, kThreads * vals);
+  if (p.chunks == 3) p.chunks = 4;
+  if (n > 4 || p.rows * p.chunks > 4 || 2 * d < kThreads * vals) {      // or half of the threads idle
+    p.rows = p.chunks = 0;
+    return;
+  }
+  const int at_once = 16 / (p.rows * p.chunks);
+  p.blocks = ceil_div(v, 2 * at_once);
+  if (p.blocks > 512) p.blocks = 512;
+  p.parts = p.blocks;
+  p.ldpart = p.chunks * kThreads * vals;
+}
 
 static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
   FewPlan p = {};
@@ -107,6 +133,7 @@ static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
   p.parts = p.grad_blocks * p.subsets;
   p.ldpart = p.slices * p.tpr * vals;
   p.wide_w = !(flags & RH_CE_COPY_WEIGHT);      // here that only says how the weights are read
+  if (flags & RH_CE_GRAD_X) plan_online(p, n, d, v, vals);
   return p;
 }
 
@@ -118,6 +145,7 @@ static FewSpace few_space(void* base, const FewPlan& p, int n, int flags) {
   s.row = c.take<float2>(kFewRows);
   s.scale = c.take<float>(1);
   if (flags & RH_CE_GRAD_X) s.dx_part = c.take<float>((size_t)p.parts * n * p.ldpart);
+  if (p.rows) s.share = c.take<float>((size_t)n * p.parts);
   s.bytes = c.off;
   return s;
 }
@@ -215,6 +243,140 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
   }
 }
 
+template <int kRotate>
+__device__ __forceinline__ float rotated(const float x) {      // within each 16 lanes
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + kRotate, 0xf, 0xf, true));
+}
+// Of every 16 lanes, over those whose number is the same modulo kN.
+template <int kN, typename F>
+__device__ __forceinline__ float over_classes(float x, const F f) {
+  x = f(x, rotated<8>(x));
+  if constexpr (kN <= 4) x = f(x, rotated<4>(x));
+  if constexpr (kN <= 2) x = f(x, rotated<2>(x));
+  if constexpr (kN <= 1) x = f(x, rotated<1>(x));
+  return x;
+}
+
+// kA classes at a time, a value (class, row) each lane of 16: value i = class i / kN, row i % kN.
+template <typename T, int kN, int kC, bool kWide>
+__global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restrict__ x, const long long ldx, const int n,
+                                                              const int d, const T* __restrict__ w, const long long ldw,
+                                                              const int v, const T* __restrict__ bias, const Labels y,
+                                                              float* __restrict__ z, const int ldz,
+                                                              float2* __restrict__ part, float* __restrict__ dx_part,
+                                                              const int ldpart) {
+  constexpr int kV = 16 / (int)sizeof(T), kA = 16 / (kN * kC), kVals = kA * kN;
+  __shared__ f32x4 s_z[2][16];      // [value], one sum of each wave
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15;
+  float xs[kN][kC][kV], acc[kN][kC][kV];
+#pragma unroll
+  for (int r = 0; r < kN; ++r) {
+    const bool keep = r < n && y.counts(y.at(r));      // what a row left out holds must not meet its zeros
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+      const int c = (j * kThreads + t) * kV;
+      to_floats<T>(keep ? load_values<T, false>(x + r * ldx + c, d - c) : u32x4{0, 0, 0, 0}, xs[r][j]);
+#pragma unroll
+      for (int k = 0; k < kV; ++k) acc[r][j][k] = 0.0f;
+    }
+  }
+  float top = -__builtin_inff(), sum = 0.0f;      // of row in % kN, the same in all waves
+  int odd = 0;
+  for (int v0 = blockIdx.x * kA; v0 < v; v0 += gridDim.x * kA, odd ^= 1) {
+    u32x4 ws[kA][kC];
+#pragma unroll
+    for (int a = 0; a < kA; ++a)
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        const int c = (j * kThreads + t) * kV;
+        ws[a][j] = load_values<T, kWide>(w + (long long)min(v0 + a, v - 1) * ldw + c, d - c);
+      }
+    float part_of[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part_of[i] = 0.0f;
+#pragma unroll
+    for (int a = 0; a < kA; ++a)
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        float f[kV];
+        to_floats<T>(ws[a][j], f);
+#pragma unroll
+        for (int r = 0; r < kN; ++r)
+#pragma unroll
+          for (int k = 0; k < kV; ++k) part_of[a * kN + r] = __builtin_fmaf(f[k], xs[r][j][k], part_of[a * kN + r]);
+      }
+    // sums over the wave: values 4 g .. 4 g + 3 end in the 16 lanes of row g
+    float eight[8], four[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, part_of[i]),
+                                                      __builtin_bit_cast(unsigned, part_of[i + 8]), false, false);
+      const unsigned s0 = s[0], s1 = s[1];
+      eight[i] = __builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, eight[i]),
+                                                      __builtin_bit_cast(unsigned, eight[i + 4]), false, false);
+      const unsigned s0 = s[0], s1 = s[1];
+      four[i] = over_classes<1>(__builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1),
+                                [](float p, float q) { return p + q; });
+    }
+    const int value = in + 4 * (lane >> 4);      // of lanes 0 .. 3 of a row
+    const float mine = in == 0 ? four[0] : in == 1 ? four[1] : in == 2 ? four[2] : four[3];
+    if (in < 4) ((float*)&s_z[odd][value])[wave] = mine;
+    __syncthreads();      // the other half is written next time, when all have read this one
+    const f32x4 of_waves = s_z[odd][in];
+    const int a = in / kN, r = in % kN, c = v0 + a;
+    const bool real = in < kVals && c < v;
+    float logit = (of_waves[0] + of_waves[1]) + (of_waves[2] + of_waves[3]);
+    if (bias && real) logit += TypeOf<T>::to_float(bias[c]);
+    if (!real) logit = -__builtin_inff();
+    if (real && t < 16 && r < n) z[(long long)r * ldz + c] = logit;
+    const float up = fmaxf(top, over_classes<kN>(logit, [](float p, float q) { return fmaxf(p, q); }));
+    const float base = up == -__builtin_inff() ? 0.0f : up;
+    const float e = expf(logit - base), shrink = expf(top - base);
+    sum = sum * shrink + over_classes<kN>(e, [](float p, float q) { return p + q; });
+    if (__builtin_amdgcn_ballot_w64(top != up)) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, shrink), i));
+#pragma unroll
+        for (int j = 0; j < kC; ++j)
+#pragma unroll
+          for (int k = 0; k < kV; ++k) acc[i][j][k] *= f;
+      }
+    }
+    top = up;
+#pragma unroll
+    for (int i = 0; i < kA; ++i)
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        float f[kV];
+        to_floats<T>(ws[i][j], f);
+#pragma unroll
+        for (int q = 0; q < kN; ++q) {
+          const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), i * kN + q));
+#pragma unroll
+          for (int k = 0; k < kV; ++k) acc[q][j][k] = __builtin_fmaf(p, f[k], acc[q][j][k]);
+        }
+      }
+  }
+  if (t < kN) part[t * gridDim.x + blockIdx.x] = make_float2(top, sum);
+#pragma unroll
+  for (int r = 0; r < kN; ++r)
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+      const int c = (j * kThreads + t) * kV;
+      if (r < n) {
+        float* to = dx_part + ((long long)blockIdx.x * n + r) * ldpart + c;
+#pragma unroll
+        for (int k = 0; k < kV; k += 4)
+          *(f32x4*)(to + k) = f32x4{acc[r][j][k], acc[r][j][k + 1], acc[r][j][k + 2], acc[r][j][k + 3]};
+      }
+    }
+}
+
 // One wave a row.
 __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* __restrict__ part, const int blocks,
                                                                  const Labels y, const int n,
@@ -223,17 +385,19 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
                                                                  const float grad, float2* __restrict__ row,
                                                                  float* __restrict__ scale,
                                                                  float* __restrict__ row_loss,
-                                                                 float* __restrict__ small, int* __restrict__ status) {
+                                                                 float* __restrict__ small, int* __restrict__ status,
+                                                                 float* __restrict__ share) {
   __shared__ float s_loss[kFewRows];
   __shared__ int s_keep[kFewRows], s_bad[kFewRows];
   const int r = threadIdx.x >> 6, lane = threadIdx.x & 63;
   float top = -__builtin_inff(), sum = 0.0f;
-  for (int i = lane; i < blocks; i += 64) {
-    const float2 p = part[r * blocks + i];
-    const float up = fmaxf(top, p.x), base = up == -__builtin_inff() ? 0.0f : up;
-    sum = sum * expf(top - base) + p.y * expf(p.x - base);
-    top = up;
-  }
+  if (r < n)
+    for (int i = lane; i < blocks; i += 64) {
+      const float2 p = part[r * blocks + i];
+      const float up = fmaxf(top, p.x), base = up == -__builtin_inff() ? 0.0f : up;
+      sum = sum * expf(top - base) + p.y * expf(p.x - base);
+      top = up;
+    }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float other = __shfl_xor(top, o, 64), more = __shfl_xor(sum, o, 64);
@@ -241,9 +405,14 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
     sum = sum * expf(top - base) + more * expf(other - base);
     top = up;
   }
+  const long long label = r < n ? y.at(r) : y.ignore;
+  const bool keep = r < n && y.counts(label);
+  if (share && r < n) {
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    for (int i = lane; i < blocks; i += 64)
+      share[r * blocks + i] = keep ? expf(part[r * blocks + i].x - base) / sum : 0.0f;
+  }
   if (lane == 0) {
-    const long long label = r < n ? y.at(r) : y.ignore;
-    const bool keep = r < n && y.counts(label);
     float loss = 0.0f;
     if (keep) {
       loss = (top - z[(long long)r * ldz + label]) + logf(sum);
@@ -398,24 +567,48 @@ __global__ __launch_bounds__(kThreads) void few_gradients_kernel(
   }
 }
 
-// Four columns of a row by 16 threads, each every 16th part.
+// Four columns of a row by 64 threads, each every 64th part.  With `share` (online) the parts are weighed
+// by it, the label's weights taken off and the sum scaled here.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __restrict__ part, const int parts,
                                                                 const int n, const int ldpart, const int d,
+                                                                const float* __restrict__ share,
+                                                                const float* __restrict__ scale, const Labels y,
+                                                                const T* __restrict__ w, const long long ldw,
                                                                 T* __restrict__ dx) {
-  __shared__ f32x4 s_sum[16][16];
-  const int quad = threadIdx.x & 15, slice = threadIdx.x >> 4;
-  const int c = (blockIdx.x * 16 + quad) * 4, r = blockIdx.y;
+  __shared__ f32x4 s_sum[64][4];
+  const int quad = threadIdx.x & 3, slice = threadIdx.x >> 2;
+  const int c = (blockIdx.x * 4 + quad) * 4, r = blockIdx.y;
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  long long label = 0;
+  if (share) {
+    label = y.at(r);
+    if (!y.counts(label)) {      // its sums may hold anything
+      if (slice == 0)
+        for (int k = 0; k < 4 && c + k < d; ++k) dx[(long long)r * d + c + k] = TypeOf<T>::from_float(0.0f);
+      return;
+    }
+  }
   if (c < ldpart) {
 #pragma unroll 4
-    for (int i = slice; i < parts; i += 16) sum += *(const f32x4*)(part + ((long long)i * n + r) * ldpart + c);
+    for (int i = slice; i < parts; i += 64) {
+      const f32x4 p = *(const f32x4*)(part + ((long long)i * n + r) * ldpart + c);
+      const float f = share ? share[r * parts + i] : 1.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] = __builtin_fmaf(p[k], f, sum[k]);
+    }
   }
   s_sum[slice][quad] = sum;
-  __syncthreads();
+  for (int half = 32; half > 0; half >>= 1) {
+    __syncthreads();
+    if (slice < half) s_sum[slice][quad] = sum = sum + s_sum[slice + half][quad];
+  }
   if (slice == 0 && c < d) {
-    for (int k = 1; k < 16; ++k) sum += s_sum[k][quad];
-    for (int k = 0; k < 4 && c + k < d; ++k) dx[(long long)r * d + c + k] = TypeOf<T>::from_float(sum[k]);
+    for (int k = 0; k < 4 && c + k < d; ++k) {
+      float out = sum[k];
+      if (share) out = (out - TypeOf<T>::to_float(w[label * ldw + c + k])) * *scale;
+      dx[(long long)r * d + c + k] = TypeOf<T>::from_float(out);
+    }
   }
 }
 
@@ -425,8 +618,19 @@ static int launch_gradients(const rh_linear_ce_args& q, const FewPlan& p, const 
   auto kernel = p.wide_w ? few_gradients_kernel<T, kN, true> : few_gradients_kernel<T, kN, false>;
   hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
                      (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per, p.tpr,
-                     (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart);
+                     (T*)q.dw, (T*)q.db, p.rows ? nullptr : s.dx_part, p.ldpart);
   RH_CHECK_LAUNCH("few_gradients_kernel");
+  return RH_OK;
+}
+
+template <typename T, int kN, int kC>
+static int launch_online(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
+                         hipStream_t stream) {
+  auto kernel = p.wide_w ? few_online_kernel<T, kN, kC, true> : few_online_kernel<T, kN, kC, false>;
+  hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx, (int)q.n, q.d,
+                     (const T*)q.w, (long long)q.ldw, (int)q.v, (const T*)q.bias, y, s.z, p.ldz, s.part, s.dx_part,
+                     p.ldpart);
+  RH_CHECK_LAUNCH("few_online_kernel");
   return RH_OK;
 }
 
@@ -436,23 +640,34 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
   const FewPlan p = few_plan(n, q.d, v, q.dtype, flags);
   const FewSpace s = few_space(q.workspace, p, n, flags);
   const Labels y{q.labels, q.labels_int64, q.ignore_index, v};
-  auto logits = p.wide_w ? few_logits_kernel<T, true> : few_logits_kernel<T, false>;
-  hipLaunchKernelGGL(logits, dim3(p.blocks), dim3(kThreads), 16 * kPitch, stream, (const T*)q.x, (long long)q.ldx, n, q.d,
-                     (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, s.z, p.ldz, s.part);
-  RH_CHECK_LAUNCH("few_logits_kernel");
+  if (p.rows) {
+    if (int rc = p.rows == 1 ? p.chunks == 1   ? launch_online<T, 1, 1>(q, p, s, y, stream)
+                               : p.chunks == 2 ? launch_online<T, 1, 2>(q, p, s, y, stream)
+                                               : launch_online<T, 1, 4>(q, p, s, y, stream)
+                 : p.rows == 2 ? p.chunks == 1 ? launch_online<T, 2, 1>(q, p, s, y, stream)
+                                               : launch_online<T, 2, 2>(q, p, s, y, stream)
+                               : launch_online<T, 4, 1>(q, p, s, y, stream))
+      return rc;
+  } else {
+    auto logits = p.wide_w ? few_logits_kernel<T, true> : few_logits_kernel<T, false>;
+    hipLaunchKernelGGL(logits, dim3(p.blocks), dim3(kThreads), 16 * kPitch, stream, (const T*)q.x, (long long)q.ldx, n, q.d,
+                       (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, s.z, p.ldz, s.part);
+    RH_CHECK_LAUNCH("few_logits_kernel");
+  }
   hipLaunchKernelGGL(few_rows_kernel, dim3(1), dim3(64 * kFewRows), 0, stream, s.part, p.blocks, y, n, s.z, p.ldz, q.divisor,
-                     q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3));
+                     q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3), s.share);
   RH_CHECK_LAUNCH("few_rows_kernel");
   if (!q.dx && !q.dw && !q.db) return RH_OK;
-  if (int rc = n <= 1   ? launch_gradients<T, 1>(q, p, s, y, stream)
+  if (p.rows && !q.dw && !q.db) {
+  } else if (int rc = n <= 1   ? launch_gradients<T, 1>(q, p, s, y, stream)
                : n <= 2 ? launch_gradients<T, 2>(q, p, s, y, stream)
                : n <= 4 ? launch_gradients<T, 4>(q, p, s, y, stream)
                : n <= 8 ? launch_gradients<T, 8>(q, p, s, y, stream)
                         : launch_gradients<T, 16>(q, p, s, y, stream))
     return rc;
   if (q.dx) {
-    hipLaunchKernelGGL(few_features_kernel<T>, dim3(ceil_div(q.d, 64), n), dim3(kThreads), 0, stream, s.dx_part, p.parts, n,
-                       p.ldpart, q.d, (T*)q.dx);
+    hipLaunchKernelGGL(few_features_kernel<T>, dim3(ceil_div(q.d, 16), n), dim3(kThreads), 0, stream, s.dx_part, p.parts, n,
+                       p.ldpart, q.d, s.share, s.scale, y, (const T*)q.w, (long long)q.ldw, (T*)q.dx);
     RH_CHECK_LAUNCH("few_features_kernel");
   }
   return RH_OK;

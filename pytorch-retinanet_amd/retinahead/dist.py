@@ -36,6 +36,10 @@ def _all_reduce_(t, op, group):
         host = t.detach().cpu()
         dist_.all_reduce(host, op=op, group=group)
         t.copy_(host)
+    elif not t.is_cuda and dist_.get_backend(group) == "nccl":
+        card = t.cuda()
+        dist_.all_reduce(card, op=op, group=group)
+        t.copy_(card)
     else:
         dist_.all_reduce(t, op=op, group=group)
     return t
@@ -154,6 +158,15 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     from .modules import _clip
     if not (dist_.is_available() and dist_.is_initialized()) or dist_.get_world_size(group) == 1:
         return _clip(parameters, max_norm, norm_type, error_if_nonfinite, None)
-    op = dist_.ReduceOp.MAX if float(norm_type) == float("inf") else dist_.ReduceOp.SUM
+    reduce_total = _max_total_ if float(norm_type) == float("inf") else all_reduce_sum_
     return _clip(parameters, max_norm, norm_type, error_if_nonfinite,
-                 lambda total: _all_reduce_(total, op, group))
+                 lambda total: reduce_total(total, group))
+
+
+def _max_total_(total, group):
+    """The largest over ranks, NaN if one has it (what a reduction's maximum makes of a NaN is its
+    library's own affair)."""
+    none = total.isnan()
+    pair = torch.cat([total.masked_fill(none, 0.0), none.to(total.dtype)])
+    _all_reduce_(pair, dist_.ReduceOp.MAX, group)
+    return total.copy_(pair[:1].masked_fill(pair[1:] > 0, float("nan")))

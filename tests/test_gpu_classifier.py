@@ -147,6 +147,43 @@ def test_few_rows(rh, n, d, v, dtype):
     check_all(rh, x, w, y, b)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d", [(1, 4096), (1, 2056), (2, 1032), (2, 4096), (3, 1024), (4, 2048), (4, 520), (7, 1024)])
+def test_few_rows_masked_and_strided(rh, n, d, dtype):
+    """The first classes masked (workgroups that see nothing else), a row left out that holds anything,
+    rows of any stride, and the gradients that a frozen weight leaves."""
+    v = 1500
+    x, w, y, b = make(n, d, v, dtype, True, seed=17)
+    for low in (float("-inf"), torch.finfo(b.dtype).min):
+        b[:700] = low
+        y.clamp_(min=700)
+        got = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+        want = oracle(x, w[700:], y - 700, b[700:])
+        for k in ("loss", "row_loss", "d_features"):
+            close(k, got[k], want[k])
+        for k in ("d_weight", "d_bias"):
+            assert (got[k][:700] == 0).all()
+            close(k, got[k][700:], want[k])
+    only = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, False, False))
+    assert torch.equal(only["d_features"], got["d_features"]) and torch.equal(only["loss"], got["loss"])
+    odd = torch.full((n, d + 3), float("nan"), dtype=x.dtype, device="cuda")
+    odd[:, 1:d + 1] = x
+    ww = torch.full((v, d + 5), float("nan"), dtype=x.dtype, device="cuda")
+    ww[:, 3:d + 3] = w
+    for xs, ws in ((odd[:, 1:d + 1], w), (x, ww[:, 3:d + 3])):
+        again = rh.functional.linear_cross_entropy(xs, ws, y, b, grads=(True, True, True))
+        for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+            assert torch.equal(again[k], got[k]), k
+    y[n - 1] = -100
+    want = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    for value in (float("nan"), float("inf"), torch.finfo(x.dtype).min):
+        x[n - 1] = value
+        got = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+        for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+            assert torch.equal(got[k], want[k]), k
+        assert (got["d_features"][n - 1] == 0).all()
+
+
 def test_few_rows_of_very_many_classes(rh):
     """More classes than the waves take in one go, and a workspace row past 2^31 bytes of weights."""
     x, w, y, b = make(3, 16, 300_001, "bf16", True, seed=14)

@@ -14,19 +14,6 @@
 namespace rh {
 namespace ce {
 
-
-// P is the matrix units' operand and so is rounded to the inputs' type.  float16 has no room for
-// small probabilities (2^-24 is its smallest value, one of 131 072 equal classes has 2^-17): there P
-// is kept times 2^15, which |P| <= 1 allows, and the products' results are scaled back, both exact.
-template <typename T>
-struct PScale {
-  static constexpr float up = 1.0f, down = 1.0f;
-};
-template <>
-struct PScale<_Float16> {
-  static constexpr float up = 32768.0f, down = 1.0f / 32768.0f;
-};
-
 // ---------------------------------------------------------------------------------------------
 // Labels, rows
 // ---------------------------------------------------------------------------------------------
@@ -51,11 +38,6 @@ struct RowInfo {
   int* n_valid;    // [1]
   float* scale;    // [1] s * expected upstream gradient
 };
-
-// Where column `c` of row `r` lies in an array of panels of `rows` rows (in elements).
-__device__ __forceinline__ long long in_panels(const int r, const int c, const long long rows) {
-  return ((long long)(c / kStepK) * rows + r) * kStepK + c % kStepK;
-}
 
 // Eight values as the matrix units' operand: the values themselves, or a float's three parts.
 template <typename T>
@@ -265,14 +247,6 @@ __device__ __forceinline__ void add_losses(const double* __restrict__ parts, con
   __syncthreads();
   if (threadIdx.x == 0) small[0] = (float)(((s_red[0] + s_red[1]) + (s_red[2] + s_red[3])) * (double)small[2]);
 }
-
-// The rows of a call come in chunks: this chunk's are `first` on, at most `most` of them.
-struct Chunk {
-  int first, most;
-  __device__ __forceinline__ int rows(const int* n_valid) const {
-    return min(most, *n_valid - first);
-  }
-};
 
 // How a logit waits for its row's sum where it is kept: as it is (float), or for the 16-bit types as
 // its distance below the largest of its group of columns in the row, in steps of 1 / kSteps of a
@@ -792,6 +766,7 @@ struct Plan {
   int ldw_pad;                  // row of the copied weights (0: not copied)
   int chunk, chunks;            // rows at a time
   int ldp;                      // columns of P
+  bool whole;                   // a workgroup holds rows of logits whole
   bool large_logits;
   int group, groups;            // classes a wave of the logits' tiles takes
   Cut dx, dw;
@@ -806,6 +781,7 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
   p.per = n > 65536 ? 256 : 32;
   p.row_blocks = ceil_div(n, p.per);
   p.panels = ceil_div(d, kStepK);
+  p.whole = dtype != RH_F32 && (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) && whole_pays(d, v);
   p.ldw_pad = dtype != RH_F32 && (flags & RH_CE_COPY_WEIGHT) ? p.panels * kStepK : 0;
   p.ldp = ceil_div(v, 64) * 64;
   long long rows = kKeptBytes / ((long long)p.ldp * p.kept_size) / 256 * 256;
@@ -878,7 +854,7 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw.splits > 1))
     s.dw_part = c.take<float>((size_t)p.dw.splits * v * p.ldpart);
   if (flags & RH_CE_GRAD_B) {
-    s.db_parts = ceil_div(p.chunk, kProbRows) * p.chunks;
+    s.db_parts = ceil_div(p.chunk, p.whole ? kWholeRows : kProbRows) * p.chunks;
     s.db_part = c.take<float>((size_t)s.db_parts * v);
   }
   s.bytes = c.off;
@@ -998,6 +974,39 @@ static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Spac
   return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, p.dw.splits, false, stream) : RH_OK;
 }
 
+// A chunk's loss, P, column sums and dX by workgroups that hold their rows' logits whole.
+template <typename T>
+static int whole_rows(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a, int chunk,
+                      hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    WholeArgs<T> g = {};
+    g.x = a.x;
+    g.x_bytes = a.x_bytes;
+    g.chunk_rows = p.chunk;
+    g.w = a.w;
+    g.ldw = a.ldw;
+    g.w_bytes = a.w_bytes;
+    g.steps = a.steps;
+    g.w_limit = a.w_limit;
+    g.bias = a.bias;
+    g.v = a.v;
+    g.d = q.d;
+    g.chunk = a.chunk;
+    g.n_valid = a.n_valid;
+    g.label = a.label;
+    g.map = s.info.map + a.chunk.first;
+    g.scale = s.info.scale;
+    g.p = s.p;
+    g.ldp = p.ldp;
+    g.column_sums = s.db_part ? s.db_part + (long long)chunk * ceil_div(p.chunk, kWholeRows) * a.v : nullptr;
+    g.dx = (T*)q.dx;
+    g.row_loss = q.row_loss;
+    g.loss = s.loss + a.chunk.first / kWholeRows;
+    return run_whole<T>(g, stream);
+  }
+  return RH_EINVAL;      // no plan leads here
+}
+
 template <typename T>
 static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStream_t stream) {
   const int n = (int)q.n, d = q.d, v = (int)q.v;
@@ -1051,6 +1060,12 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     a.x = s.x + (long long)first * p.panels * kStepBytes;
     a.label = s.info.label + first;
     a.z_label = s.z_label + first;
+    if (p.whole) {
+      if (int rc = whole_rows(q, p, s, a, c, stream)) return rc;
+      if (q.dw)
+        if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
+      continue;
+    }
     if (int rc = grads ? p.large_logits ? launch_logits<T, Large, kKeep>(a, stream)
                                         : launch_logits<T, Small, kKeep>(a, stream)
                        : p.large_logits ? launch_logits<T, Large, kStats>(a, stream)
@@ -1069,8 +1084,9 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     if (q.dw)
       if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
   }
-  if (!grads) {
-    hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, 32), q.small);
+  if (!grads || p.whole) {
+    hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, p.whole ? kWholeRows : 32),
+                       q.small);
     RH_CHECK_LAUNCH("finish_loss_kernel");
   }
   if (q.db) {

@@ -243,10 +243,6 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
   }
 }
 
-template <int kRotate>
-__device__ __forceinline__ float rotated(const float x) {      // within each 16 lanes
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + kRotate, 0xf, 0xf, true));
-}
 // Of every 16 lanes, over those whose number is the same modulo kN.
 template <int kN, typename F>
 __device__ __forceinline__ float over_classes(float x, const F f) {
@@ -308,20 +304,9 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
     // sums over the wave: values 4 g .. 4 g + 3 end in the 16 lanes of row g
     float eight[8], four[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, part_of[i]),
-                                                      __builtin_bit_cast(unsigned, part_of[i + 8]), false, false);
-      const unsigned s0 = s[0], s1 = s[1];
-      eight[i] = __builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1);
-    }
+    for (int i = 0; i < 8; ++i) eight[i] = fold32(part_of[i], part_of[i + 8]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, eight[i]),
-                                                      __builtin_bit_cast(unsigned, eight[i + 4]), false, false);
-      const unsigned s0 = s[0], s1 = s[1];
-      four[i] = over_classes<1>(__builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1),
-                                [](float p, float q) { return p + q; });
-    }
+    for (int i = 0; i < 4; ++i) four[i] = sum16(fold16(eight[i], eight[i + 4]));
     const int value = in + 4 * (lane >> 4);      // of lanes 0 .. 3 of a row
     const float mine = in == 0 ? four[0] : in == 1 ? four[1] : in == 2 ? four[2] : four[3];
     if (in < 4) ((float*)&s_z[odd][value])[wave] = mine;

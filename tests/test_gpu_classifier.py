@@ -139,6 +139,35 @@ def test_wide_features(rh, n, d, v, dtype, bias):
     check_all(rh, x, w, y, b)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,d,v", [(17, 8, 1), (64, 256, 80), (63, 40, 127), (129, 33, 128), (65, 257, 129), (200, 264, 256),
+                                   (127, 512, 300), (130, 72, 384), (70, 300, 385), (128, 500, 512), (66, 256, 513),
+                                   (193, 256, 601), (100, 31, 640), (100, 64, 641), (1000, 2048, 100)])
+def test_whole_rows(rh, n, d, v, dtype):
+    """Around the sizes whose logits a workgroup holds whole: each gradient by itself too, in every reduction."""
+    x, w, y, b = make(n, d, v, dtype, True, ignored=0.3, seed=18)
+    got = check_all(rh, x, w, y, b)
+    check_all(rh, x, w, y, None, reduction="sum")
+    for i, k in enumerate(("d_features", "d_weight", "d_bias")):
+        only = rh.functional.linear_cross_entropy(x, w, y, b, grads=tuple(j == i for j in range(3)))
+        assert torch.equal(only[k], got[k]) and torch.equal(only["loss"], got["loss"]), k
+    low = b.clone()
+    low[: v // 2] = float("-inf")
+    y = torch.where(y >= 0, y.clamp(min=v // 2), y)
+    got = rh.functional.linear_cross_entropy(x, w, y, low, grads=(True, True, True))
+    want = oracle(x, w[v // 2:], torch.where(y >= 0, y - v // 2, y), b[v // 2:])
+    for k in ("loss", "row_loss", "d_features"):
+        close(k, got[k], want[k])
+    for k in ("d_weight", "d_bias"):
+        assert (got[k][: v // 2] == 0).all()
+        close(k, got[k][v // 2:], want[k])
+    keep = torch.full((v, d + 24), float("nan"), dtype=x.dtype, device="cuda")      # NaN between the rows
+    keep[:, 8:d + 8] = w
+    again = rh.functional.linear_cross_entropy(x, keep[:, 8:d + 8], y, low, grads=(True, True, True))
+    for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+        assert torch.equal(again[k], got[k]), k
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17])
 @pytest.mark.parametrize("d,v", [(8, 17), (33, 200), (2048, 40), (2056, 3000), (5000, 130), (256, 40001)])

@@ -231,8 +231,7 @@ struct Grid {
 
 // Tiles in groups of eight rows of tiles, down a group's column first: the workgroups that run side
 // by side on an XCD share both operands' rows in its L2.
-__device__ __forceinline__ int2 tile_at(const Grid g, const int id) {
-  const int t = xcd_run(id, g.m * g.n);
+__device__ __forceinline__ int2 tile_at(const Grid g, const int t) {
   const int span = 8 * g.n, first = t / span * 8, rows = min(8, g.m - first), in = t % span;
   return make_int2(first + in % rows, in / rows);
 }
@@ -406,7 +405,7 @@ template <typename T, typename S, What kWhat>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_kernel(const LogitArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  const int2 at = tile_at(a.grid, blockIdx.x);
+  const int2 at = tile_at(a.grid, xcd_run(blockIdx.x, gridDim.x));
   const int rows = a.chunk.rows(a.n_valid), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   if (m0 >= rows) return;
   constexpr bool kPW = sizeof(T) == 4;
@@ -586,11 +585,12 @@ template <typename T, Layout kLA, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  const int2 at = tile_at(a.grid, blockIdx.x);
+  const int id = xcd_run(blockIdx.x, gridDim.x), split = id / (a.grid.m * a.grid.n);      // a split's tiles share its L2
+  const int2 at = tile_at(a.grid, id - split * (a.grid.m * a.grid.n));
   const int rows = max(a.chunk.rows(a.n_valid), 0), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   const int m = kLA == kRows ? rows : a.m, k = kLA == kCols ? rows : a.k;
   if (m0 >= m) return;
-  const int k0 = blockIdx.y * a.split_steps * kStepK;
+  const int k0 = split * a.split_steps * kStepK;
   const int steps = max(0, min(a.split_steps, (k - k0 + kStepK - 1) / kStepK));
   const int last = k - k0 - (steps - 1) * kStepK;      // values of k in the last step
   const long long panel = (long long)a.chunk_rows * kStepBytes;
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
     const int row = m0 + wm + 32 * i + (lane & 31);
     if (row < m) {
       if constexpr (kTo == kParts) {      // ldpart is a multiple of four, 16-byte aligned
-        float* part = a.part + blockIdx.y * a.plane + row * a.ldpart + n0 + wn;
+        float* part = a.part + split * a.plane + row * a.ldpart + n0 + wn;
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
@@ -885,7 +885,7 @@ static int launch_product(ProductArgs<T> a, int splits, hipStream_t stream) {
                 : a.n % (sizeof(T) == 2 ? 8 : 4) == 0 ? product_kernel<T, kLA, S, kWide>
                                                       : product_kernel<T, kLA, S, kSingly>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n, splits), dim3(S::kThreads), S::kLdsBytes, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n * splits), dim3(S::kThreads), S::kLdsBytes, stream, a);
   RH_CHECK_LAUNCH("product_kernel");
   return RH_OK;
 }

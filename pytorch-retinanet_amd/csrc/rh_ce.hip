@@ -405,9 +405,11 @@ template <typename T, typename S, What kWhat>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_kernel(const LogitArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  const int2 at = tile_at(a.grid, xcd_run(blockIdx.x, gridDim.x));
-  const int rows = a.chunk.rows(a.n_valid), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
-  if (m0 >= rows) return;
+  const int rows = a.chunk.rows(a.n_valid);
+  const Grid g = {(max(rows, 0) + S::kBM - 1) / S::kBM, a.grid.n};      // tiles that hold rows
+  if ((int)blockIdx.x >= g.m * g.n) return;
+  const int2 at = tile_at(g, xcd_run(blockIdx.x, g.m * g.n));
+  const int m0 = at.x * S::kBM, n0 = at.y * S::kBN;
   constexpr bool kPW = sizeof(T) == 4;
   const long long from = n0 * (kPW ? (long long)kStepBytes : a.ldw);
   Tile<T, kRows, kPanels, kRows, kPW, S> tile;
@@ -555,6 +557,17 @@ __global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __r
 // ---------------------------------------------------------------------------------------------
 // Gradients
 // ---------------------------------------------------------------------------------------------
+// How many splits a product of fewer rows than it was launched for takes: its workgroups share the tiles there are.
+struct Sharing {
+  int bm, tiles_n;         // of a tile's rows; tiles side by side
+  int workgroups;
+  int least, most;         // splits
+  __device__ __forceinline__ int tiles_m(const int rows) const { return (rows + bm - 1) / bm; }
+  __device__ __forceinline__ int splits(const int rows) const {
+    return least == most || rows <= 0 ? least : min(most, workgroups / (tiles_m(rows) * tiles_n));
+  }
+};
+
 template <typename T>
 struct ProductArgs {
   const char* p;               // P in panels of chunk_rows
@@ -565,15 +578,14 @@ struct ProductArgs {
   int m, n, k;                 // rows that count bound m (dX) or k (dW) on the device
   const int* n_valid;
   Chunk chunk;
-  Grid grid;
-  int split_steps;             // k steps a split takes
+  Sharing sharing;
   const float* scale;
   float down;
   T* out;                      // [map[m] or m][ldo]
   const int* map;
   long long ldo;
   float* part;                 // [split][m][ldpart] instead of out
-  long long ldpart, plane;
+  long long ldpart;
   int add;                     // part += instead of part =
 };
 
@@ -585,13 +597,17 @@ template <typename T, Layout kLA, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  const int id = xcd_run(blockIdx.x, gridDim.x), split = id / (a.grid.m * a.grid.n);      // a split's tiles share its L2
-  const int2 at = tile_at(a.grid, id - split * (a.grid.m * a.grid.n));
-  const int rows = max(a.chunk.rows(a.n_valid), 0), m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  const int rows = max(a.chunk.rows(a.n_valid), 0);
   const int m = kLA == kRows ? rows : a.m, k = kLA == kCols ? rows : a.k;
-  if (m0 >= m) return;
-  const int k0 = split * a.split_steps * kStepK;
-  const int steps = max(0, min(a.split_steps, (k - k0 + kStepK - 1) / kStepK));
+  const Grid g = {a.sharing.tiles_m(m), a.sharing.tiles_n};
+  const int tiles = g.m * g.n, splits = a.sharing.splits(m), k_steps = (k + kStepK - 1) / kStepK;
+  if ((int)blockIdx.x >= tiles * splits) return;
+  const int id = xcd_run(blockIdx.x, tiles * splits), split = id / tiles;      // a split's tiles share its L2
+  const int2 at = tile_at(g, id - split * tiles);
+  const int m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  const int split_steps = (k_steps + splits - 1) / splits;
+  const int k0 = split * split_steps * kStepK;
+  const int steps = max(0, min(split_steps, (k - k0 + kStepK - 1) / kStepK));
   const int last = k - k0 - (steps - 1) * kStepK;      // values of k in the last step
   const long long panel = (long long)a.chunk_rows * kStepBytes;
   const long long from = kLA == kRows ? k0 / kStepK * panel + (long long)m0 * kStepBytes
@@ -610,7 +626,7 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
     const int row = m0 + wm + 32 * i + (lane & 31);
     if (row < m) {
       if constexpr (kTo == kParts) {      // ldpart is a multiple of four, 16-byte aligned
-        float* part = a.part + split * a.plane + row * a.ldpart + n0 + wn;
+        float* part = a.part + ((long long)split * g.m * S::kBM + row) * a.ldpart + n0 + wn;
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
 #pragma unroll
@@ -654,20 +670,34 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
 
 // out[map[m] or m][:] = scale * sum of the splits' parts, in their order.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __restrict__ part, const int splits,
-                                                              const long long plane, const long long ldpart,
-                                                              const int m, const int n,
+__global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __restrict__ part, const Sharing sharing,
+                                                              const long long ldpart, const int m, const int n,
                                                               const Chunk chunk, const int* __restrict__ n_valid,
                                                               const float* __restrict__ scale, const float down,
                                                               const int* __restrict__ map, T* __restrict__ out,
                                                               const long long ldo) {
-  const long long quads = (n + 3) / 4, top = (n_valid ? chunk.rows(n_valid) : m) * quads;
+  const int rows = n_valid ? max(chunk.rows(n_valid), 0) : m, splits = sharing.splits(rows);
+  const long long quads = (n + 3) / 4, top = rows * quads;
+  const long long plane = (long long)sharing.tiles_m(rows) * sharing.bm * ldpart;
   const float s = *scale * down;
   for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < top; i += (long long)gridDim.x * kThreads) {
     const long long r = i / quads;
     const int c = (int)(i - r * quads) * 4;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < splits; ++k) v += *(const f32x4*)(part + k * plane + r * ldpart + c);
+    const float* from = part + r * ldpart + c;
+    int k = 0;
+    for (; k + 8 <= splits; k += 8) {      // eight loads on their way together
+      f32x4 p[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) p[u] = *(const f32x4*)(from + (k + u) * plane);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += p[u];
+    }
+    for (; k + 2 <= splits; k += 2) {
+      const f32x4 p = *(const f32x4*)(from + k * plane), q = *(const f32x4*)(from + (k + 1) * plane);
+      v = (v + p) + q;
+    }
+    if (k < splits) v += *(const f32x4*)(from + k * plane);
     T* to = out + (map ? map[r] : r) * ldo + c;
     if ((n & 3) == 0) {
       Vec4<T> o;
@@ -680,21 +710,25 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __res
   }
 }
 
-// db from the row blocks' column sums: 32 columns a workgroup, eight threads a column.
+// db from the row blocks' column sums: eight columns a workgroup, 32 threads a column.  The first workgroup also
+// adds up the loss (losses > 0).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_columns_kernel(const float* __restrict__ part, const int parts,
                                                                 const int v, const float* __restrict__ scale,
-                                                                T* __restrict__ db) {
-  __shared__ float s_sum[8][32];
-  const int in = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + in;
+                                                                T* __restrict__ db,
+                                                                const double* __restrict__ loss_parts, const int losses,
+                                                                float* __restrict__ small) {
+  __shared__ float s_sum[32][8];
+  if (losses && blockIdx.x == 0) add_losses(loss_parts, losses, small);
+  const int in = threadIdx.x & 7, slice = threadIdx.x >> 3, c = blockIdx.x * 8 + in;
   float sum = 0.0f;
   if (c < v)
 #pragma unroll 8
-    for (int k = slice; k < parts; k += 8) sum += part[(long long)k * v + c];
+    for (int k = slice; k < parts; k += 32) sum += part[(long long)k * v + c];
   s_sum[slice][in] = sum;
   __syncthreads();
   if (slice == 0 && c < v) {
-    for (int k = 1; k < 8; ++k) sum += s_sum[k][in];
+    for (int k = 1; k < 32; ++k) sum += s_sum[k][in];
     db[c] = TypeOf<T>::from_float(sum * *scale);
   }
 }
@@ -825,6 +859,8 @@ struct Space {
   size_t bytes;
 };
 
+static long long whole_tiles(const Cut& c, int rows) { return (long long)ceil_div(rows, c.large ? 256 : 128) * (c.large ? 256 : 128); }
+
 static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   Carver c(base);
   Space s = {};
@@ -850,9 +886,9 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
     s.p = p.parts > 1 ? c.take<char>((size_t)s.p_part * p.parts) : s.z;
   }
   if ((flags & RH_CE_GRAD_X) && p.dx.splits > 1)
-    s.dx_part = c.take<float>((size_t)p.dx.splits * p.chunk * p.ldpart);
+    s.dx_part = c.take<float>((size_t)p.dx.splits * whole_tiles(p.dx, p.chunk) * p.ldpart);
   if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw.splits > 1))
-    s.dw_part = c.take<float>((size_t)p.dw.splits * v * p.ldpart);
+    s.dw_part = c.take<float>((size_t)p.dw.splits * whole_tiles(p.dw, v) * p.ldpart);
   if (flags & RH_CE_GRAD_B) {
     s.db_parts = ceil_div(p.chunk, p.whole ? kWholeRows : kProbRows) * p.chunks;
     s.db_part = c.take<float>((size_t)s.db_parts * v);
@@ -878,14 +914,13 @@ static int launch_logits(LogitArgs<T> a, hipStream_t stream) {
 }
 
 template <typename T, Layout kLA, typename S>
-static int launch_product(ProductArgs<T> a, int splits, hipStream_t stream) {
-  a.grid = Grid{ceil_div(a.m, S::kBM), ceil_div(a.n, S::kBN)};
+static int launch_product(const ProductArgs<T>& a, hipStream_t stream) {
   constexpr To kWide = sizeof(T) == 2 ? kOctets : kQuads;
   auto kernel = a.part                                ? product_kernel<T, kLA, S, kParts>
                 : a.n % (sizeof(T) == 2 ? 8 : 4) == 0 ? product_kernel<T, kLA, S, kWide>
                                                       : product_kernel<T, kLA, S, kSingly>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n * splits), dim3(S::kThreads), S::kLdsBytes, stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)a.sharing.workgroups), dim3(S::kThreads), S::kLdsBytes, stream, a);
   RH_CHECK_LAUNCH("product_kernel");
   return RH_OK;
 }
@@ -903,13 +938,18 @@ static int launch_probs(const rh_linear_ce_args& q, const Plan& p, const Space& 
 }
 
 template <typename T>
-static int join_parts(const ProductArgs<T>& g, int splits, bool by_rows, hipStream_t stream) {
+static int join_parts(const ProductArgs<T>& g, bool by_rows, hipStream_t stream) {
   long long blocks = ((long long)g.m * ((g.n + 3) / 4) + kThreads - 1) / kThreads;
   if (blocks > 256 * 8) blocks = 256 * 8;
-  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, g.part, splits, g.plane,
+  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, g.part, g.sharing,
                      g.ldpart, g.m, g.n, g.chunk, by_rows ? g.n_valid : nullptr, g.scale, g.down, g.map, g.out, g.ldo);
   RH_CHECK_LAUNCH("join_parts_kernel");
   return RH_OK;
+}
+
+static Sharing share(const Cut& c, int m, int n, int most) {
+  const int side = c.large ? 256 : 128, across = ceil_div(n, side);
+  return Sharing{side, across, ceil_div(m, side) * across * c.splits, c.splits, most < c.splits ? c.splits : most};
 }
 
 // What the two products share.
@@ -941,15 +981,15 @@ static int features_gradient(const rh_linear_ce_args& q, const Plan& p, const Sp
   g.b_part = a.w_part;
   g.m = a.chunk.most;
   g.k = a.v;
-  g.split_steps = p.dx.steps;
+  // as many splits as four steps of k each leave, should fewer rows count
+  g.sharing = share(p.dx, p.chunk, q.d, s.dx_part ? p.ldp / kStepK / 4 : 1);
   g.out = (T*)q.dx;
   g.map = s.info.map + a.chunk.first;
   g.part = s.dx_part;
-  g.plane = (long long)p.chunk * p.ldpart;
-  if (int rc = p.dx.large ? launch_product<T, kRows, Large>(g, p.dx.splits, stream)
-                          : launch_product<T, kRows, Small>(g, p.dx.splits, stream))
+  if (int rc = p.dx.large ? launch_product<T, kRows, Large>(g, stream)
+                          : launch_product<T, kRows, Small>(g, stream))
     return rc;
-  return s.dx_part ? join_parts(g, p.dx.splits, true, stream) : RH_OK;
+  return s.dx_part ? join_parts(g, true, stream) : RH_OK;
 }
 
 // dW, or a chunk's part of it.
@@ -963,15 +1003,14 @@ static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Spac
   g.b_part = a.x_part;
   g.m = a.v;
   g.k = a.chunk.most;
-  g.split_steps = p.dw.steps;
+  g.sharing = share(p.dw, a.v, q.d, p.dw.splits);
   g.out = (T*)q.dw;
   g.part = s.dw_part;
-  g.plane = (long long)a.v * p.ldpart;
   g.add = chunk > 0;
-  if (int rc = p.dw.large ? launch_product<T, kCols, Large>(g, p.dw.splits, stream)
-                          : launch_product<T, kCols, Small>(g, p.dw.splits, stream))
+  if (int rc = p.dw.large ? launch_product<T, kCols, Large>(g, stream)
+                          : launch_product<T, kCols, Small>(g, stream))
     return rc;
-  return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, p.dw.splits, false, stream) : RH_OK;
+  return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, false, stream) : RH_OK;
 }
 
 // A chunk's loss, P, column sums and dX by workgroups that hold their rows' logits whole.
@@ -1084,14 +1123,14 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     if (q.dw)
       if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
   }
-  if (!grads || p.whole) {
+  if (!grads || (p.whole && !q.db)) {
     hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, p.whole ? kWholeRows : 32),
                        q.small);
     RH_CHECK_LAUNCH("finish_loss_kernel");
   }
   if (q.db) {
-    hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(v, 32)), dim3(kThreads), 0, stream, s.db_part, s.db_parts, v,
-                       s.info.scale, (T*)q.db);
+    hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(v, 8)), dim3(kThreads), 0, stream, s.db_part, s.db_parts, v,
+                       s.info.scale, (T*)q.db, s.loss, p.whole ? ceil_div(n, kWholeRows) : 0, q.small);
     RH_CHECK_LAUNCH("join_columns_kernel");
   }
   return RH_OK;

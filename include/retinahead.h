@@ -429,11 +429,13 @@ enum rh_ce_flags {
                              element size or the address): the call works on a padded copy */
 };
 
-/* Softmax cross entropy of the logits x w^T + bias, with its gradients, in pieces: no more than 2 GiB of
- * logits (or 256 rows of them) exist at a time.  A row whose label is ignore_index takes no part (no loss, zero gradient,
- * whatever its features hold); so does one with a label outside [0, v), which also sets
+/* Softmax cross entropy of the logits x w^T + bias, with its gradients, in chunks of rows: no more than 2 GiB
+ * of logits (or 256 rows of them) exist at a time.  A row whose label is ignore_index takes no part (no loss,
+ * zero gradient, whatever its features hold); so does one with a label outside [0, v), which also sets
  * RH_STATUS_LABEL_RANGE.  A call without a counted row has loss 0 and zero gradients.
- * dx / dw / db (each may be NULL) hold the gradients times `grad`, for an upstream gradient of that size. */
+ * dx / dw / db (each may be NULL) hold the gradients times `grad`, for an upstream gradient of that size.
+ * RH_F32 products are made of bfloat16 ones (three parts a number): an infinite feature or weight makes the
+ * losses it meets NaN, whatever its sign; a bias may be -inf to take a class out. */
 typedef struct rh_linear_ce_args {
   const void* x;           /* device [n][ldx]: features                                           */
   const void* w;           /* device [v][ldw]: one row a class                                    */

@@ -62,16 +62,19 @@ struct Chunk {
 // Within each 16 lanes.
 template <int kRotate>
 __device__ __forceinline__ float rotated(const float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + kRotate, 0xf, 0xf, true));
+  const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + kRotate, 0xf, 0xf, true);
+  return __builtin_bit_cast(float, y);
 }
 // The sums of both lanes of a pair 32, or 16, lanes apart: of a in the pair's lower lane, of b in its upper one.
 __device__ __forceinline__ float fold32(const float a, const float b) {
-  const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+  const unsigned x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
+  const auto s = __builtin_amdgcn_permlane32_swap(x, y, false, false);
   const unsigned s0 = s[0], s1 = s[1];
   return __builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1);
 }
 __device__ __forceinline__ float fold16(const float a, const float b) {
-  const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+  const unsigned x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
+  const auto s = __builtin_amdgcn_permlane16_swap(x, y, false, false);
   const unsigned s0 = s[0], s1 = s[1];
   return __builtin_bit_cast(float, s0) + __builtin_bit_cast(float, s1);
 }

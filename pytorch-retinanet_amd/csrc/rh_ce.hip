@@ -1,5 +1,5 @@
 // Softmax cross entropy of a classifier's last projection over a large label set, forward and
-// backward, without the logits ever being kept (gfx950).
+// backward (gfx950).
 //
 //   z[n][v] = x[n] . w[v] + b[v],   lse[n] = log sum_v exp z[n][v]
 //   row[n]  = lse[n] - z[n][y_n],   loss = s sum_n row[n],   s = 1 / max(1, rows counted)  or  1
@@ -9,6 +9,17 @@
 // Rows whose label is ignore_index, or outside [0, V), take no part: the features of the others are
 // laid out one after the other in a scratch copy first (its rows padded to whole tile steps), so
 // what stands in a row left out never meets a product, not even as 0 * inf, and costs nothing.
+//
+// The logits of a chunk of rows (2 GiB of them at most) are made once, each tile leaving its rows' (max,
+// sum of exponentials) behind and, for the gradients, the logits in 16 bits (float: as they are); P takes
+// their place when the rows' sums are known, and two more products make dX and dW: 6 n d v operations.
+// Making the logits again instead takes 8 n d v, and P from them no fewer bytes.  Up to 640 classes
+// (rh_ce_whole.hip) and up to 16 rows (rh_ce_few.hip) there are other ways.
+//
+// 4096 x 2048 rows, a twentieth left out, 32 768 classes, bfloat16, us on the card: logits 570, P 85,
+// dX 490, dW 525, all else 45.  The three products make 0.98, 1.07 and 1.0 PFLOP/s; what bounds them is
+// the power that the matrix units draw on values that are not zeros (see rh_gemm.h) and, for the logits,
+// the 16 us a tile's end takes (256 x 256 exponentials a workgroup).
 #include "rh_ce.h"
 
 namespace rh {
@@ -17,7 +28,7 @@ namespace ce {
 // ---------------------------------------------------------------------------------------------
 // Labels, rows
 // ---------------------------------------------------------------------------------------------
-// Per block of `per` rows: how many count, and whether a label lies outside [0, V).
+// Per block of `per` rows: how many count, and whether a label lies outside [0, V).  5 us, all of it latency.
 __global__ __launch_bounds__(64) void count_rows_kernel(const Labels y, const int n, const int per,
                                                        int2* __restrict__ blocks) {
   const long long lo = (long long)blockIdx.x * per, hi = min((long long)n, lo + per);
@@ -108,7 +119,8 @@ __device__ __forceinline__ Eight<T> load_parts(const T* p, const int have, const
 
 // Copies the rows that count to their places in the chunks' panels, padded with zeros to whole panels; sets
 // what a row left out gets: no loss, no gradient.  A workgroup takes `per` rows and every gridDim.y-th panel;
-// a wave 16 rows of a panel at a time, a kilobyte where they are neighbours.
+// a wave 16 rows of a panel at a time, a kilobyte where they are neighbours.  Bound by memory: 49 104 x 256
+// bfloat16, 22 + 22 MB: 13 us.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void place_rows_kernel(
     const T* __restrict__ x, const long long ldx, const int d, const Labels y, const int n, const int per,
@@ -195,7 +207,8 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
       }
 }
 
-// A copy of the weights with rows of whole 16-byte pieces, for a row length or stride that has none.
+// A copy of the weights with rows of whole 16-byte pieces, for a row length or stride that has none: read and
+// written once where every product would read them value by value.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* __restrict__ w, const long long ldw,
                                                             const int d, const int v, T* __restrict__ out,
@@ -205,7 +218,8 @@ __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* __restrict_
     for (int c = lane; c < ldp; c += 64) out[r * ldp + c] = c < d ? w[r * ldw + c] : (T)0.0f;
 }
 
-// The weights in panels and parts (float).
+// The weights in panels and parts (float), by 16 rows of a panel a wave.  Bound by memory: 16 384 x 1024, 67 MB read
+// and 101 written: 32 us.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void take_apart_kernel(const T* __restrict__ w, const long long ldw, const int d,
                                                               const int v, const int panels, char* __restrict__ out,
@@ -413,8 +427,8 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
   constexpr bool kPW = sizeof(T) == 4;
   const long long from = n0 * (kPW ? (long long)kStepBytes : a.ldw);
   Tile<T, kRows, kPanels, kRows, kPW, S> tile;
-  tile.run(a.x + (long long)m0 * kStepBytes, (long long)a.chunk_rows * kStepBytes, a.x_bytes - (long long)m0 * kStepBytes,
-           a.x_part, a.w + from, a.ldw, a.w_bytes - from, a.w_part, a.steps, lds, kStepBytes, a.w_limit);
+  const long long from_x = (long long)m0 * kStepBytes;
+  tile.run(a.x + from_x, (long long)a.chunk_rows * kStepBytes, a.x_bytes - from_x, a.x_part, a.w + from, a.ldw, a.w_bytes - from, a.w_part, a.steps, lds, kStepBytes, a.w_limit);
   if (!a.bias && n0 + S::kBN <= a.v)
     finish_logits<T, S, kWhat, true>(a, tile, m0, n0, rows);
   else
@@ -423,10 +437,12 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_ker
 
 constexpr int kProbRows = 256;
 
-// P from the kept logits, in their place (float: beside them, in parts): p = e^(z - group's top) * (e^(group's top - row's top) / row's
-// sum), the first factor from the code.  A workgroup takes a group of classes (kPanelsOf panels) of
-// kProbRows places, a thread eight columns of each panel's row.  column_sums (or NULL): [row block][v] sums of P
-// over its rows.  The first workgroup of the last chunk also adds up the loss (losses > 0).
+// P from the kept logits, in their place (float: beside them, in parts):
+//   p = e^(z - group's top) * (e^(group's top - row's top) / row's sum),  the first factor from the code.
+// A workgroup takes a group of classes (kPanelsOf panels) of kProbRows places, a thread eight columns of each
+// panel's row.  column_sums (or NULL): [row block][v] sums of P over its rows.  The first workgroup of the
+// last chunk also adds up the loss (losses > 0).  Bound by memory: 3891 x 32 768 in 16 bits, 255 MB each way:
+// 85 us.
 template <typename T, int kPanelsOf>
 __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict__ kept, char* __restrict__ p_out,
                                                          const long long part, const int chunk_rows, const int ldp,
@@ -499,7 +515,7 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict_
 }
 
 // Row loss and (max, 1 / sum) of every place from the tiles' pairs: eight threads a row, each an
-// eighth of the tiles.
+// eighth of the tiles.  9 us for 3891 rows of 256 pairs.
 __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __restrict__ stats,
                                                               const long long ld, const int groups,
                                                               const Chunk chunk, const int* __restrict__ n_valid,
@@ -592,7 +608,11 @@ struct ProductArgs {
 // float parts; the result, in rows of whole groups of eight 16-bit values, of four of either size, or not
 enum To { kParts, kOctets, kQuads, kSingly };
 
-// kLA = kRows: dX = P W, the sum over the classes; kCols: dW = P^T X, over the chunk's rows.
+// kLA = kRows: dX = P W, the sum over the classes; kCols: dW = P^T X, over the chunk's rows.  Bound by the matrix
+// units' power where the sums are long (8192 x 4096, 131 072 classes: 1.17 and 1.24 PFLOP/s), by filling the card
+// where the result is small; the splits that do so are cut()'s.  Workgroups that follow one another on an XCD
+// take the same split's tiles, which read the same rows: dW of 601 x 256 over 49 104 rows 26 us, 37 with a
+// split's tiles spread over the XCDs.
 template <typename T, Layout kLA, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -859,7 +879,10 @@ struct Space {
   size_t bytes;
 };
 
-static long long whole_tiles(const Cut& c, int rows) { return (long long)ceil_div(rows, c.large ? 256 : 128) * (c.large ? 256 : 128); }
+static long long whole_tiles(const Cut& c, int rows) {
+  const int side = c.large ? 256 : 128;
+  return (long long)ceil_div(rows, side) * side;
+}
 
 static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   Carver c(base);
@@ -930,7 +953,8 @@ static int launch_probs(const rh_linear_ce_args& q, const Plan& p, const Space& 
                         hipStream_t stream) {
   const int blocks = ceil_div(p.chunk, kProbRows);
   hipLaunchKernelGGL((probs_kernel<T, kPanelsOf>), dim3(ceil_div(p.ldp, p.group), blocks), dim3(kThreads), 0, stream, s.z,
-                     s.p, s.p_part, p.chunk, p.ldp, a.v, a.chunk, a.n_valid, a.label, s.row_stats + a.chunk.first, s.stats, a.ld_stats,
+                     s.p, s.p_part, p.chunk, p.ldp, a.v, a.chunk, a.n_valid, a.label, s.row_stats + a.chunk.first, s.stats,
+                     a.ld_stats,
                      s.db_part ? s.db_part + (long long)chunk * blocks * a.v : nullptr, s.loss,
                      chunk == p.chunks - 1 ? ceil_div(q.n, 32) : 0, q.small);
   RH_CHECK_LAUNCH("probs_kernel");
@@ -1077,8 +1101,8 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     a.w_limit = kStepBytes;
   }
   if (p.parts > 1) {
-    hipLaunchKernelGGL(take_apart_kernel<T>, dim3(ceil_div(v, 16), ceil_div(p.panels, 16) < 16 ? ceil_div(p.panels, 16) : 16),
-                       dim3(kThreads), 0, stream, (const T*)q.w, (long long)q.ldw, d, v, p.panels, s.w, s.w_part);
+    const int across = ceil_div(p.panels, 16) < 16 ? ceil_div(p.panels, 16) : 16;
+    hipLaunchKernelGGL(take_apart_kernel<T>, dim3(ceil_div(v, 16), across), dim3(kThreads), 0, stream, (const T*)q.w, (long long)q.ldw, d, v, p.panels, s.w, s.w_part);
     RH_CHECK_LAUNCH("take_apart_kernel");
     a.w = s.w;
     a.ldw = (long long)v * kStepBytes;
@@ -1124,8 +1148,8 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
       if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
   }
   if (!grads || (p.whole && !q.db)) {
-    hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss, ceil_div(n, p.whole ? kWholeRows : 32),
-                       q.small);
+    hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss,
+                       ceil_div(n, p.whole ? kWholeRows : 32), q.small);
     RH_CHECK_LAUNCH("finish_loss_kernel");
   }
   if (q.db) {
@@ -1199,11 +1223,14 @@ int rh_scale_gradient(void* x, int64_t count, int32_t dtype, const float* scale,
   if (blocks > 256 * 16) blocks = 256 * 16;
   const dim3 grid((unsigned)blocks), block(rh::ce::kThreads);
   if (dtype == RH_F32)
-    hipLaunchKernelGGL(rh::ce::upstream_kernel<float>, grid, block, 0, (hipStream_t)stream, (float*)x, (long long)count, scale, assumed);
+    hipLaunchKernelGGL(rh::ce::upstream_kernel<float>, grid, block, 0, (hipStream_t)stream, (float*)x, (long long)count, scale,
+                       assumed);
   else if (dtype == RH_BF16)
-    hipLaunchKernelGGL(rh::ce::upstream_kernel<__bf16>, grid, block, 0, (hipStream_t)stream, (__bf16*)x, (long long)count, scale, assumed);
+    hipLaunchKernelGGL(rh::ce::upstream_kernel<__bf16>, grid, block, 0, (hipStream_t)stream, (__bf16*)x, (long long)count, scale,
+                       assumed);
   else if (dtype == RH_F16)
-    hipLaunchKernelGGL(rh::ce::upstream_kernel<_Float16>, grid, block, 0, (hipStream_t)stream, (_Float16*)x, (long long)count, scale, assumed);
+    hipLaunchKernelGGL(rh::ce::upstream_kernel<_Float16>, grid, block, 0, (hipStream_t)stream, (_Float16*)x, (long long)count, scale,
+                       assumed);
   else
     RH_FAIL(RH_EINVAL, "unknown element type %d", dtype);
   RH_CHECK_LAUNCH("upstream_kernel");

@@ -2,11 +2,12 @@
 // The logits are never written: a workgroup makes all of its rows' logits, takes their softmax where they are,
 // writes P once (dW's operand) and multiplies it with the weights for dX while it is still in LDS.
 //
-// 49 104 x 256 against 601 classes, bfloat16: 82 us, where the logits by tiles, the joining of their sums, P from the kept
-// logits and dX by tiles took 103.  Of a workgroup's 25 us the logits take 8.5, the exponentials 5.5, P 3.6 and dX 7.2:
-// the products are bound by LDS (a wave of 32 rows reads a fragment of weights for every instruction), the rest by the
-// vector units.  Up to 256 classes two workgroups share a CU and run these against each other (80 classes: 24.5 us, 29.7
-// without).
+// 49 104 x 256 against 601 classes, bfloat16: 82 us, where the logits by tiles, the joining of their sums, P
+// from the kept logits and dX by tiles took 103.  Of a workgroup's 25 us the logits take 8.5, the exponentials
+// 5.5, P 3.6 and dX 7.2: the products are bound by LDS (a wave of 32 rows reads a fragment of weights for every
+// instruction; the matrix units are busy 18% of the time), the rest by the vector units.  Up to 256 classes two
+// workgroups share a CU and run these against each other (80 classes: 24.5 us, 29.7 one at a time).  The weights
+// in panels instead of rows: 79 us, less than laying them out costs.
 #include "rh_ce.h"
 
 namespace rh {
@@ -280,8 +281,9 @@ __global__ __launch_bounds__(kWholeThreads, kF <= 2 ? 4 : 2) void whole_kernel(c
 template <typename T, int kF>
 static int launch_whole(const WholeArgs<T>& a, hipStream_t stream) {
   auto kernel = whole_kernel<T, kF>;
-  RH_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, WholeLds<kF>::kBytes));
-  hipLaunchKernelGGL(kernel, dim3(ceil_div(a.chunk.most, kWholeRows)), dim3(kWholeThreads), WholeLds<kF>::kBytes, stream, a);
+  constexpr int kBytes = WholeLds<kF>::kBytes;
+  RH_CHECK_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  hipLaunchKernelGGL(kernel, dim3(ceil_div(a.chunk.most, kWholeRows)), dim3(kWholeThreads), kBytes, stream, a);
   RH_CHECK_LAUNCH("whole_kernel");
   return RH_OK;
 }

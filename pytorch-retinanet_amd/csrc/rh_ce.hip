@@ -475,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict_
         if (first + i * kStepK < ldp) z[i][k] = ((const u32x4*)kept)[(at + i * next) / 8 * kWords + k];
     const float2 of_row = row_stats[r];
     const int y = label[r] - c;
-    const float f = sizeof(T) == 4 ? of_row.y : exp_for<T>(top[r].x - of_row.x) * of_row.y;
+    const float inv = 1.0f / of_row.y, f = sizeof(T) == 4 ? inv : exp_for<T>(top[r].x - of_row.x) * inv;
 #pragma unroll
     for (int i = 0; i < kPanelsOf; ++i) {
       if (first + i * kStepK >= ldp) continue;
@@ -484,13 +484,14 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict_
       for (int k = 0; k < 8; ++k) {
         if constexpr (sizeof(T) == 4) {
           const unsigned w = z[i][k >> 2][k & 3];
-          p[k] = expf(__builtin_bit_cast(float, w) - of_row.x) * f;
+          // the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
+          p[k] = (expf(__builtin_bit_cast(float, w) - of_row.x) - (y == i * kStepK + k ? of_row.y : 0.0f)) * f;
         } else {
           const unsigned w = z[i][0][k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
           const float e = __builtin_amdgcn_exp2f((float)code * (-1.0f / Kept<T>::kSteps));
           p[k] = (code == 0xffffu ? 0.0f : e) * f;
+          p[k] = y == i * kStepK + k ? p[k] - 1.0f : p[k];
         }
-        p[k] = y == i * kStepK + k ? p[k] - 1.0f : p[k];
         sums[i][k] += p[k];
         p[k] *= PScale<T>::up;
       }
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict_
     column_sums[(long long)blockIdx.y * v + first + i] = (s_sum[0][i] + s_sum[1][i]) + (s_sum[2][i] + s_sum[3][i]);
 }
 
-// Row loss and (max, 1 / sum) of every place from the tiles' pairs: eight threads a row, each an
+// Row loss and (max, sum) of every place from the tiles' pairs: eight threads a row, each an
 // eighth of the tiles.  9 us for 3891 rows of 256 pairs.
 __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __restrict__ stats,
                                                               const long long ld, const int groups,
@@ -556,7 +557,7 @@ __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __re
       const float base = top == -__builtin_inff() ? 0.0f : top;
       for (int k = 0; k < 8; ++k) sum += s_sum[k][r] * expf(s_top[k][r] - base);
       const float v = (top - z_label[row]) + logf(sum);
-      row_stats[row] = make_float2(top, 1.0f / sum);
+      row_stats[row] = make_float2(top, sum);
       row_loss[map[row]] = v;
       loss = (double)v;
     }

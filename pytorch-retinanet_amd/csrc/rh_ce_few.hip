@@ -3,7 +3,7 @@
 //
 //   logits      z[row][class] in float32, 16 classes x 16 rows to a matrix instruction that takes the
 //               weights straight from memory, and each workgroup's (max, sum of exp) of every row
-//   rows        the rows' (max, 1 / sum), losses and the call's loss
+//   rows        the rows' (max, sum), losses and the call's loss
 //   gradients   one more pass over the weights: dW rows written, dX summed per workgroup; P stays float32
 //   features    the workgroups' parts of dX joined
 //
@@ -74,7 +74,8 @@ __device__ __forceinline__ void to_floats(const u32x4 u, float (&f)[16 / sizeof(
 struct FewSpace {
   float* z;            // [n][ldz]
   float2* part;        // [kFewRows][blocks]
-  float2* row;         // [kFewRows]  (max, 1 / sum), of a row that counts
+  float2* row;         // [kFewRows]  (max, sum), of a row that counts
+  float* of_label;     // [kFewRows]  the label's p - 1
   float* scale;        // [1]
   float* dx_part;      // [parts][n][ldpart]
   float* share;        // [n][parts]: what a row's part counts (online)
@@ -91,7 +92,7 @@ struct FewPlan {
   int rows, chunks;                 // online: rows (a power of two) and 16-byte pieces of columns a thread; else 0
 };
 
-// Online: dX = sum of p W without P's normalisation, which is not known before the last class.  A workgroup
+// Online: dX = sum of p W over the other classes, without P's normalisation, which is not known before the last class.  A workgroup
 // takes whole rows of weights, so what a thread read for the logits is still in its registers when their
 // exponentials are known: dX's sum is kept relative to the running maximum and joined like a softmax's.
 // The weights are read once; dW is written by the gradients' pass, which then reads none.
@@ -143,6 +144,7 @@ static FewSpace few_space(void* base, const FewPlan& p, int n, int flags) {
   s.z = c.take<float>((size_t)n * p.ldz);
   s.part = c.take<float2>((size_t)kFewRows * p.blocks);
   s.row = c.take<float2>(kFewRows);
+  s.of_label = c.take<float>(kFewRows);
   s.scale = c.take<float>(1);
   if (flags & RH_CE_GRAD_X) s.dx_part = c.take<float>((size_t)p.parts * n * p.ldpart);
   if (p.rows) s.share = c.take<float>((size_t)n * p.parts);
@@ -195,6 +197,9 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
           const int c = (me + (g0 + i) * waves) * 16 + in;
           const T* row = w + (long long)min(c, v - 1) * ldw + k0 + piece * kV;
           const char* xs = smem + in * kPitch + piece * 16;
+          f32x4 sum_of[kAhead];      // short sums of their own: one over all features rounds three times as much
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) sum_of[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
           for (int k = 0; k < len; k += kAhead * kStepK) {
             u32x4 a[kAhead];
@@ -203,8 +208,13 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
               a[u] = load_values<T, kWide>(row + k + u * kStepK, len - k - u * kStepK - piece * kV);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-              acc[i] = Mma16<T>::run(a[u], *(const u32x4*)(xs + (k + u * kStepK) * (int)sizeof(T)), acc[i]);
+              sum_of[u] = Mma16<T>::run(a[u], *(const u32x4*)(xs + (k + u * kStepK) * (int)sizeof(T)), sum_of[u]);
           }
+#pragma unroll
+          for (int half = kAhead / 2; half > 0; half >>= 1)
+#pragma unroll
+            for (int u = 0; u < half; ++u) sum_of[u] += sum_of[u + half];
+          acc[i] += sum_of[0];
         }
       }
     }
@@ -279,6 +289,7 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
     }
   }
   float top = -__builtin_inff(), sum = 0.0f;      // of row in % kN, the same in all waves
+  const long long label = in % kN < n ? y.at(in % kN) : -1;
   int odd = 0;
   for (int v0 = blockIdx.x * kA; v0 < v; v0 += gridDim.x * kA, odd ^= 1) {
     u32x4 ws[kA][kC];
@@ -335,6 +346,7 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
       }
     }
     top = up;
+    const float e_other = c == label ? 0.0f : e;      // the label's weights join in the end, times p - 1
 #pragma unroll
     for (int i = 0; i < kA; ++i)
 #pragma unroll
@@ -343,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
         to_floats<T>(ws[i][j], f);
 #pragma unroll
         for (int q = 0; q < kN; ++q) {
-          const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e), i * kN + q));
+          const float p = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, e_other), i * kN + q));
 #pragma unroll
           for (int k = 0; k < kV; ++k) acc[q][j][k] = __builtin_fmaf(p, f[k], acc[q][j][k]);
         }
@@ -373,7 +385,8 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
                                                                  float* __restrict__ scale,
                                                                  float* __restrict__ row_loss,
                                                                  float* __restrict__ small, int* __restrict__ status,
-                                                                 float* __restrict__ share) {
+                                                                 float* __restrict__ share,
+                                                                 float* __restrict__ of_label) {
   __shared__ float s_loss[kFewRows];
   __shared__ int s_keep[kFewRows], s_bad[kFewRows];
   const int r = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -402,8 +415,10 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
   if (lane == 0) {
     float loss = 0.0f;
     if (keep) {
-      loss = (top - z[(long long)r * ldz + label]) + logf(sum);
-      row[r] = make_float2(top, 1.0f / sum);
+      const float z_label = z[(long long)r * ldz + label];
+      loss = (top - z_label) + logf(sum);
+      row[r] = make_float2(top, sum);
+      of_label[r] = (expf(z_label - top) - sum) / sum;
     }
     if (r < n) row_loss[r] = loss;
     s_loss[r] = loss;
@@ -474,8 +489,9 @@ __global__ __launch_bounds__(kThreads) void few_gradients_kernel(
       const int r = i / count, a = i - r * count;
       float p = 0.0f;
       if (s_label[r] >= 0) {
-        p = expf(z[(long long)r * ldz + v0 + a] - s_row[r].x) * s_row[r].y;
-        p = (s_label[r] == v0 + a ? p - 1.0f : p) * s;
+        // the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
+        p = expf(z[(long long)r * ldz + v0 + a] - s_row[r].x) - (s_label[r] == v0 + a ? s_row[r].y : 0.0f);
+        p = p / s_row[r].y * s;
       }
       s_p[a][r] = p;
     }
@@ -556,11 +572,12 @@ __global__ __launch_bounds__(kThreads) void few_gradients_kernel(
 }
 
 // Four columns of a row by 64 threads, each every 64th part.  With `share` (online) the parts are weighed
-// by it, the label's weights taken off and the sum scaled here.
+// by it, the label's weights added times p - 1 and the sum scaled here.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __restrict__ part, const int parts,
                                                                 const int n, const int ldpart, const int d,
                                                                 const float* __restrict__ share,
+                                                                const float* __restrict__ of_label,
                                                                 const float* __restrict__ scale, const Labels y,
                                                                 const T* __restrict__ w, const long long ldw,
                                                                 T* __restrict__ dx) {
@@ -594,7 +611,7 @@ __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __r
   if (slice == 0 && c < d) {
     for (int k = 0; k < 4 && c + k < d; ++k) {
       float out = sum[k];
-      if (share) out = (out - TypeOf<T>::to_float(w[label * ldw + c + k])) * *scale;
+      if (share) out = __builtin_fmaf(of_label[r], TypeOf<T>::to_float(w[label * ldw + c + k]), out) * *scale;
       dx[(long long)r * d + c + k] = TypeOf<T>::from_float(out);
     }
   }
@@ -643,7 +660,8 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
     RH_CHECK_LAUNCH("few_logits_kernel");
   }
   hipLaunchKernelGGL(few_rows_kernel, dim3(1), dim3(64 * kFewRows), 0, stream, s.part, p.blocks, y, n, s.z, p.ldz, q.divisor,
-                     q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3), s.share);
+                     q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3), s.share,
+                     s.of_label);
   RH_CHECK_LAUNCH("few_rows_kernel");
   if (!q.dx && !q.dw && !q.db) return RH_OK;
   if (p.rows && !q.dw && !q.db) {
@@ -655,7 +673,7 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
     return rc;
   if (q.dx) {
     hipLaunchKernelGGL(few_features_kernel<T>, dim3(ceil_div(q.d, 16), n), dim3(kThreads), 0, stream, s.dx_part, p.parts, n,
-                       p.ldpart, q.d, s.share, s.scale, y, (const T*)q.w, (long long)q.ldw, (T*)q.dx);
+                       p.ldpart, q.d, s.share, s.of_label, s.scale, y, (const T*)q.w, (long long)q.ldw, (T*)q.dx);
     RH_CHECK_LAUNCH("few_features_kernel");
   }
   return RH_OK;

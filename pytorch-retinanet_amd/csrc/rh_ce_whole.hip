@@ -170,14 +170,14 @@ __global__ __launch_bounds__(kWholeThreads, kF <= 2 ? 4 : 2) void whole_kernel(c
     if (lane == 0) ((double*)s_top)[wr] = loss;      // all have read the maxima
   }
 
-  // P
+  // P; the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
   const float inv = 1.0f / sum;
 #pragma unroll
   for (int f = 0; f < kF; ++f) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float p = acc[f][i] * inv;
-      acc[f][i] = y == 32 * f + 8 * (i >> 2) + (i & 3) ? p - 1.0f : p;
+      const float less = y == 32 * f + 8 * (i >> 2) + (i & 3) ? sum : 0.0f;
+      acc[f][i] = (acc[f][i] - less) * inv;
     }
   }
   if (rows < kWholeRows && row >= rows) {

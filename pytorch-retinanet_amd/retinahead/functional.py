@@ -585,7 +585,8 @@ def _dtype_code(t):
 def linear_cross_entropy(features, weight, labels, bias=None, ignore_index=-100, reduction="mean",
                          divisor=None, expected_grad=1.0, grads=(False, False, False)):
     """Softmax cross entropy of ``features @ weight.T + bias`` against ``labels``, and the gradients
-    that ``grads`` asks for (features, weight, bias), without the logits ever being stored whole.
+    that ``grads`` asks for (features, weight, bias); ``retinahead.LinearCrossEntropy`` says what is
+    stored and rounded.
 
     ``features`` [..., D], ``weight`` [V, D], ``bias`` [V] share one of float32 / bfloat16 / float16;
     ``labels`` [...] is int64 or int32.  Sums and softmax statistics are float32, the loss is a

@@ -468,8 +468,9 @@ class LinearCrossEntropy(nn.Module):
     """Softmax cross entropy of a classifier's last projection, for label sets too large to keep the
     logits of: ``forward(features[..., D], weight[V, D], labels[...], bias[V]=None)`` returns the
     float32 [1] loss of ``features @ weight.T + bias``, differentiable with respect to features,
-    weight and bias.  The logits are made in pieces of the classes and never stored whole; as in
-    ``FocalLoss`` the forward call makes the gradients too.
+    weight and bias.  As in ``FocalLoss`` the forward call makes the gradients too.  Its workspace holds
+    the logits of a chunk of rows in 16 bits (32 for float32), 2 GiB of them at most, whatever the batch
+    and the label set; for up to 640 classes or 16 rows none at all.
 
     Where ``FocalLoss`` scores every class by itself, this is the head for mutually exclusive classes
     (the 601 of datasets/oid_dataset.py:47-50 count the background as one).
@@ -477,6 +478,8 @@ class LinearCrossEntropy(nn.Module):
     Element types: float32, bfloat16, float16 (one for all three; the gradients have it too).
     Products are summed in float32, softmax statistics and losses are float32.  For 16-bit types the
     softmax minus one-hot matrix is rounded once to the type, as an operand of the matrix units.
+    float32 products are made of bfloat16 ones, three parts a number: as accurate as float32's own, but an
+    infinite feature or weight makes the losses it meets NaN (a class is masked by a bias of -inf).
 
     ignore_index: rows with this label take no part: no loss, zero gradient, whatever their features
         hold.  A batch without a counted row has loss 0 and zero gradients.

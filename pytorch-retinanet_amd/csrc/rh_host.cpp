@@ -269,10 +269,9 @@ CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, cons
   Py_DECREF(ws);
   a.workspace = room.data_ptr();
   a.workspace_bytes = room.numel();
-  int code_of_call = RH_OK;
-  Py_BEGIN_ALLOW_THREADS;
-  code_of_call = entry.run(&a, stream);
-  Py_END_ALLOW_THREADS;
+  // under the interpreter's lock: two threads on one stream share the workspace, so a call's launches must not
+  // fall between another's
+  const int code_of_call = entry.run(&a, stream);
   if (code_of_call != RH_OK)
     throw Refusal{"rh_linear_ce failed (" + std::to_string(code_of_call) + "): " + last_error()};
   return out;

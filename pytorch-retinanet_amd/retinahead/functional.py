@@ -658,6 +658,9 @@ def _norm_code(norm_type):
     return code
 
 
+_clip_lock = threading.Lock()
+
+
 def grad_clip(tensors, max_norm=None, norm_type=2.0, stages=_lib.CLIP_ALL, out=None, grads=False):
     """The norm over every value of ``tensors`` (stage ``CLIP_NORM``) and their scaling in place by
     min(1, max_norm / (norm + 1e-6)) (stage ``CLIP_SCALE``), without a host read; with ``grads`` of the
@@ -685,7 +688,8 @@ def grad_clip(tensors, max_norm=None, norm_type=2.0, stages=_lib.CLIP_ALL, out=N
         args = _lib.GradClipArgs(at, count, code, int(stages), 0.0 if max_norm is None else float(max_norm),
                                  out["total"].data_ptr(), out["norm"].data_ptr(),
                                  None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-        _lib.check(lib.rh_grad_clip(C.byref(args), stream), "rh_grad_clip")
+        with _clip_lock:      # two threads on one stream share the workspace: one call's launches at a time
+            _lib.check(lib.rh_grad_clip(C.byref(args), stream), "rh_grad_clip")
     return out
 
 

@@ -470,7 +470,8 @@ class LinearCrossEntropy(nn.Module):
     float32 [1] loss of ``features @ weight.T + bias``, differentiable with respect to features,
     weight and bias.  As in ``FocalLoss`` the forward call makes the gradients too.  Its workspace holds
     the logits of a chunk of rows in 16 bits (32 for float32), 2 GiB of them at most, whatever the batch
-    and the label set; for up to 640 classes or 16 rows none at all.
+    and the label set (P of float32 takes as much and a half again); for up to 640 classes or 16 rows none
+    at all.  It is kept for the stream's later calls.
 
     Where ``FocalLoss`` scores every class by itself, this is the head for mutually exclusive classes
     (the 601 of datasets/oid_dataset.py:47-50 count the background as one).

@@ -263,6 +263,56 @@ def test_rows_in_chunks(rh):
         close(k, some[k], want[k])
 
 
+@pytest.mark.parametrize("n,d,v,dtype", [(9001, 72, 70001, "f32"), (1_700_001, 24, 600, "bf16")])
+def test_rows_in_chunks_of_other_ways(rh, n, d, v, dtype):
+    """float32, whose P lies beside the logits, and whole rows of few classes: more than one chunk of each."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(n, d, generator=g, device="cuda").to(TYPES[dtype])
+    w = (torch.randn(v, d, generator=g, device="cuda") * 0.3).to(TYPES[dtype])
+    b = (torch.randn(v, generator=g, device="cuda") * 0.1).to(TYPES[dtype])
+    y = torch.randint(0, v, (n,), generator=g, device="cuda")
+    y[5::7] = -100
+    out = rh.functional.linear_cross_entropy(x, w, y, b, reduction="sum", grads=(True, True, True))
+    for part in (slice(0, 200), slice(n // 2, n // 2 + 200), slice(n - 200, n)):
+        want = oracle(x[part], w, y[part], b, reduction="sum")
+        close("row_loss", out["row_loss"][part], want["row_loss"])
+        close("d_features", out["d_features"][part], want["d_features"])
+    # the sums over all rows, in 64 bits piece by piece; the bounds of the pieces add up
+    total = {k: [0.0, 0.0] for k in ("loss", "d_weight", "d_bias")}
+    step = 2 ** 27 // v
+    for lo in range(0, n, step):
+        want = oracle(x[lo:lo + step], w, y[lo:lo + step], b, reduction="sum")
+        for k, sums in total.items():
+            sums[0] = sums[0] + want[k][0]
+            sums[1] = sums[1] + want[k][1]
+    for k, sums in total.items():
+        close(k, out[k], sums)
+
+
+def test_two_threads_on_one_stream(rh):
+    """They share a workspace: a call's launches do not fall between another's."""
+    import threading
+    cases = [make(200, 96, 700, "bf16", True, seed=19), make(90, 64, 5000, "f32", True, seed=20),
+             make(3, 1024, 900, "f16", True, seed=21)]
+    want = [rh.functional.linear_cross_entropy(*c, grads=(True, True, True)) for c in cases]
+    wrong = []
+
+    def work(i):
+        for k in range(40):
+            j = (i + k) % len(cases)
+            got = rh.functional.linear_cross_entropy(*cases[j], grads=(True, True, True))
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(q for q in ("loss", "row_loss", "d_features", "d_weight", "d_bias")
+                         if not torch.equal(got[q], want[j][q]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("reduction,grad", [("sum", 1.0), ("mean", 0.25)])
 def test_reductions_and_expected_gradient(rh, dtype, reduction, grad):

@@ -369,7 +369,7 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
           } else {
             const float below = z[j][r] - base;      // first: z and base may be the type's lowest
             sum += exp_for<T>(below);
-            z[j][r] = __builtin_fmaf(below, -kLog2e * Kept<T>::kSteps, 0.5f);
+            z[j][r] = below * (-kLog2e * Kept<T>::kSteps / 65535.0f);
           }
         }
       sum += __shfl_xor(sum, 32, 64);
@@ -398,10 +398,9 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
             for (int g = 0; g < 2; ++g) {
               unsigned w[2];
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const float lo = z[j][4 * (q + g) + 2 * k], hi = z[j][4 * (q + g) + 2 * k + 1];
-                w[k] = (unsigned)fminf(lo, 65535.0f) | (unsigned)fminf(hi, 65535.0f) << 16;
-              }
+              for (int k = 0; k < 2; ++k)      // both times 65 535 to the nearest integer, 65 535 at most
+                w[k] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(z[j][4 * (q + g) + 2 * k],
+                                                                                    z[j][4 * (q + g) + 2 * k + 1]));
               half_group[g] = (unsigned long long)w[1] << 32 | w[0];
             }
             const u32x4 eight = whole_group(half_group[0], half_group[1]);

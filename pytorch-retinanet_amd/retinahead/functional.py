@@ -594,7 +594,7 @@ def linear_cross_entropy(features, weight, labels, bias=None, ignore_index=-100,
     row left out), ``num_valid``, ``status`` and the gradients asked for as ``d_features``,
     ``d_weight``, ``d_bias``."""
     small, row_loss, *made = _classifier_loss(features, weight, labels, bias, divisor, ignore_index,
-                                              reduction, expected_grad, grads, False)
+                                              reduction, expected_grad, grads, None)
     out = ClassifierOutputs(small=small, row_loss=row_loss)
     for key, grad in zip(("d_features", "d_weight", "d_bias"), made):
         if grad is not None:

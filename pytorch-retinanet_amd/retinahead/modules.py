@@ -461,6 +461,7 @@ class GenericFocalLoss(nn.Module):
                                      bool(self.logits), bool(self.reduce))
 
 
+_SEEDED = object()
 _NO_GRADS = (False, False, False)      # the autograd node asks for those that are needed
 
 
@@ -517,13 +518,12 @@ class LinearCrossEntropy(nn.Module):
 
     def forward(self, features, weight, labels, bias=None, divisor=None):
         cfg = self.cfg
-        loss, small, row_loss = F._classifier_loss(features, weight, labels, bias, divisor, cfg["ignore_index"],
-                                                   cfg["reduction"], cfg["expected_grad"], _NO_GRADS, True)
+        loss, (small, row_loss) = F._classifier_loss(features, weight, labels, bias, divisor, cfg["ignore_index"],
+                                                   cfg["reduction"], cfg["expected_grad"], _NO_GRADS, _LossTensor)
         cfg["state"].set(features.device, F.ClassifierOutputs(small=small, row_loss=row_loss))
         if self.check_labels and int(self.last["status"].item()) & _lib.RH_STATUS_LABEL_RANGE:
             raise IndexError("label outside [0, classes)")
-        loss = loss.as_subclass(_LossTensor)
-        loss._token = object()      # backward() without a gradient: seeded with the cached ones
+        loss._token = _SEEDED      # backward() without a gradient: seeded with the cached ones
         return loss
 
 

@@ -282,6 +282,17 @@ struct Kept<float> {
   static constexpr float kSteps = 1.0f;
 };
 
+// How many splits a product of fewer rows than it was launched for takes: its workgroups share the tiles there are.
+struct Sharing {
+  int bm, tiles_n;         // of a tile's rows; tiles side by side
+  int workgroups;
+  int least, most;         // splits
+  __device__ __forceinline__ int tiles_m(const int rows) const { return (rows + bm - 1) / bm; }
+  __device__ __forceinline__ int splits(const int rows) const {
+    return least == most || rows <= 0 ? least : min(most, workgroups / (tiles_m(rows) * tiles_n));
+  }
+};
+
 template <typename T>
 struct LogitArgs {
   const char* x;       // the chunk's placed rows, in panels of chunk_rows
@@ -302,11 +313,13 @@ struct LogitArgs {
   float* z_label;      // [place]
   void* z;             // the logits kept, in panels of chunk_rows, of ldp columns
   int ldp;
+  Sharing sharing;
+  float* part;         // [split][place of whole tiles][ldp]  kParted's sums
 };
 
 // kStats: the groups' (max, sum) only, a group being a wave's part of the tile's classes.  kKeep: and the
-// logits.
-enum What { kStats, kKeep };
+// logits.  kParted: float sums over a part of the features only, for sum_logits_kernel.
+enum What { kStats, kKeep, kParted };
 
 // What becomes of a tile's logits.  kPlain: every class is there and none has a bias; else each column
 // gets something, minus infinity where there is no class.
@@ -418,20 +431,104 @@ template <typename T, typename S, What kWhat>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void logits_kernel(const LogitArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
-  const int rows = a.chunk.rows(a.n_valid);
-  const Grid g = {(max(rows, 0) + S::kBM - 1) / S::kBM, a.grid.n};      // tiles that hold rows
-  if ((int)blockIdx.x >= g.m * g.n) return;
-  const int2 at = tile_at(g, xcd_run(blockIdx.x, g.m * g.n));
+  const int rows = max(a.chunk.rows(a.n_valid), 0);
+  const Grid g = {(rows + S::kBM - 1) / S::kBM, a.grid.n};      // tiles that hold rows
+  const int tiles = g.m * g.n, splits = kWhat == kParted ? a.sharing.splits(rows) : 1;
+  if ((int)blockIdx.x >= tiles * splits) return;
+  const int id = xcd_run(blockIdx.x, tiles * splits), split = kWhat == kParted ? id / tiles : 0;
+  const int2 at = tile_at(g, id - split * tiles);
   const int m0 = at.x * S::kBM, n0 = at.y * S::kBN;
+  const int most = kWhat == kParted ? (a.steps + splits - 1) / splits : a.steps, k0 = split * most;
+  const int steps = max(0, min(most, a.steps - k0));
   constexpr bool kPW = sizeof(T) == 4;
-  const long long from = n0 * (kPW ? (long long)kStepBytes : a.ldw);
+  const long long panel = (long long)a.chunk_rows * kStepBytes, from_x = k0 * panel + (long long)m0 * kStepBytes;
+  const long long from = kPW ? k0 * a.ldw + n0 * (long long)kStepBytes : n0 * a.ldw + k0 * kStepBytes;
   Tile<T, kRows, kPanels, kRows, kPW, S> tile;
-  const long long from_x = (long long)m0 * kStepBytes;
-  tile.run(a.x + from_x, (long long)a.chunk_rows * kStepBytes, a.x_bytes - from_x, a.x_part, a.w + from, a.ldw, a.w_bytes - from, a.w_part, a.steps, lds, kStepBytes, a.w_limit);
+  tile.run(a.x + from_x, panel, a.x_bytes - from_x, a.x_part, a.w + from, a.ldw, a.w_bytes - from, a.w_part, steps, lds,
+           kStepBytes, k0 + steps == a.steps ? a.w_limit : kStepBytes);
+  if constexpr (kWhat == kParted) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = (wave / S::kWN) * S::kFM * 32, c0 = n0 + (wave % S::kWN) * S::kFN * 32 + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < S::kFM; ++i) {
+      const int row = m0 + wm + 32 * i + (lane & 31);
+      float* to = a.part + ((long long)split * g.m * S::kBM + row) * a.ldp + c0;
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (row < rows && c0 + 32 * j + 8 * q < a.ldp)
+            *(f32x4*)(to + 32 * j + 8 * q) = f32x4{tile.acc[i][j][4 * q], tile.acc[i][j][4 * q + 1],
+                                                   tile.acc[i][j][4 * q + 2], tile.acc[i][j][4 * q + 3]};
+    }
+    return;
+  }
   if (!a.bias && n0 + S::kBN <= a.v)
     finish_logits<T, S, kWhat, true>(a, tile, m0, n0, rows);
   else
     finish_logits<T, S, kWhat, false>(a, tile, m0, n0, rows);
+}
+
+// The parts' sums, and what finish_logits makes of them, for groups of 64 classes: 16 lanes a row, four classes
+// each.  Bound by the parts' bytes.
+constexpr int kSumRows = 64;      // of a workgroup
+constexpr int kSumGroup = 64;
+template <typename T, bool kKeeps>
+__global__ __launch_bounds__(kThreads) void sum_logits_kernel(const LogitArgs<T> a) {
+  const int rows = max(a.chunk.rows(a.n_valid), 0), splits = a.sharing.splits(rows);
+  const long long plane = (long long)a.sharing.tiles_m(rows) * a.sharing.bm * a.ldp;
+  const int in = threadIdx.x & 15, c = blockIdx.x * kSumGroup + in * 4;
+  f32x4 bias;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    bias[k] = c + k >= a.v ? -__builtin_inff() : a.bias ? TypeOf<T>::to_float(a.bias[c + k]) : 0.0f;
+  const int lo = blockIdx.y * kSumRows, hi = min(rows, lo + kSumRows);
+  for (int r0 = lo; r0 < hi; r0 += kThreads / 16) {
+    const int r = min(r0 + ((int)threadIdx.x >> 4), hi - 1);      // the last row by several: the same values
+    const float* from = a.part + (long long)r * a.ldp + c;
+    f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+    int k = 0;
+    for (; k + 4 <= splits; k += 4) {
+      f32x4 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) p[u] = *(const f32x4*)(from + (k + u) * plane);
+      z += (p[0] + p[1]) + (p[2] + p[3]);
+    }
+    for (; k < splits; ++k) z += *(const f32x4*)(from + k * plane);
+    const int y = a.label[r] - c;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      // what stands behind the last class may be anything
+      z[u] = c + u >= a.v ? -__builtin_inff() : z[u] + bias[u];
+      top = fmaxf(top, z[u]);
+      if (y == u) a.z_label[r] = z[u];
+    }
+    top = fmaxf(top, rotated<8>(top));
+    top = fmaxf(top, rotated<4>(top));
+    top = fmaxf(top, rotated<2>(top));
+    top = fmaxf(top, rotated<1>(top));
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum += exp_for<T>(z[u] - base);
+    sum = sum16(sum);
+    if (in == 0) a.stats[blockIdx.x * a.ld_stats + r] = make_float2(top, sum);
+    if constexpr (kKeeps) {
+      if constexpr (sizeof(T) == 4) {
+        *(f32x4*)((float*)a.z + in_panels(r, c, a.chunk_rows)) = z;
+      } else {
+        unsigned w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          w[u] = __builtin_bit_cast(
+              unsigned, __builtin_amdgcn_cvt_pknorm_u16((z[2 * u] - base) * (-kLog2e * Kept<T>::kSteps / 65535.0f),
+                                                        (z[2 * u + 1] - base) * (-kLog2e * Kept<T>::kSteps / 65535.0f)));
+        *(unsigned long long*)((unsigned short*)a.z + in_panels(r, c, a.chunk_rows)) =
+            (unsigned long long)w[1] << 32 | w[0];
+      }
+    }
+  }
 }
 
 constexpr int kProbRows = 256;
@@ -573,17 +670,6 @@ __global__ __launch_bounds__(kThreads) void finish_loss_kernel(const double* __r
 // ---------------------------------------------------------------------------------------------
 // Gradients
 // ---------------------------------------------------------------------------------------------
-// How many splits a product of fewer rows than it was launched for takes: its workgroups share the tiles there are.
-struct Sharing {
-  int bm, tiles_n;         // of a tile's rows; tiles side by side
-  int workgroups;
-  int least, most;         // splits
-  __device__ __forceinline__ int tiles_m(const int rows) const { return (rows + bm - 1) / bm; }
-  __device__ __forceinline__ int splits(const int rows) const {
-    return least == most || rows <= 0 ? least : min(most, workgroups / (tiles_m(rows) * tiles_n));
-  }
-};
-
 template <typename T>
 struct ProductArgs {
   const char* p;               // P in panels of chunk_rows
@@ -821,8 +907,8 @@ struct Plan {
   int chunk, chunks;            // rows at a time
   int ldp;                      // columns of P
   bool whole;                   // a workgroup holds rows of logits whole
-  bool large_logits;
-  int group, groups;            // classes a wave of the logits' tiles takes
+  Cut logits;
+  int group, groups;            // classes that share a maximum: a wave's of a tile, or kSumGroup
   Cut dx, dw;
   long long ldpart;
 };
@@ -849,9 +935,14 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
     p.chunks = ceil_div(n, p.chunk);
   }
   const int terms = dtype == RH_F32 ? TypeOf<float>::kTerms : 1;
-  p.large_logits = cut(p.chunk, v, p.panels, terms, 1).large;
-  p.group = p.large_logits ? Large::kFN * 32 : Small::kFN * 32;
-  p.groups = ceil_div(v, p.large_logits ? Large::kBN : Small::kBN) * (p.large_logits ? Large::kWN : Small::kWN);
+  p.logits = cut(p.chunk, v, p.panels, terms, p.whole ? 1 : 64);
+  if (p.logits.splits > 1) {
+    p.group = kSumGroup;
+    p.groups = p.ldp / kSumGroup;
+  } else {
+    p.group = p.logits.large ? Large::kFN * 32 : Small::kFN * 32;
+    p.groups = ceil_div(v, p.logits.large ? Large::kBN : Small::kBN) * (p.logits.large ? Large::kWN : Small::kWN);
+  }
   p.dx = cut(p.chunk, d, p.ldp / kStepK, terms, 64);
   p.dw = cut(v, d, ceil_div(p.chunk, kStepK), terms, 64);
   p.ldpart = ceil_div(d, 4) * 4;
@@ -869,6 +960,7 @@ struct Space {
   float* z_label;
   float2* row_stats;
   double* loss;
+  float* z_part;
   char* z;
   char* p;               // z's place for the 16-bit types
   long long p_part;
@@ -901,6 +993,8 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   }
   s.stats = c.take<float2>((size_t)p.groups * p.chunk);
   s.z_label = c.take<float>(n);
+  if (p.logits.splits > 1)
+    s.z_part = c.take<float>((size_t)p.logits.splits * whole_tiles(p.logits, p.chunk) * p.ldp);
   s.row_stats = c.take<float2>(n);
   s.loss = c.take<double>(ceil_div(n, 32));
   if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) {
@@ -931,8 +1025,27 @@ static int launch_logits(LogitArgs<T> a, hipStream_t stream) {
   a.grid = Grid{ceil_div(a.chunk.most, S::kBM), ceil_div(a.v, S::kBN)};
   auto kernel = logits_kernel<T, S, kWhat>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)a.grid.m * a.grid.n), dim3(S::kThreads), S::kLdsBytes, stream, a);
+  const unsigned workgroups = kWhat == kParted ? a.sharing.workgroups : a.grid.m * a.grid.n;
+  hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(S::kThreads), S::kLdsBytes, stream, a);
   RH_CHECK_LAUNCH("logits_kernel");
+  return RH_OK;
+}
+
+template <typename T, What kWhat>
+static int launch_logits(const LogitArgs<T>& a, bool large, hipStream_t stream) {
+  return large ? launch_logits<T, Large, kWhat>(a, stream) : launch_logits<T, Small, kWhat>(a, stream);
+}
+
+// A chunk's logits, in parts where the plan says so.
+template <typename T>
+static int make_logits(const Plan& p, const LogitArgs<T>& a, bool keep, hipStream_t stream) {
+  if (p.logits.splits == 1)
+    return keep ? launch_logits<T, kKeep>(a, p.logits.large, stream) : launch_logits<T, kStats>(a, p.logits.large, stream);
+  if (int rc = launch_logits<T, kParted>(a, p.logits.large, stream)) return rc;
+  const dim3 grid(p.groups, ceil_div(a.chunk.most, kSumRows));
+  if (keep) hipLaunchKernelGGL((sum_logits_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
+  else hipLaunchKernelGGL((sum_logits_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
+  RH_CHECK_LAUNCH("sum_logits_kernel");
   return RH_OK;
 }
 
@@ -1117,6 +1230,8 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   a.ld_stats = p.chunk;
   a.z = s.z;
   a.ldp = p.ldp;
+  a.sharing = share(p.logits, p.chunk, v, p.logits.splits > 1 ? p.panels / 4 : 1);
+  a.part = s.z_part;
   for (int c = 0; c < p.chunks; ++c) {
     a.chunk = Chunk{c * p.chunk, n - c * p.chunk < p.chunk ? n - c * p.chunk : p.chunk};
     const int first = a.chunk.first;
@@ -1129,18 +1244,14 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
         if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
       continue;
     }
-    if (int rc = grads ? p.large_logits ? launch_logits<T, Large, kKeep>(a, stream)
-                                        : launch_logits<T, Small, kKeep>(a, stream)
-                       : p.large_logits ? launch_logits<T, Large, kStats>(a, stream)
-                                        : launch_logits<T, Small, kStats>(a, stream))
-      return rc;
+    if (int rc = make_logits(p, a, grads, stream)) return rc;
     hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, 32)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
                        p.groups, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,
                        s.loss + first / 32);
     RH_CHECK_LAUNCH("join_stats_kernel");
     if (!grads) continue;
-    if (int rc = p.large_logits ? launch_probs<T, Large::kFN * 32 / kStepK>(q, p, s, a, c, stream)
-                                : launch_probs<T, Small::kFN * 32 / kStepK>(q, p, s, a, c, stream))
+    if (int rc = p.group == 128 ? launch_probs<T, 128 / kStepK>(q, p, s, a, c, stream)
+                                : launch_probs<T, 64 / kStepK>(q, p, s, a, c, stream))
       return rc;
     if (q.dx)
       if (int rc = features_gradient(q, p, s, a, stream)) return rc;

@@ -103,11 +103,12 @@ static void plan_online(FewPlan& p, int n, int d, int v, int vals) {
   p.rows = n <= 1 ? 1 : n <= 2 ? 2 : 4;
   p.chunks = ceil_div(d, kThreads * vals);
   if (p.chunks == 3) p.chunks = 4;
-  if (n > 4 || p.rows * p.chunks > 4 || 2 * d < kThreads * vals) {      // or half of the threads idle
+  // 128 registers of rows and their sums at most; or half of the threads idle
+  if (n > 4 || p.chunks > 4 || p.rows * p.chunks * vals > 64 || 2 * d < kThreads * vals) {
     p.rows = p.chunks = 0;
     return;
   }
-  const int at_once = 16 / (p.rows * p.chunks);
+  const int at_once = 16 / (p.rows > p.chunks ? p.rows : p.chunks);
   p.blocks = ceil_div(v, 2 * at_once);
   if (p.blocks > 512) p.blocks = 512;
   p.parts = p.blocks;
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
                                                               float* __restrict__ z, const int ldz,
                                                               float2* __restrict__ part, float* __restrict__ dx_part,
                                                               const int ldpart) {
-  constexpr int kV = 16 / (int)sizeof(T), kA = 16 / (kN * kC), kVals = kA * kN;
+  constexpr int kV = 16 / (int)sizeof(T), kA = 16 / (kN > kC ? kN : kC), kVals = kA * kN;
   __shared__ f32x4 s_z[2][16];      // [value], one sum of each wave
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15;
   float xs[kN][kC][kV], acc[kN][kC][kV];
@@ -639,6 +640,15 @@ static int launch_online(const rh_linear_ce_args& q, const FewPlan& p, const Few
   return RH_OK;
 }
 
+template <typename T, int kN>
+static int online_chunks(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
+                         hipStream_t stream) {
+  if (p.chunks == 1) return launch_online<T, kN, 1>(q, p, s, y, stream);
+  if (p.chunks == 2) return launch_online<T, kN, 2>(q, p, s, y, stream);
+  if constexpr (kN * 4 * (16 / (int)sizeof(T)) <= 64) return launch_online<T, kN, 4>(q, p, s, y, stream);
+  return RH_EINVAL;      // no plan leads here
+}
+
 template <typename T>
 static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) {
   const int n = (int)q.n, v = (int)q.v;
@@ -646,12 +656,9 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
   const FewSpace s = few_space(q.workspace, p, n, flags);
   const Labels y{q.labels, q.labels_int64, q.ignore_index, v};
   if (p.rows) {
-    if (int rc = p.rows == 1 ? p.chunks == 1   ? launch_online<T, 1, 1>(q, p, s, y, stream)
-                               : p.chunks == 2 ? launch_online<T, 1, 2>(q, p, s, y, stream)
-                                               : launch_online<T, 1, 4>(q, p, s, y, stream)
-                 : p.rows == 2 ? p.chunks == 1 ? launch_online<T, 2, 1>(q, p, s, y, stream)
-                                               : launch_online<T, 2, 2>(q, p, s, y, stream)
-                               : launch_online<T, 4, 1>(q, p, s, y, stream))
+    if (int rc = p.rows == 1   ? online_chunks<T, 1>(q, p, s, y, stream)
+                 : p.rows == 2 ? online_chunks<T, 2>(q, p, s, y, stream)
+                               : online_chunks<T, 4>(q, p, s, y, stream))
       return rc;
   } else {
     auto logits = p.wide_w ? few_logits_kernel<T, true> : few_logits_kernel<T, false>;

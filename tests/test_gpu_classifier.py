@@ -263,6 +263,23 @@ def test_rows_in_chunks(rh):
         close(k, some[k], want[k])
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,v", [(17, 4001, 70), (40, 3000, 700), (300, 2100, 130), (130, 4096, 1000), (70, 1030, 65),
+                                   (600, 2048, 641), (33, 8200, 3)])
+def test_long_sums_of_few_logits(rh, n, d, v, dtype):
+    """Logits of few tiles and many features, whose sums are split; forward alone too."""
+    x, w, y, b = make(n, d, v, dtype, True, ignored=0.2, seed=22)
+    check_all(rh, x, w, y, b)
+    alone = rh.functional.linear_cross_entropy(x, w, y, b)
+    close("row_loss", alone["row_loss"], oracle(x, w, y, b)["row_loss"])
+    y[:] = -100
+    y[n - 1] = v - 1      # one row counts: its tile's sum in as many parts as there are workgroups
+    check_all(rh, x, w, y, b)
+    b[: v - 1] = float("-inf")
+    out = rh.functional.linear_cross_entropy(x, w, y, b, grads=(True, True, True))
+    assert float(out["loss"]) == 0.0 and (out["d_weight"] == 0).all() and (out["d_features"] == 0).all()
+
+
 @pytest.mark.parametrize("n,d,v,dtype", [(9001, 72, 70001, "f32"), (1_700_001, 24, 600, "bf16")])
 def test_rows_in_chunks_of_other_ways(rh, n, d, v, dtype):
     """float32, whose P lies beside the logits, and whole rows of few classes: more than one chunk of each."""

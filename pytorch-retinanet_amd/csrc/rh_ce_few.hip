@@ -4,7 +4,7 @@
 //   logits      z[row][class] in float32, 16 classes x 16 rows to a matrix instruction that takes the
 //               weights straight from memory, and each workgroup's (max, sum of exp) of every row
 //   rows        the rows' (max, sum), losses and the call's loss
-//   gradients   one more pass over the weights: dW rows written, dX summed per workgroup; P stays float32
+//   products    one more pass over the weights: dW rows written, dX summed per workgroup; P stays float32
 //   features    the workgroups' parts of dX joined
 //
 // Up to four rows whose sums fit a workgroup's registers read the weights once: see `online`.
@@ -85,7 +85,8 @@ struct FewSpace {
 struct FewPlan {
   int groups, waves, blocks;        // logits: groups of 16 classes
   int ldz;
-  int tpr, subsets, slices;         // gradients: threads a row of weights, rows side by side, column slices
+  // products: 16-lane columns of four waves; weights: threads a row; rows side by side, slices of columns
+  int tpr, subsets, slices;
   int grad_blocks, per;             // classes a workgroup takes
   int parts, ldpart;
   bool wide_w;
@@ -95,7 +96,7 @@ struct FewPlan {
 // Online: dX = sum of p W over the other classes, without P's normalisation, which is not known before the last class.  A workgroup
 // takes whole rows of weights, so what a thread read for the logits is still in its registers when their
 // exponentials are known: dX's sum is kept relative to the running maximum and joined like a softmax's.
-// The weights are read once; dW is written by the gradients' pass, which then reads none.
+// The weights are read once; dW is written by a pass that reads none.
 // 1 x 2048 rows, 65 536 classes, bfloat16 (268 MB of weights, as much of dW): 208 us with two readings, 145
 // with one (87 this pass, 45 the one that writes), 4.1 TB/s over both.  Loads for the next classes issued ahead, more
 // workgroups or contiguous runs of classes for each: no faster; what they read was written behind the caches.
@@ -122,20 +123,23 @@ static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
   p.waves = p.groups < 2048 ? p.groups : 2048;
   p.blocks = ceil_div(p.waves, 4);
   p.ldz = ceil_div(v, 16) * 16;
-  p.tpr = 16;
-  while (p.tpr < kThreads && p.tpr * vals < d) p.tpr *= 2;
-  p.subsets = kThreads / p.tpr;
-  p.slices = ceil_div(d, p.tpr * vals);
-  int blocks = 512 / (p.slices < 512 ? p.slices : 512);
-  const int most = ceil_div(v, 4 * p.subsets);
-  if (blocks > most) blocks = most;
-  if (blocks < 1) blocks = 1;
-  p.per = ceil_div(ceil_div(v, blocks), p.subsets) * p.subsets;
-  p.grad_blocks = ceil_div(v, p.per);
-  p.parts = p.grad_blocks * p.subsets;
-  p.ldpart = p.slices * p.tpr * vals;
   p.wide_w = !(flags & RH_CE_COPY_WEIGHT);      // here that only says how the weights are read
   if (flags & RH_CE_GRAD_X) plan_online(p, n, d, v, vals);
+  const int whole = p.rows ? kThreads : 64;      // threads, or sixteen times the waves, of a row of weights
+  p.tpr = 16;
+  while (p.tpr < whole && p.tpr * vals < d) p.tpr *= 2;
+  p.subsets = whole / p.tpr;
+  p.slices = ceil_div(d, p.tpr * vals);
+  int blocks = (p.rows ? 512 : 1024) / (p.slices < 512 ? p.slices : 512);
+  const int step = p.rows ? p.subsets : 16 * p.subsets, most = ceil_div(v, 4 * p.subsets);
+  if (blocks > most) blocks = most;
+  if (blocks < 1) blocks = 1;
+  p.per = ceil_div(ceil_div(v, blocks), step) * step;
+  p.grad_blocks = ceil_div(v, p.per);
+  if (!p.rows) {
+    p.parts = p.grad_blocks * p.subsets;
+    p.ldpart = p.slices * p.tpr * vals;
+  }
   return p;
 }
 
@@ -444,15 +448,14 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
   }
 }
 
-// A thread has 16 bytes of columns; kN rows of features beside them in registers.  The workgroup's
-// classes are taken `subsets` at a time, a class by tpr threads.  Bound by memory where there is much: dW of
-// 65 536 x 2048 bfloat16 alone (268 MB written) 45 us, with the weights read again for dX 131.
-template <typename T, int kN, bool kWide>
-__global__ __launch_bounds__(kThreads) void few_gradients_kernel(
-    const T* __restrict__ x, const long long ldx, const int n, const int d, const T* __restrict__ w,
-    const long long ldw, const int v, const Labels y, const float* __restrict__ z, const int ldz,
-    const float2* __restrict__ row, const float* __restrict__ scale, const int per, const int tpr,
-    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ dx_part, const int ldpart) {
+// dW and db of up to four rows whose dX is made online.  A thread has 16 bytes of columns, the rows' features
+// beside them in registers; the workgroup's classes are taken `subsets` at a time, a class by tpr threads.  Bound
+// by the bytes it writes: 65 536 x 2048 bfloat16 (268 MB) 45 us.
+template <typename T, int kN>
+__global__ __launch_bounds__(kThreads) void few_weights_kernel(
+    const T* __restrict__ x, const long long ldx, const int n, const int d, const int v, const Labels y,
+    const float* __restrict__ z, const int ldz, const float2* __restrict__ row, const float* __restrict__ scale,
+    const int per, const int tpr, T* __restrict__ dw, T* __restrict__ db) {
   constexpr int kV = 16 / (int)sizeof(T);
   constexpr int kAtOnce = 128;      // classes whose probabilities wait in LDS
   __shared__ float s_p[kAtOnce][kN];
@@ -464,24 +467,13 @@ __global__ __launch_bounds__(kThreads) void few_gradients_kernel(
   if (t < kN) {
     const long long label = t < n ? y.at(t) : y.ignore;
     s_label[t] = t < n && y.counts(label) ? (int)label : -1;
-    s_row[t] = s_label[t] >= 0 ? row[t] : make_float2(0.0f, 0.0f);
+    s_row[t] = s_label[t] >= 0 ? row[t] : make_float2(0.0f, 1.0f);
   }
   __syncthreads();
-  // 16 rows beside 16 sums of eight columns each leave no room for the rows as floats
-  constexpr bool kPacked = kN * kV > 64;
-  constexpr int kAtATime = kN <= 2 ? 4 : kN <= 8 ? 2 : 1;      // rows of weights in flight a thread
-  [[maybe_unused]] float xs[kPacked ? 1 : kN][kV];
-  [[maybe_unused]] u32x4 xp[kPacked ? kN : 1];
-  float acc[kN][kV];
+  float xs[kN][kV];
 #pragma unroll
-  for (int r = 0; r < kN; ++r) {
-    // what a row left out holds must not meet its zeros
-    const u32x4 u = s_label[r] >= 0 ? load_values<T, false>(x + r * ldx + c, d - c) : u32x4{0, 0, 0, 0};
-    if constexpr (kPacked) xp[r] = u;
-    else to_floats<T>(u, xs[r]);
-#pragma unroll
-    for (int k = 0; k < kV; ++k) acc[r][k] = 0.0f;
-  }
+  for (int r = 0; r < kN; ++r)      // what a row left out holds must not meet its zeros
+    to_floats<T>(s_label[r] >= 0 ? load_values<T, false>(x + r * ldx + c, d - c) : u32x4{0, 0, 0, 0}, xs[r]);
   const int lo = blockIdx.x * per, hi = min(v, lo + per);
   for (int v0 = lo; v0 < hi; v0 += kAtOnce) {
     const int count = min(kAtOnce, hi - v0);
@@ -504,70 +496,146 @@ __global__ __launch_bounds__(kThreads) void few_gradients_kernel(
         for (int r = 0; r < kN; ++r) sum += s_p[a][r];
         db[v0 + a] = TypeOf<T>::from_float(sum);
       }
-    if (c >= d) continue;
-#pragma unroll 1
-    for (int a0 = subset; a0 < count; a0 += kAtATime * subsets) {
-      u32x4 ws[kAtATime];
+    if (!dw || c >= d) continue;
+#pragma unroll 4
+    for (int a = subset; a < count; a += subsets) {
+      union {
+        T v[kV];
+        u32x4 u;
+      } out;
+#pragma unroll
+      for (int k = 0; k < kV; ++k) {
+        float g = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kN; ++r) g = __builtin_fmaf(s_p[a][r], xs[r][k], g);
+        out.v[k] = TypeOf<T>::from_float(g);
+      }
+      T* to = dw + (long long)(v0 + a) * d + c;
+      if (d % kV == 0) {
+        *(u32x4*)to = out.u;
+      } else {
+#pragma unroll
+        for (int k = 0; k < kV; ++k)
+          if (c + k < d) to[k] = out.v[k];
+      }
+    }
+  }
+}
+
+// The gradients otherwise, by float32 matrix instructions (16 x 16 x 4) where vector ones would take 32
+// operations a weight: a wave takes 16 classes by 16 lanes' 16 bytes of columns.  dX = P W needs no transposition: a
+// lane's one weight of k is the class of its load, and the columns of its kV instructions are its own kV neighbours.
+// dW = P^T X has the rows as k.  P and both products stay float32.  Bound by memory: 16 x 2048 rows, 65 536 classes,
+// bfloat16 (268 MB read, 268 written) 139 us; 16 x 572, 62 202 classes, float32 74.  By vector instructions 484, 174.
+template <typename T, bool kWide>
+__global__ __launch_bounds__(kThreads) void few_products_kernel(
+    const T* __restrict__ x, const long long ldx, const int n, const int d, const T* __restrict__ w,
+    const long long ldw, const int v, const Labels y, const float* __restrict__ z, const int ldz,
+    const float2* __restrict__ row, const float* __restrict__ scale, const int per, const int waves_a_row,
+    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ dx_part, const int ldpart) {
+  constexpr int kV = 16 / (int)sizeof(T), kAtOnce = 128, kPitch = kFewRows + 1;      // rows a bank apart
+  __shared__ float s_p[kAtOnce * kPitch];
+  __shared__ float2 s_row[kFewRows];
+  __shared__ int s_label[kFewRows];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15, piece = lane >> 4;
+  const int subsets = 4 / waves_a_row, subset = wave / waves_a_row;
+  const int c = ((blockIdx.y * waves_a_row + wave % waves_a_row) * 16 + in) * kV;
+  const float s = *scale;
+  if (t < kFewRows) {
+    const long long label = t < n ? y.at(t) : y.ignore;
+    s_label[t] = t < n && y.counts(label) ? (int)label : -1;
+    s_row[t] = s_label[t] >= 0 ? row[t] : make_float2(0.0f, 1.0f);
+  }
+  __syncthreads();
+  float xs[4][kV];      // [k / 4]: rows 4 k + piece
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = 4 * k + piece;
+    // what a row left out holds must not meet its zeros
+    to_floats<T>(s_label[r] >= 0 ? load_values<T, false>(x + r * ldx + c, d - c) : u32x4{0, 0, 0, 0}, xs[k]);
+  }
+  f32x4 acc[kV];
+#pragma unroll
+  for (int j = 0; j < kV; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int lo = blockIdx.x * per, hi = min(v, lo + per);
+  for (int v0 = lo; v0 < hi; v0 += kAtOnce) {
+    const int count = min(kAtOnce, hi - v0);
+    __syncthreads();
+    for (int i = t; i < kAtOnce * kFewRows; i += kThreads) {
+      const int r = i / kAtOnce, a = i % kAtOnce;
+      float p = 0.0f;
+      if (a < count && s_label[r] >= 0) {
+        // the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
+        p = expf(z[(long long)r * ldz + v0 + a] - s_row[r].x) - (s_label[r] == v0 + a ? s_row[r].y : 0.0f);
+        p = p / s_row[r].y * s;
+      }
+      s_p[a * kPitch + r] = p;
+    }
+    __syncthreads();
+    if (db && blockIdx.y == 0)
+      for (int a = t; a < count; a += kThreads) {
+        float sum = 0.0f;
+        for (int r = 0; r < n; ++r) sum += s_p[a * kPitch + r];
+        db[v0 + a] = TypeOf<T>::from_float(sum);
+      }
+    for (int a0 = subset * 16; a0 < count; a0 += subsets * 16) {
+      u32x4 ws[4];
       if (dx_part) {
 #pragma unroll
-        for (int u = 0; u < kAtATime; ++u) {
-          const int a = min(a0 + u * subsets, count - 1);
-          ws[u] = load_values<T, kWide>(w + (long long)(v0 + a) * ldw + c, d - c);
-        }
+        for (int k = 0; k < 4; ++k)
+          ws[k] = load_values<T, kWide>(w + (long long)min(v0 + a0 + 4 * k + piece, v - 1) * ldw + c, d - c);
       }
+      if (dw) {
+        f32x4 out[kV];
 #pragma unroll
-      for (int u = 0; u < kAtATime; ++u) {
-        const int a = a0 + u * subsets;
-        if (a >= count) continue;
-        float f[kV], g[kV];
-        if (dx_part) to_floats<T>(ws[u], f);
+        for (int j = 0; j < kV; ++j) out[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < kV; ++k) g[k] = 0.0f;
+        for (int k = 0; k < 4; ++k) {
+          const float p = s_p[(a0 + in) * kPitch + 4 * k + piece];
 #pragma unroll
-        for (int r = 0; r < kN; ++r) {
-          const float p = s_p[a][r];
-          if (dx_part)
-#pragma unroll
-            for (int k = 0; k < kV; ++k) acc[r][k] = __builtin_fmaf(p, f[k], acc[r][k]);
-          if (dw) {
-            float xr[kV];
-            if constexpr (kPacked) {
-              to_floats<T>(xp[r], xr);
-            } else {
-#pragma unroll
-              for (int k = 0; k < kV; ++k) xr[k] = xs[r][k];
-            }
-#pragma unroll
-            for (int k = 0; k < kV; ++k) g[k] = __builtin_fmaf(p, xr[k], g[k]);
-          }
+          for (int j = 0; j < kV; ++j) out[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, xs[k][j], out[j], 0, 0, 0);
         }
-        if (dw) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int a = a0 + 4 * piece + r;
           union {
             T v[kV];
             u32x4 u;
-          } out;
+          } values;
 #pragma unroll
-          for (int k = 0; k < kV; ++k) out.v[k] = TypeOf<T>::from_float(g[k]);
+          for (int j = 0; j < kV; ++j) values.v[j] = TypeOf<T>::from_float(out[j][r]);
           T* to = dw + (long long)(v0 + a) * d + c;
-          if (d % kV == 0) {
-            *(u32x4*)to = out.u;
-          } else {
+          if (a < count) {
+            if (d % kV == 0) {
+              if (c < d) *(u32x4*)to = values.u;
+            } else {
 #pragma unroll
-            for (int k = 0; k < kV; ++k)
-              if (c + k < d) to[k] = out.v[k];
+              for (int j = 0; j < kV; ++j)
+                if (c + j < d) to[j] = values.v[j];
+            }
           }
+        }
+      }
+      if (dx_part) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p = s_p[(a0 + 4 * k + piece) * kPitch + in];
+          float f[kV];
+          to_floats<T>(ws[k], f);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, f[j], acc[j], 0, 0, 0);
         }
       }
     }
   }
-  if (dx_part && c < ldpart) {
+  if (dx_part) {
 #pragma unroll
-    for (int r = 0; r < kN; ++r) {
-      if (r < n) {
-      float* to = dx_part + ((long long)(blockIdx.x * subsets + subset) * n + r) * ldpart + c;
+    for (int r = 0; r < 4; ++r) {
+      const int at = 4 * piece + r;
+      float* to = dx_part + ((long long)(blockIdx.x * subsets + subset) * n + at) * ldpart + c;
+      if (at < n)
 #pragma unroll
-      for (int k = 0; k < kV; k += 4) *(f32x4*)(to + k) = f32x4{acc[r][k], acc[r][k + 1], acc[r][k + 2], acc[r][k + 3]};
-      }
+        for (int j = 0; j < kV; j += 4) *(f32x4*)(to + j) = f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
     }
   }
 }
@@ -619,13 +687,23 @@ __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __r
 }
 
 template <typename T, int kN>
-static int launch_gradients(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
-                            hipStream_t stream) {
-  auto kernel = p.wide_w ? few_gradients_kernel<T, kN, true> : few_gradients_kernel<T, kN, false>;
+static int launch_weights(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
+                          hipStream_t stream) {
+  hipLaunchKernelGGL((few_weights_kernel<T, kN>), dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x,
+                     (long long)q.ldx, (int)q.n, q.d, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per, p.tpr, (T*)q.dw,
+                     (T*)q.db);
+  RH_CHECK_LAUNCH("few_weights_kernel");
+  return RH_OK;
+}
+
+template <typename T>
+static int launch_products(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
+                           hipStream_t stream) {
+  auto kernel = p.wide_w ? few_products_kernel<T, true> : few_products_kernel<T, false>;
   hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
-                     (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per, p.tpr,
-                     (T*)q.dw, (T*)q.db, p.rows ? nullptr : s.dx_part, p.ldpart);
-  RH_CHECK_LAUNCH("few_gradients_kernel");
+                     (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per,
+                     p.tpr / 16, (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart);
+  RH_CHECK_LAUNCH("few_products_kernel");
   return RH_OK;
 }
 
@@ -671,13 +749,14 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
                      s.of_label);
   RH_CHECK_LAUNCH("few_rows_kernel");
   if (!q.dx && !q.dw && !q.db) return RH_OK;
-  if (p.rows && !q.dw && !q.db) {
-  } else if (int rc = n <= 1   ? launch_gradients<T, 1>(q, p, s, y, stream)
-               : n <= 2 ? launch_gradients<T, 2>(q, p, s, y, stream)
-               : n <= 4 ? launch_gradients<T, 4>(q, p, s, y, stream)
-               : n <= 8 ? launch_gradients<T, 8>(q, p, s, y, stream)
-                        : launch_gradients<T, 16>(q, p, s, y, stream))
-    return rc;
+  if (!p.rows) {
+    if (int rc = launch_products<T>(q, p, s, y, stream)) return rc;
+  } else if (q.dw || q.db) {
+    if (int rc = p.rows == 1   ? launch_weights<T, 1>(q, p, s, y, stream)
+                 : p.rows == 2 ? launch_weights<T, 2>(q, p, s, y, stream)
+                               : launch_weights<T, 4>(q, p, s, y, stream))
+      return rc;
+  }
   if (q.dx) {
     hipLaunchKernelGGL(few_features_kernel<T>, dim3(ceil_div(q.d, 16), n), dim3(kThreads), 0, stream, s.dx_part, p.parts, n,
                        p.ldpart, q.d, s.share, s.of_label, s.scale, y, (const T*)q.w, (long long)q.ldw, (T*)q.dx);

@@ -611,8 +611,9 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict_
     column_sums[(long long)blockIdx.y * v + first + i] = (s_sum[0][i] + s_sum[1][i]) + (s_sum[2][i] + s_sum[3][i]);
 }
 
-// Row loss and (max, sum) of every place from the tiles' pairs: eight threads a row, each an
-// eighth of the tiles.  9 us for 3891 rows of 256 pairs.
+// Row loss and (max, sum) of every place from the groups' pairs: 32 threads a row, each a 32nd of the groups.
+// 9 us for 3891 rows of 256 pairs.
+constexpr int kJoinRows = 8;      // of a workgroup
 __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __restrict__ stats,
                                                               const long long ld, const int groups,
                                                               const Chunk chunk, const int* __restrict__ n_valid,
@@ -621,17 +622,18 @@ __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __re
                                                               float2* __restrict__ row_stats,
                                                               float* __restrict__ row_loss,
                                                               double* __restrict__ partial) {
-  __shared__ float s_top[8][32], s_sum[8][32];
-  const int rows = chunk.rows(n_valid), r = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int row = blockIdx.x * 32 + r;
+  constexpr int kParts = kThreads / kJoinRows;
+  __shared__ float s_top[kParts][kJoinRows], s_sum[kParts][kJoinRows];
+  const int rows = chunk.rows(n_valid), r = threadIdx.x % kJoinRows, part = threadIdx.x / kJoinRows;
+  const int row = blockIdx.x * kJoinRows + r;
   float top = -__builtin_inff(), sum = 0.0f;
   if (row < rows) {
-    for (int t0 = part; t0 < groups; t0 += 64) {      // eight at a time, their loads together
+    for (int t0 = part; t0 < groups; t0 += 8 * kParts) {      // eight at a time, their loads together
       float2 p[8];
       float up = top;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        p[k] = t0 + 8 * k < groups ? stats[(t0 + 8 * k) * ld + row] : make_float2(-__builtin_inff(), 0.0f);
+        p[k] = t0 + kParts * k < groups ? stats[(t0 + kParts * k) * ld + row] : make_float2(-__builtin_inff(), 0.0f);
         up = fmaxf(up, p[k].x);
       }
       const float base = up == -__builtin_inff() ? 0.0f : up;
@@ -649,9 +651,9 @@ __global__ __launch_bounds__(kThreads) void join_stats_kernel(const float2* __re
     if (part == 0 && row < rows) {
       top = -__builtin_inff();
       sum = 0.0f;
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, s_top[k][r]);
+      for (int k = 0; k < kParts; ++k) top = fmaxf(top, s_top[k][r]);
       const float base = top == -__builtin_inff() ? 0.0f : top;
-      for (int k = 0; k < 8; ++k) sum += s_sum[k][r] * expf(s_top[k][r] - base);
+      for (int k = 0; k < kParts; ++k) sum += s_sum[k][r] * expf(s_top[k][r] - base);
       const float v = (top - z_label[row]) + logf(sum);
       row_stats[row] = make_float2(top, sum);
       row_loss[map[row]] = v;
@@ -727,6 +729,30 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
   const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32 + 4 * (lane >> 5);
   const float s = *a.scale * a.down;
   const int room = a.n - n0 - wn;      // this lane's columns (32 j + 8 q + r) below it exist
+  if constexpr (kTo == kSingly) {
+    // Rows of any alignment: 32 rows at a time through LDS, so that a store's lanes are neighbours in a row.  dW of
+    // 8997 x 3087 over 57 rows, float: 50 us, 119 with a lane's four columns stored as they are.
+    constexpr int kWide = S::kFN * 32, kPitch = kWide + 1;
+    RH_LDS float* const mine = (RH_LDS float*)lds + wave * 32 * kPitch;
+    const int first = n0 + (wave % S::kWN) * kWide;
+#pragma unroll
+    for (int i = 0; i < S::kFM; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::kFN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          mine[(lane & 31) * kPitch + 32 * j + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = tile.acc[i][j][r] * s;
+      const int base = m0 + wm + 32 * i, rows_here = min(32, m - base);
+#pragma unroll 4
+      for (int r = 0; r < rows_here; ++r) {
+        T* const out = a.out + (a.map ? a.map[base + r] : base + r) * a.ldo + first;
+#pragma unroll
+        for (int c = 0; c < kWide; c += 64)
+          if (first + c + lane < a.n) out[c + lane] = TypeOf<T>::from_float(mine[r * kPitch + c + lane]);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < S::kFM; ++i) {
     const int row = m0 + wm + 32 * i + (lane & 31);
@@ -763,10 +789,6 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
                 const int c = 32 * j + 8 * (q - 1) + 4 * (lane >> 5);      // from this lane's first column
                 if (c < room) *(u32x4*)(out + c) = eight;
               }
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (32 * j + 8 * q + r < room) to[r] = v.v[r];
             }
           }
       }
@@ -996,7 +1018,7 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   if (p.logits.splits > 1)
     s.z_part = c.take<float>((size_t)p.logits.splits * whole_tiles(p.logits, p.chunk) * p.ldp);
   s.row_stats = c.take<float2>(n);
-  s.loss = c.take<double>(ceil_div(n, 32));
+  s.loss = c.take<double>(ceil_div(n, kJoinRows));
   if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) {
     s.z = c.take<char>((size_t)p.chunk * p.ldp * p.kept_size);
     s.p_part = (long long)p.chunk * p.ldp * 2;
@@ -1069,7 +1091,7 @@ static int launch_probs(const rh_linear_ce_args& q, const Plan& p, const Space& 
                      s.p, s.p_part, p.chunk, p.ldp, a.v, a.chunk, a.n_valid, a.label, s.row_stats + a.chunk.first, s.stats,
                      a.ld_stats,
                      s.db_part ? s.db_part + (long long)chunk * blocks * a.v : nullptr, s.loss,
-                     chunk == p.chunks - 1 ? ceil_div(q.n, 32) : 0, q.small);
+                     chunk == p.chunks - 1 ? ceil_div(q.n, kJoinRows) : 0, q.small);
   RH_CHECK_LAUNCH("probs_kernel");
   return RH_OK;
 }
@@ -1189,7 +1211,10 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   const Labels labels{q.labels, q.labels_int64, q.ignore_index, v};
   hipLaunchKernelGGL(count_rows_kernel, dim3(p.row_blocks), dim3(64), 0, stream, labels, n, p.per, s.blocks);
   RH_CHECK_LAUNCH("count_rows_kernel");
-  const int side = ceil_div(p.panels, 16) < 8 ? ceil_div(p.panels, 16) : 8;
+  // a panel a wave where there are few rows
+  int side = ceil_div(p.panels, 16) < 8 ? ceil_div(p.panels, 16) : 8;
+  if (side < 256 / p.row_blocks) side = 256 / p.row_blocks;
+  if (side > ceil_div(p.panels, 4)) side = ceil_div(p.panels, 4);
   hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks, side), dim3(kThreads), 0, stream, (const T*)q.x,
                      (long long)q.ldx, d, labels, n, p.per, s.blocks, s.x, s.x_part, p.panels, p.chunk, s.info, q.row_loss,
                      (T*)q.dx, q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
@@ -1245,9 +1270,9 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
       continue;
     }
     if (int rc = make_logits(p, a, grads, stream)) return rc;
-    hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, 32)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
+    hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, kJoinRows)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
                        p.groups, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,
-                       s.loss + first / 32);
+                       s.loss + first / kJoinRows);
     RH_CHECK_LAUNCH("join_stats_kernel");
     if (!grads) continue;
     if (int rc = p.group == 128 ? launch_probs<T, 128 / kStepK>(q, p, s, a, c, stream)
@@ -1260,7 +1285,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   }
   if (!grads || (p.whole && !q.db)) {
     hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss,
-                       ceil_div(n, p.whole ? kWholeRows : 32), q.small);
+                       ceil_div(n, p.whole ? kWholeRows : kJoinRows), q.small);
     RH_CHECK_LAUNCH("finish_loss_kernel");
   }
   if (q.db) {

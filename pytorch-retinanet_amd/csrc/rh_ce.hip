@@ -85,16 +85,17 @@ __device__ __forceinline__ Eight<T> in_parts(const float (&f)[8]) {
   return out;
 }
 
-// Eight values from p on, of which `have` exist (the others are zero), in parts.
+// Eight values from p on, of which `have` exist (the others are zero), in parts.  p is aligned to its elements only:
+// the card's wide loads ask for no more.
 template <typename T>
-__device__ __forceinline__ Eight<T> load_parts(const T* p, const int have, const bool wide) {
+__device__ __forceinline__ Eight<T> load_parts(const T* p, const int have) {
   if constexpr (sizeof(T) == 2) {
     union {
       T v[8];
       Eight<T> e;
     } w;
-    if (wide && have >= 8) {
-      w.e.part[0] = *(const u32x4*)p;
+    if (have >= 8) {
+      __builtin_memcpy(&w, p, 16);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) w.v[k] = k < have ? p[k] : (T)0.0f;
@@ -102,13 +103,8 @@ __device__ __forceinline__ Eight<T> load_parts(const T* p, const int have, const
     return w.e;
   } else {
     float f[8];
-    if (wide && have >= 8) {
-      const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f[k] = a[k];
-        f[4 + k] = b[k];
-      }
+    if (have >= 8) {
+      __builtin_memcpy(f, p, 32);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = k < have ? p[k] : 0.0f;
@@ -185,14 +181,13 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
     }
   }
   __syncthreads();
-  const bool wide = ((ldx * (long long)sizeof(T)) & 15) == 0 && ((uintptr_t)x & 15) == 0;
   for (int p = blockIdx.y + gridDim.y * wave; p < panels; p += gridDim.y * 4) {
     const int c = p * kStepK + (lane & 3) * 8;
 #pragma unroll 2
     for (int r = lane >> 2; r < rows; r += 16) {
       const int to = s_place[r];
       if (to < 0) continue;
-      const Eight<T> w = load_parts<T>(x + (lo + r) * ldx + c, d - c, wide);
+      const Eight<T> w = load_parts<T>(x + (lo + r) * ldx + c, d - c);
       const int in = to / chunk;
       char* dst = xp + ((long long)in * chunk * panels * kStepK + in_panels(to - in * chunk, c, chunk)) * 2;
 #pragma unroll
@@ -207,15 +202,17 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
       }
 }
 
-// A copy of the weights with rows of whole 16-byte pieces, for a row length or stride that has none: read and
-// written once where every product would read them value by value.
+// A copy of the weights with rows of whole 16-byte pieces (ldp: of whole panels), for a row length or stride that
+// has none: the products' loads to LDS need them.  Bound by memory.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* __restrict__ w, const long long ldw,
                                                             const int d, const int v, T* __restrict__ out,
                                                             const int ldp) {
   const int lane = threadIdx.x & 63;
   for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < v; r += (long long)gridDim.x * 4)
-    for (int c = lane; c < ldp; c += 64) out[r * ldp + c] = c < d ? w[r * ldw + c] : (T)0.0f;
+#pragma unroll 4
+    for (int c = lane * 8; c < ldp; c += 512)
+      *(u32x4*)(out + r * ldp + c) = load_parts<T>(w + r * ldw + c, d - c).part[0];
 }
 
 // The weights in panels and parts (float), by 16 rows of a panel a wave.  Bound by memory: 16 384 x 1024, 67 MB read
@@ -224,12 +221,11 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void take_apart_kernel(const T* __restrict__ w, const long long ldw, const int d,
                                                               const int v, const int panels, char* __restrict__ out,
                                                               const long long part) {
-  const bool wide = ((ldw * (long long)sizeof(T)) & 15) == 0 && ((uintptr_t)w & 15) == 0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 16 + (lane >> 2);
   if (r >= v) return;
   for (int p = blockIdx.y * 4 + wave; p < panels; p += gridDim.y * 4) {
     const int c = p * kStepK + (lane & 3) * 8;
-    const Eight<T> e = load_parts<T>(w + (long long)r * ldw + c, d - c, wide);
+    const Eight<T> e = load_parts<T>(w + (long long)r * ldw + c, d - c);
     char* dst = out + in_panels(r, c, v) * 2;
 #pragma unroll
     for (int i = 0; i < TypeOf<T>::kParts; ++i) *(u32x4*)(dst + i * part) = e.part[i];

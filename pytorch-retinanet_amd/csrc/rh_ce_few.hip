@@ -54,8 +54,12 @@ __device__ __forceinline__ u32x4 load_values(const T* p, const int have) {
       T v[kV];
       u32x4 u;
     } r;
+    if (have >= kV) {
+      __builtin_memcpy(&r, p, 16);      // aligned to its elements: the card's wide loads ask for no more
+    } else {
 #pragma unroll
-    for (int i = 0; i < kV; ++i) r.v[i] = i < have ? p[i] : (T)0.0f;
+      for (int i = 0; i < kV; ++i) r.v[i] = i < have ? p[i] : (T)0.0f;
+    }
     return r.u;
   }
 }

@@ -689,8 +689,8 @@ struct ProductArgs {
   int add;                     // part += instead of part =
 };
 
-// float parts; the result, in rows of whole groups of eight 16-bit values, of four of either size, or not
-enum To { kParts, kOctets, kQuads, kSingly };
+// float parts; the result, in rows of whole 16 bytes or not
+enum To { kParts, kWhole, kSingly };
 
 // kLA = kRows: dX = P W, the sum over the classes; kCols: dW = P^T X, over the chunk's rows.  Bound by the matrix
 // units' power where the sums are long (8192 x 4096, 131 072 classes: 1.17 and 1.24 PFLOP/s), by filling the card
@@ -725,30 +725,6 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
   const int wm = (wave / S::kWN) * S::kFM * 32, wn = (wave % S::kWN) * S::kFN * 32 + 4 * (lane >> 5);
   const float s = *a.scale * a.down;
   const int room = a.n - n0 - wn;      // this lane's columns (32 j + 8 q + r) below it exist
-  if constexpr (kTo == kSingly) {
-    // Rows of any alignment: 32 rows at a time through LDS, so that a store's lanes are neighbours in a row.  dW of
-    // 8997 x 3087 over 57 rows, float: 50 us, 119 with a lane's four columns stored as they are.
-    constexpr int kWide = S::kFN * 32, kPitch = kWide + 1;
-    RH_LDS float* const mine = (RH_LDS float*)lds + wave * 32 * kPitch;
-    const int first = n0 + (wave % S::kWN) * kWide;
-#pragma unroll
-    for (int i = 0; i < S::kFM; ++i) {
-#pragma unroll
-      for (int j = 0; j < S::kFN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          mine[(lane & 31) * kPitch + 32 * j + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)] = tile.acc[i][j][r] * s;
-      const int base = m0 + wm + 32 * i, rows_here = min(32, m - base);
-#pragma unroll 4
-      for (int r = 0; r < rows_here; ++r) {
-        T* const out = a.out + (a.map ? a.map[base + r] : base + r) * a.ldo + first;
-#pragma unroll
-        for (int c = 0; c < kWide; c += 64)
-          if (first + c + lane < a.n) out[c + lane] = TypeOf<T>::from_float(mine[r * kPitch + c + lane]);
-      }
-    }
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < S::kFM; ++i) {
     const int row = m0 + wm + 32 * i + (lane & 31);
@@ -767,6 +743,22 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
             }
       } else {
         T* out = a.out + (a.map ? a.map[row] : row) * a.ldo + n0 + wn;
+        // 16 bytes a store, eight neighbouring columns of a 16-bit type or four of float; kSingly: of rows of any
+        // alignment, and the last of a row one by one
+        auto store = [&](T* to, const int left, const auto v) {
+          constexpr int kV = 16 / (int)sizeof(T);
+          if (kTo == kWhole) {
+            if (left > 0) *(u32x4*)to = __builtin_bit_cast(u32x4, v);
+          } else if (left >= kV) {
+            __builtin_memcpy(to, &v, 16);
+          } else {
+            T single[kV];
+            __builtin_memcpy(single, &v, 16);
+#pragma unroll
+            for (int r = 0; r < kV; ++r)
+              if (r < left) to[r] = single[r];
+          }
+        };
         [[maybe_unused]] unsigned long long half_group[2];
 #pragma unroll
         for (int j = 0; j < S::kFN; ++j)
@@ -775,15 +767,13 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
             Vec4<T> v;
 #pragma unroll
             for (int r = 0; r < 4; ++r) v.v[r] = TypeOf<T>::from_float(tile.acc[i][j][4 * q + r] * s);
-            T* to = out + 32 * j + 8 * q;
-            if constexpr (kTo == kQuads) {
-              if (32 * j + 8 * q < room) *(Vec4<T>*)to = v;
-            } else if constexpr (kTo == kOctets) {
+            if constexpr (sizeof(T) == 4) {
+              store(out + 32 * j + 8 * q, room - 32 * j - 8 * q, v);
+            } else {
               half_group[q & 1] = __builtin_bit_cast(unsigned long long, v);
-              if (q & 1) {      // eight neighbouring columns a lane
-                const u32x4 eight = whole_group(half_group[0], half_group[1]);
+              if (q & 1) {
                 const int c = 32 * j + 8 * (q - 1) + 4 * (lane >> 5);      // from this lane's first column
-                if (c < room) *(u32x4*)(out + c) = eight;
+                store(out + c, room - c, whole_group(half_group[0], half_group[1]));
               }
             }
           }
@@ -1069,10 +1059,9 @@ static int make_logits(const Plan& p, const LogitArgs<T>& a, bool keep, hipStrea
 
 template <typename T, Layout kLA, typename S>
 static int launch_product(const ProductArgs<T>& a, hipStream_t stream) {
-  constexpr To kWide = sizeof(T) == 2 ? kOctets : kQuads;
-  auto kernel = a.part                                ? product_kernel<T, kLA, S, kParts>
-                : a.n % (sizeof(T) == 2 ? 8 : 4) == 0 ? product_kernel<T, kLA, S, kWide>
-                                                      : product_kernel<T, kLA, S, kSingly>;
+  auto kernel = a.part                            ? product_kernel<T, kLA, S, kParts>
+                : a.n * (int)sizeof(T) % 16 == 0 ? product_kernel<T, kLA, S, kWhole>
+                                                 : product_kernel<T, kLA, S, kSingly>;
   if (int rc = raise_lds(kernel, S::kLdsBytes)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.sharing.workgroups), dim3(S::kThreads), S::kLdsBytes, stream, a);
   RH_CHECK_LAUNCH("product_kernel");

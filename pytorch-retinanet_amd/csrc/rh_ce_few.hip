@@ -517,6 +517,8 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
       T* to = dw + (long long)(v0 + a) * d + c;
       if (d % kV == 0) {
         *(u32x4*)to = out.u;
+      } else if (c + kV <= d) {
+        __builtin_memcpy(to, &out, 16);
       } else {
 #pragma unroll
         for (int k = 0; k < kV; ++k)
@@ -612,6 +614,8 @@ __global__ __launch_bounds__(kThreads) void few_products_kernel(
           if (a < count) {
             if (d % kV == 0) {
               if (c < d) *(u32x4*)to = values.u;
+            } else if (c + kV <= d) {
+              __builtin_memcpy(to, &values, 16);
             } else {
 #pragma unroll
               for (int j = 0; j < kV; ++j)

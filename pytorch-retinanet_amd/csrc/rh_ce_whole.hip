@@ -260,18 +260,21 @@ __global__ __launch_bounds__(kWholeThreads, kF <= 2 ? 4 : 2) void whole_kernel(c
         Vec4<T> v;
 #pragma unroll
         for (int r = 0; r < 4; ++r) v.v[r] = TypeOf<T>::from_float(out[j][4 * q + r] * scale);
-        const int c = wc * 64 + 32 * j + 8 * q + 4 * half;
-        if (wide) {
-          group[q & 1] = __builtin_bit_cast(unsigned long long, v);
-          if (q & 1) {
-            const u32x4 eight = whole_group(group[0], group[1]);
-            const int c8 = wc * 64 + 32 * j + 8 * (q - 1 + half);
-            if (n0 + c8 < a.d) *(u32x4*)(to + c8) = eight;
-          }
-        } else {
+        group[q & 1] = __builtin_bit_cast(unsigned long long, v);
+        if (q & 1) {
+          const u32x4 eight = whole_group(group[0], group[1]);
+          const int c = wc * 64 + 32 * j + 8 * (q - 1 + half), left = a.d - n0 - c;
+          if (wide) {
+            if (left > 0) *(u32x4*)(to + c) = eight;
+          } else if (left >= 8) {
+            __builtin_memcpy(to + c, &eight, 16);
+          } else {
+            T single[8];
+            __builtin_memcpy(single, &eight, 16);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n0 + c + r < a.d) to[c + r] = v.v[r];
+            for (int r = 0; r < 8; ++r)
+              if (r < left) to[c + r] = single[r];
+          }
         }
       }
     }

@@ -12,15 +12,17 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// exp as the loss needs it: for float results the accurate one; for 16-bit ones the hardware exp2 of a
-// rounded product (|x| * 6e-8 relative, far below the 2^-9 of the type the result is rounded to).
+// exp of many logits: the hardware's exp2 of a rounded product, an error of |x| * 2^-24 relative (and of log2 e's own
+// rounding, which float's takes back).  That is far below the 2^-9 that a 16-bit result is rounded by; for float it is
+// what rounding z itself does to e^z where |x| is no larger than |z|, and e^x is small where it is.
 template <typename T>
 __device__ __forceinline__ float exp_for(const float x) {
   return __builtin_amdgcn_exp2f(x * kLog2e);
 }
 template <>
 __device__ __forceinline__ float exp_for<float>(const float x) {
-  return expf(x);
+  constexpr float kRest = 1.925963033500853e-08f;      // log2 e - kLog2e
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, x * kRest));
 }
 
 struct Labels {

@@ -374,7 +374,7 @@ __device__ __forceinline__ void finish_logits(const LogitArgs<T>& a, const Acc& 
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           if constexpr (sizeof(T) == 4) {
-            sum += expf(z[j][r] - base);
+            sum += exp_for<T>(z[j][r] - base);
           } else {
             const float below = z[j][r] - base;      // first: z and base may be the type's lowest
             sum += exp_for<T>(below);
@@ -577,7 +577,7 @@ __global__ __launch_bounds__(kThreads) void probs_kernel(const void* __restrict_
         if constexpr (sizeof(T) == 4) {
           const unsigned w = z[i][k >> 2][k & 3];
           // the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
-          p[k] = (expf(__builtin_bit_cast(float, w) - of_row.x) - (y == i * kStepK + k ? of_row.y : 0.0f)) * f;
+          p[k] = (exp_for<T>(__builtin_bit_cast(float, w) - of_row.x) - (y == i * kStepK + k ? of_row.y : 0.0f)) * f;
         } else {
           const unsigned w = z[i][0][k >> 1], code = k & 1 ? w >> 16 : w & 0xffffu;
           const float e = __builtin_amdgcn_exp2f((float)code * (-1.0f / Kept<T>::kSteps));
@@ -880,7 +880,7 @@ struct Cut {
 // each pair is the small tiles' time: 80 / 94 us; over 1024: 194 / 182.  49 104 x 601 over 256: 40 / 67.
 // dX of 2048 x 1024 over 16 384 classes, float: 893 us unsplit, 499 of four splits, large and eight of
 // them 380.  200 x 512 over 10 000, bfloat16: 83 unsplit, 18 of sixteen, large 29 at best.
-static Cut cut(long long m, long long n, int steps, int terms, int most_splits) {
+static Cut cut(long long m, long long n, int steps, int terms, int most_splits, float large_end = 14.0f) {
   Cut best = {};
   float least = 0.0f;
   for (int large = 0; large < 2; ++large) {
@@ -892,7 +892,7 @@ static Cut cut(long long m, long long n, int steps, int terms, int most_splits) 
       const long long work = tiles * splits;
       const float filled = work < slots ? (float)work / slots : 1.0f;
       float us = (float)((work + slots - 1) / slots) *
-                 (((large ? 0.58f : 0.26f) + 0.30f * filled) * (float)c.steps * (float)terms + (large ? 14.0f : 6.0f));
+                 (((large ? 0.58f : 0.26f) + 0.30f * filled) * (float)c.steps * (float)terms + (large ? splits > 1 ? 14.0f : large_end : 6.0f));
       if (splits > 1) us += 4.0f + (float)splits * (float)m * (float)n * (4.0f / 4.5e6f);
       if (least == 0.0f || us < least) {
         least = us;
@@ -943,7 +943,8 @@ static Plan make_plan(int n, int d, int v, int dtype, int flags) {
     p.chunks = ceil_div(n, p.chunk);
   }
   const int terms = dtype == RH_F32 ? TypeOf<float>::kTerms : 1;
-  p.logits = cut(p.chunk, v, p.panels, terms, p.whole ? 1 : 64);
+  // float's logits: more registers than there are at the end of a large tile
+  p.logits = cut(p.chunk, v, p.panels, terms, p.whole ? 1 : 64, dtype == RH_F32 ? 30.0f : 14.0f);
   if (p.logits.splits > 1) {
     p.group = kSumGroup;
     p.groups = p.ldp / kSumGroup;

@@ -13,23 +13,35 @@
 namespace rh {
 namespace ce {
 
-typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(4))) double f64x4;
 
+// A row's largest logit, rounded to float, and the sum of the exponentials of the others' distance to it.
+struct TopSum {
+  double sum;
+  float top;
+};
+
+// Logits of so few rows are not averaged over many: float's are held and summed in 64 bits (Z), since rounding a
+// logit of 10 to float alone changes its probability by 5e-7.
 template <typename T>
 struct Mma16;      // 16 classes x 16 rows, 16 bytes of k a lane: lane % 16 is the class / row, lane / 16 the piece
 template <>
 struct Mma16<float> {
-  static __device__ __forceinline__ f32x4 run(const u32x4 a, const u32x4 b, f32x4 c) {
+  typedef double Z;
+  typedef f64x4 Acc;      // of lane l: row 4 r + l / 16
+  static __device__ __forceinline__ int row(const int piece, const int r) { return 4 * r + piece; }
+  static __device__ __forceinline__ Acc run(const u32x4 a, const u32x4 b, Acc c) {
     const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[0], y[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[1], y[1], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[2], y[2], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], y[3], c, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f64_16x16x4f64((double)x[i], (double)y[i], c, 0, 0, 0);
     return c;
   }
 };
 template <>
 struct Mma16<__bf16> {
+  typedef float Z;
+  typedef f32x4 Acc;      // row 4 (l / 16) + r
+  static __device__ __forceinline__ int row(const int piece, const int r) { return 4 * piece + r; }
   static __device__ __forceinline__ f32x4 run(const u32x4 a, const u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                    0, 0, 0);
@@ -37,6 +49,9 @@ struct Mma16<__bf16> {
 };
 template <>
 struct Mma16<_Float16> {
+  typedef float Z;
+  typedef f32x4 Acc;      // row 4 (l / 16) + r
+  static __device__ __forceinline__ int row(const int piece, const int r) { return 4 * piece + r; }
   static __device__ __forceinline__ f32x4 run(const u32x4 a, const u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                   0, 0);
@@ -76,9 +91,9 @@ __device__ __forceinline__ void to_floats(const u32x4 u, float (&f)[16 / sizeof(
 }
 
 struct FewSpace {
-  float* z;            // [n][ldz]
-  float2* part;        // [kFewRows][blocks]
-  float2* row;         // [kFewRows]  (max, sum), of a row that counts
+  void* z;             // [n][ldz]  float's are double
+  TopSum* part;        // [kFewRows][blocks]
+  TopSum* row;         // [kFewRows]  (max, sum), of a row that counts
   float* of_label;     // [kFewRows]  the label's p - 1
   float* scale;        // [1]
   float* dx_part;      // [parts][n][ldpart]
@@ -88,7 +103,7 @@ struct FewSpace {
 
 struct FewPlan {
   int groups, waves, blocks;        // logits: groups of 16 classes
-  int ldz;
+  int ldz, z_size;
   // products: 16-lane columns of four waves; weights: threads a row; rows side by side, slices of columns
   int tpr, subsets, slices;
   int grad_blocks, per;             // classes a workgroup takes
@@ -127,6 +142,7 @@ static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
   p.waves = p.groups < 2048 ? p.groups : 2048;
   p.blocks = ceil_div(p.waves, 4);
   p.ldz = ceil_div(v, 16) * 16;
+  p.z_size = dtype == RH_F32 ? 8 : 4;
   p.wide_w = !(flags & RH_CE_COPY_WEIGHT);      // here that only says how the weights are read
   if (flags & RH_CE_GRAD_X) plan_online(p, n, d, v, vals);
   const int whole = p.rows ? kThreads : 64;      // threads, or sixteen times the waves, of a row of weights
@@ -150,9 +166,9 @@ static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
 static FewSpace few_space(void* base, const FewPlan& p, int n, int flags) {
   Carver c(base);
   FewSpace s = {};
-  s.z = c.take<float>((size_t)n * p.ldz);
-  s.part = c.take<float2>((size_t)kFewRows * p.blocks);
-  s.row = c.take<float2>(kFewRows);
+  s.z = c.take<char>((size_t)n * p.ldz * p.z_size);
+  s.part = c.take<TopSum>((size_t)kFewRows * p.blocks);
+  s.row = c.take<TopSum>(kFewRows);
   s.of_label = c.take<float>(kFewRows);
   s.scale = c.take<float>(1);
   if (flags & RH_CE_GRAD_X) s.dx_part = c.take<float>((size_t)p.parts * n * p.ldpart);
@@ -177,18 +193,21 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
                                                               const int d, const T* __restrict__ w, const long long ldw,
                                                               const int v, const T* __restrict__ bias,
                                                               const int groups, const int waves,
-                                                              float* __restrict__ z, const int ldz,
-                                                              float2* __restrict__ part) {
+                                                              typename Mma16<T>::Z* __restrict__ z, const int ldz,
+                                                              TopSum* __restrict__ part) {
+  typedef typename Mma16<T>::Z Z;
+  typedef typename Mma16<T>::Acc Acc;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float2 s_part[4][16];
+  __shared__ TopSum s_part[4][16];
   constexpr int kV = 16 / (int)sizeof(T), kStepK = 4 * kV, kChunk = kChunkBytes / (int)sizeof(T);
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15, piece = lane >> 4;
   const int me = blockIdx.x * 4 + wave;
-  float top = -__builtin_inff(), sum = 0.0f;      // of row `in`, over this lane's classes
+  float top = -__builtin_inff();      // of row `in`, over this lane's classes
+  double sum = 0.0;
   for (int g0 = 0; g0 * waves < groups; g0 += kBatch) {
-    f32x4 acc[kBatch];
+    Acc acc[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kBatch; ++i) acc[i] = Acc{0, 0, 0, 0};
     const int mine = me < waves ? min(kBatch, (groups - me + waves - 1) / waves - g0) : 0;
     for (int k0 = 0; k0 < d; k0 += kChunk) {
       const int len = min(kChunk, d - k0);
@@ -206,9 +225,10 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
           const int c = (me + (g0 + i) * waves) * 16 + in;
           const T* row = w + (long long)min(c, v - 1) * ldw + k0 + piece * kV;
           const char* xs = smem + in * kPitch + piece * 16;
-          f32x4 sum_of[kAhead];      // short sums of their own: one over all features rounds three times as much
+          constexpr int kSums = sizeof(Z) == 4 ? kAhead : 1;      // short ones: one over all features rounds more
+          Acc sum_of[kSums];
 #pragma unroll
-          for (int u = 0; u < kAhead; ++u) sum_of[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int u = 0; u < kSums; ++u) sum_of[u] = Acc{0, 0, 0, 0};
 #pragma unroll 1
           for (int k = 0; k < len; k += kAhead * kStepK) {
             u32x4 a[kAhead];
@@ -217,61 +237,96 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
               a[u] = load_values<T, kWide>(row + k + u * kStepK, len - k - u * kStepK - piece * kV);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-              sum_of[u] = Mma16<T>::run(a[u], *(const u32x4*)(xs + (k + u * kStepK) * (int)sizeof(T)), sum_of[u]);
+              sum_of[u % kSums] =
+                  Mma16<T>::run(a[u], *(const u32x4*)(xs + (k + u * kStepK) * (int)sizeof(T)), sum_of[u % kSums]);
           }
 #pragma unroll
-          for (int half = kAhead / 2; half > 0; half >>= 1)
+          for (int half = kSums / 2; half > 0; half >>= 1)
 #pragma unroll
             for (int u = 0; u < half; ++u) sum_of[u] += sum_of[u + half];
           acc[i] += sum_of[0];
         }
       }
     }
-    // acc: row `in`, classes 4 * piece + r of the group
+    // acc: row `in`, classes row(piece, r) of the group
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (i < mine) {
-      const int c = (me + (g0 + i) * waves) * 16 + 4 * piece;
-      f32x4 out;
+        const int c = (me + (g0 + i) * waves) * 16;
+        Acc out;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float b = bias && c + r < v ? TypeOf<T>::to_float(bias[c + r]) : 0.0f;
-        out[r] = c + r < v ? acc[i][r] + b : -__builtin_inff();
-        const float up = fmaxf(top, out[r]), base = up == -__builtin_inff() ? 0.0f : up;
-        sum = sum * expf(top - base) + expf(out[r] - base);
-        top = up;
-      }
-      if (in < n) *(f32x4*)(z + (long long)in * ldz + c) = out;
+        for (int r = 0; r < 4; ++r) {
+          const int at = c + Mma16<T>::row(piece, r);
+          const Z b = bias && at < v ? (Z)TypeOf<T>::to_float(bias[at]) : (Z)0;
+          out[r] = at < v ? acc[i][r] + b : -(Z)__builtin_inff();
+          const float up = fmaxf(top, (float)out[r]), base = up == -__builtin_inff() ? 0.0f : up;
+          sum = sum * (double)expf(top - base) + (double)expf((float)(out[r] - (Z)base));
+          top = up;
+        }
+        if (in < n) {
+          Z* to = z + (long long)in * ldz + c;
+          if constexpr (sizeof(Z) == 4) {
+            *(Acc*)(to + 4 * piece) = out;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[Mma16<T>::row(piece, r)] = out[r];
+          }
+        }
       }
     }
   }
 #pragma unroll
   for (int o = 16; o < 64; o <<= 1) {
-    const float other = __shfl_xor(top, o, 64), more = __shfl_xor(sum, o, 64);
+    const float other = __shfl_xor(top, o, 64);
+    const double more = __shfl_xor(sum, o, 64);
     const float up = fmaxf(top, other), base = up == -__builtin_inff() ? 0.0f : up;
-    sum = sum * expf(top - base) + more * expf(other - base);
+    sum = sum * (double)expf(top - base) + more * (double)expf(other - base);
     top = up;
   }
-  if (lane < 16) s_part[wave][lane] = make_float2(top, sum);
+  if (lane < 16) s_part[wave][lane] = TopSum{sum, top};
   __syncthreads();
   if (t < 16) {
     top = -__builtin_inff();
-    sum = 0.0f;
-    for (int k = 0; k < 4; ++k) top = fmaxf(top, s_part[k][t].x);
+    sum = 0.0;
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, s_part[k][t].top);
     const float base = top == -__builtin_inff() ? 0.0f : top;
-    for (int k = 0; k < 4; ++k) sum += s_part[k][t].y * expf(s_part[k][t].x - base);
-    part[t * gridDim.x + blockIdx.x] = make_float2(top, sum);
+    for (int k = 0; k < 4; ++k) sum += s_part[k][t].sum * (double)expf(s_part[k][t].top - base);
+    part[t * gridDim.x + blockIdx.x] = TopSum{sum, top};
   }
 }
 
+template <int kRotate>
+__device__ __forceinline__ double rotated(const double x) {
+  const unsigned long long w = __builtin_bit_cast(unsigned long long, x);
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)w, 0x120 + kRotate, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(w >> 32), 0x120 + kRotate, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (unsigned long long)(unsigned)hi << 32 | (unsigned)lo);
+}
 // Of every 16 lanes, over those whose number is the same modulo kN.
-template <int kN, typename F>
-__device__ __forceinline__ float over_classes(float x, const F f) {
+template <int kN, typename X, typename F>
+__device__ __forceinline__ X over_classes(X x, const F f) {
   x = f(x, rotated<8>(x));
   if constexpr (kN <= 4) x = f(x, rotated<4>(x));
   if constexpr (kN <= 2) x = f(x, rotated<2>(x));
   if constexpr (kN <= 1) x = f(x, rotated<1>(x));
   return x;
+}
+// fold32, fold16 and sum16 for both kinds of logit
+template <bool k32>
+__device__ __forceinline__ double fold(const double a, const double b) {
+  const unsigned long long x = __builtin_bit_cast(unsigned long long, a), y = __builtin_bit_cast(unsigned long long, b);
+  const auto swap = [](const unsigned p, const unsigned q) {
+    if constexpr (k32) return __builtin_amdgcn_permlane32_swap(p, q, false, false);
+    else return __builtin_amdgcn_permlane16_swap(p, q, false, false);
+  };
+  const auto lo = swap((unsigned)x, (unsigned)y), hi = swap((unsigned)(x >> 32), (unsigned)(y >> 32));
+  const unsigned l0 = lo[0], l1 = lo[1], h0 = hi[0], h1 = hi[1];
+  return __builtin_bit_cast(double, (unsigned long long)h0 << 32 | l0) +
+         __builtin_bit_cast(double, (unsigned long long)h1 << 32 | l1);
+}
+template <bool k32>
+__device__ __forceinline__ float fold(const float a, const float b) {
+  return k32 ? fold32(a, b) : fold16(a, b);
 }
 
 // kA classes at a time, a value (class, row) each lane of 16: value i = class i / kN, row i % kN.
@@ -279,11 +334,13 @@ template <typename T, int kN, int kC, bool kWide>
 __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restrict__ x, const long long ldx, const int n,
                                                               const int d, const T* __restrict__ w, const long long ldw,
                                                               const int v, const T* __restrict__ bias, const Labels y,
-                                                              float* __restrict__ z, const int ldz,
-                                                              float2* __restrict__ part, float* __restrict__ dx_part,
+                                                              typename Mma16<T>::Z* __restrict__ z, const int ldz,
+                                                              TopSum* __restrict__ part, float* __restrict__ dx_part,
                                                               const int ldpart) {
   constexpr int kV = 16 / (int)sizeof(T), kA = 16 / (kN > kC ? kN : kC), kVals = kA * kN;
-  __shared__ f32x4 s_z[2][16];      // [value], one sum of each wave
+  typedef typename Mma16<T>::Z Z;
+  typedef typename Mma16<T>::Acc Four;
+  __shared__ Four s_z[2][16];      // [value], one sum of each wave
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15;
   float xs[kN][kC][kV], acc[kN][kC][kV];
 #pragma unroll
@@ -297,7 +354,8 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
       for (int k = 0; k < kV; ++k) acc[r][j][k] = 0.0f;
     }
   }
-  float top = -__builtin_inff(), sum = 0.0f;      // of row in % kN, the same in all waves
+  float top = -__builtin_inff();      // of row in % kN, the same in all waves
+  double sum = 0.0;
   const long long label = in % kN < n ? y.at(in % kN) : -1;
   int odd = 0;
   for (int v0 = blockIdx.x * kA; v0 < v; v0 += gridDim.x * kA, odd ^= 1) {
@@ -309,9 +367,17 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
         const int c = (j * kThreads + t) * kV;
         ws[a][j] = load_values<T, kWide>(w + (long long)min(v0 + a, v - 1) * ldw + c, d - c);
       }
-    float part_of[16];
+    if constexpr (sizeof(Z) == 8) {      // not to be kept in 64 bits from one round to the next: they take registers
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part_of[i] = 0.0f;
+      for (int r = 0; r < kN; ++r)
+#pragma unroll
+        for (int j = 0; j < kC; ++j)
+#pragma unroll
+          for (int k = 0; k < kV; ++k) asm volatile("" : "+v"(xs[r][j][k]));
+    }
+    Z part_of[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) part_of[i] = 0;
 #pragma unroll
     for (int a = 0; a < kA; ++a)
 #pragma unroll
@@ -321,29 +387,33 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
 #pragma unroll
         for (int r = 0; r < kN; ++r)
 #pragma unroll
-          for (int k = 0; k < kV; ++k) part_of[a * kN + r] = __builtin_fmaf(f[k], xs[r][j][k], part_of[a * kN + r]);
+          for (int k = 0; k < kV; ++k) {
+            if constexpr (sizeof(Z) == 4) part_of[a * kN + r] = __builtin_fmaf(f[k], xs[r][j][k], part_of[a * kN + r]);
+            else part_of[a * kN + r] = __builtin_fma((double)f[k], (double)xs[r][j][k], part_of[a * kN + r]);
+          }
       }
     // sums over the wave: values 4 g .. 4 g + 3 end in the 16 lanes of row g
-    float eight[8], four[4];
+    Z eight[8], four[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) eight[i] = fold32(part_of[i], part_of[i + 8]);
+    for (int i = 0; i < 8; ++i) eight[i] = fold<true>(part_of[i], part_of[i + 8]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) four[i] = sum16(fold16(eight[i], eight[i + 4]));
+    for (int i = 0; i < 4; ++i)
+      four[i] = over_classes<1>(fold<false>(eight[i], eight[i + 4]), [](const Z p, const Z q) { return p + q; });
     const int value = in + 4 * (lane >> 4);      // of lanes 0 .. 3 of a row
-    const float mine = in == 0 ? four[0] : in == 1 ? four[1] : in == 2 ? four[2] : four[3];
-    if (in < 4) ((float*)&s_z[odd][value])[wave] = mine;
+    const Z mine = in == 0 ? four[0] : in == 1 ? four[1] : in == 2 ? four[2] : four[3];
+    if (in < 4) ((Z*)&s_z[odd][value])[wave] = mine;
     __syncthreads();      // the other half is written next time, when all have read this one
-    const f32x4 of_waves = s_z[odd][in];
+    const Four of_waves = s_z[odd][in];
     const int a = in / kN, r = in % kN, c = v0 + a;
     const bool real = in < kVals && c < v;
-    float logit = (of_waves[0] + of_waves[1]) + (of_waves[2] + of_waves[3]);
-    if (bias && real) logit += TypeOf<T>::to_float(bias[c]);
-    if (!real) logit = -__builtin_inff();
+    Z logit = (of_waves[0] + of_waves[1]) + (of_waves[2] + of_waves[3]);
+    if (bias && real) logit += (Z)TypeOf<T>::to_float(bias[c]);
+    if (!real) logit = -(Z)__builtin_inff();
     if (real && t < 16 && r < n) z[(long long)r * ldz + c] = logit;
-    const float up = fmaxf(top, over_classes<kN>(logit, [](float p, float q) { return fmaxf(p, q); }));
+    const float up = fmaxf(top, over_classes<kN>((float)logit, [](float p, float q) { return fmaxf(p, q); }));
     const float base = up == -__builtin_inff() ? 0.0f : up;
-    const float e = expf(logit - base), shrink = expf(top - base);
-    sum = sum * shrink + over_classes<kN>(e, [](float p, float q) { return p + q; });
+    const float e = expf((float)(logit - (Z)base)), shrink = expf(top - base);
+    sum = sum * (double)shrink + over_classes<kN>((double)e, [](double p, double q) { return p + q; });
     if (__builtin_amdgcn_ballot_w64(top != up)) {
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
@@ -370,7 +440,7 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
         }
       }
   }
-  if (t < kN) part[t * gridDim.x + blockIdx.x] = make_float2(top, sum);
+  if (t < kN) part[t * gridDim.x + blockIdx.x] = TopSum{sum, top};
 #pragma unroll
   for (int r = 0; r < kN; ++r)
 #pragma unroll
@@ -386,11 +456,12 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
 }
 
 // One wave a row.  4 to 8 us, all of it latency.
-__global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* __restrict__ part, const int blocks,
+template <typename Z>
+__global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const TopSum* __restrict__ part, const int blocks,
                                                                  const Labels y, const int n,
-                                                                 const float* __restrict__ z, const int ldz,
+                                                                 const Z* __restrict__ z, const int ldz,
                                                                  const float* __restrict__ divisor, const int mean,
-                                                                 const float grad, float2* __restrict__ row,
+                                                                 const float grad, TopSum* __restrict__ row,
                                                                  float* __restrict__ scale,
                                                                  float* __restrict__ row_loss,
                                                                  float* __restrict__ small, int* __restrict__ status,
@@ -399,19 +470,21 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
   __shared__ float s_loss[kFewRows];
   __shared__ int s_keep[kFewRows], s_bad[kFewRows];
   const int r = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float top = -__builtin_inff(), sum = 0.0f;
+  float top = -__builtin_inff();
+  double sum = 0.0;
   if (r < n)
     for (int i = lane; i < blocks; i += 64) {
-      const float2 p = part[r * blocks + i];
-      const float up = fmaxf(top, p.x), base = up == -__builtin_inff() ? 0.0f : up;
-      sum = sum * expf(top - base) + p.y * expf(p.x - base);
+      const TopSum p = part[r * blocks + i];
+      const float up = fmaxf(top, p.top), base = up == -__builtin_inff() ? 0.0f : up;
+      sum = sum * (double)expf(top - base) + p.sum * (double)expf(p.top - base);
       top = up;
     }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    const float other = __shfl_xor(top, o, 64), more = __shfl_xor(sum, o, 64);
+    const float other = __shfl_xor(top, o, 64);
+    const double more = __shfl_xor(sum, o, 64);
     const float up = fmaxf(top, other), base = up == -__builtin_inff() ? 0.0f : up;
-    sum = sum * expf(top - base) + more * expf(other - base);
+    sum = sum * (double)expf(top - base) + more * (double)expf(other - base);
     top = up;
   }
   const long long label = r < n ? y.at(r) : y.ignore;
@@ -419,15 +492,15 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
   if (share && r < n) {
     const float base = top == -__builtin_inff() ? 0.0f : top;
     for (int i = lane; i < blocks; i += 64)
-      share[r * blocks + i] = keep ? expf(part[r * blocks + i].x - base) / sum : 0.0f;
+      share[r * blocks + i] = keep ? (float)((double)expf(part[r * blocks + i].top - base) / sum) : 0.0f;
   }
   if (lane == 0) {
     float loss = 0.0f;
     if (keep) {
-      const float z_label = z[(long long)r * ldz + label];
-      loss = (top - z_label) + logf(sum);
-      row[r] = make_float2(top, sum);
-      of_label[r] = (expf(z_label - top) - sum) / sum;
+      const Z below = z[(long long)r * ldz + label] - (Z)top;
+      loss = (float)(log(sum) - (double)below);
+      row[r] = TopSum{sum, top};
+      of_label[r] = (float)(((double)expf((float)below) - sum) / sum);
     }
     if (r < n) row_loss[r] = loss;
     s_loss[r] = loss;
@@ -458,12 +531,13 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const float2* _
 template <typename T, int kN>
 __global__ __launch_bounds__(kThreads) void few_weights_kernel(
     const T* __restrict__ x, const long long ldx, const int n, const int d, const int v, const Labels y,
-    const float* __restrict__ z, const int ldz, const float2* __restrict__ row, const float* __restrict__ scale,
+    const typename Mma16<T>::Z* __restrict__ z, const int ldz, const TopSum* __restrict__ row,
+    const float* __restrict__ scale,
     const int per, const int tpr, T* __restrict__ dw, T* __restrict__ db) {
   constexpr int kV = 16 / (int)sizeof(T);
   constexpr int kAtOnce = 128;      // classes whose probabilities wait in LDS
   __shared__ float s_p[kAtOnce][kN];
-  __shared__ float2 s_row[kN];
+  __shared__ TopSum s_row[kN];
   __shared__ int s_label[kN];
   const int t = threadIdx.x, subsets = kThreads / tpr, subset = t / tpr;
   const int c = (blockIdx.y * tpr + t % tpr) * kV;
@@ -471,7 +545,7 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
   if (t < kN) {
     const long long label = t < n ? y.at(t) : y.ignore;
     s_label[t] = t < n && y.counts(label) ? (int)label : -1;
-    s_row[t] = s_label[t] >= 0 ? row[t] : make_float2(0.0f, 1.0f);
+    s_row[t] = s_label[t] >= 0 ? row[t] : TopSum{1.0, 0.0f};
   }
   __syncthreads();
   float xs[kN][kV];
@@ -487,8 +561,9 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
       float p = 0.0f;
       if (s_label[r] >= 0) {
         // the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
-        p = expf(z[(long long)r * ldz + v0 + a] - s_row[r].x) - (s_label[r] == v0 + a ? s_row[r].y : 0.0f);
-        p = p / s_row[r].y * s;
+        const float e = expf((float)(z[(long long)r * ldz + v0 + a] - (typename Mma16<T>::Z)s_row[r].top));
+        p = s_label[r] == v0 + a ? (float)(((double)e - s_row[r].sum) / s_row[r].sum) : e / (float)s_row[r].sum;
+        p *= s;
       }
       s_p[a][r] = p;
     }
@@ -536,12 +611,12 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
 template <typename T, bool kWide>
 __global__ __launch_bounds__(kThreads) void few_products_kernel(
     const T* __restrict__ x, const long long ldx, const int n, const int d, const T* __restrict__ w,
-    const long long ldw, const int v, const Labels y, const float* __restrict__ z, const int ldz,
-    const float2* __restrict__ row, const float* __restrict__ scale, const int per, const int waves_a_row,
+    const long long ldw, const int v, const Labels y, const typename Mma16<T>::Z* __restrict__ z, const int ldz,
+    const TopSum* __restrict__ row, const float* __restrict__ scale, const int per, const int waves_a_row,
     T* __restrict__ dw, T* __restrict__ db, float* __restrict__ dx_part, const int ldpart) {
   constexpr int kV = 16 / (int)sizeof(T), kAtOnce = 128, kPitch = kFewRows + 1;      // rows a bank apart
   __shared__ float s_p[kAtOnce * kPitch];
-  __shared__ float2 s_row[kFewRows];
+  __shared__ TopSum s_row[kFewRows];
   __shared__ int s_label[kFewRows];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, in = lane & 15, piece = lane >> 4;
   const int subsets = 4 / waves_a_row, subset = wave / waves_a_row;
@@ -550,7 +625,7 @@ __global__ __launch_bounds__(kThreads) void few_products_kernel(
   if (t < kFewRows) {
     const long long label = t < n ? y.at(t) : y.ignore;
     s_label[t] = t < n && y.counts(label) ? (int)label : -1;
-    s_row[t] = s_label[t] >= 0 ? row[t] : make_float2(0.0f, 1.0f);
+    s_row[t] = s_label[t] >= 0 ? row[t] : TopSum{1.0, 0.0f};
   }
   __syncthreads();
   float xs[4][kV];      // [k / 4]: rows 4 k + piece
@@ -572,8 +647,9 @@ __global__ __launch_bounds__(kThreads) void few_products_kernel(
       float p = 0.0f;
       if (a < count && s_label[r] >= 0) {
         // the label's p - 1 as (e - sum) / sum, which does not cancel what p was rounded by
-        p = expf(z[(long long)r * ldz + v0 + a] - s_row[r].x) - (s_label[r] == v0 + a ? s_row[r].y : 0.0f);
-        p = p / s_row[r].y * s;
+        const float e = expf((float)(z[(long long)r * ldz + v0 + a] - (typename Mma16<T>::Z)s_row[r].top));
+        p = s_label[r] == v0 + a ? (float)(((double)e - s_row[r].sum) / s_row[r].sum) : e / (float)s_row[r].sum;
+        p *= s;
       }
       s_p[a * kPitch + r] = p;
     }
@@ -698,7 +774,7 @@ template <typename T, int kN>
 static int launch_weights(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
                           hipStream_t stream) {
   hipLaunchKernelGGL((few_weights_kernel<T, kN>), dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x,
-                     (long long)q.ldx, (int)q.n, q.d, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per, p.tpr, (T*)q.dw,
+                     (long long)q.ldx, (int)q.n, q.d, (int)q.v, y, (const typename Mma16<T>::Z*)s.z, p.ldz, s.row, s.scale, p.per, p.tpr, (T*)q.dw,
                      (T*)q.db);
   RH_CHECK_LAUNCH("few_weights_kernel");
   return RH_OK;
@@ -709,7 +785,7 @@ static int launch_products(const rh_linear_ce_args& q, const FewPlan& p, const F
                            hipStream_t stream) {
   auto kernel = p.wide_w ? few_products_kernel<T, true> : few_products_kernel<T, false>;
   hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
-                     (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, s.z, p.ldz, s.row, s.scale, p.per,
+                     (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, (const typename Mma16<T>::Z*)s.z, p.ldz, s.row, s.scale, p.per,
                      p.tpr / 16, (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart);
   RH_CHECK_LAUNCH("few_products_kernel");
   return RH_OK;
@@ -720,7 +796,7 @@ static int launch_online(const rh_linear_ce_args& q, const FewPlan& p, const Few
                          hipStream_t stream) {
   auto kernel = p.wide_w ? few_online_kernel<T, kN, kC, true> : few_online_kernel<T, kN, kC, false>;
   hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx, (int)q.n, q.d,
-                     (const T*)q.w, (long long)q.ldw, (int)q.v, (const T*)q.bias, y, s.z, p.ldz, s.part, s.dx_part,
+                     (const T*)q.w, (long long)q.ldw, (int)q.v, (const T*)q.bias, y, (typename Mma16<T>::Z*)s.z, p.ldz, s.part, s.dx_part,
                      p.ldpart);
   RH_CHECK_LAUNCH("few_online_kernel");
   return RH_OK;
@@ -737,6 +813,7 @@ static int online_chunks(const rh_linear_ce_args& q, const FewPlan& p, const Few
 
 template <typename T>
 static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) {
+  typedef typename Mma16<T>::Z Z;
   const int n = (int)q.n, v = (int)q.v;
   const FewPlan p = few_plan(n, q.d, v, q.dtype, flags);
   const FewSpace s = few_space(q.workspace, p, n, flags);
@@ -749,10 +826,10 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
   } else {
     auto logits = p.wide_w ? few_logits_kernel<T, true> : few_logits_kernel<T, false>;
     hipLaunchKernelGGL(logits, dim3(p.blocks), dim3(kThreads), 16 * kPitch, stream, (const T*)q.x, (long long)q.ldx, n, q.d,
-                       (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, s.z, p.ldz, s.part);
+                       (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, (Z*)s.z, p.ldz, s.part);
     RH_CHECK_LAUNCH("few_logits_kernel");
   }
-  hipLaunchKernelGGL(few_rows_kernel, dim3(1), dim3(64 * kFewRows), 0, stream, s.part, p.blocks, y, n, s.z, p.ldz, q.divisor,
+  hipLaunchKernelGGL(few_rows_kernel<Z>, dim3(1), dim3(64 * kFewRows), 0, stream, s.part, p.blocks, y, n, (const Z*)s.z, p.ldz, q.divisor,
                      q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3), s.share,
                      s.of_label);
   RH_CHECK_LAUNCH("few_rows_kernel");

@@ -16,10 +16,10 @@
 // Making the logits again instead takes 8 n d v, and P from them no fewer bytes.  Up to 640 classes
 // (rh_ce_whole.hip) and up to 16 rows (rh_ce_few.hip) there are other ways.
 //
-// 4096 x 2048 rows, a twentieth left out, 32 768 classes, bfloat16, us on the card: logits 570, P 85,
-// dX 490, dW 525, all else 45.  The three products make 0.98, 1.07 and 1.0 PFLOP/s; what bounds them is
+// 4096 x 2048 rows, a twentieth left out, 32 768 classes, bfloat16, us on the card: logits 565, P 84,
+// dX 485, dW 535, all else 45.  The three products make 0.97, 1.08 and 0.98 PFLOP/s; what bounds them is
 // the power that the matrix units draw on values that are not zeros (see rh_gemm.h) and, for the logits,
-// the 16 us a tile's end takes (256 x 256 exponentials a workgroup).
+// the 14 us a tile's end takes (256 x 256 exponentials a workgroup).
 #include "rh_ce.h"
 
 namespace rh {

@@ -128,11 +128,21 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
   __shared__ int s_place[kThreads];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   int before = 0, all = 0, bad = 0;
-  for (int i = t; i < (int)gridDim.x; i += kThreads) {
-    const int2 c = blocks[i];
-    if (i < (int)blockIdx.x) before += c.x;
-    all += c.x;
-    bad |= c.y;
+  if (blocks) {
+    for (int i = t; i < (int)gridDim.x; i += kThreads) {
+      const int2 c = blocks[i];
+      if (i < (int)blockIdx.x) before += c.x;
+      all += c.x;
+      bad |= c.y;
+    }
+  } else {      // few rows: every workgroup counts them all
+    for (int i = t; i < n; i += kThreads) {
+      const long long l = y.at(i);
+      const int c = y.counts(l);
+      if (i < (int)blockIdx.x * per) before += c;
+      all += c;
+      bad |= l != y.ignore && (l < 0 || l >= y.v);
+    }
   }
   before = wave_sum(before);
   all = wave_sum(all);
@@ -514,12 +524,12 @@ __global__ __launch_bounds__(kThreads) void sum_logits_kernel(const LogitArgs<T>
       if constexpr (sizeof(T) == 4) {
         *(f32x4*)((float*)a.z + in_panels(r, c, a.chunk_rows)) = z;
       } else {
+        constexpr float kCode = -kLog2e * Kept<T>::kSteps / 65535.0f;
         unsigned w[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          w[u] = __builtin_bit_cast(
-              unsigned, __builtin_amdgcn_cvt_pknorm_u16((z[2 * u] - base) * (-kLog2e * Kept<T>::kSteps / 65535.0f),
-                                                        (z[2 * u + 1] - base) * (-kLog2e * Kept<T>::kSteps / 65535.0f)));
+          w[u] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16((z[2 * u] - base) * kCode,
+                                                                              (z[2 * u + 1] - base) * kCode));
         *(unsigned long long*)((unsigned short*)a.z + in_panels(r, c, a.chunk_rows)) =
             (unsigned long long)w[1] << 32 | w[0];
       }
@@ -891,8 +901,9 @@ static Cut cut(long long m, long long n, int steps, int terms, int most_splits, 
       if (ceil_div(steps, c.steps) < splits) continue;      // the last would be empty
       const long long work = tiles * splits;
       const float filled = work < slots ? (float)work / slots : 1.0f;
+      const float end = !large ? 6.0f : splits > 1 ? 14.0f : large_end;
       float us = (float)((work + slots - 1) / slots) *
-                 (((large ? 0.58f : 0.26f) + 0.30f * filled) * (float)c.steps * (float)terms + (large ? splits > 1 ? 14.0f : large_end : 6.0f));
+                 (((large ? 0.58f : 0.26f) + 0.30f * filled) * (float)c.steps * (float)terms + end);
       if (splits > 1) us += 4.0f + (float)splits * (float)m * (float)n * (4.0f / 4.5e6f);
       if (least == 0.0f || us < least) {
         least = us;
@@ -1195,15 +1206,19 @@ template <typename T>
 static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStream_t stream) {
   const int n = (int)q.n, d = q.d, v = (int)q.v;
   const Labels labels{q.labels, q.labels_int64, q.ignore_index, v};
-  hipLaunchKernelGGL(count_rows_kernel, dim3(p.row_blocks), dim3(64), 0, stream, labels, n, p.per, s.blocks);
-  RH_CHECK_LAUNCH("count_rows_kernel");
+  // up to 2048 rows counting them takes less than the launch (5 us)
+  const bool counted = n > 2048;
+  if (counted) {
+    hipLaunchKernelGGL(count_rows_kernel, dim3(p.row_blocks), dim3(64), 0, stream, labels, n, p.per, s.blocks);
+    RH_CHECK_LAUNCH("count_rows_kernel");
+  }
   // a panel a wave where there are few rows
   int side = ceil_div(p.panels, 16) < 8 ? ceil_div(p.panels, 16) : 8;
   if (side < 256 / p.row_blocks) side = 256 / p.row_blocks;
   if (side > ceil_div(p.panels, 4)) side = ceil_div(p.panels, 4);
   hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks, side), dim3(kThreads), 0, stream, (const T*)q.x,
-                     (long long)q.ldx, d, labels, n, p.per, s.blocks, s.x, s.x_part, p.panels, p.chunk, s.info, q.row_loss,
-                     (T*)q.dx, q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
+                     (long long)q.ldx, d, labels, n, p.per, counted ? s.blocks : nullptr, s.x, s.x_part, p.panels,
+                     p.chunk, s.info, q.row_loss, (T*)q.dx, q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
   RH_CHECK_LAUNCH("place_rows_kernel");
   const bool grads = q.dx || q.dw || q.db;
   LogitArgs<T> a = {};
@@ -1226,7 +1241,8 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   }
   if (p.parts > 1) {
     const int across = ceil_div(p.panels, 16) < 16 ? ceil_div(p.panels, 16) : 16;
-    hipLaunchKernelGGL(take_apart_kernel<T>, dim3(ceil_div(v, 16), across), dim3(kThreads), 0, stream, (const T*)q.w, (long long)q.ldw, d, v, p.panels, s.w, s.w_part);
+    hipLaunchKernelGGL(take_apart_kernel<T>, dim3(ceil_div(v, 16), across), dim3(kThreads), 0, stream, (const T*)q.w,
+                       (long long)q.ldw, d, v, p.panels, s.w, s.w_part);
     RH_CHECK_LAUNCH("take_apart_kernel");
     a.w = s.w;
     a.ldw = (long long)v * kStepBytes;

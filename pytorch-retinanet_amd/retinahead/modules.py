@@ -540,7 +540,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """Scales the gradients of ``parameters`` in place so that their norm over all of them is at most
     ``max_norm`` (each times min(1, max_norm / (norm + 1e-6))), and returns that norm from before as a
     float32 [] device tensor: the step between ``loss.backward()`` and ``optimizer.step()`` of
-    train.py:190-203.  The signature is that of torch.nn.utils.clip_grad_norm_; nothing is read back
+    train.py:190-203.  Arguments and result are torch's own; nothing is read back
     unless ``error_if_nonfinite`` asks for it.
 
     Gradients may be float32, bfloat16 and float16 in one call, in any dense order of dimensions and at

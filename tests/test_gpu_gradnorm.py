@@ -244,7 +244,7 @@ def test_training_step_of_a_classifier(rh, dtype):
         with torch.no_grad():
             pw -= pw.grad
             pb -= pb.grad
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
     assert all(math.isfinite(v) for v in losses)
 
 

@@ -90,6 +90,17 @@ __device__ __forceinline__ void to_floats(const u32x4 u, float (&f)[16 / sizeof(
   for (int i = 0; i < 16 / (int)sizeof(T); ++i) f[i] = TypeOf<T>::to_float(r.v[i]);
 }
 
+// dW that the caches could not hold beside the weights is written past them, so that they keep weights: a call of
+// 1 x 2048 rows and 65 536 classes in bfloat16 (268 MB each) takes 118 us so, 140 with ordinary stores, the next
+// call's reading 42 instead of 84; 8 x 2048 191 instead of 227 on the card.  (The same in the products of many rows costs:
+// dW of 32 768 x 2048 578 us instead of 535.)
+constexpr long long kPastCaches = 128ll << 20;
+template <bool kPast>
+__device__ __forceinline__ void store16(void* to, const u32x4 v) {
+  if constexpr (kPast) __builtin_nontemporal_store(v, (u32x4*)to);
+  else *(u32x4*)to = v;
+}
+
 struct FewSpace {
   void* z;             // [n][ldz]  float's are double
   TopSum* part;        // [kFewRows][blocks]
@@ -108,7 +119,7 @@ struct FewPlan {
   int tpr, subsets, slices;
   int grad_blocks, per;             // classes a workgroup takes
   int parts, ldpart;
-  bool wide_w;
+  bool wide_w, past;                // how the weights are read; dW is written past the caches
   int rows, chunks;                 // online: rows (a power of two) and 16-byte pieces of columns a thread; else 0
 };
 
@@ -116,9 +127,8 @@ struct FewPlan {
 // takes whole rows of weights, so what a thread read for the logits is still in its registers when their
 // exponentials are known: dX's sum is kept relative to the running maximum and joined like a softmax's.
 // The weights are read once; dW is written by a pass that reads none.
-// 1 x 2048 rows, 65 536 classes, bfloat16 (268 MB of weights, as much of dW): 208 us with two readings, 145
-// with one (87 this pass, 45 the one that writes), 4.1 TB/s over both.  Loads for the next classes issued ahead, more
-// workgroups or contiguous runs of classes for each: no faster; what they read was written behind the caches.
+// 1 x 2048 rows, 65 536 classes, bfloat16 (268 MB of weights, as much of dW): 208 us with two readings, 145 with
+// one.  Loads for the next classes issued ahead, more workgroups or contiguous runs of classes for each: no faster.
 static void plan_online(FewPlan& p, int n, int d, int v, int vals) {
   p.rows = n <= 1 ? 1 : n <= 2 ? 2 : 4;
   p.chunks = ceil_div(d, kThreads * vals);
@@ -144,6 +154,7 @@ static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
   p.ldz = ceil_div(v, 16) * 16;
   p.z_size = dtype == RH_F32 ? 8 : 4;
   p.wide_w = !(flags & RH_CE_COPY_WEIGHT);      // here that only says how the weights are read
+  p.past = (long long)v * d * (16 / vals) >= kPastCaches;
   if (flags & RH_CE_GRAD_X) plan_online(p, n, d, v, vals);
   const int whole = p.rows ? kThreads : 64;      // threads, or sixteen times the waves, of a row of weights
   p.tpr = 16;
@@ -527,8 +538,8 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const TopSum* _
 
 // dW and db of up to four rows whose dX is made online.  A thread has 16 bytes of columns, the rows' features
 // beside them in registers; the workgroup's classes are taken `subsets` at a time, a class by tpr threads.  Bound
-// by the bytes it writes: 65 536 x 2048 bfloat16 (268 MB) 45 us.
-template <typename T, int kN>
+// by the bytes it writes: 65 536 x 2048 bfloat16 (268 MB) 53 us past the caches, 43 into them.
+template <typename T, int kN, bool kPast>
 __global__ __launch_bounds__(kThreads) void few_weights_kernel(
     const T* __restrict__ x, const long long ldx, const int n, const int d, const int v, const Labels y,
     const typename Mma16<T>::Z* __restrict__ z, const int ldz, const TopSum* __restrict__ row,
@@ -591,7 +602,7 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
       }
       T* to = dw + (long long)(v0 + a) * d + c;
       if (d % kV == 0) {
-        *(u32x4*)to = out.u;
+        store16<kPast>(to, out.u);
       } else if (c + kV <= d) {
         __builtin_memcpy(to, &out, 16);
       } else {
@@ -608,7 +619,7 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
 // lane's one weight of k is the class of its load, and the columns of its kV instructions are its own kV neighbours.
 // dW = P^T X has the rows as k.  P and both products stay float32.  Bound by memory: 16 x 2048 rows, 65 536 classes,
 // bfloat16 (268 MB read, 268 written) 139 us; 16 x 572, 62 202 classes, float32 74.  By vector instructions 484, 174.
-template <typename T, bool kWide>
+template <typename T, bool kWide, bool kPast>
 __global__ __launch_bounds__(kThreads) void few_products_kernel(
     const T* __restrict__ x, const long long ldx, const int n, const int d, const T* __restrict__ w,
     const long long ldw, const int v, const Labels y, const typename Mma16<T>::Z* __restrict__ z, const int ldz,
@@ -689,7 +700,7 @@ __global__ __launch_bounds__(kThreads) void few_products_kernel(
           T* to = dw + (long long)(v0 + a) * d + c;
           if (a < count) {
             if (d % kV == 0) {
-              if (c < d) *(u32x4*)to = values.u;
+              if (c < d) store16<kPast>(to, values.u);
             } else if (c + kV <= d) {
               __builtin_memcpy(to, &values, 16);
             } else {
@@ -773,7 +784,8 @@ __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __r
 template <typename T, int kN>
 static int launch_weights(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
                           hipStream_t stream) {
-  hipLaunchKernelGGL((few_weights_kernel<T, kN>), dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x,
+  auto kernel = p.past ? few_weights_kernel<T, kN, true> : few_weights_kernel<T, kN, false>;
+  hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x,
                      (long long)q.ldx, (int)q.n, q.d, (int)q.v, y, (const typename Mma16<T>::Z*)s.z, p.ldz, s.row, s.scale, p.per, p.tpr, (T*)q.dw,
                      (T*)q.db);
   RH_CHECK_LAUNCH("few_weights_kernel");
@@ -783,7 +795,8 @@ static int launch_weights(const rh_linear_ce_args& q, const FewPlan& p, const Fe
 template <typename T>
 static int launch_products(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
                            hipStream_t stream) {
-  auto kernel = p.wide_w ? few_products_kernel<T, true> : few_products_kernel<T, false>;
+  auto kernel = p.wide_w ? p.past ? few_products_kernel<T, true, true> : few_products_kernel<T, true, false>
+                         : few_products_kernel<T, false, false>;
   hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
                      (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, (const typename Mma16<T>::Z*)s.z, p.ldz, s.row, s.scale, p.per,
                      p.tpr / 16, (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart);

@@ -92,8 +92,8 @@ __device__ __forceinline__ void to_floats(const u32x4 u, float (&f)[16 / sizeof(
 
 // dW that the caches could not hold beside the weights is written past them, so that they keep weights: a call of
 // 1 x 2048 rows and 65 536 classes in bfloat16 (268 MB each) takes 118 us so, 140 with ordinary stores, the next
-// call's reading 42 instead of 84; 8 x 2048 191 instead of 227 on the card.  (The same in the products of many rows costs:
-// dW of 32 768 x 2048 578 us instead of 535.)
+// call's reading 42 instead of 84; 8 x 2048 191 instead of 227 on the card.  (In the products of many rows it costs: dW
+// of 32 768 x 2048 578 us instead of 535.)
 constexpr long long kPastCaches = 128ll << 20;
 template <bool kPast>
 __device__ __forceinline__ void store16(void* to, const u32x4 v) {
@@ -123,9 +123,9 @@ struct FewPlan {
   int rows, chunks;                 // online: rows (a power of two) and 16-byte pieces of columns a thread; else 0
 };
 
-// Online: dX = sum of p W over the other classes, without P's normalisation, which is not known before the last class.  A workgroup
-// takes whole rows of weights, so what a thread read for the logits is still in its registers when their
-// exponentials are known: dX's sum is kept relative to the running maximum and joined like a softmax's.
+// Online: dX = sum of p W over the other classes, without P's normalisation, which is not known before the last
+// class.  A workgroup takes whole rows of weights, so what a thread read for the logits is still in its registers
+// when their exponentials are known: dX's sum is kept relative to the running maximum and joined like a softmax's.
 // The weights are read once; dW is written by a pass that reads none.
 // 1 x 2048 rows, 65 536 classes, bfloat16 (268 MB of weights, as much of dW): 208 us with two readings, 145 with
 // one.  Loads for the next classes issued ahead, more workgroups or contiguous runs of classes for each: no faster.

@@ -792,19 +792,58 @@ __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_ke
   }
 }
 
-// out[map[m] or m][:] = scale * sum of the splits' parts, in their order.
+// What is left of a call beside dW: db from the row blocks' column sums (parts [parts][v]), eight columns a workgroup
+// and 32 threads a column, and where losses > 0 the call's loss, by the first workgroup.
+template <typename T>
+struct Rest {
+  const float* columns;
+  int parts, v;
+  const float* scale;
+  T* db;
+  const double* loss_parts;
+  int losses;
+  float* small;
+  __device__ __forceinline__ void join(const int block) const {
+    __shared__ float s_sum[32][8];
+    if (losses && block == 0) add_losses(loss_parts, losses, small);
+    const int in = threadIdx.x & 7, slice = threadIdx.x >> 3, c = block * 8 + in;
+    float sum = 0.0f;
+    if (c < v)
+#pragma unroll 8
+      for (int k = slice; k < parts; k += 32) sum += columns[(long long)k * v + c];
+    s_sum[slice][in] = sum;
+    __syncthreads();
+    if (slice == 0 && c < v) {
+      for (int k = 1; k < 32; ++k) sum += s_sum[k][in];
+      db[c] = TypeOf<T>::from_float(sum * *scale);
+    }
+  }
+  int workgroups() const { return db ? (v + 7) / 8 : 0; }
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_rest_kernel(const Rest<T> rest) {
+  rest.join(blockIdx.x);
+}
+
+// out[map[m] or m][:] = scale * sum of the splits' parts, in their order.  The workgroups from `of_rest` on do that.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __restrict__ part, const Sharing sharing,
                                                               const long long ldpart, const int m, const int n,
                                                               const Chunk chunk, const int* __restrict__ n_valid,
                                                               const float* __restrict__ scale, const float down,
                                                               const int* __restrict__ map, T* __restrict__ out,
-                                                              const long long ldo) {
+                                                              const long long ldo, const Rest<T> rest,
+                                                              const int of_rest) {
+  if ((int)blockIdx.x >= of_rest) {
+    rest.join(blockIdx.x - of_rest);
+    return;
+  }
   const int rows = n_valid ? max(chunk.rows(n_valid), 0) : m, splits = sharing.splits(rows);
   const long long quads = (n + 3) / 4, top = rows * quads;
   const long long plane = (long long)sharing.tiles_m(rows) * sharing.bm * ldpart;
   const float s = *scale * down;
-  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < top; i += (long long)gridDim.x * kThreads) {
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < top; i += (long long)of_rest * kThreads) {
     const long long r = i / quads;
     const int c = (int)(i - r * quads) * 4;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -831,29 +870,6 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __res
     } else {
       for (int j = 0; j < 4 && c + j < n; ++j) to[j] = TypeOf<T>::from_float(v[j] * s);
     }
-  }
-}
-
-// db from the row blocks' column sums: eight columns a workgroup, 32 threads a column.  The first workgroup also
-// adds up the loss (losses > 0).
-template <typename T>
-__global__ __launch_bounds__(kThreads) void join_columns_kernel(const float* __restrict__ part, const int parts,
-                                                                const int v, const float* __restrict__ scale,
-                                                                T* __restrict__ db,
-                                                                const double* __restrict__ loss_parts, const int losses,
-                                                                float* __restrict__ small) {
-  __shared__ float s_sum[32][8];
-  if (losses && blockIdx.x == 0) add_losses(loss_parts, losses, small);
-  const int in = threadIdx.x & 7, slice = threadIdx.x >> 3, c = blockIdx.x * 8 + in;
-  float sum = 0.0f;
-  if (c < v)
-#pragma unroll 8
-    for (int k = slice; k < parts; k += 32) sum += part[(long long)k * v + c];
-  s_sum[slice][in] = sum;
-  __syncthreads();
-  if (slice == 0 && c < v) {
-    for (int k = 1; k < 32; ++k) sum += s_sum[k][in];
-    db[c] = TypeOf<T>::from_float(sum * *scale);
   }
 }
 
@@ -1094,11 +1110,12 @@ static int launch_probs(const rh_linear_ce_args& q, const Plan& p, const Space& 
 }
 
 template <typename T>
-static int join_parts(const ProductArgs<T>& g, bool by_rows, hipStream_t stream) {
+static int join_parts(const ProductArgs<T>& g, bool by_rows, const Rest<T>& rest, hipStream_t stream) {
   long long blocks = ((long long)g.m * ((g.n + 3) / 4) + kThreads - 1) / kThreads;
   if (blocks > 256 * 8) blocks = 256 * 8;
-  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, g.part, g.sharing,
-                     g.ldpart, g.m, g.n, g.chunk, by_rows ? g.n_valid : nullptr, g.scale, g.down, g.map, g.out, g.ldo);
+  hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks + rest.workgroups()), dim3(kThreads), 0, stream, g.part,
+                     g.sharing, g.ldpart, g.m, g.n, g.chunk, by_rows ? g.n_valid : nullptr, g.scale, g.down, g.map, g.out,
+                     g.ldo, rest, (int)blocks);
   RH_CHECK_LAUNCH("join_parts_kernel");
   return RH_OK;
 }
@@ -1145,13 +1162,13 @@ static int features_gradient(const rh_linear_ce_args& q, const Plan& p, const Sp
   if (int rc = p.dx.large ? launch_product<T, kRows, Large>(g, stream)
                           : launch_product<T, kRows, Small>(g, stream))
     return rc;
-  return s.dx_part ? join_parts(g, true, stream) : RH_OK;
+  return s.dx_part ? join_parts(g, true, Rest<T>{}, stream) : RH_OK;
 }
 
-// dW, or a chunk's part of it.
+// dW, or a chunk's part of it; with the last part the rest, of which nothing is left then.
 template <typename T>
 static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Space& s, const LogitArgs<T>& a,
-                           int chunk, hipStream_t stream) {
+                           int chunk, Rest<T>& rest, hipStream_t stream) {
   ProductArgs<T> g = product_args(q, p, s, a);
   g.b = a.x;
   g.ldb = (long long)p.chunk * kStepBytes;
@@ -1166,7 +1183,10 @@ static int weight_gradient(const rh_linear_ce_args& q, const Plan& p, const Spac
   if (int rc = p.dw.large ? launch_product<T, kCols, Large>(g, stream)
                           : launch_product<T, kCols, Small>(g, stream))
     return rc;
-  return s.dw_part && chunk == p.chunks - 1 ? join_parts(g, false, stream) : RH_OK;
+  if (!s.dw_part || chunk < p.chunks - 1) return RH_OK;
+  const Rest<T> now = rest;
+  rest = Rest<T>{};
+  return join_parts(g, false, now, stream);
 }
 
 // A chunk's loss, P, column sums and dX by workgroups that hold their rows' logits whole.
@@ -1259,6 +1279,10 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   a.ldp = p.ldp;
   a.sharing = share(p.logits, p.chunk, v, p.logits.splits > 1 ? p.panels / 4 : 1);
   a.part = s.z_part;
+  Rest<T> rest = {};
+  if (q.db)
+    rest = Rest<T>{s.db_part, s.db_parts, v, s.info.scale, (T*)q.db, s.loss, p.whole ? ceil_div(n, kWholeRows) : 0,
+                   q.small};
   for (int c = 0; c < p.chunks; ++c) {
     a.chunk = Chunk{c * p.chunk, n - c * p.chunk < p.chunk ? n - c * p.chunk : p.chunk};
     const int first = a.chunk.first;
@@ -1268,7 +1292,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     if (p.whole) {
       if (int rc = whole_rows(q, p, s, a, c, stream)) return rc;
       if (q.dw)
-        if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
+        if (int rc = weight_gradient(q, p, s, a, c, rest, stream)) return rc;
       continue;
     }
     if (int rc = make_logits(p, a, grads, stream)) return rc;
@@ -1283,17 +1307,16 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     if (q.dx)
       if (int rc = features_gradient(q, p, s, a, stream)) return rc;
     if (q.dw)
-      if (int rc = weight_gradient(q, p, s, a, c, stream)) return rc;
+      if (int rc = weight_gradient(q, p, s, a, c, rest, stream)) return rc;
   }
   if (!grads || (p.whole && !q.db)) {
     hipLaunchKernelGGL(finish_loss_kernel, dim3(1), dim3(kThreads), 0, stream, s.loss,
                        ceil_div(n, p.whole ? kWholeRows : kJoinRows), q.small);
     RH_CHECK_LAUNCH("finish_loss_kernel");
   }
-  if (q.db) {
-    hipLaunchKernelGGL(join_columns_kernel<T>, dim3(ceil_div(v, 8)), dim3(kThreads), 0, stream, s.db_part, s.db_parts, v,
-                       s.info.scale, (T*)q.db, s.loss, p.whole ? ceil_div(n, kWholeRows) : 0, q.small);
-    RH_CHECK_LAUNCH("join_columns_kernel");
+  if (rest.db) {
+    hipLaunchKernelGGL(join_rest_kernel<T>, dim3(rest.workgroups()), dim3(kThreads), 0, stream, rest);
+    RH_CHECK_LAUNCH("join_rest_kernel");
   }
   return RH_OK;
 }

@@ -1043,7 +1043,9 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
   if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw.splits > 1))
     s.dw_part = c.take<float>((size_t)p.dw.splits * whole_tiles(p.dw, v) * p.ldpart);
   if (flags & RH_CE_GRAD_B) {
-    s.db_parts = ceil_div(p.chunk, p.whole ? kWholeRows : kProbRows) * p.chunks;
+    // as many as are written: whole rows' launches have a workgroup for every kWholeRows rows there are (a chunk before
+    // the last is a multiple of them), the others' for every kProbRows of every chunk
+    s.db_parts = p.whole ? ceil_div(n, kWholeRows) : ceil_div(p.chunk, kProbRows) * p.chunks;
     s.db_part = c.take<float>((size_t)s.db_parts * v);
   }
   s.bytes = c.off;

@@ -583,3 +583,50 @@ def test_captured_training_step(rh):
         torch.cuda.synchronize()
         assert torch.equal(static.detach(), want["loss"])
         assert torch.equal(sx.grad, want["d_features"]) and torch.equal(sw.grad, want["d_weight"])
+
+
+# ------------------------------------------------------------------ what an earlier call leaves in the workspace
+def with_spoilt_workspaces(rh, call):
+    """``call`` with every byte of the workspaces that it uses 0xFF before it (a NaN in every type)."""
+    call()      # it has its workspace now
+    torch.cuda.synchronize()
+    for room in rh.functional._workspaces.values():
+        room.fill_(255)
+    return call()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,v", [(1, 2056, 900), (4, 1032, 700), (13, 72, 300), (70, 40, 200), (193, 256, 601), (300, 100, 1000),
+                                   (40, 3000, 700), (3000, 64, 129)])
+def test_nothing_is_read_that_the_call_did_not_write(rh, n, d, v, dtype):
+    x, w, y, b = make(n, d, v, dtype, True, ignored=0.3 if n > 4 else 0.0, seed=23)
+    kw = dict(grads=(True, True, True))
+    first = rh.functional.linear_cross_entropy(x, w, y, b, **kw)
+    again = with_spoilt_workspaces(rh, lambda: rh.functional.linear_cross_entropy(x, w, y, b, **kw))
+    want = oracle(x, w, y, b)
+    for k in ("loss", "row_loss", "d_features", "d_weight", "d_bias"):
+        assert torch.equal(again[k], first[k]), k
+        close(k, again[k], want[k])
+    alone = with_spoilt_workspaces(rh, lambda: rh.functional.linear_cross_entropy(x, w, y, b))
+    close("row_loss", alone["row_loss"], want["row_loss"])
+
+
+@pytest.mark.parametrize("n,d,v", [(1_700_001, 8, 600), (1_680_000, 8, 640)])
+def test_nothing_is_read_that_a_shorter_last_chunk_did_not_write(rh, n, d, v):
+    """Whole rows in two chunks, the last with fewer workgroups than the first."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(n, d, generator=g, device="cuda").bfloat16()
+    w, b = torch.randn(v, d, generator=g, device="cuda").bfloat16(), torch.randn(v, generator=g, device="cuda").bfloat16()
+    y = torch.randint(0, v, (n,), generator=g, device="cuda")
+    y[3::11] = -100
+    out = with_spoilt_workspaces(rh, lambda: rh.functional.linear_cross_entropy(x, w, y, b, reduction="sum",
+                                                                                grads=(True, True, True)))
+    total = {k: [0.0, 0.0] for k in ("loss", "d_weight", "d_bias")}
+    step = 2 ** 27 // v
+    for lo in range(0, n, step):      # the bounds of the pieces add up
+        want = oracle(x[lo:lo + step], w, y[lo:lo + step], b, reduction="sum")
+        for k, sums in total.items():
+            sums[0] = sums[0] + want[k][0]
+            sums[1] = sums[1] + want[k][1]
+    for k, sums in total.items():
+        close(k, out[k], sums)

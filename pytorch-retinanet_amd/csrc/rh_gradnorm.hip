@@ -226,12 +226,13 @@ __device__ __forceinline__ double total_of(const double* __restrict__ partial, c
   return sum.value();
 }
 
+// partials < 0: the total is there, only the norm is made of it.
 template <int kKind>
-__global__ __launch_bounds__(kThreads) void total_kernel(const double* __restrict__ partial, const int n,
+__global__ __launch_bounds__(kThreads) void total_kernel(const double* __restrict__ partial, const int partials,
                                                          double* __restrict__ total, float* __restrict__ norm) {
-  const double s = total_of<kKind>(partial, n);
+  const double s = partials < 0 ? *total : total_of<kKind>(partial, partials);
   if (threadIdx.x == 0) {
-    *total = s;
+    if (partials >= 0) *total = s;
     *norm = (float)(kKind == kSquares ? __builtin_sqrt(s) : s);
   }
 }
@@ -352,17 +353,23 @@ static int run(const rh_grad_clip_args& q, hipStream_t stream) {
     });
     if (rc) return rc;
   }
-  if (!(q.stages & RH_CLIP_SCALE) || (blocks == 0 && (q.stages & RH_CLIP_NORM))) {
-    hipLaunchKernelGGL(total_kernel<kKind>, dim3(1), dim3(kThreads), 0, stream, partial, blocks, q.total, q.norm);
-    RH_CHECK_LAUNCH("total_kernel");
-    return RH_OK;
+  bool written = false;      // a list without values launches none of these
+  if (q.stages & RH_CLIP_SCALE) {
+    int rc = each_table(q.tensors, q.count, [&](const Table& t, int b) -> int {
+      hipLaunchKernelGGL(clip_kernel<kKind>, dim3(b), dim3(kThreads), 0, stream, t, partial, blocks, q.total, q.max_norm,
+                         q.norm);
+      RH_CHECK_LAUNCH("clip_kernel");
+      written = true;
+      return RH_OK;
+    });
+    if (rc) return rc;
   }
-  return each_table(q.tensors, q.count, [&](const Table& t, int b) -> int {
-    hipLaunchKernelGGL(clip_kernel<kKind>, dim3(b), dim3(kThreads), 0, stream, t, partial, blocks, q.total, q.max_norm,
-                       q.norm);
-    RH_CHECK_LAUNCH("clip_kernel");
-    return RH_OK;
-  });
+  if (!written) {
+    hipLaunchKernelGGL(total_kernel<kKind>, dim3(1), dim3(kThreads), 0, stream, partial,
+                       q.stages & RH_CLIP_NORM ? blocks : -1, q.total, q.norm);
+    RH_CHECK_LAUNCH("total_kernel");
+  }
+  return RH_OK;
 }
 
 }  // namespace norm

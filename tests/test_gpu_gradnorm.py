@@ -275,3 +275,21 @@ def test_sharded_stages(rh):
     for t, b in zip(a, before):
         exact = b.double() * (1.0 / (both + 1e-6))
         assert ((t.double() - exact).abs() <= exact.abs() * (torch.finfo(t.dtype).eps / 2 + 2.0 ** -22)).all()
+
+
+@pytest.mark.parametrize("p,total,norm", [(2.0, 9.0, 3.0), (1.0, 5.0, 5.0), (math.inf, 7.0, 7.0)])
+def test_scaling_of_empty_tensors_writes_the_norm(rh, p, total, norm):
+    """A rank whose shards are all of size 0 has the norm that the ranks' totals make."""
+    from retinahead import _lib
+    from retinahead.modules import _clip
+    F = rh.functional
+    empty = [torch.empty(0, device="cuda"), torch.empty(3, 0, device="cuda", dtype=torch.bfloat16)]
+    out = F.grad_clip(empty, norm_type=p, stages=_lib.CLIP_NORM)
+    assert float(out["norm"]) == 0.0 and float(out["total"]) == 0.0
+    out["total"].fill_(total)
+    F.grad_clip(empty, 1.0, p, stages=_lib.CLIP_SCALE, out=out)
+    assert float(out["norm"]) == norm and float(out["total"]) == total
+    got = _clip(params_of(empty), 1.0, p, False, lambda t: t.add_(total))      # as the ranks' reduction adds to it
+    assert float(got) == norm
+    assert float(rh.clip_grad_norm_(params_of(empty), 1.0, p, error_if_nonfinite=True)) == 0.0
+    assert float(rh.clip_grad_norm_(params_of(empty), 1.0, p)) == 0.0

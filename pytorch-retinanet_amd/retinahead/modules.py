@@ -566,12 +566,13 @@ def _clip(parameters, max_norm, norm_type, error_if_nonfinite, reduce_total):
         total = out["total"]
     if reduce_total is not None:
         reduce_total(total)
-    norm = total.sqrt() if float(norm_type) == 2.0 else total
+    # as the kernels make it of the total: what clips is a float32, infinity beyond its range
+    norm = (total.sqrt() if float(norm_type) == 2.0 else total).float()
     if error_if_nonfinite and not bool(torch.isfinite(norm)):
         raise RuntimeError(f"the norm of order {norm_type} of the gradients is not finite, so they "
                            "cannot be clipped")
     if out is None:
-        return norm.float().reshape(())
+        return norm.reshape(())
     return F.grad_clip(parameters, max_norm, norm_type, grads=True, stages=_lib.CLIP_SCALE, out=out)["norm"]
 
 

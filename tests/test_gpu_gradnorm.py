@@ -293,3 +293,17 @@ def test_scaling_of_empty_tensors_writes_the_norm(rh, p, total, norm):
     assert float(got) == norm
     assert float(rh.clip_grad_norm_(params_of(empty), 1.0, p, error_if_nonfinite=True)) == 0.0
     assert float(rh.clip_grad_norm_(params_of(empty), 1.0, p)) == 0.0
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0])
+def test_a_norm_beyond_float32_is_not_finite(rh, p):
+    """It is infinity where it clips, so that is what error_if_nonfinite asks about."""
+    top = torch.finfo(torch.float32).max
+    g = torch.full((100,), top, device="cuda")
+    kept = g.clone()
+    with pytest.raises(RuntimeError, match="not finite"):
+        rh.clip_grad_norm_(params_of([g]), 1.0, p, error_if_nonfinite=True)
+    assert torch.equal(g, kept)
+    one = g[:1].clone()      # the largest that is finite
+    assert float(rh.clip_grad_norm_(params_of([one]), math.inf, p, error_if_nonfinite=True)) == top
+    assert float(rh.clip_grad_norm_(params_of([g]), 1.0, p)) == math.inf and (g == 0).all()

@@ -34,6 +34,8 @@ int type_code(const at::ScalarType t) {      // -1: not one of the operators' ty
   }
 }
 const char* const kTypes = "float32, bfloat16 or float16 tensors needed";
+// a tangent would be dropped, which counts as zero
+const char* const kNoTangents = "retinahead operators do not support forward-mode differentiation";
 const char* const kNoFallback = "retinahead operators need tensors on a HIP device (there is no CPU fallback)";
 
 // (device index, bytes of rh_tensor_ref [count]), or a text that says what is wrong with the list.
@@ -49,6 +51,7 @@ PyObject* table_of(PyObject* list, const bool grads) {
     const at::Tensor& item = THPVariable_Unpack(items[i]);
     const at::Tensor t = grads ? item.grad() : item;
     if (!t.defined()) continue;
+    if (t._fw_grad(0).defined()) return PyUnicode_FromString(kNoTangents);
     if (t.layout() != at::kStrided) return PyUnicode_FromString("gradients must be dense tensors, not sparse ones");
     if (!t.is_cuda())
       return PyUnicode_FromString(kNoFallback);
@@ -184,6 +187,8 @@ struct Settings {
 CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, const at::Tensor& labels,
                       const at::Tensor& bias, const at::Tensor& divisor, const Settings& q,
                       const std::array<bool, 3>& want) {
+  for (const at::Tensor* t : {&features, &weight, &bias, &divisor})
+    refuse_unless(!t->defined() || !t->_fw_grad(0).defined(), kNoTangents);
   at::AutoDispatchBelowAutograd below;
   const int code = type_code(features.scalar_type());
   refuse_unless(code >= 0, kTypes);

@@ -101,3 +101,17 @@ def test_scale_gradient_refuses():
     assert lib.rh_scale_gradient(None, -1, 0, None, 1.0, None) == -2
     assert lib.rh_scale_gradient(None, 4, 0, None, 0.0, None) == -1
     assert lib.rh_scale_gradient(None, 0, 0, None, 1.0, None) == 0
+
+
+@pytest.mark.parametrize("which", ["features", "weight", "bias", "divisor"])
+def test_refuses_tangents(which):
+    """Forward-mode differentiation has no rule here: a tangent must not count as zero."""
+    import torch.autograd.forward_ad as forward_ad
+    args = dict(features=torch.ones(4, 8), weight=torch.ones(5, 8), labels=torch.zeros(4, dtype=torch.int64),
+                bias=torch.ones(5), divisor=torch.ones(1))
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(rh.RetinaHeadError, match="forward-mode"):
+            F.linear_cross_entropy(**args)
+        with pytest.raises(rh.RetinaHeadError, match="forward-mode"):
+            rh.LinearCrossEntropy()(**args)

@@ -76,3 +76,15 @@ def test_workspace_query():
     assert q(None, 1) == 0 and q(one.ctypes.data, -1) == 0
     big = _refs((4096, 1 << 34, 0))
     assert q(big.ctypes.data, 1) < 1 << 20
+
+
+def test_refuses_tangents():
+    """Forward-mode differentiation has no rule here: a tangent must not count as zero."""
+    import torch.autograd.forward_ad as forward_ad
+    p = torch.nn.Parameter(torch.ones(4))
+    with forward_ad.dual_level():
+        p.grad = forward_ad.make_dual(torch.ones(4), torch.ones(4))
+        with pytest.raises(rh.RetinaHeadError, match="forward-mode"):
+            rh.grad_norm(p.grad)
+        with pytest.raises(rh.RetinaHeadError, match="forward-mode"):
+            rh.clip_grad_norm_([p], 1.0)

@@ -459,13 +459,17 @@ typedef struct rh_linear_ce_args {
   void* db;                /* device [v] out                                                      */
   void* workspace;
   size_t workspace_bytes;
+  const float* upstream;   /* device [1] or NULL: the gradients are made for *upstream instead of `grad`.  Where it
+                              equals `grad`, dx, dw and db are left as an earlier call made them, and row_loss
+                              and small may hold anything                                       */
 } rh_linear_ce_args;
 
 /* 0 for sizes out of range: n <= 2^26, d <= 2^17, v <= 2^21. */
 size_t rh_linear_ce_workspace_bytes(int64_t n, int32_t d, int64_t v, int32_t dtype, int32_t flags);
 int rh_linear_ce(const rh_linear_ce_args* args, rh_stream_t stream);
 
-/* x *= *scale / assumed in place; nothing is touched when *scale == assumed (no host read). */
+/* x *= *scale / assumed in place; nothing is touched when *scale == assumed (no host read).  RH_F16 values that
+ * were too small or too large for the type when they were made do not come back: see rh_linear_ce_args.upstream. */
 int rh_scale_gradient(void* x, int64_t count, int32_t dtype, const float* scale, float assumed,
                       rh_stream_t stream);
 

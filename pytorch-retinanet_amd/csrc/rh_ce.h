@@ -36,6 +36,16 @@ struct Labels {
   __device__ __forceinline__ bool counts(const long long y) const { return y != ignore && y >= 0 && y < v; }
 };
 
+// The upstream gradient that a call's gradients are for: what the host was told, or a value on the device; one that
+// is what the host was told already has its gradients.
+struct Upstream {
+  const float* at;
+  float made;
+  __device__ __forceinline__ float value() const { return at ? *at : made; }
+  __device__ __forceinline__ bool there() const { return at && *at == made; }
+};
+constexpr int kThere = -1;      // rows counted, of a call whose gradients are there: no kernel has any
+
 // P is the matrix units' operand and so is rounded to the inputs' type.  float16 has no room for
 // small probabilities (2^-24 is its smallest value, one of 131 072 equal classes has 2^-17): there P
 // is kept times 2^15, which |P| <= 1 allows, and the products' results are scaled back, both exact.

@@ -123,7 +123,11 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
     const int2* __restrict__ blocks, char* __restrict__ xp, const long long part, const int panels, const int chunk,
     const RowInfo info,
     float* __restrict__ row_loss, T* __restrict__ dx, float* __restrict__ small, int* __restrict__ status,
-    const float* __restrict__ total, const int mean, const float grad) {
+    const float* __restrict__ total, const int mean, const Upstream up) {
+  if (up.there()) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *info.n_valid = kThere;
+    return;
+  }
   __shared__ int s_red[4], s_all[4], s_bad[4];
   __shared__ int s_place[kThreads];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
     all = s_all[0] + s_all[1] + s_all[2] + s_all[3];
     *info.n_valid = all;
     const float div = mean ? fmaxf(total ? *total : (float)all, 1.0f) : 1.0f;
-    *info.scale = grad / div;
+    *info.scale = up.value() / div;
     small[1] = (float)all;
     small[2] = 1.0f / div;
     *status = (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) ? RH_STATUS_LABEL_RANGE : 0;
@@ -217,7 +221,8 @@ __global__ __launch_bounds__(kThreads) void place_rows_kernel(
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* __restrict__ w, const long long ldw,
                                                             const int d, const int v, T* __restrict__ out,
-                                                            const int ldp) {
+                                                            const int ldp, const int* __restrict__ n_valid) {
+  if (*n_valid == kThere) return;
   const int lane = threadIdx.x & 63;
   for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < v; r += (long long)gridDim.x * 4)
 #pragma unroll 4
@@ -711,6 +716,7 @@ template <typename T, Layout kLA, typename S, To kTo>
 __global__ __launch_bounds__(S::kThreads, S::kBM == 256 ? 1 : 2) void product_kernel(const ProductArgs<T> a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   RH_LDS char* lds = (RH_LDS char*)smem;
+  if (kLA == kCols && *a.n_valid == kThere) return;
   const int rows = max(a.chunk.rows(a.n_valid), 0);
   const int m = kLA == kRows ? rows : a.m, k = kLA == kCols ? rows : a.k;
   const Grid g = {a.sharing.tiles_m(m), a.sharing.tiles_n};
@@ -798,12 +804,14 @@ template <typename T>
 struct Rest {
   const float* columns;
   int parts, v;
+  const int* n_valid;
   const float* scale;
   T* db;
   const double* loss_parts;
   int losses;
   float* small;
   __device__ __forceinline__ void join(const int block) const {
+    if (*n_valid == kThere) return;
     __shared__ float s_sum[32][8];
     if (losses && block == 0) add_losses(loss_parts, losses, small);
     const int in = threadIdx.x & 7, slice = threadIdx.x >> 3, c = block * 8 + in;
@@ -831,6 +839,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __restrict__ part, const Sharing sharing,
                                                               const long long ldpart, const int m, const int n,
                                                               const Chunk chunk, const int* __restrict__ n_valid,
+                                                              const int by_rows,
                                                               const float* __restrict__ scale, const float down,
                                                               const int* __restrict__ map, T* __restrict__ out,
                                                               const long long ldo, const Rest<T> rest,
@@ -839,7 +848,8 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __res
     rest.join(blockIdx.x - of_rest);
     return;
   }
-  const int rows = n_valid ? max(chunk.rows(n_valid), 0) : m, splits = sharing.splits(rows);
+  if (*n_valid == kThere) return;
+  const int rows = by_rows ? max(chunk.rows(n_valid), 0) : m, splits = sharing.splits(rows);
   const long long quads = (n + 3) / 4, top = rows * quads;
   const long long plane = (long long)sharing.tiles_m(rows) * sharing.bm * ldpart;
   const float s = *scale * down;
@@ -1116,7 +1126,7 @@ static int join_parts(const ProductArgs<T>& g, bool by_rows, const Rest<T>& rest
   long long blocks = ((long long)g.m * ((g.n + 3) / 4) + kThreads - 1) / kThreads;
   if (blocks > 256 * 8) blocks = 256 * 8;
   hipLaunchKernelGGL(join_parts_kernel<T>, dim3((unsigned)blocks + rest.workgroups()), dim3(kThreads), 0, stream, g.part,
-                     g.sharing, g.ldpart, g.m, g.n, g.chunk, by_rows ? g.n_valid : nullptr, g.scale, g.down, g.map, g.out,
+                     g.sharing, g.ldpart, g.m, g.n, g.chunk, g.n_valid, (int)by_rows, g.scale, g.down, g.map, g.out,
                      g.ldo, rest, (int)blocks);
   RH_CHECK_LAUNCH("join_parts_kernel");
   return RH_OK;
@@ -1240,7 +1250,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   if (side > ceil_div(p.panels, 4)) side = ceil_div(p.panels, 4);
   hipLaunchKernelGGL(place_rows_kernel<T>, dim3(p.row_blocks, side), dim3(kThreads), 0, stream, (const T*)q.x,
                      (long long)q.ldx, d, labels, n, p.per, counted ? s.blocks : nullptr, s.x, s.x_part, p.panels,
-                     p.chunk, s.info, q.row_loss, (T*)q.dx, q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, q.grad);
+                     p.chunk, s.info, q.row_loss, (T*)q.dx, q.small, (int*)(q.small + 3), q.divisor, q.reduction == RH_CE_MEAN, Upstream{q.upstream, q.grad});
   RH_CHECK_LAUNCH("place_rows_kernel");
   const bool grads = q.dx || q.dw || q.db;
   LogitArgs<T> a = {};
@@ -1254,7 +1264,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   a.w_limit = d * 2 - (a.steps - 1) * kStepBytes;
   if (p.ldw_pad) {
     hipLaunchKernelGGL(pad_rows_kernel<T>, dim3(v < 8192 ? ceil_div(v, 4) : 2048), dim3(kThreads), 0, stream, (const T*)q.w,
-                       (long long)q.ldw, d, v, (T*)s.w, p.ldw_pad);
+                       (long long)q.ldw, d, v, (T*)s.w, p.ldw_pad, s.info.n_valid);
     RH_CHECK_LAUNCH("pad_rows_kernel");
     a.w = s.w;
     a.ldw = (long long)p.ldw_pad * p.size;
@@ -1283,7 +1293,7 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
   a.part = s.z_part;
   Rest<T> rest = {};
   if (q.db)
-    rest = Rest<T>{s.db_part, s.db_parts, v, s.info.scale, (T*)q.db, s.loss, p.whole ? ceil_div(n, kWholeRows) : 0,
+    rest = Rest<T>{s.db_part, s.db_parts, v, s.info.n_valid, s.info.scale, (T*)q.db, s.loss, p.whole ? ceil_div(n, kWholeRows) : 0,
                    q.small};
   for (int c = 0; c < p.chunks; ++c) {
     a.chunk = Chunk{c * p.chunk, n - c * p.chunk < p.chunk ? n - c * p.chunk : p.chunk};

@@ -205,7 +205,8 @@ __global__ __launch_bounds__(kThreads) void few_logits_kernel(const T* __restric
                                                               const int v, const T* __restrict__ bias,
                                                               const int groups, const int waves,
                                                               typename Mma16<T>::Z* __restrict__ z, const int ldz,
-                                                              TopSum* __restrict__ part) {
+                                                              TopSum* __restrict__ part, const Upstream up) {
+  if (up.there()) return;
   typedef typename Mma16<T>::Z Z;
   typedef typename Mma16<T>::Acc Acc;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -347,7 +348,8 @@ __global__ __launch_bounds__(kThreads) void few_online_kernel(const T* __restric
                                                               const int v, const T* __restrict__ bias, const Labels y,
                                                               typename Mma16<T>::Z* __restrict__ z, const int ldz,
                                                               TopSum* __restrict__ part, float* __restrict__ dx_part,
-                                                              const int ldpart) {
+                                                              const int ldpart, const Upstream up) {
+  if (up.there()) return;
   constexpr int kV = 16 / (int)sizeof(T), kA = 16 / (kN > kC ? kN : kC), kVals = kA * kN;
   typedef typename Mma16<T>::Z Z;
   typedef typename Mma16<T>::Acc Four;
@@ -472,12 +474,13 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const TopSum* _
                                                                  const Labels y, const int n,
                                                                  const Z* __restrict__ z, const int ldz,
                                                                  const float* __restrict__ divisor, const int mean,
-                                                                 const float grad, TopSum* __restrict__ row,
+                                                                 const Upstream up_to, TopSum* __restrict__ row,
                                                                  float* __restrict__ scale,
                                                                  float* __restrict__ row_loss,
                                                                  float* __restrict__ small, int* __restrict__ status,
                                                                  float* __restrict__ share,
                                                                  float* __restrict__ of_label) {
+  if (up_to.there()) return;
   __shared__ float s_loss[kFewRows];
   __shared__ int s_keep[kFewRows], s_bad[kFewRows];
   const int r = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(64 * kFewRows) void few_rows_kernel(const TopSum* _
       bad |= s_bad[i];
     }
     const float div = mean ? fmaxf(divisor ? *divisor : (float)count, 1.0f) : 1.0f;
-    *scale = grad / div;
+    *scale = up_to.value() / div;
     small[0] = (float)(total * (double)(1.0f / div));
     small[1] = (float)count;
     small[2] = 1.0f / div;
@@ -544,7 +547,8 @@ __global__ __launch_bounds__(kThreads) void few_weights_kernel(
     const T* __restrict__ x, const long long ldx, const int n, const int d, const int v, const Labels y,
     const typename Mma16<T>::Z* __restrict__ z, const int ldz, const TopSum* __restrict__ row,
     const float* __restrict__ scale,
-    const int per, const int tpr, T* __restrict__ dw, T* __restrict__ db) {
+    const int per, const int tpr, T* __restrict__ dw, T* __restrict__ db, const Upstream up) {
+  if (up.there()) return;
   constexpr int kV = 16 / (int)sizeof(T);
   constexpr int kAtOnce = 128;      // classes whose probabilities wait in LDS
   __shared__ float s_p[kAtOnce][kN];
@@ -624,7 +628,8 @@ __global__ __launch_bounds__(kThreads) void few_products_kernel(
     const T* __restrict__ x, const long long ldx, const int n, const int d, const T* __restrict__ w,
     const long long ldw, const int v, const Labels y, const typename Mma16<T>::Z* __restrict__ z, const int ldz,
     const TopSum* __restrict__ row, const float* __restrict__ scale, const int per, const int waves_a_row,
-    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ dx_part, const int ldpart) {
+    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ dx_part, const int ldpart, const Upstream up) {
+  if (up.there()) return;
   constexpr int kV = 16 / (int)sizeof(T), kAtOnce = 128, kPitch = kFewRows + 1;      // rows a bank apart
   __shared__ float s_p[kAtOnce * kPitch];
   __shared__ TopSum s_row[kFewRows];
@@ -744,7 +749,8 @@ __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __r
                                                                 const float* __restrict__ of_label,
                                                                 const float* __restrict__ scale, const Labels y,
                                                                 const T* __restrict__ w, const long long ldw,
-                                                                T* __restrict__ dx) {
+                                                                T* __restrict__ dx, const Upstream up) {
+  if (up.there()) return;
   __shared__ f32x4 s_sum[64][4];
   const int quad = threadIdx.x & 3, slice = threadIdx.x >> 2;
   const int c = (blockIdx.x * 4 + quad) * 4, r = blockIdx.y;
@@ -781,13 +787,15 @@ __global__ __launch_bounds__(kThreads) void few_features_kernel(const float* __r
   }
 }
 
+static Upstream upstream_of(const rh_linear_ce_args& q) { return Upstream{q.upstream, q.grad}; }
+
 template <typename T, int kN>
 static int launch_weights(const rh_linear_ce_args& q, const FewPlan& p, const FewSpace& s, const Labels& y,
                           hipStream_t stream) {
   auto kernel = p.past ? few_weights_kernel<T, kN, true> : few_weights_kernel<T, kN, false>;
   hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x,
                      (long long)q.ldx, (int)q.n, q.d, (int)q.v, y, (const typename Mma16<T>::Z*)s.z, p.ldz, s.row, s.scale, p.per, p.tpr, (T*)q.dw,
-                     (T*)q.db);
+                     (T*)q.db, upstream_of(q));
   RH_CHECK_LAUNCH("few_weights_kernel");
   return RH_OK;
 }
@@ -799,7 +807,7 @@ static int launch_products(const rh_linear_ce_args& q, const FewPlan& p, const F
                          : few_products_kernel<T, false, false>;
   hipLaunchKernelGGL(kernel, dim3(p.grad_blocks, p.slices), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx,
                      (int)q.n, q.d, (const T*)q.w, (long long)q.ldw, (int)q.v, y, (const typename Mma16<T>::Z*)s.z, p.ldz, s.row, s.scale, p.per,
-                     p.tpr / 16, (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart);
+                     p.tpr / 16, (T*)q.dw, (T*)q.db, s.dx_part, p.ldpart, upstream_of(q));
   RH_CHECK_LAUNCH("few_products_kernel");
   return RH_OK;
 }
@@ -810,7 +818,7 @@ static int launch_online(const rh_linear_ce_args& q, const FewPlan& p, const Few
   auto kernel = p.wide_w ? few_online_kernel<T, kN, kC, true> : few_online_kernel<T, kN, kC, false>;
   hipLaunchKernelGGL(kernel, dim3(p.blocks), dim3(kThreads), 0, stream, (const T*)q.x, (long long)q.ldx, (int)q.n, q.d,
                      (const T*)q.w, (long long)q.ldw, (int)q.v, (const T*)q.bias, y, (typename Mma16<T>::Z*)s.z, p.ldz, s.part, s.dx_part,
-                     p.ldpart);
+                     p.ldpart, upstream_of(q));
   RH_CHECK_LAUNCH("few_online_kernel");
   return RH_OK;
 }
@@ -839,11 +847,11 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
   } else {
     auto logits = p.wide_w ? few_logits_kernel<T, true> : few_logits_kernel<T, false>;
     hipLaunchKernelGGL(logits, dim3(p.blocks), dim3(kThreads), 16 * kPitch, stream, (const T*)q.x, (long long)q.ldx, n, q.d,
-                       (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, (Z*)s.z, p.ldz, s.part);
+                       (const T*)q.w, (long long)q.ldw, v, (const T*)q.bias, p.groups, p.waves, (Z*)s.z, p.ldz, s.part, upstream_of(q));
     RH_CHECK_LAUNCH("few_logits_kernel");
   }
   hipLaunchKernelGGL(few_rows_kernel<Z>, dim3(1), dim3(64 * kFewRows), 0, stream, s.part, p.blocks, y, n, (const Z*)s.z, p.ldz, q.divisor,
-                     q.reduction == RH_CE_MEAN, q.grad, s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3), s.share,
+                     q.reduction == RH_CE_MEAN, upstream_of(q), s.row, s.scale, q.row_loss, q.small, (int*)(q.small + 3), s.share,
                      s.of_label);
   RH_CHECK_LAUNCH("few_rows_kernel");
   if (!q.dx && !q.dw && !q.db) return RH_OK;
@@ -857,7 +865,8 @@ static int run_typed(const rh_linear_ce_args& q, int flags, hipStream_t stream) 
   }
   if (q.dx) {
     hipLaunchKernelGGL(few_features_kernel<T>, dim3(ceil_div(q.d, 16), n), dim3(kThreads), 0, stream, s.dx_part, p.parts, n,
-                       p.ldpart, q.d, s.share, s.of_label, s.scale, y, (const T*)q.w, (long long)q.ldw, (T*)q.dx);
+                       p.ldpart, q.d, s.share, s.of_label, s.scale, y, (const T*)q.w, (long long)q.ldw, (T*)q.dx,
+                       upstream_of(q));
     RH_CHECK_LAUNCH("few_features_kernel");
   }
   return RH_OK;

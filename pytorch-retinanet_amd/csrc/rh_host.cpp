@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <array>
 #include <atomic>
 #include <map>
@@ -115,63 +116,21 @@ void refuse_unless(const bool ok, const char* text) {
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
+struct WithInterpreter {
+  const PyGILState_STATE state = PyGILState_Ensure();
+  ~WithInterpreter() { PyGILState_Release(state); }
+};
+
 // In a node's backward: RetinaHeadError for the caller of backward().
 [[noreturn]] void raise_in_backward(const std::string& text) {
-  const PyGILState_STATE state = PyGILState_Ensure();
-  PyErr_SetString(entry.error, text.c_str());
   python_error e;
-  e.persist();
-  PyGILState_Release(state);
+  {
+    const WithInterpreter held;
+    PyErr_SetString(entry.error, text.c_str());
+    e.persist();
+  }
   throw e;
 }
-
-// The forward call makes the gradients, backward hands them out, times the upstream one where that is not
-// the one they were made for.
-struct LinearCrossEntropyBackward : public torch::autograd::Node {
-  std::array<at::Tensor, 3> grads;
-  double expected = 1.0;
-  bool spent = false;
-  std::mutex once;
-
-  std::string name() const override { return "LinearCrossEntropyBackward"; }
-
-  torch::autograd::variable_list apply(torch::autograd::variable_list&& upstream) override {
-    torch::autograd::variable_list out(3);
-    {
-      std::lock_guard<std::mutex> lock(once);
-      if (spent)
-        raise_in_backward("the fused loss keeps one set of gradients: backward() can run once per forward()");
-      spent = true;
-      for (int i = 0; i < 3; ++i) out[i] = std::move(grads[i]);
-    }
-    const at::Tensor& g = upstream[0];
-    if (!g.defined()) return torch::autograd::variable_list(3);
-    const bool as_made = expected == 1.0 && g.numel() == 1 && g.is_cuda() && g.get_device() < kDevices &&
-                         g.const_data_ptr() == unit[g.get_device()].load();
-    if (!as_made) {
-      at::AutoDispatchBelowAutograd below;
-      const at::Tensor scale = g.reshape({-1}).slice(0, 0, 1).to(at::kFloat).contiguous();
-      for (const at::Tensor& d : out) {
-        if (!d.defined()) continue;
-        c10::DeviceGuard on(d.device());
-        if (entry.scale(d.data_ptr(), d.numel(), type_code(d.scalar_type()), scale.const_data_ptr<float>(),
-                        (float)expected, stream_of(d)) != RH_OK)
-          raise_in_backward("rh_scale_gradient failed: " + last_error());
-      }
-    }
-    if (!at::GradMode::is_enabled()) return out;
-    // create_graph: the gradients are there, their own gradients are not
-    for (at::Tensor& d : out)
-      if (d.defined()) d = d.detach().requires_grad_(true);
-    return torch::autograd::DelayedError("the classifier loss's gradients cannot be differentiated", 3).apply(std::move(out));
-  }
-
-  void release_variables() override {
-    std::lock_guard<std::mutex> lock(once);
-    for (at::Tensor& d : grads) d.reset();
-    spent = true;
-  }
-};
 
 struct CeOut {
   at::Tensor small, row_loss;
@@ -184,9 +143,12 @@ struct Settings {
   double expected;
 };
 
+// Under the interpreter's lock.  made: gradients of an earlier call with these arguments, to be made again where the
+// upstream gradient is not the expected one.
 CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, const at::Tensor& labels,
                       const at::Tensor& bias, const at::Tensor& divisor, const Settings& q,
-                      const std::array<bool, 3>& want) {
+                      const std::array<bool, 3>& want, const std::array<at::Tensor, 3>& made = {},
+                      const at::Tensor& upstream = {}) {
   for (const at::Tensor* t : {&features, &weight, &bias, &divisor})
     refuse_unless(!t->defined() || !t->_fw_grad(0).defined(), kNoTangents);
   at::AutoDispatchBelowAutograd below;
@@ -216,6 +178,7 @@ CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, cons
   const at::TensorOptions as_features = at::TensorOptions().dtype(features.scalar_type()).device(device);
   const at::TensorOptions floats = at::TensorOptions().dtype(at::kFloat).device(device);
   CeOut out;
+  out.grads = made;
   out.small = at::empty({4}, floats);
   out.row_loss = at::empty(labels.sizes(), floats);
   if (want[0]) out.grads[0] = at::empty(features.sizes(), as_features);
@@ -249,6 +212,7 @@ CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, cons
   a.reduction = q.reduction;
   a.ignore_index = q.ignore_index;
   a.divisor = divisor.defined() ? divisor.const_data_ptr<float>() : nullptr;
+  a.upstream = upstream.defined() ? upstream.const_data_ptr<float>() : nullptr;
   a.grad = (float)q.expected;
   a.flags = d * size % 16 || w.stride(0) * size % 16 || (uintptr_t)a.w % 16 || w.stride(0) >= 1 << 20
                 ? RH_CE_COPY_WEIGHT : 0;
@@ -281,6 +245,81 @@ CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, cons
     throw Refusal{"rh_linear_ce failed (" + std::to_string(code_of_call) + "): " + last_error()};
   return out;
 }
+
+// The forward call makes the gradients, backward hands them out, times the upstream one where that is not
+// the one they were made for.  float16 has no room for that: gradients made for 1 may be too small for it where those
+// of a scaled loss are not (a mean over many rows), or too large, so there they are made anew from the inputs.
+struct LinearCrossEntropyBackward : public torch::autograd::Node {
+  std::array<at::Tensor, 3> grads;
+  // float16: features, weight, labels, bias, divisor; those made under inference mode as they are
+  std::array<torch::autograd::SavedVariable, 5> inputs;
+  std::array<at::Tensor, 5> frozen;
+  bool anew = false;
+  Settings settings = {};
+  bool spent = false;
+  std::mutex once;
+
+  std::string name() const override { return "LinearCrossEntropyBackward"; }
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& upstream) override {
+    torch::autograd::variable_list out(3);
+    std::array<at::Tensor, 5> of;
+    const at::Tensor& g = upstream[0];
+    const bool as_made = settings.expected == 1.0 && g.defined() && g.numel() == 1 && g.is_cuda() &&
+                         g.get_device() < kDevices && g.const_data_ptr() == unit[g.get_device()].load();
+    {
+      std::lock_guard<std::mutex> lock(once);
+      if (spent)
+        raise_in_backward("the fused loss keeps one set of gradients: backward() can run once per forward()");
+      if (anew && g.defined() && !as_made)
+        for (int i = 0; i < 5; ++i)
+          of[i] = frozen[i].defined() ? frozen[i] : inputs[i].unpack();      // refuses what was changed in place
+      spent = true;
+      for (int i = 0; i < 3; ++i) out[i] = std::move(grads[i]);
+    }
+    if (!g.defined()) return torch::autograd::variable_list(3);
+    if (!as_made) {
+      at::AutoDispatchBelowAutograd below;
+      const at::Tensor scale = g.reshape({-1}).slice(0, 0, 1).to(at::kFloat).contiguous();
+      if (anew)
+        make_anew(of, scale, out);
+      else
+        for (const at::Tensor& d : out) {
+          if (!d.defined()) continue;
+          c10::DeviceGuard on(d.device());
+          if (entry.scale(d.data_ptr(), d.numel(), type_code(d.scalar_type()), scale.const_data_ptr<float>(),
+                          (float)settings.expected, stream_of(d)) != RH_OK)
+            raise_in_backward("rh_scale_gradient failed: " + last_error());
+        }
+    }
+    if (!at::GradMode::is_enabled()) return out;
+    // create_graph: the gradients are there, their own gradients are not
+    for (at::Tensor& d : out)
+      if (d.defined()) d = d.detach().requires_grad_(true);
+    return torch::autograd::DelayedError("the classifier loss's gradients cannot be differentiated", 3).apply(std::move(out));
+  }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(once);
+    for (at::Tensor& d : grads) d.reset();
+    for (torch::autograd::SavedVariable& v : inputs) v.reset_data();
+    for (at::Tensor& t : frozen) t.reset();
+    spent = true;
+  }
+
+ private:
+  void make_anew(const std::array<at::Tensor, 5>& of, const at::Tensor& scale, const torch::autograd::variable_list& out) {
+    const WithInterpreter held;      // classifier_loss wants it
+    try {
+      classifier_loss(of[0], of[1], of[2], of[3], of[4], settings, {}, {out[0], out[1], out[2]}, scale);
+    } catch (const Refusal& e) {
+      raise_in_backward(e.text);
+    } catch (python_error& e) {
+      e.persist();
+      throw;
+    }
+  }
+};
 
 bool tensor_or_none(PyObject* o, at::Tensor& t) {
   if (o == Py_None) return true;
@@ -344,7 +383,14 @@ PyObject* linear_ce(PyObject*, PyObject* args) {
       auto made = std::shared_ptr<LinearCrossEntropyBackward>(new LinearCrossEntropyBackward(), torch::autograd::deleteNode);
       made->set_next_edges(torch::autograd::collect_next_edges(features, weight, bias));
       made->grads = std::move(out.grads);
-      made->expected = q.expected;
+      made->settings = q;
+      made->anew = features.scalar_type() == at::kHalf;
+      if (made->anew) {
+        const at::Tensor* const of[5] = {&features, &weight, &labels, &bias, &divisor};
+        for (int i = 0; i < 5; ++i)
+          if (of[i]->defined() && of[i]->is_inference()) made->frozen[i] = *of[i];
+          else made->inputs[i] = torch::autograd::SavedVariable(*of[i], false);
+      }
       torch::autograd::set_history(loss, made);
     }
     PyObject* const as_class = THPVariable_Wrap(loss, reinterpret_cast<PyTypeObject*>(node));

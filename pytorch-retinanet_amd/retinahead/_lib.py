@@ -92,6 +92,7 @@ class LinearCeArgs(C.Structure):
         ("db", C.c_void_p),
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_size_t),
+        ("upstream", C.c_void_p),
     ]
 
 

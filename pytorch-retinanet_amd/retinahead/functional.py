@@ -628,7 +628,8 @@ def _bind_host():
 
 def scale_gradient_(grad, scale, assumed=1.0):
     """In place and without a host read: grad *= scale / assumed, one rounding; a gradient whose
-    scale equals ``assumed`` is not touched."""
+    scale equals ``assumed`` is not touched.  What a float16 gradient lost when it was made (below
+    2^-24, beyond 65 504) does not come back."""
     dev = _dev_check(grad, scale)
     if not grad.is_contiguous():
         raise RetinaHeadError("scale_gradient_ needs a contiguous tensor")

@@ -486,8 +486,12 @@ class LinearCrossEntropy(nn.Module):
     ignore_index: rows with this label take no part: no loss, zero gradient, whatever their features
         hold.  A batch without a counted row has loss 0 and zero gradients.
     reduction: 'mean' over the counted rows, or 'sum'.
-    expected_grad: the upstream gradient the stored gradients are made for (see ``FocalLoss``); any
-        other one is applied in place by ``backward``, with one more rounding for 16-bit types.
+    expected_grad: the upstream gradient the stored gradients are made for (see ``FocalLoss``).  Any
+        other one is applied in place by ``backward``: for bfloat16 with one more rounding.  float16
+        gradients made for 1 may be zero or infinite where those of a scaled loss are not, so
+        ``backward`` makes them anew there, which costs the call again (and keeps its inputs, which must
+        not be changed before); with the loss scale as expected_grad it need not.  Whether the upstream
+        gradient is the expected one is found on the device.
     check_labels: read the status word after the call (one host synchronisation) and raise IndexError
         for a label outside [0, V) other than ignore_index; without it such a row is left out.
 

@@ -630,3 +630,170 @@ def test_nothing_is_read_that_a_shorter_last_chunk_did_not_write(rh, n, d, v):
             sums[1] = sums[1] + want[k][1]
     for k, sums in total.items():
         close(k, out[k], sums)
+
+
+# ------------------------------------------------------------------ upstream gradients other than the expected one
+def leaves_of(*tensors):
+    return [None if t is None else t.clone().requires_grad_(True) for t in tensors]
+
+
+UPSTREAM = [(1, 2056, 900, 64.0), (4, 1032, 5000, 256.0), (4, 40, 5000, 256.0), (13, 72, 30000, 1024.0), (16, 2048, 300, 512.0),
+            (300, 40, 601, 65536.0), (4096, 256, 601, 65536.0), (700, 1001, 20011, 65536.0), (2100, 64, 9000, 65536.0),
+            (40, 3000, 700, 2048.0)]
+
+
+@pytest.mark.parametrize("n,d,v,up", UPSTREAM)
+def test_float16_under_a_loss_scale(rh, n, d, v, up):
+    """A scaled loss's gradients are those that were made for its scale, whatever 1 would have left of them."""
+    x, w, y, b = make(n, d, v, "f16", True, ignored=0.2 if n > 4 else 0.0, seed=24, scale=3.0)
+    want = oracle(x, w, y, b, upstream=up)
+    made = rh.functional.linear_cross_entropy(x, w, y, b, expected_grad=up, grads=(True, True, True))
+    for how in range(3):
+        leaves = leaves_of(x, w, b)
+        fn = rh.LinearCrossEntropy(expected_grad=(1.0, 1.0, 8.0)[how])
+        loss = fn(leaves[0], leaves[1], y, leaves[2])
+        if how == 1:
+            loss.backward(torch.full((1,), up, device="cuda"))
+        else:
+            (loss * up).backward()
+        close("loss", loss.detach(), want["loss"])
+        for t, k in zip(leaves, ("d_features", "d_weight", "d_bias")):
+            close(k, t.grad, want[k])
+            assert torch.equal(t.grad, made[k]), (k, how)
+        assert torch.equal(fn.last["row_loss"], made["row_loss"]) and torch.equal(loss.detach(), made["loss"])
+
+
+@pytest.mark.parametrize("n,d,v", [(2, 1032, 700), (13, 72, 300), (193, 256, 601), (300, 100, 1000), (40, 3000, 700)])
+def test_float16_gradients_made_for_the_loss_scale_stay(rh, n, d, v):
+    """expected_grad is the loss scale: what forward made is what backward hands out, of any leaves."""
+    x, w, y, b = make(n, d, v, "f16", True, ignored=0.2 if n > 4 else 0.0, seed=25)
+    fn = rh.LinearCrossEntropy(expected_grad=512.0)
+    for need in ((True, True, True), (True, False, False), (False, True, False), (False, False, True)):
+        for up in (512.0, 96.0):
+            # (other leaves may be other kernels)
+            ref = rh.functional.linear_cross_entropy(x, w, y, b, expected_grad=up, grads=need)
+            args = [t.clone().requires_grad_(r) for t, r in zip((x, w, b), need)]
+            torch.cuda.synchronize()
+            for room in rh.functional._workspaces.values():
+                room.fill_(255)
+            (fn(args[0], args[1], y, args[2]) * up).backward()
+            for t, r, k in zip(args, need, ("d_features", "d_weight", "d_bias")):
+                assert t.grad is None if not r else torch.equal(t.grad, ref[k]), (k, need, up)
+
+
+def test_float16_upstream_of_special_calls(rh):
+    fn = rh.LinearCrossEntropy()
+    # rows left out that hold anything; a sum beyond the type's range that the upstream gradient brings back
+    x, w, y, _ = make(3000, 72, 90, "f16", False, ignored=0.4, seed=26)
+    x[(y == -100).nonzero()[::2, 0]] = float("nan")
+    for reduction, up in (("mean", 4096.0), ("sum", 2.0 ** -10)):
+        px, pw = leaves_of(x, w)
+        (rh.LinearCrossEntropy(reduction=reduction)(px, pw, y) * up).backward()
+        want = oracle(torch.where((y == -100)[:, None], 0.0, x), w, y, None, reduction=reduction, upstream=up)
+        close("d_features", px.grad, want["d_features"])
+        close("d_weight", pw.grad, want["d_weight"])
+        assert (px.grad[y == -100] == 0).all()
+    y5 = torch.full_like(y, 5)
+    x5 = torch.full_like(x, 100.0)
+    x5[:, 0] = -100.0      # dW of class 5 is about -3000 x
+    px, pw = leaves_of(x5, w)
+    (rh.LinearCrossEntropy(reduction="sum")(px, pw, y5) * 2.0 ** -10).backward()
+    close("d_weight", pw.grad, oracle(x5, w, y5, None, reduction="sum", upstream=2.0 ** -10)["d_weight"])
+    # no row counts; no rows
+    px, pw = leaves_of(x, w)
+    (fn(px, pw, torch.full_like(y, -100)) * 3.0).backward()
+    assert (px.grad == 0).all() and (pw.grad == 0).all()
+    px, pw = leaves_of(x[:0], w)
+    (fn(px, pw, y[:0]) * 3.0).backward()
+    assert px.grad.shape == (0, 72) and (pw.grad == 0).all()
+    # a divisor, strided and batched features, int32 labels, a label outside
+    x, w, y, b = make(60, 72, 130, "f16", True, seed=27)
+    y[7] = 130
+    wide = torch.full((60, 100), float("nan"), dtype=x.dtype, device="cuda")
+    wide[:, 5:77] = x
+    leaf = wide.requires_grad_(True)
+    pw, pb = leaves_of(w, b)
+    div = torch.full((1,), 50.0, device="cuda")
+    (fn(leaf[:, 5:77].reshape(5, 12, 72), pw, y.view(5, 12).int(), pb, divisor=div) * 1000.0).backward()
+    ref = rh.functional.linear_cross_entropy(x, w, y, b, divisor=div, expected_grad=1000.0, grads=(True, True, True))
+    assert torch.equal(leaf.grad[:, 5:77], ref["d_features"]) and (leaf.grad[:, 77:] == 0).all()
+    assert torch.equal(pw.grad, ref["d_weight"]) and torch.equal(pb.grad, ref["d_bias"])
+    # inputs changed in between are refused, and one set of gradients it stays
+    px, pw = leaves_of(x, w)
+    loss = fn(px, pw, y)
+    with torch.no_grad():
+        pw += 1.0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        (loss * 2.0).backward()
+    px, pw = leaves_of(x, w)
+    loss = fn(px, pw, y)
+    (loss * 2.0).backward(retain_graph=True)
+    with pytest.raises(rh.RetinaHeadError, match="once"):
+        (loss * 2.0).backward()
+    # labels made under inference mode
+    with torch.inference_mode():
+        seen = y.clone()
+    first = pw.grad.clone()
+    px, pw = leaves_of(x, w)
+    (fn(px, pw, seen) * 2.0).backward()
+    assert torch.equal(pw.grad, first)
+
+
+def test_float16_scaled_step_captured(rh):
+    """A graph of forward and scaled backward, replayed with other inputs and scales, the expected one among them."""
+    x, w, y, _ = make(200, 64, 300, "f16", False, ignored=0.1, seed=28)
+    fn = rh.LinearCrossEntropy(expected_grad=128.0)
+    sx, sw, sy = x.clone().requires_grad_(True), w.clone().requires_grad_(True), y.clone()
+    scale = torch.full((1,), 64.0, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = fn(sx, sw, sy)
+        (loss * scale).backward()
+        del loss
+        sx.grad = sw.grad = None
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = fn(sx, sw, sy)
+        (static * scale).backward()
+    for i, up in enumerate((128.0, 4096.0, 1.0, 128.0, 65536.0)):
+        x2, w2, y2, _ = make(200, 64, 300, "f16", False, ignored=0.1 * i, seed=40 + i)
+        with torch.no_grad():
+            sx.copy_(x2)
+            sw.copy_(w2)
+            sy.copy_(y2)
+            scale.fill_(up)
+        graph.replay()
+        want = rh.functional.linear_cross_entropy(x2, w2, y2, expected_grad=up, grads=(True, True, False))
+        torch.cuda.synchronize()
+        assert torch.equal(static.detach(), want["loss"])
+        assert torch.equal(sx.grad, want["d_features"]) and torch.equal(sw.grad, want["d_weight"]), up
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,d,v", [(3, 1032, 700), (13, 72, 300), (193, 256, 601), (300, 101, 1000)])
+def test_upstream_of_the_other_types(rh, n, d, v, dtype):
+    """Stored gradients times the upstream one: its quotient, the product and the result are rounded once more."""
+    x, w, y, b = make(n, d, v, dtype, True, ignored=0.2 if n > 4 else 0.0, seed=29)
+    want = oracle(x, w, y, b, upstream=300.0)
+    leaves = leaves_of(x, w, b)
+    (rh.LinearCrossEntropy(expected_grad=7.0)(leaves[0], leaves[1], y, leaves[2]) * 300.0).backward()
+    for t, k in zip(leaves, ("d_features", "d_weight", "d_bias")):
+        value, tol = want[k]
+        more = torch.finfo(t.dtype).eps / 2 + 2 * E
+        close(k, t.grad, (value, tol * (1 + more) + more * value.abs()))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [0, 1, 255, 100_003])
+def test_scale_gradient(rh, n, dtype):
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g).to(TYPES[dtype]).cuda()
+    was = x.clone()
+    F = rh.functional
+    assert F.scale_gradient_(x, torch.full((1,), 2.5, device="cuda"), 2.5) is x and torch.equal(x, was)
+    F.scale_gradient_(x, torch.full((1,), 6.0, device="cuda"), 0.5)
+    exact = was.double() * 12.0
+    f = torch.finfo(x.dtype)
+    assert ((x.double() - exact).abs() <= f.eps / 2 * exact.abs() + f.smallest_normal * f.eps / 2).all()

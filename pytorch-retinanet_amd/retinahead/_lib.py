@@ -216,6 +216,24 @@ def load():
     return lib
 
 
+_host = None
+
+
+def load_host():
+    """Returns the extension module retinahead._host, which the classifier loss and the multi-tensor
+    operators go through; raises if it is missing or does not fit the torch that runs."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise RetinaHeadError(
+                f"retinahead._host cannot be loaded ({e}): build it with `make -C pytorch-retinanet_amd/csrc` "
+                "against the torch that is installed") from e
+        _host = module
+    return _host
+
+
 def last_error():
     buf = C.create_string_buffer(512)
     load().rh_last_error(buf, 512)

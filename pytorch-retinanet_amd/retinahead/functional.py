@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from . import _host, _lib
+from . import _lib
 from ._lib import RetinaHeadError
 
 # Caches shared by every thread that calls into the package (nn.DataParallel drives its replicas
@@ -608,22 +608,22 @@ def _classifier_loss(features, weight, labels, bias, divisor, ignore_index, redu
         raise ValueError("reduction must be 'mean' or 'sum'")
     if float(expected_grad) == 0.0:
         raise ValueError("expected_grad must not be zero")
-    if not _bound:
+    if _host is None:
         _bind_host()
     return _host.linear_ce(features, weight, labels, bias, divisor, ignore_index, _lib.CE_REDUCTIONS[reduction],
                            expected_grad, *grads, node)
 
 
-_bound = False
+_host = None      # the extension module, bound to the library's entry points
 
 
 def _bind_host():
-    global _bound
-    lib = _lib.load()
+    global _host
+    lib, host = _lib.load(), _lib.load_host()
     at = lambda f: C.cast(f, C.c_void_p).value
-    _host.bind(at(lib.rh_linear_ce_workspace_bytes), at(lib.rh_linear_ce), at(lib.rh_scale_gradient),
-               at(lib.rh_last_error), workspace, RetinaHeadError)
-    _bound = True
+    host.bind(at(lib.rh_linear_ce_workspace_bytes), at(lib.rh_linear_ce), at(lib.rh_scale_gradient),
+              at(lib.rh_last_error), workspace, RetinaHeadError)
+    _host = host
 
 
 def scale_gradient_(grad, scale, assumed=1.0):
@@ -645,7 +645,7 @@ def scale_gradient_(grad, scale, assumed=1.0):
 def _tensor_table(tensors, grads=False):
     """(device, list as rh_tensor_ref in bytes) of the tensors, or of their gradients where they have
     one; device None where there is nothing."""
-    table = _host.tensor_table(tensors, grads)
+    table = _lib.load_host().tensor_table(tensors, grads)
     if isinstance(table, str):
         raise RetinaHeadError(table)
     index, refs = table

@@ -340,3 +340,33 @@ def test_bench_multi_rank_skeleton_under_gloo():
     with pytest.raises(SystemExit):
         bench.require_ranks(2, 2, 1, "nccl")
     bench.require_ranks(2, 2, 1, "gloo")                  # the one-card rehearsal is asked for by name
+
+
+def test_package_loads_without_the_extension_module():
+    """The detection operators need none of it; what does says so when it is called."""
+    import subprocess
+    code = """
+import sys
+sys.path.insert(0, %r)
+sys.modules["retinahead._host"] = None      # as if it were not there
+import torch
+import retinahead as rh
+rh.load_library()
+rh.FocalLoss(), rh.postprocess, rh.functional.make_anchor_cfg(), rh.LinearCrossEntropy()
+p = torch.nn.Parameter(torch.ones(3))
+p.grad = torch.ones(3)
+for call in (lambda: rh.LinearCrossEntropy()(torch.ones(2, 3), torch.ones(4, 3), torch.zeros(2, dtype=torch.int64)),
+             lambda: rh.clip_grad_norm_([p], 1.0), lambda: rh.grad_norm(p.grad)):
+    try:
+        call()
+    except rh.RetinaHeadError as e:
+        assert "retinahead._host cannot be loaded" in str(e) and "make -C" in str(e), e
+    else:
+        raise AssertionError("not refused")
+from retinahead import modules
+modules.torch = type("T", (), {"ones": staticmethod(lambda *a, **k: torch.ones(1)), "float32": torch.float32})
+assert modules._unit_gradient(torch.device("cuda", 0)).item() == 1.0
+print("fine")
+""" % PKG_DIR
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert done.returncode == 0 and done.stdout.strip().endswith("fine"), done.stdout + done.stderr

@@ -118,8 +118,9 @@ __device__ __forceinline__ u32x4 make_rsrc(const char* base, const long long byt
 // the compiler waits for every such load of its own before any LDS read; here stage_wait() does.
 template <int kAt>
 __device__ __forceinline__ void load_to_lds(const u32x4 rsrc, const unsigned lds, const int offset) {
-  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
+  [[maybe_unused]] unsigned m0;      // an output, so that the compiler keeps nothing of its own there
+  asm volatile("s_add_u32 m0, %1, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+               : "={m0}"(m0)
                : "s"(lds), "v"(offset), "s"(rsrc), "n"(kAt)
                : "memory", "scc");
 }

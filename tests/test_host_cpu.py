@@ -370,3 +370,16 @@ print("fine")
 """ % PKG_DIR
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert done.returncode == 0 and done.stdout.strip().endswith("fine"), done.stdout + done.stderr
+
+
+def test_inline_assembly_declares_the_m0_it_writes():
+    """m0 is no register that the compiler hands out, but it uses it: what overwrites it has to be an output."""
+    import glob
+    seen = 0
+    for path in glob.glob(os.path.join(PKG_DIR, "csrc", "*.h*")):
+        with open(path) as f:
+            for block in re.findall(r"asm volatile\((.*?)\);", f.read(), re.S):
+                if re.search(r"\bs_\w+ m0,", block):
+                    seen += 1
+                    assert '"={m0}"' in block, (path, block)
+    assert seen == 1

@@ -244,12 +244,14 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(const Table t, const dou
                                                         const int partials, double* __restrict__ total,
                                                         const float max_norm, float* __restrict__ norm) {
   const double s = partials ? total_of<kKind>(partial, partials) : *total;
-  const float length = (float)(kKind == kSquares ? __builtin_sqrt(s) : s);
+  const double length = kKind == kSquares ? __builtin_sqrt(s) : s;
+  const float rounded = (float)length;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     if (partials) *total = s;
-    *norm = length;
+    *norm = rounded;
   }
-  const float c = max_norm / (length + 1e-6f);
+  // of the unrounded length, unless what is returned is infinity: the factor is rounded once
+  const float c = (float)((double)max_norm / ((rounded < __builtin_inff() ? length : (double)rounded) + 1e-6));
   if (c >= 1.0f) return;      // times one: nothing to write (a NaN goes on, and into every gradient)
   // from the list's end, which the norm's pass has read last and the caches still hold
   each_piece<true>(t, [&](const int type, const Range& r) {

@@ -307,3 +307,16 @@ def test_a_norm_beyond_float32_is_not_finite(rh, p):
     one = g[:1].clone()      # the largest that is finite
     assert float(rh.clip_grad_norm_(params_of([one]), math.inf, p, error_if_nonfinite=True)) == top
     assert float(rh.clip_grad_norm_(params_of([g]), 1.0, p)) == math.inf and (g == 0).all()
+
+
+@pytest.mark.parametrize("p", NORMS)
+def test_the_factor_is_rounded_once(rh, p):
+    """min(1, max_norm / (norm + 1e-6)) in 64 bits, then to float32 (2^-24), times a float32 value (2^-24); the norm's
+    own 64-bit sums are granted 2^-40."""
+    for seed in range(24):
+        g = rand(3001 + seed, "f32", 60 + seed, 1.0 + seed)
+        was = g.double()
+        c = 0.125 / (norm64([g], p) + 1e-6)
+        rh.clip_grad_norm_(params_of([g]), 0.125, p)
+        off = ((g.double() - was * c).abs() / (was.abs() * c).clamp(min=1e-30)).max()
+        assert float(off) <= 2.0 ** -23 + 2.0 ** -40, seed

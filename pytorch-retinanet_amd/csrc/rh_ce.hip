@@ -1037,18 +1037,20 @@ static Space carve(void* base, const Plan& p, int n, int d, int v, int flags) {
     s.w_part = (long long)v * p.panels * kStepBytes;
     s.w = c.take<char>((size_t)s.w_part * p.parts);
   }
-  s.stats = c.take<float2>((size_t)p.groups * p.chunk);
-  s.z_label = c.take<float>(n);
-  if (p.logits.splits > 1)
-    s.z_part = c.take<float>((size_t)p.logits.splits * whole_tiles(p.logits, p.chunk) * p.ldp);
-  s.row_stats = c.take<float2>(n);
+  if (!p.whole) {
+    s.stats = c.take<float2>((size_t)p.groups * p.chunk);
+    s.z_label = c.take<float>(n);
+    if (p.logits.splits > 1)
+      s.z_part = c.take<float>((size_t)p.logits.splits * whole_tiles(p.logits, p.chunk) * p.ldp);
+    s.row_stats = c.take<float2>(n);
+  }
   s.loss = c.take<double>(ceil_div(n, kJoinRows));
   if (flags & (RH_CE_GRAD_X | RH_CE_GRAD_W | RH_CE_GRAD_B)) {
-    s.z = c.take<char>((size_t)p.chunk * p.ldp * p.kept_size);
+    s.z = c.take<char>((size_t)p.chunk * p.ldp * p.kept_size);      // whole rows: P alone
     s.p_part = (long long)p.chunk * p.ldp * 2;
     s.p = p.parts > 1 ? c.take<char>((size_t)s.p_part * p.parts) : s.z;
   }
-  if ((flags & RH_CE_GRAD_X) && p.dx.splits > 1)
+  if ((flags & RH_CE_GRAD_X) && !p.whole && p.dx.splits > 1)
     s.dx_part = c.take<float>((size_t)p.dx.splits * whole_tiles(p.dx, p.chunk) * p.ldpart);
   if ((flags & RH_CE_GRAD_W) && (p.chunks > 1 || p.dw.splits > 1))
     s.dw_part = c.take<float>((size_t)p.dw.splits * whole_tiles(p.dw, v) * p.ldpart);
@@ -1300,13 +1302,13 @@ static int run(const rh_linear_ce_args& q, const Plan& p, const Space& s, hipStr
     const int first = a.chunk.first;
     a.x = s.x + (long long)first * p.panels * kStepBytes;
     a.label = s.info.label + first;
-    a.z_label = s.z_label + first;
     if (p.whole) {
       if (int rc = whole_rows(q, p, s, a, c, stream)) return rc;
       if (q.dw)
         if (int rc = weight_gradient(q, p, s, a, c, rest, stream)) return rc;
       continue;
     }
+    a.z_label = s.z_label + first;
     if (int rc = make_logits(p, a, grads, stream)) return rc;
     hipLaunchKernelGGL(join_stats_kernel, dim3(ceil_div(a.chunk.most, kJoinRows)), dim3(kThreads), 0, stream, s.stats, a.ld_stats,
                        p.groups, a.chunk, s.info.n_valid, s.info.map + first, a.z_label, s.row_stats + first, q.row_loss,

@@ -115,3 +115,14 @@ def test_refuses_tangents(which):
             F.linear_cross_entropy(**args)
         with pytest.raises(rh.RetinaHeadError, match="forward-mode"):
             rh.LinearCrossEntropy()(**args)
+
+
+@pytest.mark.parametrize("n,d,v", [(49104, 256, 601), (850_176, 24, 600), (100_000, 512, 512)])
+def test_workspace_of_whole_rows(n, d, v):
+    """The placed features, P, the places and the sums of columns: nothing of what the logits by tiles need."""
+    q = rh.load_library().rh_linear_ce_workspace_bytes
+    columns = (v + 63) // 64 * 64
+    p, x, rows = n * columns * 2, n * ((d + 31) // 32 * 64), n * 12 + n
+    sums = (n + 63) // 64 * v * 4
+    got = q(n, d, v, _lib.RH_BF16, _lib.CE_GRAD_X | _lib.CE_GRAD_B)
+    assert got <= p + x + rows + sums + (1 << 20), (got, p, x, rows, sums)

@@ -90,11 +90,15 @@ __device__ __forceinline__ void to_floats(const u32x4 u, float (&f)[16 / sizeof(
   for (int i = 0; i < 16 / (int)sizeof(T); ++i) f[i] = TypeOf<T>::to_float(r.v[i]);
 }
 
-// dW that the caches could not hold beside the weights is written past them, so that they keep weights: a call of
-// 1 x 2048 rows and 65 536 classes in bfloat16 (268 MB each) takes 118 us so, 140 with ordinary stores, the next
-// call's reading 42 instead of 84; 8 x 2048 191 instead of 227 on the card.  (In the products of many rows it costs: dW
-// of 32 768 x 2048 578 us instead of 535.)
-constexpr long long kPastCaches = 128ll << 20;
+// dW is written past the caches where what is read next is not dW: beside the weights that the same kernel reads, if
+// the caches cannot hold both, and else where dW alone is more than they hold.  Steps of loss, clipping and an update
+// of the weights (each reads dW next), bfloat16, 2048 features, us, past them / into them:
+//   16 rows (weights read beside)   160 MiB of dW 305 / 315, 256 MiB 505 / 506, 384 MiB 744 / 778
+//   1 row (read before)             160 MiB 236 / 225, 256 MiB 400 / 380, 320 MiB 510 / 499, 384 MiB 618 / 627
+//   4 rows, frozen features (the same)   256 MiB 402 / 396, 320 MiB 519 / 514, 384 MiB 620 / 646
+// A loss called again and again, its weights still in the caches, gains more and earlier (1 row, 256 MiB: 109 / 141), but
+// that is no step.  (In the products of many rows it costs: dW of 32 768 x 2048 578 us instead of 535.)
+constexpr long long kPastBeside = 128ll << 20, kPastAlone = 352ll << 20;
 template <bool kPast>
 __device__ __forceinline__ void store16(void* to, const u32x4 v) {
   if constexpr (kPast) __builtin_nontemporal_store(v, (u32x4*)to);
@@ -154,8 +158,8 @@ static FewPlan few_plan(int n, int d, int v, int dtype, int flags) {
   p.ldz = ceil_div(v, 16) * 16;
   p.z_size = dtype == RH_F32 ? 8 : 4;
   p.wide_w = !(flags & RH_CE_COPY_WEIGHT);      // here that only says how the weights are read
-  p.past = (long long)v * d * (16 / vals) >= kPastCaches;
   if (flags & RH_CE_GRAD_X) plan_online(p, n, d, v, vals);
+  p.past = (long long)v * d * (16 / vals) >= ((flags & RH_CE_GRAD_X) && !p.rows ? kPastBeside : kPastAlone);
   const int whole = p.rows ? kThreads : 64;      // threads, or sixteen times the waves, of a row of weights
   p.tpr = 16;
   while (p.tpr < whole && p.tpr * vals < d) p.tpr *= 2;

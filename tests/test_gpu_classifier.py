@@ -797,3 +797,67 @@ def test_scale_gradient(rh, n, dtype):
     exact = was.double() * 12.0
     f = torch.finfo(x.dtype)
     assert ((x.double() - exact).abs() <= f.eps / 2 * exact.abs() + f.smallest_normal * f.eps / 2).all()
+
+
+def test_float16_scaled_backward_from_other_streams_and_threads(rh):
+    """The gradients are made anew on the forward call's stream, wherever backward is called from."""
+    import threading
+    cases = [make(200, 96, 700, "f16", True, seed=50), make(90, 64, 5000, "f16", True, seed=51),
+             make(3, 1032, 900, "f16", True, seed=52)]
+    want = [rh.functional.linear_cross_entropy(*c, expected_grad=96.0, grads=(True, True, True)) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)] + [torch.cuda.default_stream()]
+    wrong = []
+
+    def work(i):
+        fn = rh.LinearCrossEntropy()
+        for k in range(12):
+            j, s = (i + k) % 3, streams[(i + k // 3) % 3]
+            x, w, y, b = cases[j]
+            leaves = leaves_of(x, w, b)
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                loss = fn(leaves[0], leaves[1], y, leaves[2])
+                scaled = loss * 96.0
+            torch.cuda.current_stream().wait_stream(s)
+            scaled.backward()
+            torch.cuda.synchronize()
+            wrong.extend((j, q) for t, q in zip(leaves, ("d_features", "d_weight", "d_bias")) if not torch.equal(t.grad, want[j][q]))
+
+    work(0)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_float16_as_a_scaler_and_checkpointing_call_it(rh):
+    from torch.utils.checkpoint import checkpoint
+    x, w, y, b = make(150, 72, 400, "f16", True, ignored=0.1, seed=53)
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 14)
+    want = rh.functional.linear_cross_entropy(x, w, y, b, expected_grad=2.0 ** 14, grads=(True, True, True))
+    for expected in (1.0, 2.0 ** 14):
+        fn = rh.LinearCrossEntropy(expected_grad=expected)
+        leaves = leaves_of(x, w, b)
+        scaler.scale(fn(leaves[0], leaves[1], y, leaves[2])).backward()
+        for t, k in zip(leaves, ("d_features", "d_weight", "d_bias")):
+            assert torch.equal(t.grad, want[k]), (k, expected)
+        for reentrant in (False, True):
+            leaves = leaves_of(x, w, b)
+            loss = checkpoint(lambda p, q, r: fn(p, q, y, r), *leaves, use_reentrant=reentrant)
+            scaler.scale(loss).backward()
+            for t, k in zip(leaves, ("d_features", "d_weight", "d_bias")):
+                assert torch.equal(t.grad, want[k]), (k, expected, reentrant)
+    # two calls of one weight: their gradients add up
+    fn = rh.LinearCrossEntropy()
+    leaves = leaves_of(x, w, b)
+    ((fn(leaves[0], leaves[1], y, leaves[2]) + fn(leaves[0], leaves[1], y, leaves[2])) * 2.0 ** 14).backward()
+    assert torch.equal(leaves[1].grad, want["d_weight"] * 2.0)
+    # a graph of the gradients still refuses to be differentiated
+    leaves = leaves_of(x, w, b)
+    (g,) = torch.autograd.grad(fn(leaves[0], leaves[1], y, leaves[2]) * 2.0 ** 14, leaves[0], create_graph=True)
+    assert torch.equal(g.detach(), want["d_features"])
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.float().sum().backward()

@@ -671,10 +671,19 @@ def grad_clip(tensors, max_norm=None, norm_type=2.0, stages=_lib.CLIP_ALL, out=N
     code = _norm_code(norm_type)
     if stages & _lib.CLIP_SCALE and (max_norm is None or not float(max_norm) >= 0.0):
         raise ValueError("max_norm must be a number from 0 on")
+    if out is None and not stages & _lib.CLIP_NORM:
+        raise ValueError("scaling alone needs the dict of the norm's stage as out")
+    if out is not None and not (out["total"].dtype == torch.float64 and out["norm"].dtype == torch.float32
+                                and out["total"].numel() == out["norm"].numel() == 1):
+        raise ValueError("out needs one float64 total and one float32 norm")
     dev, refs = _tensor_table(tensors, grads)
     if dev is None:
         return None
-    if out is None:
+    if out is not None:
+        made_on = _dev_check(out["total"], out["norm"])
+        if made_on != dev:
+            raise RetinaHeadError(f"tensors on different devices: {dev} and {made_on}")
+    else:
         out = {"norm": torch.empty((), dtype=torch.float32, device=dev),
                "total": torch.empty((1,), dtype=torch.float64, device=dev)}
     lib = _lib.load()

@@ -320,3 +320,13 @@ def test_the_factor_is_rounded_once(rh, p):
         rh.clip_grad_norm_(params_of([g]), 0.125, p)
         off = ((g.double() - was * c).abs() / (was.abs() * c).clamp(min=1e-30)).max()
         assert float(off) <= 2.0 ** -23 + 2.0 ** -40, seed
+
+
+def test_scaling_refuses_an_out_of_the_host(rh):
+    from retinahead import _lib
+    g = rand(100, "f32", 90)
+    kept = g.clone()
+    with pytest.raises(rh.RetinaHeadError, match="HIP device"):
+        rh.functional.grad_clip([g], 1.0, stages=_lib.CLIP_SCALE,
+                                out=dict(total=torch.ones(1, dtype=torch.float64), norm=torch.ones(())))
+    assert torch.equal(g, kept)

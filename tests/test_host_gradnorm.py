@@ -88,3 +88,15 @@ def test_refuses_tangents():
             rh.grad_norm(p.grad)
         with pytest.raises(rh.RetinaHeadError, match="forward-mode"):
             rh.clip_grad_norm_([p], 1.0)
+
+
+def test_stages_refuse_what_they_cannot_use():
+    F = rh.functional
+    p = torch.ones(4)
+    with pytest.raises(ValueError, match="as out"):      # its total would be anything
+        F.grad_clip([p], 1.0, stages=_lib.CLIP_SCALE)
+    total, norm = torch.ones(1, dtype=torch.float64), torch.ones(())
+    for out in (dict(total=total.float(), norm=norm), dict(total=total, norm=norm.double()),
+                dict(total=total.expand(2), norm=norm)):
+        with pytest.raises(ValueError, match="one float64 total"):
+            F.grad_clip([p], 1.0, stages=_lib.CLIP_SCALE, out=out)

@@ -123,10 +123,10 @@ struct WholeArgs {
 };
 constexpr int kWholeRows = 64;          // of a workgroup
 // Every 64 rows take the weights through LDS anew, twice, which costs more the larger they are; what it saves is
-// the logits' way to memory and back.  A whole call with its gradients, bfloat16, this way / the general one, us:
-// 49 104 x 256: 80 classes 83 / 97, 200 classes 100 / 133, 601 classes 164 / 182; 49 104 x 512, 300 classes 169 / 174;
-// 196 416 x 256, 80 classes 207 / 221; 8192 x 2048, 80 classes 95 / 99.  Against: 8192 x 512, 601 classes 87 / 86,
-// 8192 x 1024, 601 classes 119 / 102, 16 384 x 4096, 90 classes 278 / 224.
+// the logits' way to memory and back.  A whole call with its gradients, bfloat16, bias, this way / the general one, us:
+// 49 104 x 256: 80 classes 61 / 87, 200 classes 65 / 116, 601 classes 125 / 155; 49 104 x 512, 300 classes 129 / 154;
+// 196 416 x 256, 80 classes 162 / 238; 8192 x 2048, 80 classes 79 / 89.  Beyond: 8192 x 512, 601 classes 70 / 74,
+// 8192 x 1024, 601 classes 100 / 91, 16 384 x 4096, 90 classes 270 / 219.
 inline bool whole_pays(int d, int v) { return v <= 640 && (long long)ceil_div(v, 128) * d <= 2048; }
 template <typename T>
 int run_whole(const WholeArgs<T>& a, hipStream_t stream);

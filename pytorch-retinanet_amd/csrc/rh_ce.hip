@@ -16,10 +16,11 @@
 // Making the logits again instead takes 8 n d v, and P from them no fewer bytes.  Up to 640 classes
 // (rh_ce_whole.hip) and up to 16 rows (rh_ce_few.hip) there are other ways.
 //
-// 4096 x 2048 rows, a twentieth left out, 32 768 classes, bfloat16, us on the card: logits 565, P 84,
-// dX 485, dW 535, all else 45.  The three products make 0.97, 1.08 and 0.98 PFLOP/s; what bounds them is
-// the power that the matrix units draw on values that are not zeros (see rh_gemm.h) and, for the logits,
-// the 14 us a tile's end takes (256 x 256 exponentials a workgroup).
+// 4096 x 2048 rows, a twentieth left out, 32 768 classes, bfloat16, us, the least of eight passes: logits 504, P 82,
+// dX 426, dW 468, all else 42.  The three products make 1.04, 1.23 and 1.12 PFLOP/s.  The matrix units are busy
+// for 57, 70 and 60 % of the CUs' cycles (8192 x 4096: 69, 73 and 66 %): a tile's start and end are not hidden (the
+// logits' end, 256 x 256 exponentials a workgroup, takes 14 us).  And the clock is 1.9 GHz there (1.75) where the same
+// launches in the same cycles run at 2.4 on zeros.
 #include "rh_ce.h"
 
 namespace rh {
@@ -708,8 +709,8 @@ struct ProductArgs {
 enum To { kParts, kWhole, kSingly };
 
 // kLA = kRows: dX = P W, the sum over the classes; kCols: dW = P^T X, over the chunk's rows.  Bound by the matrix
-// units' power where the sums are long (8192 x 4096, 131 072 classes: 1.17 and 1.24 PFLOP/s), by filling the card
-// where the result is small; the splits that do so are cut()'s.  Workgroups that follow one another on an XCD
+// units (busy 73 and 66 % of the cycles) and their clock where the sums are long (8192 x 4096, 131 072 classes: 1.26 and
+// 1.18 PFLOP/s), by filling the card where the result is small; the splits that do so are cut()'s.  Workgroups that follow one another on an XCD
 // take the same split's tiles, which read the same rows: dW of 601 x 256 over 49 104 rows 26 us, 37 with a
 // split's tiles spread over the XCDs.
 template <typename T, Layout kLA, typename S, To kTo>
@@ -883,7 +884,8 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const float* __res
   }
 }
 
-// x *= scale / assumed in place, one rounding; an array whose scale is the assumed one is not touched.
+// x *= scale / assumed in place, one rounding; an array whose scale is the assumed one is not touched.  Bound by
+// memory: 268 MB of bfloat16 97 us (5.5 TB/s over both ways), of float32 75.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void upstream_kernel(T* __restrict__ x, const long long n,
                                                             const float* __restrict__ scale, const float assumed) {

@@ -2,7 +2,7 @@
 // The logits are never written: a workgroup makes all of its rows' logits, takes their softmax where they are,
 // writes P once (dW's operand) and multiplies it with the weights for dX while it is still in LDS.
 //
-// 49 104 x 256 against 601 classes, bfloat16: 82 us, where the logits by tiles, the joining of their sums, P
+// 49 104 x 256 against 601 classes, bfloat16: 80 us, where the logits by tiles, the joining of their sums, P
 // from the kept logits and dX by tiles took 103.  Of a workgroup's 25 us the logits take 8.5, the exponentials
 // 5.5, P 3.6 and dX 7.2: the products are bound by LDS (a wave of 32 rows reads a fragment of weights for every
 // instruction; the matrix units are busy 18% of the time), the rest by the vector units.  Up to 256 classes two

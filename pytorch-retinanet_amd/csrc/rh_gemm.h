@@ -283,7 +283,7 @@ struct Tile {
   // Fragments are read one half step ahead of the instructions that take them, and the loads of a
   // stage are spread over the step that frees its place in the ring, nearly three steps before it is
   // read.  8192 x 4096 x 16384 in bfloat16, uniform values: two stages of twice the depth, their loads in one
-  // burst, 1.04-1.10 PFLOP/s; this 1.12-1.16 (1.6-1.7 on zeros: the card's power sets its clock).
+  // burst, 1.04-1.10 PFLOP/s; this 1.12-1.16 (1.6-1.7 on zeros, where the clock stays at 2.4 GHz; here it is below 1.8).
   __device__ __forceinline__ void run(const void* a, long long lda, long long a_bytes, long long a_part,
                                       const void* b, long long ldb, long long b_bytes, long long b_part,
                                       const int steps_of_k, RH_LDS char* lds, const int a_limit = kStepBytes,

@@ -488,8 +488,8 @@ class LinearCrossEntropy(nn.Module):
     Element types: float32, bfloat16, float16 (one for all three; the gradients have it too).
     Products are summed in float32, softmax statistics and losses are float32.  For 16-bit types the
     softmax minus one-hot matrix is rounded once to the type, as an operand of the matrix units, and the
-    logits kept for it are accurate to 2^-12 (bfloat16) or 2^-13 (float16) of a probability, zero below
-    2^-32 or 2^-23 of the row's largest: gradients are off by up to a sixth more than rounding them to the
+    logits kept for it give a probability to 2^-12 (bfloat16) or 2^-13 (float16) of itself, and 0 below
+    2^-32 or 2^-23 of the largest of its 64 or 128 neighbours: gradients are off by up to a sixth more than rounding them to the
     type alone makes them (49 104 x 256, 601 classes, bfloat16: 1.94e-3 of their norm for 1.66e-3).
     float32 products are made of bfloat16 ones, three parts a number: as accurate as float32's own, but an
     infinite feature or weight makes the losses it meets NaN (a class is masked by a bias of -inf).
@@ -545,7 +545,7 @@ class LinearCrossEntropy(nn.Module):
 def grad_norm(tensors, norm_type=2.0):
     """float32 [] device tensor: the 2-, 1- or infinity norm over every value of ``tensors`` (one
     tensor or an iterable; float32, bfloat16 and float16 may be mixed).  Values and squares are summed
-    in float64.  An empty list has norm 0."""
+    in float64.  An empty list has norm 0.  Not differentiable."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     out = F.grad_clip(tensors, norm_type=norm_type, stages=_lib.CLIP_NORM)
     return torch.tensor(0.0) if out is None else out["norm"]
@@ -555,11 +555,13 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """Scales the gradients of ``parameters`` in place so that their norm over all of them is at most
     ``max_norm`` (each times min(1, max_norm / (norm + 1e-6))), and returns that norm from before as a
     float32 [] device tensor: the step between ``loss.backward()`` and ``optimizer.step()`` of
-    train.py:190-203.  Arguments and result are torch's own; nothing is read back
-    unless ``error_if_nonfinite`` asks for it.
+    train.py:190-203.  Arguments and result are as of torch's function of that name, without its
+    ``foreach`` (there is one way); the order of the norm is 2, 1 or infinity, ``max_norm`` from 0 on.
+    Nothing is read back unless ``error_if_nonfinite`` asks for it.
 
     Gradients may be float32, bfloat16 and float16 in one call, in any dense order of dimensions and at
-    any address, but two must not share memory.  A NaN or infinite gradient has the effect it has in
+    any address.  Refused are other types, sparse gradients, those that do not fill their memory (an
+    expanded one), two that share memory, and tangents of forward-mode differentiation.  A NaN or infinite gradient has the effect it has in
     torch: a NaN norm makes every gradient NaN, an infinite one makes them 0 (NaN where infinite).
     When every rank of a data-parallel job holds the same (already reduced) gradients this is the call;
     for parameters sharded over ranks see ``retinahead.dist.clip_grad_norm_``."""

@@ -20,6 +20,7 @@
 #include <array>
 #include <atomic>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <string>
 #include "retinahead.h"
@@ -251,10 +252,11 @@ CeOut classifier_loss(const at::Tensor& features, const at::Tensor& weight, cons
 // of a scaled loss are not (a mean over many rows), or too large, so there they are made anew from the inputs.
 struct LinearCrossEntropyBackward : public torch::autograd::Node {
   std::array<at::Tensor, 3> grads;
-  // float16: features, weight, labels, bias, divisor; those made under inference mode as they are
-  std::array<torch::autograd::SavedVariable, 5> inputs;
-  std::array<at::Tensor, 5> frozen;
-  bool anew = false;
+  struct Inputs {      // features, weight, labels, bias, divisor; those made under inference mode as they are
+    std::array<torch::autograd::SavedVariable, 5> saved;
+    std::array<at::Tensor, 5> frozen;
+  };
+  std::unique_ptr<Inputs> inputs;      // float16
   Settings settings = {};
   bool spent = false;
   std::mutex once;
@@ -264,6 +266,7 @@ struct LinearCrossEntropyBackward : public torch::autograd::Node {
   torch::autograd::variable_list apply(torch::autograd::variable_list&& upstream) override {
     torch::autograd::variable_list out(3);
     std::array<at::Tensor, 5> of;
+    bool anew = false;
     const at::Tensor& g = upstream[0];
     const bool as_made = settings.expected == 1.0 && g.defined() && g.numel() == 1 && g.is_cuda() &&
                          g.get_device() < kDevices && g.const_data_ptr() == unit[g.get_device()].load();
@@ -271,9 +274,10 @@ struct LinearCrossEntropyBackward : public torch::autograd::Node {
       std::lock_guard<std::mutex> lock(once);
       if (spent)
         raise_in_backward("the fused loss keeps one set of gradients: backward() can run once per forward()");
-      if (anew && g.defined() && !as_made)
-        for (int i = 0; i < 5; ++i)
-          of[i] = frozen[i].defined() ? frozen[i] : inputs[i].unpack();      // refuses what was changed in place
+      anew = inputs != nullptr && g.defined() && !as_made;
+      if (anew)
+        for (int i = 0; i < 5; ++i)      // unpack() refuses what was changed in place
+          of[i] = inputs->frozen[i].defined() ? inputs->frozen[i] : inputs->saved[i].unpack();
       spent = true;
       for (int i = 0; i < 3; ++i) out[i] = std::move(grads[i]);
     }
@@ -302,8 +306,7 @@ struct LinearCrossEntropyBackward : public torch::autograd::Node {
   void release_variables() override {
     std::lock_guard<std::mutex> lock(once);
     for (at::Tensor& d : grads) d.reset();
-    for (torch::autograd::SavedVariable& v : inputs) v.reset_data();
-    for (at::Tensor& t : frozen) t.reset();
+    inputs.reset();
     spent = true;
   }
 
@@ -384,12 +387,12 @@ PyObject* linear_ce(PyObject*, PyObject* args) {
       made->set_next_edges(torch::autograd::collect_next_edges(features, weight, bias));
       made->grads = std::move(out.grads);
       made->settings = q;
-      made->anew = features.scalar_type() == at::kHalf;
-      if (made->anew) {
+      if (features.scalar_type() == at::kHalf) {
+        made->inputs = std::make_unique<LinearCrossEntropyBackward::Inputs>();
         const at::Tensor* const of[5] = {&features, &weight, &labels, &bias, &divisor};
         for (int i = 0; i < 5; ++i)
-          if (of[i]->defined() && of[i]->is_inference()) made->frozen[i] = *of[i];
-          else made->inputs[i] = torch::autograd::SavedVariable(*of[i], false);
+          if (of[i]->defined() && of[i]->is_inference()) made->inputs->frozen[i] = *of[i];
+          else made->inputs->saved[i] = torch::autograd::SavedVariable(*of[i], false);
       }
       torch::autograd::set_history(loss, made);
     }
